@@ -122,6 +122,10 @@ _SIGNATURES = {
     'momentum_update_many': (_i, [ct.c_int, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
                                   ct.c_void_p, ct.c_void_p]),
     'softmax_ce_grad': (_i, [_M, _M, _M, _M, _M, _f]),
+    'layer_norm': (_i, [_M, _M, _M, _M, _f]), 'layer_norm_grad': (_i, [_M, _M, _M, _M, _M, _M, _f, _f, _f]),
+    'dot_gated': (_i, [_M, _M, _M, _M, _M, _i]), 'dot_gated_grad': (_i, [_M, _M, _M, _M, _M, _M, _M, _M, _i, _f, _f]),
+    'counter_dropout': (_i, [_M, _M, _M, _M, _f, _f, _u, _u, _u]),
+    'log_probs': (_i, [_M, _M, _M, _M, _M, _M, _M]), 'log_probs_grad': (_i, [_M, _M, _M, _M, _M, _M, _M]),
     'init_from_sparse_array': (None, [_S, ct.POINTER(ct.c_float), ct.POINTER(ct.c_int), ct.POINTER(ct.c_int),
                                       _i, _i, _i]),
     'allocate_device_memory_sparse': (_i, [_S]), 'copy_sparse_to_device': (_i, [_S]),
@@ -985,6 +989,119 @@ def softmax_ce_grad(mat, labels, probs=None, loss=None, grad=None, tiny=1e-10):
     _check(_cudamat.softmax_ce_grad(mat.p_mat, labels.p_mat, probs.p_mat, loss.p_mat if loss is not None else None,
                                     grad.p_mat if grad is not None else None, ct.c_float(tiny)))
     return probs
+
+
+def _p(mat):
+    return mat.p_mat if mat is not None else None
+
+
+def layer_norm(mat, gain=None, bias=None, target=None, eps=1e-5):
+    """Extension of this backend (not in the reference): target = gain * (mat - mean) / sqrt(variance + eps) + bias with
+    the mean and the variance of every column (the features of a case); gain and bias are rows x 1 or None (ones, zeros).
+    In place without a target."""
+    if target is None:
+        target = mat
+    _check(_cudamat.layer_norm(mat.p_mat, _p(gain), _p(bias), target.p_mat, float(eps)))
+    return target
+
+
+def layer_norm_grad(deriv, mat, gain=None, target=None, gain_grad=None, bias_grad=None, eps=1e-5, mult=1.0, beta=0.0):
+    """Extension of this backend (not in the reference): the backward pass of layer_norm(mat, gain, bias, eps=eps) from
+    deriv, the derivative by its result.  target = the derivative by mat (in the place of deriv by default);
+        gain_grad = beta * gain_grad + mult * (sums along the rows of deriv * normalised mat)
+        bias_grad = beta * bias_grad + mult * (sums along the rows of deriv)
+    where they are given (beta = 0 does not read them)."""
+    if target is None:
+        target = deriv
+    _check(_cudamat.layer_norm_grad(deriv.p_mat, mat.p_mat, _p(gain), target.p_mat, _p(gain_grad), _p(bias_grad), float(eps),
+                                    float(beta), float(mult)))
+    return target
+
+
+_GATES = dict(_ACTS, silu=4, swish=4, gelu=5)
+
+
+def _gate(act):
+    if act not in _GATES:
+        raise ValueError("act must be one of %s" % sorted(k for k in _GATES if k))
+    return _GATES[act]
+
+
+def dot_gated(m1, m2, bias=None, target=None, act='silu', pre=None):
+    """Extension of this backend (not in the reference): the gated half of a feed-forward block.  With the 2 f rows of
+    P = m1 . m2 + bias, target = act(P[0:f]) * P[f:2f]: the first f rows of m1 (columns of a weight matrix w given as w.T) make the
+    gate, the others what it lets through.  act: None, 'sigmoid', 'relu', 'tanh', 'silu' (x sigmoid(x)), 'gelu' (x times the
+    normal distribution function of x); bias: 2 f x 1 or None; pre, where given, receives P for dot_gated_grad."""
+    if target is None:
+        m = _cudamat.get_leading_dimension(m1.p_mat)
+        if m % 2:
+            raise generate_exception(-1)
+        target = empty((m // 2, _cudamat.get_nonleading_dimension(m2.p_mat)))
+    _check(_cudamat.dot_gated(m1.p_mat, m2.p_mat, _p(bias), target.p_mat, _p(pre), _gate(act)))
+    return target
+
+
+def dot_gated_grad(deriv, m1, m2, pre, target=None, m1_grad=None, m2_grad=None, bias_grad=None, act='silu', mult=1.0, beta=0.0):
+    """Extension of this backend (not in the reference): the backward pass of dot_gated(m1, m2, bias, act=act, pre=pre) from deriv, the
+    derivative by its target.  target = the derivative by P (in the place of pre by default); where they are given,
+        m1_grad = beta * m1_grad + mult * (derivative by m1), bias_grad = beta * bias_grad + mult * (derivative by bias)
+        m2_grad = derivative by m2
+    in the shapes that the operands are stored in: m1_grad of w.T is that of w."""
+    if target is None:
+        target = pre
+    _check(_cudamat.dot_gated_grad(deriv.p_mat, m1.p_mat, m2.p_mat, pre.p_mat, target.p_mat, _p(m1_grad), _p(m2_grad), _p(bias_grad),
+                                   _gate(act), float(beta), float(mult)))
+    return target
+
+
+def counter_dropout(mat, dropprob, seed, stream=0, step=None, mult=None, residual=None, target=None):
+    """Extension of this backend (not in the reference): target = [residual +] mult * mat with each entry dropped (0 in its place)
+    with probability dropprob, by a generator that is a function of seed (64 bits), stream (32 bits: one a layer), step and
+    the entry's place (Philox4x32-10).  No mask is stored: the backward pass is the same call on the derivative, without residual.
+        step    a 1 x 1 matrix that counts training steps on the device (step.add(1); a recorded graph counts too), or None
+        mult    1 / (1 - dropprob) by default (0 where everything is dropped); 1 for deepnet's own rule, which scales at test time
+    In place without a target, which may be mat or residual."""
+    if not 0.0 <= dropprob <= 1.0:
+        raise ValueError("dropprob must be between 0 and 1.")
+    if not 0 <= seed < 1 << 64 or not 0 <= stream < 1 << 32:
+        raise ValueError("seed must be a whole number of 64 bits, stream one of 32.")
+    if mult is None:
+        mult = 1.0 / (1.0 - dropprob) if dropprob < 1.0 else 0.0
+    if target is None:
+        target = mat
+    _check(_cudamat.counter_dropout(mat.p_mat, _p(residual), target.p_mat, _p(step), float(dropprob), float(mult), int(seed) & 0xffffffff,
+                                    int(seed) >> 32, int(stream)))
+    return target
+
+
+LOG_PROBS_MAX_TOP = 64
+
+
+def log_probs(mat, labels=None, logp=None, entropy=None, log_z=None, top=None, top_labels=None):
+    """Extension of this backend (not in the reference): of softmax(mat), mat being vocabulary x columns of logits, in one read
+    and without storing probabilities, as far as matrices are given for it (logp is made where only labels are):
+        logp (1 x columns)        log probability of the token labels[c]; 0 where that is no token (outside [0, vocabulary): padding)
+        entropy, log_z (1 x columns)   entropy, and log of the sum of exponentials
+        top, top_labels (k x columns)  log probabilities and places of the k <= 64 greatest entries, the greatest first, of equal ones
+                                  the one further up
+    Entries of -infinity have probability 0; a column of nothing else has log_z = log probabilities = -infinity and entropy 0.  NaN and
+    +infinity make their column NaN."""
+    if logp is None and labels is not None:
+        logp = empty((1, mat.shape[1]))
+    _check(_cudamat.log_probs(mat.p_mat, _p(labels), _p(logp), _p(entropy), _p(log_z), _p(top), _p(top_labels)))
+    return logp
+
+
+def log_probs_grad(mat, labels, log_z, logp_weight=None, entropy=None, entropy_weight=None, target=None):
+    """Extension of this backend (not in the reference): target (mat by default) = the derivative by mat of
+        sum over the columns of  logp_weight * logp + entropy_weight * entropy
+    from log_z and entropy as log_probs returns them (1 x columns each).  labels None: no first term; logp_weight None: ones;
+    entropy and entropy_weight None: no second term.  Columns without a token have no first term.  The gradient of the
+    cross-entropy loss is that of logp_weight = -1."""
+    if target is None:
+        target = mat
+    _check(_cudamat.log_probs_grad(mat.p_mat, _p(labels), log_z.p_mat, _p(logp_weight), _p(entropy), _p(entropy_weight), target.p_mat))
+    return target
 
 
 def momentum_update(w, w_delta, gradient, momentum, epsilon, l2_decay=None, l1_decay=None, reset_gradient=True):

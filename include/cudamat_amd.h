@@ -329,6 +329,53 @@ int launch_deferred(void);
  * of up to 128 the products and sums of the six calls themselves, in one launch: the same bits). ---- */
 int cd_update(cudamat* W, cudamat* bv, cudamat* bh, cudamat* v, cudamat* h, cudamat* v2, cudamat* h2, float eps);
 
+/* ---- Extension: the parts of a net over tokens that work on one column (a token's features or logits) at a time; no
+ * counterpart in the reference.  Nothing is held back, nothing waits.  Matrices that are written may be one that is read where
+ * that is said, and share no memory with the others (-9). ---- */
+
+/* Layer norm: target = gain * (mat - mean) / sqrt(variance + eps) + bias, mean and (biased) variance of each column.
+ * gain, bias: rows x 1 or NULL (ones, zeros); target may be mat; eps >= 0. */
+int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, float eps);
+/* Its gradients from the derivative by its result: target = derivative by mat (may be deriv or mat);
+ * gain_grad = beta * gain_grad + mult * (sums over the columns), bias_grad likewise (each may be NULL; beta = 0 reads nothing). */
+int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target, cudamat* gain_grad, cudamat* bias_grad, float eps,
+                    float beta, float mult);
+
+/* Gated product: with P = op(mat1) * op(mat2) + bias, of 2 f rows, target = act(P[0:f]) * P[f:2f].
+ * bias: 2 f x 1 or NULL.  pre: 2 f x columns, receives P for the backward pass, or NULL.
+ * act: 0 none, 1 sigmoid, 2 max(x, 0), 3 tanh, 4 x sigmoid(x), 5 x Phi(x) (Phi: the normal distribution function). */
+int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cudamat* pre, int act);
+/* Its gradients from deriv, the derivative by its target: target = derivative by P (2 f x columns, may be pre);
+ * mat1_grad = beta * mat1_grad + mult * (derivative by mat1 as it is stored), bias_grad likewise from the sums over the
+ * columns, mat2_grad = derivative by mat2 as it is stored (each may be NULL). */
+int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, cudamat* target, cudamat* mat1_grad, cudamat* mat2_grad,
+                   cudamat* bias_grad, int act, float beta, float mult);
+
+/* Dropout without a mask: target = [residual +] mult * mat, of dropped entries [residual +] 0.  Entry i (column-major) is
+ * dropped when word i % 4 of Philox4x32-10 (Salmon et al., SC 2011) at the counter (i / 4, i / 4 >> 32, step, stream) with
+ * the key (seed_lo, seed_hi) is below floor(dropprob * 2^32).  The same arguments drop the same entries, so the backward pass is the same
+ * call on the derivative.  step: a 1 x 1 matrix on the device whose 32 bits count (add 1 to it every training step,
+ * recorded graphs too; as a float it counts to 2^24), or NULL (0).  residual: NULL or mat's shape; target may be mat or residual. */
+int counter_dropout(cudamat* mat, cudamat* residual, cudamat* target, cudamat* step, float dropprob, float mult,
+                    unsigned seed_lo, unsigned seed_hi, unsigned stream);
+
+/* Log probabilities of tokens under softmax(mat), mat: vocabulary x columns.  labels: 1 x columns, the given tokens as
+ * floats; a label outside [0, vocabulary) is no token (padding).  Each output may be NULL:
+ *   logp 1 x columns      log probability of the given token; 0 for no token
+ *   entropy 1 x columns   of the column's distribution
+ *   log_z 1 x columns     log of the sum of exponentials (what log_probs_grad takes)
+ *   top, top_labels  k x columns, k <= 64: log probabilities and places of the k greatest entries, the greatest first, of
+ *                         equal ones the one further up; NaN ranks with -infinity
+ * Entries of -infinity have probability 0; a column of nothing else has log_z and log probabilities of -infinity and entropy 0.
+ * A column with NaN or +infinity has NaN in all but top_labels and the 0 of no token.  Vocabularies of up to 2^24. */
+#define LOG_PROBS_MAX_TOP 64
+int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cudamat* log_z, cudamat* top, cudamat* top_labels);
+/* target (may be mat) = derivative by mat of  sum over the columns of  logp_weight * logp + entropy_weight * entropy, from log_z and
+ * entropy as log_probs returns them.  labels NULL: no first term; logp_weight NULL: ones; entropy and entropy_weight NULL (both): no second
+ * term.  A column that is no token has no first term; a column of -infinity gives zeros. */
+int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_weight, cudamat* entropy, cudamat* entropy_weight,
+                   cudamat* target);
+
 /* ---- HIP graphs: no counterpart in the reference.  graph_capture_begin() makes the library
  * record every following call (with the pointers and scalars it is given) into a HIP graph
  * instead of running it, until graph_capture_end() returns the executable graph;

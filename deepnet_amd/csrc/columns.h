@@ -1,0 +1,59 @@
+// Teams of lanes on the columns of a matrix: sums over a team, and columns as 16-byte groups at any 4-byte boundary.
+#pragma once
+#include "common.h"
+
+// Sums over the 16 lanes of a row, or over a wavefront, by the cross-lane paths of the vector unit (a shuffle through LDS takes some
+// 60 cycles a step, these 8).  Every lane gets the same bits: each step adds the same two numbers on both sides.
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int T>
+__device__ __forceinline__ float lanes_sum(float v) {
+  static_assert(T == 16 || T == 64, "a row or a wavefront");
+  v += lane_move<0xB1>(v);         // neighbours
+  v += lane_move<0x4E>(v);         // pairs
+  v += lane_move<0x141>(v);        // halves of a row, mirrored
+  v += lane_move<0x140>(v);        // the row, mirrored
+  if (T == 64) {                   // the four rows' sums, as scalars (the whole wavefront is here)
+    const int x = __builtin_bit_cast(int, v);
+    auto row = [&](int l) __attribute__((always_inline)) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, l)); };
+    v = (row(0) + row(16)) + (row(32) + row(48));
+  }
+  return v;
+}
+
+// A column of h >= 4 floats as groups of four: group j starts at row 4 j, the last one at h - 4; the rows that it has in common with the
+// one before (`lap`, only where h is no multiple of 4) are that one's.
+struct __attribute__((packed, aligned(4))) ColGroupAny { float x, y, z, w; };
+template <bool STREAM>
+__device__ __forceinline__ void col_load(float (&v)[4], const float* p) {
+  if (STREAM) {
+    const float4 q = dn_ld4<true>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  } else {
+    const ColGroupAny q = *reinterpret_cast<const ColGroupAny*>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  }
+}
+template <bool STREAM>
+__device__ __forceinline__ void col_store(float* p, const float (&v)[4]) {
+  if (STREAM) dn_st4<true>(p, make_float4(v[0], v[1], v[2], v[3]));
+  else *reinterpret_cast<ColGroupAny*>(p) = ColGroupAny{v[0], v[1], v[2], v[3]};
+}
+template <int NV, bool TAIL>
+struct ColGroups {
+  int row[NV];                  // first row of a lane's group, or -1 for none
+  int lap;                      // rows of the last group that are its neighbour's, for the lane that has it (TAIL)
+  int last;                     // which of its groups that is, or -1
+  __device__ __forceinline__ void init(int lane, int T, int h) {
+    lap = 0; last = -1;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int r = 4 * (lane + k * T);
+      row[k] = r < h ? r : -1;
+      if (TAIL && r < h && r + 4 > h) { row[k] = h - 4; lap = r - (h - 4); last = k; }
+    }
+  }
+  __device__ __forceinline__ bool own(int k, int e) const { return !TAIL || k != last || e >= lap; }
+};

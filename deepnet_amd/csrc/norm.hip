@@ -1,5 +1,5 @@
 // Layer norm of columns and its gradients (no counterpart in cudamat.cu): a column is the h features of one case.
-#include "common.h"
+#include "columns.h"
 #include <math.h>
 
 // Sums over the 256 lanes of a workgroup; every lane gets them.  `red` is free again after the next barrier.
@@ -100,6 +100,332 @@ __global__ void __launch_bounds__(256) k_layer_norm_grad_inputs(const float* der
   }
 }
 
+// ------------------------------------------------------------------ columns that stay in registers
+// A team (16 or 64 lanes, or T = 0: the workgroup) holds a column, NV groups of four rows a lane, from its one read to its one write; gain and bias stay in
+// registers for all columns that the team takes, and the next column is on its way while this one is reduced.  Arithmetic of
+// k_layer_norm: sum, then deviations from the rounded mean.
+__device__ __forceinline__ float norm_rstd(float sq, float d, float inv_h, float eps) {
+  const float var = sq * inv_h - d * d;
+  return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);       // (NaN stays)
+}
+
+// A team's sums of deviations.  A wavefront (or a row of 16 lanes) takes deviations from the rounded mean of its own n rows, so that
+// nothing is exchanged for the mean first; the wavefronts of a team meet once, in LDS, where each shifts every other's sums to the team's mean
+// m: sum (x - m) = S1 + n (m_i - m), sum (x - m)^2 = S2 + 2 (m_i - m) S1 + n (m_i - m)^2, sum g (x - m) = GX + (m_i - m) G.
+// `v` holds x on entry and x - m on return (0 outside).
+struct NormSums { float d, sq, g, gx; };      // sums of x - m, of its square, of g and of g (x - m)
+template <int T, int NV, bool TAIL, bool GRAD>
+__device__ __forceinline__ NormSums norm_sums(const ColGroups<NV, TAIL>& at, float (&v)[NV][4], const float (&g)[NV][4], const float (&dy)[NV][4],
+                                              float* part, float n, float inv_n, float inv_h, int lane, int W) {
+#pragma clang fp contract(off)      // (the deviations are from the rounded means that the wavefronts exchange)
+  constexpr int R = T == 16 ? 16 : 64;
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += at.own(k, e) ? v[k][e] : 0.f;
+  const float mi = lanes_sum<R>(s) * inv_n;
+  NormSums o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[k][e] = at.row[k] >= 0 ? v[k][e] - mi : 0.f;
+      const float x = at.own(k, e) ? v[k][e] : 0.f;
+      o.d += x;
+      o.sq = __fmaf_rn(x, x, o.sq);
+      if (GRAD) {
+        const float y = at.own(k, e) ? g[k][e] * dy[k][e] : 0.f;
+        o.g += y;
+        o.gx = __fmaf_rn(y, x, o.gx);
+      }
+    }
+  o.d = lanes_sum<R>(o.d); o.sq = lanes_sum<R>(o.sq);
+  if (GRAD) { o.g = lanes_sum<R>(o.g); o.gx = lanes_sum<R>(o.gx); }
+  if (T) return o;
+  // (six arrays of 16)
+  if (lane % 64 == 0) {
+    float* p = part + lane / 64;
+    p[0] = mi; p[16] = n; p[32] = o.d; p[48] = o.sq;
+    if (GRAD) { p[64] = o.g; p[80] = o.gx; }
+  }
+  __syncthreads();
+  const int q = lane % 16;
+  const bool in = q < W;
+  const float mq = in ? part[q] : 0.f, nq = in ? part[16 + q] : 0.f, dq = in ? part[32 + q] : 0.f, sq = in ? part[48 + q] : 0.f;
+  const float gq = GRAD && in ? part[64 + q] : 0.f, gxq = GRAD && in ? part[80 + q] : 0.f;
+  const float m = lanes_sum<16>(nq * mq) * inv_h, by = mq - m;
+  o.d = lanes_sum<16>(__fmaf_rn(nq, by, dq));
+  o.sq = lanes_sum<16>(__fmaf_rn(by, __fmaf_rn(nq, by, 2.f * dq), sq));
+  if (GRAD) { o.g = lanes_sum<16>(gq); o.gx = lanes_sum<16>(__fmaf_rn(by, gq, gxq)); }
+  const float mine = mi - m;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[k][e] += mine;
+  return o;
+}
+// The rows of a wavefront of a team (T = 0), or of a team.
+template <int T, int NV>
+__device__ __forceinline__ float norm_rows(int lane, int lanes, int h) {
+  if (T) return (float)h;
+  int n = 0;
+  const int first = 4 * (lane & ~63);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int left = h - first - 4 * k * lanes;
+    n += left < 0 ? 0 : left < 256 ? left : 256;
+  }
+  return (float)n;
+}
+
+template <int T, int NV, bool TAIL, bool STREAM>
+__global__ void __launch_bounds__(T ? 256 : 1024)
+k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float* target, int h, int w, float eps) {
+  constexpr int TEAMS = T ? 256 / T : 1;
+  __shared__ float part[2][T ? 1 : 64];      // (two in turn: one may be read still when the other is written)
+  const int lane = T ? threadIdx.x % (T ? T : 1) : threadIdx.x, W = blockDim.x / 64;
+  ColGroups<NV, TAIL> at;
+  at.init(lane, T ? T : blockDim.x, h);
+  const float inv_h = 1.f / (float)h, rows = norm_rows<T, NV>(lane, T ? T : blockDim.x, h), inv_rows = 1.f / rows;
+  int turn = 0;
+  float gv[NV][4], bv[NV][4], x[NV][4], next[NV][4];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { gv[k][e] = 1.f; bv[k][e] = 0.f; x[k][e] = next[k][e] = 0.f; }
+    if (at.row[k] >= 0) {
+      if (gain) col_load<false>(gv[k], gain + at.row[k]);
+      if (bias) col_load<false>(bv[k], bias + at.row[k]);
+    }
+  }
+  const int stride = gridDim.x * TEAMS;
+  int c = blockIdx.x * TEAMS + (T ? threadIdx.x / (T ? T : 1) : 0);
+  if (c >= w) return;                                      // (whole workgroups where teams meet at barriers)
+  auto fetch = [&](float (&v)[NV][4], int col) __attribute__((always_inline)) {
+    const float* p = mat + (size_t)col * h;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at.row[k] >= 0) col_load<STREAM>(v[k], p + at.row[k]);
+  };
+  fetch(x, c);
+  for (;;) {
+    const int n = c + stride;
+    if (n < w) fetch(next, n);
+    const NormSums o = norm_sums<T, NV, TAIL, false>(at, x, gv, x, part[turn], rows, inv_rows, inv_h, lane, W);
+    turn ^= T ? 0 : 1;
+    const float d = o.d * inv_h, r = norm_rstd(o.sq, d, inv_h, eps);
+    float* t = target + (size_t)c * h;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at.row[k] >= 0) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = __fmaf_rn(gv[k][e], (x[k][e] - d) * r, bv[k][e]);
+        col_store<STREAM>(t + at.row[k], y);
+      }
+    if (n >= w) break;
+    c = n;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] = next[k][e];
+  }
+}
+
+// Backward in one pass over mat and deriv: with m known, sums of the deviations, their squares, g = gain * deriv and g times
+// the deviations come from one round.  The gradients of gain and bias stay in the lanes that have their rows, for all columns of
+// the workgroup; its teams meet in LDS at the end, and a second kernel adds up the workgroups (a single one finishes by itself).
+struct NormGradArgs {
+  const float *deriv, *mat, *gain;
+  float *target, *partial, *gain_grad, *bias_grad;
+  int h, w, waves;                // waves: of a team of whole wavefronts
+  float eps, beta, mult;
+};
+__device__ __forceinline__ void norm_param_out(float* out, int i, float sum, float beta, float mult) {
+  out[i] = beta != 0.f ? __fmaf_rn(mult, sum, beta * out[i]) : mult * sum;
+}
+
+template <int T, int NV, bool TAIL, bool STREAM>
+__global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
+  constexpr int AHEAD = NV <= 2 ? 1 : 0;                   // columns on their way (none fit the registers of 1024 lanes beyond)
+  __shared__ float part[2][T ? 1 : 16][T ? 1 : 96];
+  __shared__ float meet[NV <= 2 ? 512 * NV * 8 : 1];
+  const int h = a.h, w = a.w, W = a.waves, lanes = T ? T : 64 * W, teams = blockDim.x / lanes;
+  const int team = T ? threadIdx.x / (T ? T : 1) : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W, lane = threadIdx.x - team * lanes;
+  ColGroups<NV, TAIL> at;
+  at.init(lane, lanes, h);
+  const float inv_h = 1.f / (float)h, rows = norm_rows<T, NV>(lane, lanes, h), inv_rows = 1.f / rows;
+  int turn = 0;
+  float gv[NV][4], x[NV][4], dy[NV][4], nx[AHEAD ? AHEAD : 1][NV][4], ny[AHEAD ? AHEAD : 1][NV][4], sg[NV][4], sb[NV][4];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      gv[k][e] = 1.f; x[k][e] = dy[k][e] = sg[k][e] = sb[k][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) nx[q][k][e] = ny[q][k][e] = 0.f;
+    }
+    if (at.row[k] >= 0 && a.gain) col_load<false>(gv[k], a.gain + at.row[k]);
+  }
+  const int stride = gridDim.x * teams;
+  auto fetch = [&](float (&u)[NV][4], float (&v)[NV][4], int col) __attribute__((always_inline)) {
+    const size_t o = (size_t)col * h;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at.row[k] >= 0) {
+        col_load<STREAM>(u[k], a.mat + o + at.row[k]);
+        col_load<STREAM>(v[k], a.deriv + o + at.row[k]);
+      }
+  };
+  // every team of a workgroup makes the same number of trips; those beyond the last column count and store nothing
+  int c = blockIdx.x * teams + team;
+  if (AHEAD && c < w) fetch(x, dy, c);
+#pragma unroll
+  for (int q = 0; q + 1 < AHEAD; ++q)
+    if (c + (q + 1) * stride < w) fetch(nx[q], ny[q], c + (q + 1) * stride);
+  for (int base = blockIdx.x * teams; base < w; base += stride) {
+    const bool live = c < w;
+    const int n = c + AHEAD * stride;
+    if (n < w) { if (AHEAD) fetch(nx[AHEAD ? AHEAD - 1 : 0], ny[AHEAD ? AHEAD - 1 : 0], n); else fetch(x, dy, n); }
+    const NormSums o = norm_sums<T, NV, TAIL, true>(at, x, gv, dy, part[T ? 0 : turn][T ? 0 : team], rows, inv_rows, inv_h, lane, W);
+    turn ^= 1;
+    const float d = o.d * inv_h, r = norm_rstd(o.sq, d, inv_h, a.eps);
+    const float mg = o.g * inv_h, mgx = r * (o.gx - d * o.g) * inv_h;
+    if (live) {
+      float* t = a.target + (size_t)c * h;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (at.row[k] >= 0) {
+          float out[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float xh = (x[k][e] - d) * r;
+            sg[k][e] = __fmaf_rn(dy[k][e], xh, sg[k][e]);
+            sb[k][e] += dy[k][e];
+            out[e] = r * (__fmaf_rn(gv[k][e], dy[k][e], -mg) - xh * mgx);
+          }
+          col_store<STREAM>(t + at.row[k], out);
+        }
+    }
+    c += stride;
+    if (AHEAD) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[k][e] = nx[0][k][e]; dy[k][e] = ny[0][k][e];
+#pragma unroll
+          for (int q = 0; q + 1 < AHEAD; ++q) { nx[q][k][e] = nx[q + 1][k][e]; ny[q][k][e] = ny[q + 1][k][e]; }
+        }
+    }
+  }
+  if (!a.gain_grad && !a.bias_grad) return;
+  if (T == 16) {                  // teams of one wavefront
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+          sg[k][e] += __shfl_xor(sg[k][e], o, WAVE);
+          sb[k][e] += __shfl_xor(sb[k][e], o, WAVE);
+        }
+  }
+  // the later half of the teams (wavefronts, of teams that share one) hands its sums to the earlier one
+  const int U = T == 16 ? 64 : lanes, unit = T == 16 ? threadIdx.x >> 6 : team;
+  for (int units = blockDim.x / U; units > 1; units = (units + 1) >> 1) {
+    const int half = (units + 1) >> 1;
+    __syncthreads();
+    if (unit >= half && unit < units) {
+      const int to = (int)threadIdx.x - half * U;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { meet[(8 * k + e) * 512 + to] = sg[k][e]; meet[(8 * k + 4 + e) * 512 + to] = sb[k][e]; }
+    }
+    __syncthreads();
+    if (unit + half < units) {
+      const int from = threadIdx.x;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { sg[k][e] += meet[(8 * k + e) * 512 + from]; sb[k][e] += meet[(8 * k + 4 + e) * 512 + from]; }
+    }
+  }
+  if ((int)threadIdx.x < lanes) {
+    float* p = a.partial + (size_t)blockIdx.x * 2 * h;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at.row[k] >= 0 && at.own(k, e)) {
+          const int i = at.row[k] + e;
+          if (gridDim.x > 1) { p[i] = sg[k][e]; p[h + i] = sb[k][e]; }
+          else {
+            if (a.gain_grad) norm_param_out(a.gain_grad, i, sg[k][e], a.beta, a.mult);
+            if (a.bias_grad) norm_param_out(a.bias_grad, i, sb[k][e], a.beta, a.mult);
+          }
+        }
+  }
+}
+// The sums of `parts` workgroups: 64 of the 2 h rows a workgroup, its 16 wavefronts take every sixteenth part.
+__global__ void __launch_bounds__(1024) k_layer_norm_grad_finish(NormGradArgs a, int parts) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, rows = 2 * a.h, i = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (i < rows)
+#pragma unroll 4
+    for (int p = wv; p < parts; p += 16) s += a.partial[(size_t)p * rows + i];
+  red[wv][lane] = s;
+  __syncthreads();
+  if (wv == 0 && i < rows) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][lane];
+    float* out = i < a.h ? a.gain_grad : a.bias_grad;
+    if (out) norm_param_out(out, i < a.h ? i : i - a.h, s, a.beta, a.mult);
+  }
+}
+
+#define NORM_COLS_MAX 16384       // tallest columns that a team holds
+#define NORM_COLS_W (1 << 29)     // most of them (they are counted in 31 bits)
+
+// waves: of the workgroup, where that is a team
+template <int T, int NV>
+static void norm_launch(const float* mat, const float* gain, const float* bias, float* target, int h, int w, float eps, int waves = 4) {
+  const int teams = T ? 256 / (T ? T : 1) : 1, nt = 64 * waves;
+  const bool tail = h % 4 != 0, stream = !tail && (long long)h * w >= DN_STREAM_MIN_ELEMS && dn_aligned16(mat) && dn_aligned16(target);
+  // as many workgroups as fit the CUs, or one for as many columns as makes them even
+  const int groups = (w + teams - 1) / teams, most = dn_num_cus() * (2048 / nt), each = (groups + most - 1) / most;
+  const dim3 grid((unsigned)((groups + each - 1) / each));
+  if (tail) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, true, false>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
+  else if (stream) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, false, true>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
+  else hipLaunchKernelGGL((k_layer_norm_cols<T, NV, false, false>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
+}
+
+template <int T, int NV>
+static int norm_grad_launch(NormGradArgs a) {
+  const int lanes = T ? T : 64 * a.waves, cus = dn_num_cus(), least = T == 16 ? 4 : 1;
+  // teams of a workgroup: all that fit, or fewer where that leaves CUs without one
+  int teams = 1024 / lanes;
+  while (teams > least && (a.w + teams - 1) / teams < cus) teams = (teams + 1) / 2 > least ? (teams + 1) / 2 : least;
+  int blocks = (a.w + teams - 1) / teams;
+  if (blocks > cus) blocks = cus;
+  const bool sums = a.gain_grad || a.bias_grad;
+  if (sums && blocks > 1) {
+    a.partial = (float*)dn_scratch((size_t)blocks * 2 * a.h * sizeof(float));
+    if (!a.partial) return CUDA_ERROR;
+  }
+  const bool tail = a.h % 4 != 0, stream = !tail && (long long)a.h * a.w >= DN_STREAM_MIN_ELEMS && dn_aligned16(a.mat) && dn_aligned16(a.deriv) && dn_aligned16(a.target);
+  const dim3 grid((unsigned)blocks), block((unsigned)(teams * lanes));
+  if (tail) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, true, false>), grid, block, 0, dn_stream(), a);
+  else if (stream) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, false, true>), grid, block, 0, dn_stream(), a);
+  else hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, false, false>), grid, block, 0, dn_stream(), a);
+  if (sums && blocks > 1)
+    hipLaunchKernelGGL(k_layer_norm_grad_finish, dim3((unsigned)((2 * a.h + 63) / 64)), dim3(1024), 0, dn_stream(), a, blocks);
+  return dn_launch_status();
+}
+
 static inline bool apart(const cudamat* a, const cudamat* b) {
   return !a || !b || a->data_device + dn_len(a) <= b->data_device || b->data_device + dn_len(b) <= a->data_device;
 }
@@ -124,6 +450,16 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, floa
   if (int e = check_vector(bias, h)) return e;
   if (!(eps >= 0.f) || !same_or_apart(mat, target) || !apart(gain, target) || !apart(bias, target)) return ERROR_UNSUPPORTED;
   if (h <= 0 || w <= 0) return 0;
+  if (h >= 4 && h <= NORM_COLS_MAX && w <= NORM_COLS_W) {
+    const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
+    float* t = target->data_device;
+    if (h <= 64) norm_launch<16, 1>(x, g, b, t, h, w, eps);
+    else if (h <= 256) norm_launch<64, 1>(x, g, b, t, h, w, eps);
+    else if (h <= 512) norm_launch<64, 2>(x, g, b, t, h, w, eps);
+    else if (h <= 1024) norm_launch<64, 4>(x, g, b, t, h, w, eps);
+    else norm_launch<0, 4>(x, g, b, t, h, w, eps, (h + 1023) / 1024);
+    return dn_launch_status();
+  }
   hipLaunchKernelGGL(k_layer_norm, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)mat->data_device,
                      (const float*)(gain ? gain->data_device : nullptr), (const float*)(bias ? bias->data_device : nullptr), target->data_device, h, eps);
   return dn_launch_status();
@@ -144,6 +480,15 @@ int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target
     if (!apart(m, gain_grad) || !apart(m, bias_grad)) return ERROR_UNSUPPORTED;
   if (!apart(gain_grad, bias_grad)) return ERROR_UNSUPPORTED;
   if (h <= 0) return 0;
+  if (h >= 4 && h <= NORM_COLS_MAX && w > 0 && w <= NORM_COLS_W) {
+    NormGradArgs a = {deriv->data_device, mat->data_device, gain ? gain->data_device : nullptr, target->data_device, nullptr,
+                            gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, h <= 8192 ? (h + 511) / 512 : (h + 1023) / 1024, eps, beta, mult};
+    if (h <= 64) return norm_grad_launch<16, 1>(a);
+    if (h <= 256) return norm_grad_launch<64, 1>(a);
+    if (h <= 512) return norm_grad_launch<64, 2>(a);
+    if (h <= 8192) return norm_grad_launch<0, 2>(a);
+    return norm_grad_launch<0, 4>(a);
+  }
   float* stats = (float*)dn_scratch((size_t)(w > 0 ? w : 1) * 5 * sizeof(float));
   if (!stats) return CUDA_ERROR;
   const float* gp = gain ? gain->data_device : nullptr;

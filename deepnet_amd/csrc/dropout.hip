@@ -18,21 +18,40 @@ __device__ __forceinline__ void philox10(uint32_t (&c)[4], PhiloxKey k) {
 }
 
 // Entry i of the matrix (column-major) is dropped when word i % 4 of counter (i / 4, i / 4 >> 32, bits of the step,
-// stream) is below border.  target may be mat or residual.
+// stream) is below border.  target may be mat or residual.  A lane has one counter and its four entries, 16 bytes at any 4-byte boundary
+// that are on their way while the generator runs (20 products of 32 bits, which issue at a quarter of the rate, take 0.6 of the time that the
+// bytes do; with all ten rounds as fast as with seven).  Bound by the bytes: 4096 x 8192 onto a residual 62.4 us, 6.46 TB/s, what a copy
+// reaches; 42.3 us without; 4097 x 4097 32.1.  Two, four, eight counters a lane: 64.0, 66.9, 68.7 us.
+struct __attribute__((packed, aligned(4))) DropGroup { float x, y, z, w; };
+template <bool RES, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_counter_dropout(const float* mat, const float* residual, float* target, const float* step, long long n, uint64_t border, float mult,
                   uint32_t stream, PhiloxKey key) {
-  const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long g = (long long)blockIdx.x * 256 + threadIdx.x, whole = n >> 2;
   if (4 * g >= n) return;
+  auto load = [](float (&v)[4], const float* p) __attribute__((always_inline)) {
+    if (STREAM) { const float4 q = dn_ld4<true>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+    else { const DropGroup q = *reinterpret_cast<const DropGroup*>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+  };
+  auto one = [&](float x, float r, uint32_t word) __attribute__((always_inline)) {
+    x = word >= border ? x : 0.f;
+    return RES ? __fmaf_rn(mult, x, r) : mult * x;
+  };
+  float x[4], r[4] = {0.f, 0.f, 0.f, 0.f};
+  if (g < whole) {
+    load(x, mat + 4 * g);
+    if (RES) load(r, residual + 4 * g);
+  }
   uint32_t c[4] = {(uint32_t)g, (uint32_t)(g >> 32), step ? __float_as_uint(*step) : 0u, stream};
   philox10(c, key);
+  if (g < whole) {
+    const float y[4] = {one(x[0], r[0], c[0]), one(x[1], r[1], c[1]), one(x[2], r[2], c[2]), one(x[3], r[3], c[3])};
+    if (STREAM) dn_st4<true>(target + 4 * g, make_float4(y[0], y[1], y[2], y[3]));
+    else *reinterpret_cast<DropGroup*>(target + 4 * g) = DropGroup{y[0], y[1], y[2], y[3]};
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const long long i = 4 * g + j;
-    if (i < n) {
-      const float x = c[j] >= border ? mat[i] : 0.f;
-      target[i] = residual ? __fmaf_rn(mult, x, residual[i]) : mult * x;
-    }
+    for (int j = 0; j < 3; ++j)
+      if (4 * g + j < n) target[4 * g + j] = one(mat[4 * g + j], RES ? residual[4 * g + j] : 0.f, c[j]);
   }
 }
 
@@ -55,9 +74,14 @@ extern "C" int counter_dropout(cudamat* mat, cudamat* residual, cudamat* target,
   if (n <= 0) return 0;
   const long long blocks = ((n + 3) / 4 + 255) / 256;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  hipLaunchKernelGGL(k_counter_dropout, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), (const float*)mat->data_device,
-                     (const float*)(residual ? residual->data_device : nullptr), target->data_device,
-                     (const float*)(step ? step->data_device : nullptr), n, (uint64_t)((double)dropprob * 4294967296.0), mult, stream,
-                     PhiloxKey{seed_lo, seed_hi});
+  const float *x = mat->data_device, *r = residual ? residual->data_device : nullptr, *s = step ? step->data_device : nullptr;
+  float* t = target->data_device;
+  const bool wide = n >= DN_STREAM_MIN_ELEMS && dn_aligned16(x) && dn_aligned16(t) && dn_aligned16(r);
+  const uint64_t border = (uint64_t)((double)dropprob * 4294967296.0);
+#define DROP_GO(R, S) hipLaunchKernelGGL((k_counter_dropout<R, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), x, r, t, s, n, border, mult, stream, PhiloxKey{seed_lo, seed_hi})
+  if (r) { if (wide) DROP_GO(true, true); else DROP_GO(true, false); }
+  else if (wide) DROP_GO(false, true);
+  else DROP_GO(false, false);
+#undef DROP_GO
   return dn_launch_status();
 }

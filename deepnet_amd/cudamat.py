@@ -1054,6 +1054,11 @@ def dot_gated_grad(deriv, m1, m2, pre, target=None, m1_grad=None, m2_grad=None, 
     return target
 
 
+def _word(bits):
+    """The low 32 bits as a signed whole number (what the callables of csrc/fastcall.c take)."""
+    return ((int(bits) + 0x80000000) & 0xffffffff) - 0x80000000
+
+
 def counter_dropout(mat, dropprob, seed, stream=0, step=None, mult=None, residual=None, target=None):
     """Extension of this backend (not in the reference): target = [residual +] mult * mat with each entry dropped (0 in its place)
     with probability dropprob, by a generator that is a function of seed (64 bits), stream (32 bits: one a layer), step and
@@ -1069,8 +1074,8 @@ def counter_dropout(mat, dropprob, seed, stream=0, step=None, mult=None, residua
         mult = 1.0 / (1.0 - dropprob) if dropprob < 1.0 else 0.0
     if target is None:
         target = mat
-    _check(_cudamat.counter_dropout(mat.p_mat, _p(residual), target.p_mat, _p(step), float(dropprob), float(mult), int(seed) & 0xffffffff,
-                                    int(seed) >> 32, int(stream)))
+    _check(_cudamat.counter_dropout(mat.p_mat, _p(residual), target.p_mat, _p(step), float(dropprob), float(mult), _word(seed),
+                                    _word(seed >> 32), _word(stream)))
     return target
 
 

@@ -2,23 +2,24 @@
 #pragma once
 #include "common.h"
 
-// Sums over the 16 lanes of a row, or over a wavefront, by the cross-lane paths of the vector unit (a shuffle through LDS takes some
-// 60 cycles a step, these 8).  Every lane gets the same bits: each step adds the same two numbers on both sides.
+// Sums or maxima over the 16 lanes of a row, or over a wavefront, by the cross-lane paths of the vector unit (a shuffle through LDS takes
+// some 60 cycles a step, these 8).  Every lane gets the same bits: each step combines the same two numbers on both sides.
 template <int CTRL>
 __device__ __forceinline__ float lane_move(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-template <int T>
+template <int T, bool MAX = false>
 __device__ __forceinline__ float lanes_sum(float v) {
   static_assert(T == 16 || T == 64, "a row or a wavefront");
-  v += lane_move<0xB1>(v);         // neighbours
-  v += lane_move<0x4E>(v);         // pairs
-  v += lane_move<0x141>(v);        // halves of a row, mirrored
-  v += lane_move<0x140>(v);        // the row, mirrored
-  if (T == 64) {                   // the four rows' sums, as scalars (the whole wavefront is here)
+  auto both = [](float a, float b) __attribute__((always_inline)) { return MAX ? fmaxf(a, b) : a + b; };
+  v = both(v, lane_move<0xB1>(v));         // neighbours
+  v = both(v, lane_move<0x4E>(v));         // pairs
+  v = both(v, lane_move<0x141>(v));        // halves of a row, mirrored
+  v = both(v, lane_move<0x140>(v));        // the row, mirrored
+  if (T == 64) {                           // the four rows' results, as scalars (the whole wavefront is here)
     const int x = __builtin_bit_cast(int, v);
     auto row = [&](int l) __attribute__((always_inline)) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, l)); };
-    v = (row(0) + row(16)) + (row(32) + row(48));
+    v = both(both(row(0), row(16)), both(row(32), row(48)));
   }
   return v;
 }

@@ -18,10 +18,10 @@ __device__ __forceinline__ void philox10(uint32_t (&c)[4], PhiloxKey k) {
 }
 
 // Entry i of the matrix (column-major) is dropped when word i % 4 of counter (i / 4, i / 4 >> 32, bits of the step,
-// stream) is below border.  target may be mat or residual.  A lane has one counter and its four entries, 16 bytes at any 4-byte boundary
-// that are on their way while the generator runs (20 products of 32 bits, which issue at a quarter of the rate, take 0.6 of the time that the
-// bytes do; with all ten rounds as fast as with seven).  Bound by the bytes: 4096 x 8192 onto a residual 62.4 us, 6.46 TB/s, what a copy
-// reaches; 42.3 us without; 4097 x 4097 32.1.  Two, four, eight counters a lane: 64.0, 66.9, 68.7 us.
+// stream) is below border.  target may be mat or residual.  A lane has one counter and its four entries, 16 bytes at any 4-byte
+// boundary that are on their way while the generator runs.  Bound by the bytes: 4096 x 8192 onto a residual 62.4 us, 6.46 TB/s, what a
+// copy reaches; 42.3 us without, 4097 x 4097 32.1.  Two, four, eight counters a lane: 64.0, 66.9, 68.7 us.  The generator is hidden: with
+// seven of its rounds instead of ten, four counters a lane take 66.4.
 struct __attribute__((packed, aligned(4))) DropGroup { float x, y, z, w; };
 template <bool RES, bool STREAM>
 __global__ void __launch_bounds__(256)

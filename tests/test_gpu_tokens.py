@@ -440,6 +440,29 @@ def test_log_probs_of_ties_masks_and_special_columns(cm, rng, h):
     assert o['logp'][0, 1] == -np.inf and o['logp'][0, 13] == 0 and o['logp'][0, 14] == 0 and (h < 100 or -1e-10 < o['logp'][0, 11] < 0)
 
 
+@pytest.mark.parametrize("h,w", [(40000, 600), (131072, 2), (60001, 700)])
+def test_log_probs_where_the_best_entries_are_close_together(cm, rng, h, w):
+    """Groups of four rows at a distance of 256 groups go to the same lane of a workgroup: with the large entries in a few lanes, far more
+    entries than asked for are candidates; with them in one run of rows, every lane has some."""
+    x = F(rng.standard_normal((h, w)))
+    rows = np.arange(h)
+    for c in range(w):
+        if c % 3 == 0:
+            x[(rows // 4) % 256 < 19, c] += 100.0
+        elif c % 3 == 1:
+            x[h // 2:h // 2 + 3000, c] += 50.0
+    labels = F(rng.integers(0, h, (1, w)))
+    X = cm.CUDAMatrix(x)
+    t, l = cm.empty((20, w)), cm.empty((20, w))
+    cm.log_probs(X, top=t, top_labels=l)
+    got, probs = l.asarray(), t.asarray()
+    for c in list(range(min(w, 9))) + [w - 1]:
+        order = np.argsort(-x[:, c].astype(np.float64), kind='stable')[:20]
+        assert np.array_equal(got[:, c], order), c
+    o = tok.log_probs(x[:, :4], labels[:, :4], 20)
+    check(probs[:, :4], o['top'][:, :w], logp_bounds(x[:, :4], labels[:, :4], o)['top'], 'top')
+
+
 def test_log_probs_gives_what_is_asked_for(cm, rng):
     x, labels = F(rng.standard_normal((300, 6))), F(rng.integers(0, 300, (1, 6)))
     X, L = cm.CUDAMatrix(x), cm.CUDAMatrix(labels)

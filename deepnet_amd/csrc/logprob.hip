@@ -21,6 +21,10 @@ __device__ __forceinline__ unsigned long long lp_key(float x, int i) {
   return ((unsigned long long)v << 32) | (unsigned)~i;
 }
 __device__ __forceinline__ int lp_key_index(unsigned long long k) { return (int)~(unsigned)k; }
+__device__ __forceinline__ float lp_key_value(unsigned long long key) {
+  const unsigned v = (unsigned)(key >> 32);
+  return __uint_as_float(v ^ ((v >> 31) ? 0x80000000u : 0xffffffffu));
+}
 
 // log(1 + r), r >= 0 (NaN stays NaN); 1 + r itself would round a small r away.
 __device__ __forceinline__ double lp_log1p(double u) {
@@ -41,57 +45,65 @@ struct LogProbArgs {
 // others r, the sum of e^(x - m), and t, that of (x - m) e^(x - m).  So log(sum of exponentials) = m + log(1 + (count - 1 + r)), to full
 // precision however small r is beside the maximum's own 1, and entropy = log(1 + ..) - t / (1 + ..).  Entries of -inf count nothing: a
 // column of nothing else has count 0.  NaN and +inf make r NaN.
-struct LogProbPart { float m, count, r, t; };
-__device__ __forceinline__ LogProbPart lp_none() { return LogProbPart{-FLT_MAX, 0.f, 0.f, 0.f}; }
-// e^d, d <= 0: the hardware's exp2 of d log2(e) in two terms (d itself is off by half a step, that is what the result is off by).
-__device__ __forceinline__ float lp_exp_fast(float d) { return __builtin_amdgcn_exp2f(__fmaf_rn(d, 1.925963033500011e-08f, d * 1.44269502162933349609375f)); }
+struct LogProbPart { float m; int count; float r, t; };
+__device__ __forceinline__ LogProbPart lp_none() { return LogProbPart{-FLT_MAX, 0, 0.f, 0.f}; }
+// e^d, d <= 0, by the hardware's exp2.  d is off by half a step already, which changes the result by u |d| of it (u = 2^-24); the product's
+// rounding is as much again, and the constant is off by 0.22 u of it.
+__device__ __forceinline__ float lp_exp_fast(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502162933349609375f); }
 // The part as seen from a maximum M >= m.
 __device__ __forceinline__ void lp_raise(LogProbPart& p, float M) {
   if (M > p.m) {
-    const float d = p.m - M, s = lp_exp_fast(d), all = p.r + p.count;
+    const float d = p.m - M, s = lp_exp_fast(d), all = p.r + (float)p.count;
     p.t = s * __fmaf_rn(fmaxf(d, -200.f), all, p.t);
     p.r = s * all;
-    p.count = 0.f;
+    p.count = 0;
     p.m = M;
   }
 }
 __device__ __forceinline__ void lp_take(LogProbPart& p, float x) {
   const float d = x - p.m, e = lp_exp_fast(d);
-  p.count += d == 0.f ? 1.f : 0.f;
+  p.count += d == 0.f ? 1 : 0;
   p.r += d == 0.f ? 0.f : e;
   p.t = __fmaf_rn(fmaxf(d, -200.f), e, p.t);               // (-inf: e is 0; what is kept of d does not matter below -200)
 }
 // Over the 64 lanes of a wavefront; every lane gets it.
 __device__ __forceinline__ LogProbPart lp_wave(LogProbPart p) {
   lp_raise(p, lanes_sum<64, true>(p.m));
-  return LogProbPart{p.m, lanes_sum<64>(p.count), lanes_sum<64>(p.r), lanes_sum<64>(p.t)};
+  return LogProbPart{p.m, (int)lanes_sum<64>((float)p.count), lanes_sum<64>(p.r), lanes_sum<64>(p.t)};
 }
 
 struct LogProbResult { float m, log_z; double lz; bool none; };
 __device__ __forceinline__ LogProbResult lp_result(const LogProbPart& p) {
   LogProbResult o;
   o.m = p.m;
-  o.none = p.count == 0.f && p.r == 0.f;
-  o.lz = lp_log1p((double)(p.count - 1.f) + (double)p.r);
+  o.none = p.count == 0 && p.r == 0.f;
+  o.lz = lp_log1p((double)(p.count - 1) + (double)p.r);
   o.log_z = o.none ? -INFINITY : p.r == p.r ? (float)((double)p.m + o.lz) : NAN;
   return o;
 }
 __device__ __forceinline__ float lp_of(const LogProbResult& o, float x) {
   return o.none ? -INFINITY : o.log_z != o.log_z ? NAN : (float)((double)x - (double)o.m - o.lz);
 }
-// The results of a column but for the top list, by one lane.
-__device__ __forceinline__ void lp_finish(const LogProbArgs& a, int col, const LogProbPart& p, const LogProbResult& o) {
-  if (a.log_z) a.log_z[col] = o.log_z;
-  if (a.entropy) a.entropy[col] = o.none ? 0.f : o.log_z != o.log_z ? NAN : (float)(o.lz - (double)p.t / ((double)p.count + (double)p.r));
+// The given token's entry, asked for before everything else: 0 for no token.
+struct LogProbLabel { float x; bool token; };
+__device__ __forceinline__ LogProbLabel lp_label(const LogProbArgs& a, int col) {
+  LogProbLabel o = {0.f, false};
   if (a.logp) {
     const float l = a.labels[col];
-    a.logp[col] = l >= 0.f && l < (float)a.h ? lp_of(o, a.mat[(size_t)col * a.h + (int)l]) : 0.f;
+    o.token = l >= 0.f && l < (float)a.h;
+    if (o.token) o.x = a.mat[(size_t)col * a.h + (int)l];
   }
+  return o;
+}
+// The results of a column but for the top list, by one lane.
+__device__ __forceinline__ void lp_finish(const LogProbArgs& a, int col, const LogProbPart& p, const LogProbResult& o, const LogProbLabel& l) {
+  if (a.log_z) a.log_z[col] = o.log_z;
+  if (a.entropy) a.entropy[col] = o.none ? 0.f : o.log_z != o.log_z ? NAN : (float)(o.lz - (double)p.t / ((double)p.count + (double)p.r));
+  if (a.logp) a.logp[col] = l.token ? lp_of(o, l.x) : 0.f;
 }
 __device__ __forceinline__ void lp_top_out(const LogProbArgs& a, int col, int rank, unsigned long long key, const LogProbResult& o) {
-  const int i = lp_key_index(key);
-  if (a.top) a.top[(size_t)col * a.k + rank] = lp_of(o, a.mat[(size_t)col * a.h + i]);
-  if (a.top_labels) a.top_labels[(size_t)col * a.k + rank] = (float)i;
+  if (a.top) a.top[(size_t)col * a.k + rank] = lp_of(o, lp_key_value(key));
+  if (a.top_labels) a.top_labels[(size_t)col * a.k + rank] = (float)lp_key_index(key);
 }
 // How many of n keys in LDS (n even, 16-byte aligned) are greater.
 __device__ __forceinline__ int lp_rank(unsigned long long key, const unsigned long long* keys, int n) {
@@ -104,21 +116,80 @@ __device__ __forceinline__ int lp_rank(unsigned long long key, const unsigned lo
   return r;
 }
 
-// The top list of a team.  The k greatest entries lie in the k lanes whose own greatest entries are the greatest: those lanes' entries
-// from the k-th of these maxima on are the candidates (k and a few more, unless a few lanes have far more than their share), and a
-// candidate's place is the number of greater ones.
+template <int CTRL>
+__device__ __forceinline__ int lane_move_int(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true); }
+__device__ __forceinline__ int lp_quad_sum(int v) { v += lane_move_int<0xB1>(v); return v + lane_move_int<0x4E>(v); }
+// How many of 64 values in LDS are greater than that of a quad of lanes, and how many are at least as great; each lane looks at 16.
+__device__ __forceinline__ void lp_standing(unsigned value, const unsigned* values, int lane, int& greater, int& least) {
+  int g = 0, l = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 q = *reinterpret_cast<const uint4*>(values + 16 * i + 4 * (lane & 3));
+    g += (q.x > value ? 1 : 0) + (q.y > value ? 1 : 0) + (q.z > value ? 1 : 0) + (q.w > value ? 1 : 0);
+    l += (q.x >= value ? 1 : 0) + (q.y >= value ? 1 : 0) + (q.z >= value ? 1 : 0) + (q.w >= value ? 1 : 0);
+  }
+  greater = lp_quad_sum(g);
+  least = lp_quad_sum(l);
+}
+// Element i of 16.
+__device__ __forceinline__ float lp_pick(const float (&x)[4][4], int i) {
+  float a[8], b[4];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) a[q] = i & 8 ? x[2 + q / 4][q % 4] : x[q / 4][q % 4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) b[q] = i & 4 ? a[4 + q] : a[q];
+  const float c0 = i & 2 ? b[2] : b[0], c1 = i & 2 ? b[3] : b[1];
+  return i & 1 ? c1 : c0;
+}
+// The greatest of the four of a quad.
+__device__ __forceinline__ unsigned lp_quad_max(unsigned v) {
+  const unsigned a = (unsigned)lane_move_int<0xB1>((int)v);
+  v = a > v ? a : v;
+  const unsigned b = (unsigned)lane_move_int<0x4E>((int)v);
+  return b > v ? b : v;
+}
+// Lanes before this one that are in the mask.
+__device__ __forceinline__ int lp_before(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+}
+// The places of the `count` keys of a list (two zeros behind them): out(place, key) of the first k.  Four lanes share a key, `lanes` are here.
+template <typename F>
+__device__ __forceinline__ void lp_places(const unsigned long long* list, int count, int k, int lane, int lanes, F out) {
+  for (int i0 = 0; i0 < count; i0 += lanes / 4) {
+    const int i = i0 + lane / 4;
+    const unsigned long long key = i < count ? list[i] : ~0ull;
+    int r = 0;
+#pragma unroll 4
+    for (int j = 2 * (lane % 4); j < count; j += 8) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + j);
+      r += (q.x > key ? 1 : 0) + (q.y > key ? 1 : 0);
+    }
+    r = lp_quad_sum(r);
+    if (lane % 4 == 0 && i < count && r < k) out(r, key);
+  }
+}
+// Upper halves of keys: the values' order; 0 is below all of them.
+__device__ __forceinline__ unsigned lp_order(float x) { return (unsigned)(lp_key(x, 0) >> 32); }
+
+// The top list of a team.  At least k entries reach the k-th of the maxima that 64 quads of lanes have of their own entries, and those that do
+// lie in lanes whose own maximum does: these are the candidates, k and a few more (unless a few lanes have far more than their
+// share), and a candidate's place is the number of greater ones.  Maxima are compared by value; where the k-th and the next one are alike
+// (a mask, a constant column), by their places too, lane by lane.
 #define LP_LIST 2048               // candidates that a workgroup holds
 
 // ---- columns (or segments of them) by a workgroup of 256 lanes, four 16-byte groups a lane in flight
-template <bool TOP>
+template <bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
   __shared__ LogProbPart parts[4];
   __shared__ __attribute__((aligned(16))) unsigned long long lane_keys[TOP ? 256 : 2], list[TOP ? LP_LIST + 2 : 2];
-  __shared__ int winners[TOP ? 64 : 1], listed, last;
-  __shared__ unsigned long long border;
+  __shared__ int winners[TOP ? 256 : 1], wave_won[4], won, listed, last;
+  __shared__ unsigned least_order;
+  __shared__ unsigned long long border_key;
+  unsigned* const orders = reinterpret_cast<unsigned*>(lane_keys);
   const int tid = threadIdx.x, col = blockIdx.x / a.segments, seg = blockIdx.x - col * a.segments;
   const int row0 = seg * a.length, n = a.h - row0 < a.length ? a.h - row0 : a.length, n4 = n >> 2, trips = (n4 + 1023) >> 10;
   const float* c = a.mat + (size_t)col * a.h + row0;
+  const LogProbLabel label = lp_label(a, col);
   LogProbPart p = lp_none();
   float best = -INFINITY;
   int best_at = 0;
@@ -126,12 +197,13 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int j = tid + 256 * u + 1024 * it;
-      if (j < n4) col_load<false>(v[u], c + 4 * j);
+      if (j < n4) col_load<STREAM>(v[u], c + 4 * j);
       else v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
     }
   };
   float v[4][4], next[4][4];
   load(v, 0);
+  if (TOP && tid == 0) listed = won = 0;
   for (int it = 0; it < trips; ++it) {
     if (it + 1 < trips) load(next, it + 1);
     float m = v[0][0];
@@ -144,90 +216,159 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { lp_take(p, v[u][e]); v[u][e] = next[u][e]; }
+      for (int e = 0; e < 4; ++e) lp_take(p, v[u][e]);
+    if (it + 1 < trips) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u][e] = next[u][e];
+    }
   }
   const bool tail = tid < (n & 3);                         // the rows behind the last group: one a lane
+  float tail_x = 0.f;
   if (tail) {
-    const float x = c[4 * n4 + tid];
-    lp_raise(p, x);
-    lp_take(p, x);
+    tail_x = c[4 * n4 + tid];
+    lp_raise(p, tail_x);
+    lp_take(p, tail_x);
   }
+  const unsigned long long tail_key = TOP && tail ? lp_key(tail_x, row0 + 4 * n4 + tid) : 0;
   p = lp_wave(p);
   if (tid % 64 == 0) parts[tid >> 6] = p;
+  unsigned long long border = 1;           // candidates have keys from it on
+  bool by_value = true;                    // ... which are those of values from its own on
   if (TOP) {
-    // this lane's greatest entry: the first of its trip's greatest, or its row of the tail
-    unsigned long long key = 0;
+    const unsigned own = tid < n4 || tail ? lp_order(tail ? fmaxf(best, tail_x) : best) : 0, order = lp_quad_max(own);
+    if (tid % 4 == 0) orders[tid >> 2] = order;
+    __syncthreads();
+    int greater, reach;
+    lp_standing(order, orders, tid, greater, reach);
+    if (order && greater < a.k && reach >= a.k) { least_order = order; won = reach; }      // (the k-th one, or several: they write the same)
+    __syncthreads();
+    border = won == a.k ? (unsigned long long)least_order << 32 : 1;
+    bool in = own >= (unsigned)(border >> 32) && own;
+    if (won > a.k) {
+      // Several are alike at the border: now lane by lane, and of those alike the first places.
+      unsigned* const lanes = orders + 64;
+      auto standing = [&](unsigned value, int& greater, int& reach) __attribute__((always_inline)) {
+        lanes[tid] = value;
+        __syncthreads();
+        greater = reach = 0;
+#pragma unroll 4
+        for (int i = 0; i < 256; i += 4) {
+          const uint4 q = *reinterpret_cast<const uint4*>(lanes + i);
+          greater += (q.x > value ? 1 : 0) + (q.y > value ? 1 : 0) + (q.z > value ? 1 : 0) + (q.w > value ? 1 : 0);
+          reach += (q.x >= value ? 1 : 0) + (q.y >= value ? 1 : 0) + (q.z >= value ? 1 : 0) + (q.w >= value ? 1 : 0);
+        }
+        __syncthreads();
+      };
+      const unsigned long long above = __ballot(own > least_order);
+      if (tid % 64 == 0) wave_won[tid >> 6] = __popcll(above);
+      __syncthreads();
+      if (wave_won[0] + wave_won[1] + wave_won[2] + wave_won[3] >= a.k) {          // (else the quads' border is the lanes' too)
+        standing(own, greater, reach);
+        if (own && greater < a.k && reach >= a.k) { least_order = own; won = reach; }
+        __syncthreads();
+      }
+      const unsigned value = least_order;
+      by_value = won == a.k;
+      // this lane's greatest entry: the first that is its trip's maximum (the last trip is still in registers), of nothing but -inf and
+      // NaN the first of all; or its row of the tail
+      int first = tid < n4 ? 4 * tid : n;
+      if (best > -INFINITY) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = tid + 256 * u + 1024 * best_at;
-      if (j < n4) {
-        col_load<false>(v[u], c + 4 * j);
+        for (int u = 3; u >= 0; --u) {
+          const int j = tid + 256 * u + 1024 * best_at;
+          float x[4] = {v[u][0], v[u][1], v[u][2], v[u][3]};
+          if (best_at != trips - 1 && j < n4) col_load<false>(x, c + 4 * j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned long long q = lp_key(v[u][e], row0 + 4 * j + e);
-          key = q > key ? q : key;
+          for (int e = 3; e >= 0; --e) first = x[e] == best ? 4 * j + e : first;
         }
       }
+      if (tail && lp_order(tail_x) == own && (first >= n || lp_order(best) != own)) first = 4 * n4 + tid;
+      const unsigned place = own == value ? (unsigned)~(row0 + first) : 0;
+      if (tid == 0) border_key = (unsigned long long)value << 32;
+      standing(own > value ? 0xffffffffu : place, greater, reach);
+      if (!by_value && place && greater == a.k - 1) border_key |= place;
+      __syncthreads();
+      border = border_key;
+      in = ((unsigned long long)own << 32 | place) >= border && own;
     }
-    if (tail) {
-      const unsigned long long q = lp_key(c[4 * n4 + tid], row0 + 4 * n4 + tid);
-      key = q > key ? q : key;
+    if (trips > 1) {
+      const unsigned long long all = __ballot(in);
+      if (tid % 64 == 0) wave_won[tid >> 6] = __popcll(all);
+      __syncthreads();
+      int at = lp_before(all);
+      for (int i = 0; i < tid >> 6; ++i) at += wave_won[i];
+      if (in) winners[at] = tid;
     }
-    lane_keys[tid] = key;
-    if (tid == 0) { listed = 0; border = 1; }
   }
   __syncthreads();
-  auto all = [&]() __attribute__((always_inline)) {
+  {
     LogProbPart q = parts[tid & 3];
-    float m = fmaxf(fmaxf(parts[0].m, parts[1].m), fmaxf(parts[2].m, parts[3].m));
-    lp_raise(q, m);
+    lp_raise(q, fmaxf(fmaxf(parts[0].m, parts[1].m), fmaxf(parts[2].m, parts[3].m)));
     // (four neighbours have the four parts: sums over them)
     auto four = [](float x) __attribute__((always_inline)) { x += lane_move<0xB1>(x); return x + lane_move<0x4E>(x); };
-    return LogProbPart{m, four(q.count), four(q.r), four(q.t)};
-  };
-  p = all();
+    p = LogProbPart{q.m, (int)four((float)q.count), four(q.r), four(q.t)};
+  }
   if (TOP) {
-    const unsigned long long mine = lane_keys[tid];
-    const int rank = lp_rank(mine, lane_keys, 256);
-    if (mine && rank < a.k) {
-      winners[rank] = tid;
-      if (rank == a.k - 1) border = mine;
-    }
-    __syncthreads();
-    const unsigned long long from = border;
-    // (fewer lanes than k have entries only where there are fewer than 256 groups: then all of them take part)
-    const int lanes = from > 1 ? a.k : 0;
+    const float least = border > 1 ? lp_key_value(border) : -INFINITY;
     auto offer = [&](unsigned long long q) __attribute__((always_inline)) {
-      if (q >= from) {
+      if (q >= border) {
         const int at = atomicAdd(&listed, 1);
         if (at < LP_LIST) list[at] = q;
       }
     };
-    if (lanes) {
-      const int items = lanes * 4 * trips;
-      for (int i = tid; i < items; i += 256) {
-        const int q = i / (4 * trips), g = i - q * (4 * trips), j = winners[q] + 256 * (g & 3) + 1024 * (g >> 2);
-        if (j < n4) {
-          float x[4];
-          col_load<false>(x, c + 4 * j);
+    // a lane has one or two candidates among its sixteen entries at most times: one a turn (every lane of the wavefront is here)
+    auto offer16 = [&](const int (&j)[4], const float (&x)[4][4]) __attribute__((always_inline)) {
+      unsigned mask = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) offer(lp_key(x[e], row0 + 4 * j + e));
-        }
+      for (int i = 0; i < 16; ++i) mask |= !(x[i >> 2][i & 3] < least) ? 1u << i : 0;
+      if (!by_value) {                                     // (of the ones alike, those from the border's place on are none)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(x[i >> 2][i & 3] > least) && row0 + 4 * j[i >> 2] + (i & 3) > lp_key_index(border)) mask &= ~(1u << i);
       }
-    } else {
-      for (int j = tid; j < n4; j += 256) {
-        float x[4];
-        col_load<false>(x, c + 4 * j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) offer(lp_key(x[e], row0 + 4 * j + e));
+      for (int u = 0; u < 4; ++u) mask &= j[u] < n4 ? ~0u : ~(15u << (4 * u));
+      while (__ballot(mask != 0)) {
+        const int i = mask ? __builtin_ctz(mask) : 0, u = i >> 2;
+        const int g = u & 2 ? (u & 1 ? j[3] : j[2]) : (u & 1 ? j[1] : j[0]);
+        const unsigned long long key = mask ? lp_key(lp_pick(x, i), row0 + 4 * g + (i & 3)) : 0, in = __ballot(key >= border);
+        int at = 0;
+        if ((tid & 63) == 0) at = atomicAdd(&listed, __popcll(in));
+        at = __builtin_amdgcn_readfirstlane(at) + lp_before(in);
+        if (key >= border && at < LP_LIST) list[at] = key;
+        mask &= mask - 1;
+      }
+    };
+    if (trips <= 1) {
+      const int j[4] = {tid, tid + 256, tid + 512, tid + 768};
+      offer16(j, v);
+    } else {
+      // (the entries of those lanes come from memory, four groups a lane on their way)
+      const int items = (wave_won[0] + wave_won[1] + wave_won[2] + wave_won[3]) * 4 * trips;
+      for (int i0 = 0; i0 < items; i0 += 1024) {
+        float x[4][4];
+        int at[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int i = i0 + tid + 256 * s, q = i / (4 * trips), g = i - q * (4 * trips);
+          at[s] = i < items ? winners[q] + 256 * (g & 3) + 1024 * (g >> 2) : n4;
+          if (at[s] < n4) col_load<false>(x[s], c + 4 * at[s]);
+          else x[s][0] = x[s][1] = x[s][2] = x[s][3] = -INFINITY;
+        }
+        offer16(at, x);
       }
     }
-    if (tail) offer(lp_key(c[4 * n4 + tid], row0 + 4 * n4 + tid));
+    if (tail) offer(tail_key);
     __syncthreads();
   }
   // one segment: the column's results; several: this one's part, and the last to arrive joins them
-  LogProbResult o = lp_result(p);
-  if (a.segments == 1 && tid == 0) lp_finish(a, col, p, o);
+  LogProbResult o = {};
+  if (a.segments == 1) {
+    o = lp_result(p);
+    if (tid == 0) lp_finish(a, col, p, o, label);
+  }
   unsigned long long* const keys = TOP ? a.keys + (size_t)blockIdx.x * a.k : nullptr;
   auto out = [&](int rank, unsigned long long key) __attribute__((always_inline)) {
     if (a.segments == 1) lp_top_out(a, col, rank, key, o);
@@ -238,11 +379,9 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
     if (count <= LP_LIST) {
       if (tid < 2) list[count + tid] = 0;
       __syncthreads();
-      for (int i = tid; i < count; i += 256) {
-        const int rank = lp_rank(list[i], list, count + (count & 1));
-        if (rank < a.k) out(rank, list[i]);
-      }
-      for (int i = count + tid; i < a.k; i += 256) out(i, 0);          // (a segment of fewer than k rows)
+      lp_places(list, count, a.k, tid, 256, out);
+      if (a.segments > 1)
+        for (int i = count + tid; i < a.k; i += 256) out(i, 0);          // (a segment of fewer than k rows)
     } else {
       // more than fit: the greatest, the next one below it, and so on, a pass each
       unsigned long long above = ~0ull;
@@ -255,15 +394,15 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
         __syncthreads();
         lane_keys[tid] = key;
         __syncthreads();
-        if (lp_rank(key, lane_keys, 256) == 0 && key) { border = key; out(j, key); }
+        if (key && lp_rank(key, lane_keys, 256) == 0) { border_key = key; out(j, key); }
         __syncthreads();
-        above = border;
+        above = border_key;
       }
     }
   }
   if (a.segments == 1) return;
   if (tid < 4) {
-    const float f[4] = {p.m, p.count, p.r, p.t};
+    const float f[4] = {p.m, __builtin_bit_cast(float, p.count), p.r, p.t};
     __hip_atomic_store(a.parts + 4 * (size_t)blockIdx.x + tid, f[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __builtin_amdgcn_s_waitcnt(0);         // the stores of this wavefront have been acknowledged
@@ -273,37 +412,60 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
     last = old == (unsigned)a.segments - 1u;
     if (last) __hip_atomic_store(a.arrived + col, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
+  if (TOP && tid == 0) listed = won = 0;
   __syncthreads();
   if (!last) return;
   // at most 64 segments: a lane each, in a fixed order whoever came last
   const float* f = a.parts + 4 * ((size_t)col * a.segments + (tid & 63));
   auto get = [&](int i) __attribute__((always_inline)) { return __hip_atomic_load(f + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  const int count = a.segments * a.k;                      // (at most LP_JOIN: two keys a lane)
+  unsigned long long q[2] = {0, 0};
+  if (TOP) {
+    const unsigned long long* from = a.keys + (size_t)col * count;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (tid + 256 * i < count) q[i] = __hip_atomic_load(from + tid + 256 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   p = lp_none();
-  if ((tid & 63) < a.segments) p = LogProbPart{get(0), get(1), get(2), get(3)};
+  if ((tid & 63) < a.segments) p = LogProbPart{get(0), __builtin_bit_cast(int, get(1)), get(2), get(3)};
   p = lp_wave(p);
   o = lp_result(p);
-  if (tid == 0) lp_finish(a, col, p, o);
+  if (tid == 0) lp_finish(a, col, p, o, label);
   if (TOP) {
-    const int count = a.segments * a.k;                    // (at most LP_LIST)
-    const unsigned long long* from = a.keys + (size_t)col * count;
-    for (int i = tid; i < count; i += 256) list[i] = __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (tid < 2) list[count + tid] = 0;
+    // candidates: keys from the k-th of 64 maxima of four lanes each on (a key has one place: none are alike, and those of equal
+    // value are taken together)
+    const unsigned order = lp_quad_max((unsigned)((q[0] > q[1] ? q[0] : q[1]) >> 32));
+    if (tid % 4 == 0) orders[tid >> 2] = order;
     __syncthreads();
-    for (int i = tid; i < count; i += 256) {
-      const int rank = list[i] ? lp_rank(list[i], list, count + (count & 1)) : a.k;
-      if (rank < a.k) lp_top_out(a, col, rank, list[i], o);
+    int greater, reach;
+    lp_standing(order, orders, tid, greater, reach);
+    if (order && greater < a.k && reach >= a.k) { least_order = order; won = reach; }
+    __syncthreads();
+    const unsigned from_order = won ? least_order : 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned long long in = __ballot((unsigned)(q[i] >> 32) >= from_order);
+      int at = 0;
+      if ((tid & 63) == 0 && in) at = atomicAdd(&listed, __popcll(in));
+      at = __builtin_amdgcn_readfirstlane(at) + lp_before(in);
+      if (in >> (tid & 63) & 1) list[at] = q[i];
     }
+    __syncthreads();
+    const int found = listed;
+    if (tid < 2) list[found + tid] = 0;
+    __syncthreads();
+    lp_places(list, found, a.k, tid, 256, [&](int place, unsigned long long key) __attribute__((always_inline)) { lp_top_out(a, col, place, key, o); });
   }
 }
 
 // ---- columns of 4 to 1024 rows by a wavefront, which holds them in registers
 template <int NV, bool TAIL, bool TOP>
 __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned long long lane_keys[TOP ? 4 : 1][TOP ? 64 : 2], lists[TOP ? 4 : 1][TOP ? 256 * NV + 2 : 2];
-  __shared__ int listed[4];
+  __shared__ __attribute__((aligned(16))) unsigned long long lists[TOP ? 4 : 1][TOP ? 256 * NV + 2 : 2];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = blockIdx.x * 4 + wv;
   const bool live = col < a.w;
   const float* c = a.mat + (size_t)(live ? col : 0) * a.h;
+  const LogProbLabel label = lp_label(a, live ? col : 0);
   ColGroups<NV, TAIL> at;
   at.init(lane, 64, a.h);
   float v[NV][4], m = -FLT_MAX;
@@ -322,44 +484,76 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) lp_take(p, v[k][e]);
-  p = LogProbPart{p.m, lanes_sum<64>(p.count), lanes_sum<64>(p.r), lanes_sum<64>(p.t)};
+  p = LogProbPart{p.m, (int)lanes_sum<64>((float)p.count), lanes_sum<64>(p.r), lanes_sum<64>(p.t)};
   const LogProbResult o = lp_result(p);
-  if (live && lane == 0) lp_finish(a, col, p, o);
+  if (live && lane == 0) lp_finish(a, col, p, o, label);
   if (!TOP) return;
-  unsigned long long best = 0, border = 1;
+  unsigned long long best = 0;
   auto key_of = [&](int k, int e) __attribute__((always_inline)) { return at.row[k] >= 0 && at.own(k, e) ? lp_key(v[k][e], at.row[k] + e) : 0ull; };
+  // the lane's greatest entry: the first that is its maximum, of nothing but -inf and NaN the first of all
+  int first = -1;
+  float most = -INFINITY;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned long long q = key_of(k, e);
-      best = q > best ? q : best;
-    }
+    for (int e = 0; e < 4; ++e) most = fmaxf(most, v[k][e]);
+#pragma unroll
+  for (int k = NV - 1; k >= 0; --k)
+#pragma unroll
+    for (int e = 3; e >= 0; --e)
+      if (at.row[k] >= 0 && at.own(k, e) && (v[k][e] == most || most == -INFINITY)) first = at.row[k] + e;
+  if (first >= 0) best = lp_key(most, first);
   // (a wavefront's own part of LDS, whose accesses are in order: the compiler has to keep them so)
   auto ordered = []() __attribute__((always_inline)) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
-  unsigned long long *keys = lane_keys[wv], *list = lists[wv];
-  keys[lane] = best;
-  if (lane == 0) listed[wv] = 0;
+  unsigned long long* list = lists[wv];
+  unsigned* const orders = reinterpret_cast<unsigned*>(list);
+  const unsigned order = (unsigned)(best >> 32);
+  orders[lane] = order;
   ordered();
-  const int rank = lp_rank(best, keys, 64);
-  const unsigned long long at_border = __ballot(best && rank == a.k - 1);
-  if (at_border) border = keys[__builtin_ctzll(at_border)];
+  int greater, reach;
+  auto stand = [&](unsigned value) __attribute__((always_inline)) {
+    greater = reach = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(orders + i);
+      greater += (q.x > value ? 1 : 0) + (q.y > value ? 1 : 0) + (q.z > value ? 1 : 0) + (q.w > value ? 1 : 0);
+      reach += (q.x >= value ? 1 : 0) + (q.y >= value ? 1 : 0) + (q.z >= value ? 1 : 0) + (q.w >= value ? 1 : 0);
+    }
+  };
+  stand(order);
+  const unsigned long long kth = __ballot(order && greater < a.k && reach >= a.k);          // the k-th maximum, or several that are alike
   ordered();
+  unsigned long long border = 1;
+  if (kth) {
+    const int first_kth = __builtin_ctzll(kth);
+    border = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)order, first_kth) << 32;
+    if (__builtin_amdgcn_readlane(reach, first_kth) != a.k) {
+      // several are alike at the border: of those the first places
+      const unsigned value = (unsigned)(border >> 32), standing = order > value ? 0xffffffffu : order == value ? (unsigned)best : 0;
+      orders[lane] = standing;
+      ordered();
+      stand(standing);
+      border |= (unsigned)__builtin_amdgcn_readlane((int)standing, __builtin_ctzll(__ballot(standing && greater < a.k && reach >= a.k)));
+      ordered();
+    }
+  }
+  const float least = border > 1 ? lp_key_value(border) : -INFINITY;
+  int count = 0;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const unsigned long long q = key_of(k, e);
-      if (q >= border) list[atomicAdd(&listed[wv], 1)] = q;
+      const bool may = !(v[k][e] < least);
+      if (__ballot(may)) {
+        const unsigned long long q = may ? key_of(k, e) : 0, in = __ballot(q >= border);
+        if (q >= border) list[count + lp_before(in)] = q;
+        count += __popcll(in);
+      }
     }
   ordered();
-  const int count = listed[wv];
   if (lane < 2) list[count + lane] = 0;
   ordered();
-  for (int i = lane; i < count; i += 64) {
-    const int r = lp_rank(list[i], list, count + (count & 1));
-    if (live && r < a.k) lp_top_out(a, col, r, list[i], o);
-  }
+  lp_places(list, count, a.k, lane, 64, [&](int place, unsigned long long key) __attribute__((always_inline)) { if (live) lp_top_out(a, col, place, key, o); });
 }
 
 // target = logp_weight (onehot(label) - p) - entropy_weight p (log p + entropy), log p = mat - log_z: one pass.
@@ -445,8 +639,12 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   const long long blocks = (long long)w * segments;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  if (k) hipLaunchKernelGGL(k_log_probs<true>, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
-  else hipLaunchKernelGGL(k_log_probs<false>, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
+  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS && h % 4 == 0 && dn_aligned16(a.mat);
+#define LP_GO(TOP, S) hipLaunchKernelGGL((k_log_probs<TOP, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
+  if (k) { if (stream) LP_GO(true, true); else LP_GO(true, false); }
+  else if (stream) LP_GO(false, true);
+  else LP_GO(false, false);
+#undef LP_GO
   return dn_launch_status();
 }
 

@@ -26,21 +26,20 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 // A column of h >= 4 floats as groups of four: group j starts at row 4 j, the last one at h - 4; the rows that it has in common with the
 // one before (`lap`, only where h is no multiple of 4) are that one's.
-struct __attribute__((packed, aligned(4))) ColGroupAny { float x, y, z, w; };
+// STREAM: non-temporal accesses, for what is touched once.
+typedef float ColGroup __attribute__((ext_vector_type(4), aligned(4)));
 template <bool STREAM>
 __device__ __forceinline__ void col_load(float (&v)[4], const float* p) {
-  if (STREAM) {
-    const float4 q = dn_ld4<true>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
-    const ColGroupAny q = *reinterpret_cast<const ColGroupAny*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  }
+  const ColGroup* g = reinterpret_cast<const ColGroup*>(p);
+  const ColGroup q = STREAM ? __builtin_nontemporal_load(g) : *g;
+  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
 }
 template <bool STREAM>
 __device__ __forceinline__ void col_store(float* p, const float (&v)[4]) {
-  if (STREAM) dn_st4<true>(p, make_float4(v[0], v[1], v[2], v[3]));
-  else *reinterpret_cast<ColGroupAny*>(p) = ColGroupAny{v[0], v[1], v[2], v[3]};
+  ColGroup* g = reinterpret_cast<ColGroup*>(p);
+  const ColGroup q = {v[0], v[1], v[2], v[3]};
+  if (STREAM) __builtin_nontemporal_store(q, g);
+  else *g = q;
 }
 template <int NV, bool TAIL>
 struct ColGroups {

@@ -4,16 +4,6 @@
 #include "wide_math.h"
 #include <float.h>
 
-// e^t for t <= 0: t log2(e) in two terms, the hardware's exp2, a correction.  -inf gives 0, NaN stays NaN.
-__device__ __forceinline__ float lp_exp(float t) {
-  t = t < -128.f ? -128.f : t;      // (e^-128 is 0 in fp32; keeps -inf out of the correction)
-  const float L2E = 1.44269502162933349609375f, L2E_LO = 1.925963033500011e-08f;
-  const float p = t * L2E;
-  const float lo = __fmaf_rn(t, L2E_LO, __fmaf_rn(t, L2E, -p));
-  const float e = __builtin_amdgcn_exp2f(p);
-  return __fmaf_rn(e, lo * 0.693147182464599609375f, e);
-}
-
 // Orders entries: the greater value first, of equal ones (0 and -0 are) the one further up; NaN ranks with -inf.
 __device__ __forceinline__ unsigned long long lp_key(float x, int i) {
   x = x != x ? -INFINITY : x + 0.f;
@@ -556,24 +546,50 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   lp_places(list, count, a.k, lane, 64, [&](int place, unsigned long long key) __attribute__((always_inline)) { if (live) lp_top_out(a, col, place, key, o); });
 }
 
-// target = logp_weight (onehot(label) - p) - entropy_weight p (log p + entropy), log p = mat - log_z: one pass.
-__global__ void __launch_bounds__(256)
-k_log_probs_grad(const float* mat, const float* labels, const float* log_z, const float* logp_weight, const float* entropy,
-                 const float* entropy_weight, float* target, int h) {
-  const int col = blockIdx.x;
-  const float z = log_z[col], l = labels ? labels[col] : -1.f;
-  const bool token = l >= 0.f && l < (float)h;
-  const int label = token ? (int)l : -1;
-  const float lw = token ? (logp_weight ? logp_weight[col] : 1.f) : 0.f;
-  const float ew = entropy_weight ? entropy_weight[col] : 0.f, ent = entropy ? entropy[col] : 0.f;
-  const float* c = mat + (size_t)col * h;
-  float* t = target + (size_t)col * h;
-  for (int i = threadIdx.x; i < h; i += 256) {
-    const float x = c[i], lp = x - z;
-    const float p = x == -INFINITY ? 0.f : lp_exp(lp);
-    const float q = p > 0.f || p != p ? p * (lp + ent) : 0.f;
-    t[i] = lw * ((i == label ? 1.f : 0.f) - p) - ew * q;
+// target = logp_weight (onehot(label) - p) - entropy_weight p (log p + entropy), log p = mat - log_z, p = e^(log p): one pass.  A unit of 64
+// lanes (columns of up to 1024 rows) or 256 (pieces of 4096) takes up to 16 rows a lane of one column; the rows behind the last group of
+// four go one a lane, so that target may be mat (no row is read by one lane when another may have written it).
+struct LogProbGradArgs {
+  const float *mat, *labels, *log_z, *logp_weight, *entropy, *entropy_weight;
+  float* target;
+  int h, w, pieces, length;        // pieces of a column, and their rows (a multiple of 4)
+};
+template <int T, bool STREAM>
+__global__ void __launch_bounds__(256) k_log_probs_grad(LogProbGradArgs a) {
+  const int lane = threadIdx.x % T;
+  const long long unit = (long long)blockIdx.x * (256 / T) + threadIdx.x / T;
+  const int col = (int)(T == 64 ? unit : unit / a.pieces), piece = T == 64 ? 0 : (int)(unit - (long long)col * a.pieces);
+  if (col >= a.w) return;
+  const int row0 = piece * a.length, n = a.h - row0 < a.length ? a.h - row0 : a.length, n4 = n >> 2;
+  const float* c = a.mat + (size_t)col * a.h + row0;
+  float* t = a.target + (size_t)col * a.h + row0;
+  float v[4][4], last = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + T * u < n4) col_load<STREAM>(v[u], c + 4 * (lane + T * u));
+  const bool tail = lane < (n & 3);
+  if (tail) last = c[4 * n4 + lane];
+  const float z = a.log_z[col], l = a.labels ? a.labels[col] : -1.f;
+  const bool token = l >= 0.f && l < (float)a.h;
+  const int label = token ? (int)l - row0 : -1;
+  const float lw = token ? (a.logp_weight ? a.logp_weight[col] : 1.f) : 0.f;
+  const float ew = a.entropy_weight ? a.entropy_weight[col] : 0.f, ent = a.entropy ? a.entropy[col] : 0.f;
+  auto one = [&](float x, int i) __attribute__((always_inline)) {
+    const float lp = x - z;
+    const float e = __builtin_amdgcn_exp2f(__fmaf_rn(lp, 1.925963033500011e-08f, lp * 1.44269502162933349609375f));
+    const float p = x == -INFINITY ? 0.f : e;                        // (of a column of nothing else log p is no number)
+    const float q = p == 0.f ? 0.f : p * (lp + ent);
+    return lw * ((i == label ? 1.f : 0.f) - p) - ew * q;
+  };
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int j = lane + T * u;
+    if (j < n4) {
+      const float y[4] = {one(v[u][0], 4 * j), one(v[u][1], 4 * j + 1), one(v[u][2], 4 * j + 2), one(v[u][3], 4 * j + 3)};
+      col_store<STREAM>(t + 4 * j, y);
+    }
   }
+  if (tail) t[4 * n4 + lane] = one(last, 4 * n4 + lane);
 }
 
 static inline long long end_of(const cudamat* a) { return dn_len(a); }
@@ -639,7 +655,8 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   const long long blocks = (long long)w * segments;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS && h % 4 == 0 && dn_aligned16(a.mat);
+  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
+  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
 #define LP_GO(TOP, S) hipLaunchKernelGGL((k_log_probs<TOP, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
   if (k) { if (stream) LP_GO(true, true); else LP_GO(true, false); }
   else if (stream) LP_GO(false, true);
@@ -662,9 +679,19 @@ int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_
     if (!apart(m, target)) return ERROR_UNSUPPORTED;
   if ((!apart(mat, target) && mat->data_device != target->data_device) || h > (1 << 24)) return ERROR_UNSUPPORTED;
   if (h <= 0 || w <= 0) return 0;
-  hipLaunchKernelGGL(k_log_probs_grad, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)mat->data_device, (const float*)DPTR(labels),
-                     (const float*)log_z->data_device, (const float*)DPTR(logp_weight), (const float*)DPTR(entropy), (const float*)DPTR(entropy_weight),
-                     target->data_device, h);
+  const bool wave = h <= 1024;
+  const int pieces = wave ? 1 : (h + 4095) / 4096;
+  const LogProbGradArgs a = {mat->data_device, DPTR(labels), log_z->data_device, DPTR(logp_weight), DPTR(entropy), DPTR(entropy_weight),
+                             target->data_device, h, w, pieces, wave ? h : ((h + pieces - 1) / pieces + 3) / 4 * 4};
+  const long long blocks = wave ? (w + 3ll) / 4 : (long long)w * a.pieces;
+  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
+  // (at any alignment: 32003 x 1000 51.7 -> 47.7 us)
+  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
+#define LP_GRAD(T, S) hipLaunchKernelGGL((k_log_probs_grad<T, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
+  if (wave) { if (stream) LP_GRAD(64, true); else LP_GRAD(64, false); }
+  else if (stream) LP_GRAD(256, true);
+  else LP_GRAD(256, false);
+#undef LP_GRAD
   return dn_launch_status();
 }
 

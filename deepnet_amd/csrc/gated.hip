@@ -1,51 +1,200 @@
 // Gated products act(G) * U of the two halves of one product, and their backward pass (no counterpart in cudamat.cu).
-#include "common.h"
-#include "wide_math.h"
-#include <math.h>
+#include "columns.h"
+#include "gated_act.h"
 
-enum { GATE_LINEAR = 0, GATE_SIGMOID = 1, GATE_RELU = 2, GATE_TANH = 3, GATE_SILU = 4, GATE_GELU = 5 };
+bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int lda, const float* B, int ldb, const GatedOut& out, int* err);
 
-// The share of a normal variable below g; erfc keeps the digits of the small ones.
-__device__ __forceinline__ float gate_phi(float g) { return 0.5f * erfcf(g * -0.70710678118654752440f); }
+// ------------------------------------------------------------------ up to eight columns
+// One to eight columns (single tokens of a few sequences) against weights whose rows are contiguous: bound by the weights' bytes.  A
+// wavefront (or the four of a workgroup, a quarter of the terms each, where there are few units) has R units, that is 2 R rows, for all
+// columns; its lanes take 16 bytes of every row at any 4-byte boundary, U pieces of 256 terms on their way at once.
+struct GatedColumnsArgs {
+  const float *A, *B;
+  int lda, ldb, K;
+  GatedOut out;
+};
+template <int N, int R, int U, bool SHARED>
+__global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
+  __shared__ float part[SHARED ? 4 : 1][2 * R * N];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), f = a.out.f;
+  const int unit0 = (SHARED ? (int)blockIdx.x : (int)blockIdx.x * 4 + wv) * R, n4 = a.K >> 2;
+  if (!SHARED && unit0 >= f) return;
+  // (units beyond the last one repeat it and store nothing)
+  const float* row[2 * R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = unit0 + r < f ? unit0 + r : f - 1;
+    row[2 * r] = a.A + (size_t)i * a.lda;
+    row[2 * r + 1] = a.A + ((size_t)f + i) * a.lda;
+  }
+  float acc[2 * R][N];
+#pragma unroll
+  for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+    for (int c = 0; c < N; ++c) acc[r][c] = 0.f;
+  const int step = 64 * U * (SHARED ? 4 : 1);
+  for (int j0 = SHARED ? 64 * U * wv : 0; j0 < n4; j0 += step) {
+    float w[U][2 * R][4], x[U][N][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 64 * u + lane;
+#pragma unroll
+      for (int r = 0; r < 2 * R; ++r) {
+        w[u][r][0] = w[u][r][1] = w[u][r][2] = w[u][r][3] = 0.f;
+        if (j < n4) col_load<true>(w[u][r], row[r] + 4 * j);
+      }
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        x[u][c][0] = x[u][c][1] = x[u][c][2] = x[u][c][3] = 0.f;
+        if (j < n4) col_load<false>(x[u][c], a.B + (size_t)c * a.ldb + 4 * j);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][c] = __fmaf_rn(w[u][r][e], x[u][c][e], acc[r][c]);
+  }
+  if (lane < (a.K & 3) && (!SHARED || wv == 0)) {
+    const int k = 4 * n4 + lane;
+#pragma unroll
+    for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+      for (int c = 0; c < N; ++c) acc[r][c] = __fmaf_rn(row[r][k], a.B[(size_t)c * a.ldb + k], acc[r][c]);
+  }
+#pragma unroll
+  for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+    for (int c = 0; c < N; ++c) acc[r][c] = lanes_sum<64>(acc[r][c]);
+  if (SHARED) {
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+        for (int c = 0; c < N; ++c) part[wv][r * N + c] = acc[r][c];
+    }
+    __syncthreads();
+    if (wv) return;
+#pragma unroll
+    for (int r = 0; r < 2 * R; ++r)
+#pragma unroll
+      for (int c = 0; c < N; ++c) acc[r][c] = (part[0][r * N + c] + part[SHARED ? 1 : 0][r * N + c]) + (part[SHARED ? 2 : 0][r * N + c] + part[SHARED ? 3 : 0][r * N + c]);
+  }
+  // lane r N + c finishes unit r, column c
+  float g = 0.f, u = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      g = lane == r * N + c ? acc[2 * r][c] : g;
+      u = lane == r * N + c ? acc[2 * r + 1][c] : u;
+    }
+  if (lane < R * N && unit0 + lane / N < f) gated_out(a.out, unit0 + lane / N, lane % N, g, u);
+}
 
-__device__ __forceinline__ float gate_act(float g, int act) {
-  switch (act) {
-    case GATE_SIGMOID: return dn_sigmoid(g);
-    case GATE_RELU: return g < 0.f ? 0.f : g;
-    case GATE_TANH: return dn_tanh(g);
-    case GATE_SILU: return g * dn_sigmoid(g);
-    case GATE_GELU: return g * gate_phi(g);
-    default: return g;
+#define GATED_COLUMNS 8
+static int gated_columns(int n, const GatedColumnsArgs& a) {
+  const int f = a.out.f;
+  const bool shared = f < 8 * dn_num_cus();        // (fewer than eight wavefronts a CU by themselves)
+#define GATED_COLS(N, R, U)                                                                                                       \
+  case N:                                                                                                                         \
+    if (shared) hipLaunchKernelGGL((k_gated_columns<N, R, U, true>), dim3((unsigned)((f + R - 1) / R)), dim3(256), 0, dn_stream(), a); \
+    else hipLaunchKernelGGL((k_gated_columns<N, R, U, false>), dim3((unsigned)((f + 4 * R - 1) / (4 * R))), dim3(256), 0, dn_stream(), a);  \
+    break
+  switch (n) {
+    GATED_COLS(1, 1, 4);
+    GATED_COLS(2, 1, 4);
+    GATED_COLS(3, 2, 2);
+    GATED_COLS(4, 2, 2);
+    GATED_COLS(5, 2, 2);
+    GATED_COLS(6, 2, 2);
+    GATED_COLS(7, 2, 2);
+    GATED_COLS(8, 2, 2);
+  }
+#undef GATED_COLS
+  return dn_launch_status();
+}
+
+// ------------------------------------------------------------------ a pass over the halves
+// A unit of 64 lanes (columns of up to 1024 rows) or 256 (pieces of 4096) takes up to four groups of rows a lane of one column; the rows behind the
+// last group of four go one a lane.
+struct GatePass {
+  const float *deriv, *pre;
+  float* target;
+  int f, w, act, pieces, length;
+};
+// GRAD: target (2 f rows, may be pre) = the derivatives by the halves; else target = act(gate) * up.
+template <int T, bool GRAD, bool STREAM>
+__global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
+  const int lane = threadIdx.x % T;
+  const long long unit = (long long)blockIdx.x * (256 / T) + threadIdx.x / T;
+  const int col = (int)(T == 64 ? unit : unit / a.pieces), piece = T == 64 ? 0 : (int)(unit - (long long)col * a.pieces);
+  if (col >= a.w) return;
+  const int row0 = piece * a.length, n = a.f - row0 < a.length ? a.f - row0 : a.length, n4 = n >> 2;
+  const float* g = a.pre + 2 * (size_t)col * a.f + row0;
+  const float* d = GRAD ? a.deriv + (size_t)col * a.f + row0 : nullptr;
+  float* t = a.target + (GRAD ? 2 : 1) * (size_t)col * a.f + row0;
+  auto one = [&](float gate, float up, float deriv, float& to_gate, float& to_up) __attribute__((always_inline)) {
+    if (GRAD) {
+      float slope;
+      const float v = gate_act_slope(gate, a.act, &slope);
+      to_gate = deriv * up * slope;
+      to_up = deriv * v;
+    } else {
+      to_gate = gate_act(gate, a.act) * up;
+    }
+  };
+  float x[4][4], y[4][4], z[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int j = lane + T * u;
+    if (j < n4) {
+      col_load<STREAM>(x[u], g + 4 * j);
+      col_load<STREAM>(y[u], g + a.f + 4 * j);
+      if (GRAD) col_load<STREAM>(z[u], d + 4 * j);
+    }
+  }
+#pragma unroll 1
+  for (int u = 0; u < 4; ++u) {
+    const int j = lane + T * u;
+    if (j < n4) {
+      float p[4], q[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) one(x[0][e], y[0][e], GRAD ? z[0][e] : 0.f, p[e], q[e]);
+      col_store<STREAM>(t + 4 * j, p);
+      if (GRAD) col_store<STREAM>(t + a.f + 4 * j, q);
+    }
+    // (one copy of the code for the four groups: they move up)
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { x[k][e] = x[k + 1][e]; y[k][e] = y[k + 1][e]; if (GRAD) z[k][e] = z[k + 1][e]; }
+  }
+  if (lane < (n & 3)) {
+    const int i = 4 * n4 + lane;
+    float p, q;
+    one(g[i], g[a.f + i], GRAD ? d[i] : 0.f, p, q);
+    t[i] = p;
+    if (GRAD) t[a.f + i] = q;
   }
 }
-// The activation and its slope.
-__device__ __forceinline__ float gate_act_slope(float g, int act, float* slope) {
-  switch (act) {
-    case GATE_SIGMOID: { const float s = dn_sigmoid(g); *slope = s * dn_sigmoid(-g); return s; }
-    case GATE_RELU: *slope = g > 0.f ? 1.f : 0.f; return g < 0.f ? 0.f : g;
-    case GATE_TANH: { const float s = dn_tanh(g); *slope = (1.f - s) * (1.f + s); return s; }
-    case GATE_SILU: { const float s = dn_sigmoid(g), v = g * s; *slope = __fmaf_rn(v, dn_sigmoid(-g), s); return v; }
-    case GATE_GELU: { const float p = gate_phi(g); *slope = __fmaf_rn(g * 0.39894228040143267794f, dn_exp(-0.5f * g * g), p); return g * p; }
-    default: *slope = 1.f; return g;
-  }
-}
-
-// pre: the halves, f rows each, one above the other.
-__global__ void __launch_bounds__(256) k_gate(const float* pre, float* target, long long n, int f, int act) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= n) return;
-  const long long c = at / f, i = at - c * f;
-  target[at] = gate_act(pre[2 * c * f + i], act) * pre[2 * c * f + f + i];
-}
-// target (may be pre): the derivatives by the halves.
-__global__ void __launch_bounds__(256) k_gate_grad(const float* deriv, const float* pre, float* target, long long n, int f, int act) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= n) return;
-  const long long c = at / f, g = 2 * c * f + (at - c * f);
-  float slope;
-  const float d = deriv[at], u = pre[g + f], v = gate_act_slope(pre[g], act, &slope);
-  target[g] = d * u * slope;
-  target[g + f] = d * v;
+template <bool GRAD>
+static int gate_pass(const float* deriv, const float* pre, float* target, int f, int w, int act) {
+  const bool wave = f <= 1024;
+  const int pieces = wave ? 1 : (f + 4095) / 4096;
+  const GatePass a = {deriv, pre, target, f, w, act, pieces, wave ? f : ((f + pieces - 1) / pieces + 3) / 4 * 4};
+  const long long blocks = wave ? (w + 3ll) / 4 : (long long)w * pieces;
+  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
+  const bool stream = (long long)f * w >= DN_STREAM_MIN_ELEMS;
+#define GATE_GO(T, S) hipLaunchKernelGGL((k_gate_pass<T, GRAD, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
+  if (wave) { if (stream) GATE_GO(64, true); else GATE_GO(64, false); }
+  else if (stream) GATE_GO(256, true);
+  else GATE_GO(256, false);
+#undef GATE_GO
+  return dn_launch_status();
 }
 
 static inline bool apart(const cudamat* a, const cudamat* b) {
@@ -74,7 +223,13 @@ int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cuda
   if (act < GATE_LINEAR || act > GATE_GELU) return ERROR_UNSUPPORTED;
   const long long count = (long long)f * n;
   if (count <= 0) return 0;
-  if ((count + 255) / 256 > 0x7fffffffll) return ERROR_UNSUPPORTED;
+  const bool ta = mat1->is_trans != 0, tb = mat2->is_trans != 0;
+  const GatedOut out = {bias ? bias->data_device : nullptr, target->data_device, pre ? pre->data_device : nullptr, f, act};
+  if (n <= GATED_COLUMNS && ta && !tb && k > 0)
+    return gated_columns(n, GatedColumnsArgs{mat1->data_device, mat2->data_device, mat1->size[0], mat2->size[0], k, out});
+  int done = 0;
+  if (n > 1 && dn_gemm_gated(ta, tb, n, k, mat1->data_device, mat1->size[0], mat2->data_device, mat2->size[0], out, &done)) return done;
+  // other products: the halves, then a pass over them
   cudamat both = *target;
   both.size[0] = 2 * f;
   both.data_device = pre ? pre->data_device : (float*)dn_scratch((size_t)2 * count * sizeof(float), 1);
@@ -84,8 +239,7 @@ int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cuda
   if (!e && bias) e = add_col_vec(&both, bias, &both);
   set_deferred_epilogues(held);
   if (e) return e;
-  hipLaunchKernelGGL(k_gate, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, dn_stream(), (const float*)both.data_device, target->data_device, count, f, act);
-  return dn_launch_status();
+  return gate_pass<false>(nullptr, both.data_device, target->data_device, f, n, act);
 }
 
 int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, cudamat* target, cudamat* mat1_grad, cudamat* mat2_grad,
@@ -107,11 +261,7 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
     for (int i = 0; i < o; ++i)
       if (!apart(all[o], all[i]) && !(o == 4 && i == 3 && target->data_device == pre->data_device)) return ERROR_UNSUPPORTED;
   const long long count = (long long)f * n;
-  if ((count + 255) / 256 > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  if (count > 0)
-    hipLaunchKernelGGL(k_gate_grad, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, dn_stream(), (const float*)deriv->data_device,
-                       (const float*)pre->data_device, target->data_device, count, f, act);
-  int e = dn_launch_status();
+  int e = count > 0 ? gate_pass<true>(deriv->data_device, pre->data_device, target->data_device, f, n, act) : 0;
   const int held = set_deferred_epilogues(0);
   cudamat d = *target, x = *mat2, w = *mat1;
   if (!e && mat1_grad) {

@@ -1227,6 +1227,8 @@ bool dn_gemm_goes_ring(bool a_trans, bool b_trans, int M, int N, int K, const fl
   return M > 0 && N > 0 && gemm_plan(a_trans, !b_trans, M, N, K, A, lda, B, ldb, beta).kind == GEMM_RING;
 }
 
+#include "gemm_gated.h"
+
 // ------------------------------------------------------------------ the open group
 // Products that leave the held-back calls (elementwise.hip) go to the open group instead of the stream, as far as one kernel
 // with an epilogue computes them in a few microseconds.  They are launched when the next call comes that is no such product,

@@ -2,6 +2,7 @@
 #include "columns.h"
 #include "gated_act.h"
 
+int dn_row_sums(const float* M, int h, int w, float* y, float alpha, float beta);
 bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int lda, const float* B, int ldb, const GatedOut& out, int* err);
 
 // ------------------------------------------------------------------ up to eight columns
@@ -119,21 +120,20 @@ static int gated_columns(int n, const GatedColumnsArgs& a) {
 }
 
 // ------------------------------------------------------------------ a pass over the halves
-// A unit of 64 lanes (columns of up to 1024 rows) or 256 (pieces of 4096) takes up to four groups of rows a lane of one column; the rows behind the
-// last group of four go one a lane.
+// A wavefront takes up to G groups of four rows a lane of a piece of one column; the rows behind the last group go one a lane.
 struct GatePass {
   const float *deriv, *pre;
   float* target;
   int f, w, act, pieces, length;
 };
 // GRAD: target (2 f rows, may be pre) = the derivatives by the halves; else target = act(gate) * up.
-template <int T, bool GRAD, bool STREAM>
+template <int G, bool GRAD, bool STREAM>
 __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
-  const int lane = threadIdx.x % T;
-  const long long unit = (long long)blockIdx.x * (256 / T) + threadIdx.x / T;
-  const int col = (int)(T == 64 ? unit : unit / a.pieces), piece = T == 64 ? 0 : (int)(unit - (long long)col * a.pieces);
+  const int lane = threadIdx.x & 63;
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long col = unit / a.pieces;
   if (col >= a.w) return;
-  const int row0 = piece * a.length, n = a.f - row0 < a.length ? a.f - row0 : a.length, n4 = n >> 2;
+  const int row0 = (int)(unit - col * a.pieces) * a.length, n = a.f - row0 < a.length ? a.f - row0 : a.length, n4 = n >> 2;
   const float* g = a.pre + 2 * (size_t)col * a.f + row0;
   const float* d = GRAD ? a.deriv + (size_t)col * a.f + row0 : nullptr;
   float* t = a.target + (GRAD ? 2 : 1) * (size_t)col * a.f + row0;
@@ -147,10 +147,10 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
       to_gate = gate_act(gate, a.act) * up;
     }
   };
-  float x[4][4], y[4][4], z[4][4];
+  float x[G][4], y[G][4], z[G][4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int j = lane + T * u;
+  for (int u = 0; u < G; ++u) {
+    const int j = lane + 64 * u;
     if (j < n4) {
       col_load<STREAM>(x[u], g + 4 * j);
       col_load<STREAM>(y[u], g + a.f + 4 * j);
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
     }
   }
 #pragma unroll 1
-  for (int u = 0; u < 4; ++u) {
-    const int j = lane + T * u;
+  for (int u = 0; u < G; ++u) {
+    const int j = lane + 64 * u;
     if (j < n4) {
       float p[4], q[4];
 #pragma unroll
@@ -167,9 +167,9 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
       col_store<STREAM>(t + 4 * j, p);
       if (GRAD) col_store<STREAM>(t + a.f + 4 * j, q);
     }
-    // (one copy of the code for the four groups: they move up)
+    // (one copy of the code for the groups: they move up)
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
+    for (int k = 0; k + 1 < G; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) { x[k][e] = x[k + 1][e]; y[k][e] = y[k + 1][e]; if (GRAD) z[k][e] = z[k + 1][e]; }
   }
@@ -183,16 +183,16 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
 }
 template <bool GRAD>
 static int gate_pass(const float* deriv, const float* pre, float* target, int f, int w, int act) {
-  const bool wave = f <= 1024;
-  const int pieces = wave ? 1 : (f + 4095) / 4096;
-  const GatePass a = {deriv, pre, target, f, w, act, pieces, wave ? f : ((f + pieces - 1) / pieces + 3) / 4 * 4};
-  const long long blocks = wave ? (w + 3ll) / 4 : (long long)w * pieces;
+  // four groups a lane, or one where that makes less than two wavefronts for every SIMD
+  const bool wide = (long long)w * ((f + 1023) / 1024) >= 8 * dn_num_cus();
+  const int most = wide ? 1024 : 256, pieces = (f + most - 1) / most;
+  const GatePass a = {deriv, pre, target, f, w, act, pieces, ((f + pieces - 1) / pieces + 3) / 4 * 4};
+  const long long blocks = ((long long)w * pieces + 3) / 4;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
   const bool stream = (long long)f * w >= DN_STREAM_MIN_ELEMS;
-#define GATE_GO(T, S) hipLaunchKernelGGL((k_gate_pass<T, GRAD, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
-  if (wave) { if (stream) GATE_GO(64, true); else GATE_GO(64, false); }
-  else if (stream) GATE_GO(256, true);
-  else GATE_GO(256, false);
+#define GATE_GO(G, S) hipLaunchKernelGGL((k_gate_pass<G, GRAD, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
+  if (wide) { if (stream) GATE_GO(4, true); else GATE_GO(4, false); }
+  else GATE_GO(1, false);
 #undef GATE_GO
   return dn_launch_status();
 }
@@ -262,26 +262,28 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
       if (!apart(all[o], all[i]) && !(o == 4 && i == 3 && target->data_device == pre->data_device)) return ERROR_UNSUPPORTED;
   const long long count = (long long)f * n;
   int e = count > 0 ? gate_pass<true>(deriv->data_device, pre->data_device, target->data_device, f, n, act) : 0;
-  const int held = set_deferred_epilogues(0);
-  cudamat d = *target, x = *mat2, w = *mat1;
-  if (!e && mat1_grad) {
-    // by op(mat1): d op(mat2)^T; where mat1 is stored transposed, so is that
-    if (mat1->is_trans) { d.is_trans = 1; e = dot(&x, &d, mat1_grad, beta, mult); d.is_trans = 0; }
-    else { x.is_trans = !x.is_trans; e = dot(&d, &x, mat1_grad, beta, mult); x.is_trans = mat2->is_trans; }
+  if (e) return e;
+  const float *w = mat1->data_device, *x = mat2->data_device, *d = target->data_device;
+  const bool wt = mat1->is_trans != 0, xt = mat2->is_trans != 0;
+  // The sums go with the weights' gradient where a kernel takes both, and the two products, which have nothing to do with each
+  // other, share a launch where their tiles do.
+  DnRowSumJob job = {d, bias_grad ? bias_grad->data_device : nullptr, 2 * f, n, mult, beta, 0};
+  const int kind = bias_grad && mat1_grad && n > 0 && k > 0 ? dn_row_sum_job_kind(d, 2 * f, n) : 0;
+  job.scalar = kind == 2;
+  dn_group_allow(true);
+  // by op(mat1): d op(mat2)^T; where mat1 is stored transposed, so is that
+  if (mat1_grad && f > 0 && k > 0) {
+    e = wt ? dn_gemm_sums(xt, true, k, 2 * f, n, mult, x, mat2->size[0], d, 2 * f, beta, mat1_grad->data_device, k, &job, kind ? 1 : 0)
+           : dn_gemm_sums(false, !xt, 2 * f, k, n, mult, d, 2 * f, x, mat2->size[0], beta, mat1_grad->data_device, 2 * f, &job, kind ? 1 : 0);
   }
-  if (!e && mat2_grad) {
-    // by op(mat2): op(mat1)^T d
-    if (mat2->is_trans) { d.is_trans = 1; e = dot(&d, &w, mat2_grad, 0.f, 1.f); d.is_trans = 0; }
-    else { w.is_trans = !w.is_trans; e = dot(&w, &d, mat2_grad, 0.f, 1.f); }
-  }
-  if (!e && bias_grad) e = beta == 0.f && mult == 1.f ? sum_by_axis(&d, bias_grad, 1) : 0;
-  if (!e && bias_grad && !(beta == 0.f && mult == 1.f)) {
-    if (beta == 0.f) e = assign_scalar(bias_grad, 0.f);
-    else if (beta != 1.f) e = mult_by_scalar(bias_grad, beta, bias_grad);
-    if (!e) e = add_sum_by_axis(&d, bias_grad, 1, mult);
-  }
-  set_deferred_epilogues(held);
-  return e;
+  // by op(mat2): op(mat1)^T d
+  if (!e && mat2_grad && k > 0 && n > 0)
+    e = xt ? dn_gemm(true, wt, n, k, 2 * f, 1.f, d, 2 * f, w, mat1->size[0], 0.f, mat2_grad->data_device, n)
+           : dn_gemm(!wt, false, k, n, 2 * f, 1.f, w, mat1->size[0], d, 2 * f, 0.f, mat2_grad->data_device, k);
+  dn_group_allow(false);
+  dn_close_group();
+  if (!e && bias_grad && !kind) e = dn_row_sums(d, 2 * f, n, bias_grad->data_device, mult, beta);
+  return e ? e : dn_launch_status();
 }
 
 }  // extern "C"

@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(RING_THREADS, 4) k_gated_ring(GatedArgs a) {
   const int tid = threadIdx.x, f = a.out.f, N = g.N, K = g.K;
   int bx, by;
   if (!gated_tile(g, bx, by)) return;
-  const int m_lo = bx * HALF, n_lo = by * BN, m0 = m_lo + HALF <= f ? m_lo : f - HALF, n0 = n_lo + BN <= N ? n_lo : N - BN;
+  // (a single tile of fewer columns reads zeros behind the last one, the buffer's range check gives them; dn_gemm_gated)
+  const int m_lo = bx * HALF, n_lo = by * BN, m0 = m_lo + HALF <= f ? m_lo : f - HALF, n0 = n_lo + BN <= N || N < BN ? n_lo : N - BN;
   const int nst = (K + BK - 1) / BK;
   OA oa; OB ob;
   oa.init(g.A, g.a_bytes, g.lda, m0, f, K, tid);
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(RING_THREADS, 4) k_gated_ring(GatedArgs a) {
       x += lds[w * (BM * BN) + c * BM + i];
       y += lds[w * (BM * BN) + c * BM + HALF + i];
     }
-    if (m0 + i >= m_lo && n0 + c >= n_lo) gated_out(a.out, m0 + i, n0 + c, x, y);
+    if (m0 + i >= m_lo && n0 + c >= n_lo && n0 + c < N) gated_out(a.out, m0 + i, n0 + c, x, y);
   }
 }
 
@@ -95,7 +96,12 @@ bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int
   const int f = out.f, M = 2 * f;
   const bool a_kc = a_trans, b_kc = !b_trans;
   if (f <= 0 || N <= 0 || K <= 0) return false;
-  const GemmPlan plan = gemm_plan(a_kc, b_kc, M, N, K, A, lda, B, ldb, 0.f);
+  GemmPlan plan = gemm_plan(a_kc, b_kc, M, N, K, A, lda, B, ldb, 0.f);
+  // Strips of 9 to 15 columns, whose other kernels read the weights several times (2048 -> 5632 of 9 44.3 -> 22 us): the tile of 16 columns,
+  // where a column beyond the last one lies behind the operand's bytes.
+  if (N > 8 && N < 16 && f >= 16 && K > 128 && b_kc && (size_t)lda * (a_kc ? M : K) * sizeof(float) < (1ull << 31) &&
+      (size_t)16 * ldb * sizeof(float) < (1ull << 31))
+    plan = GemmPlan{GEMM_RING, RingPlan{4, 0.}, false};
   GatedArgs a = {RingArgs{A, B, nullptr, (unsigned)((size_t)lda * (a_kc ? M : K) * sizeof(float)), (unsigned)((size_t)ldb * (b_kc ? N : K) * sizeof(float)),
                           lda, ldb, 0, M, N, K, 0, 0, 1.f, 0.f}, out};
   auto grid = [&](int half, int bn) {

@@ -1091,6 +1091,10 @@ int dn_gemv_cols(const float* M, int ld, int h, int w, const float* x, float* y,
 int dn_gemv_rows(const float* M, int ld, int h, int w, const float* x, float* y, float alpha, float beta) {
   return rows_reduce<ROW_DOT>(M, ld, h, w, x, y, alpha, beta);
 }
+// y = beta * y + alpha * (sums along the rows)
+int dn_row_sums(const float* M, int h, int w, float* y, float alpha, float beta) {
+  return rows_reduce<ROW_SUM>(M, h, h, w, nullptr, y, alpha, beta);
+}
 
 // ------------------------------------------------------------------ flat dot / norm
 

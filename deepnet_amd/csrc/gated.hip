@@ -197,6 +197,153 @@ static int gate_pass(const float* deriv, const float* pre, float* target, int f,
   return dn_launch_status();
 }
 
+// ------------------------------------------------------------------ the backward products of up to eight columns
+// Both are bound by the weights' bytes: their gradient mult d x^T is written (k rows, 2 f columns), the inputs' gradient W d reads them.  A
+// wavefront has 256 rows, four a lane at any 4-byte boundary; the derivatives d of a slice of the 2 f units wait in LDS.
+#define FEW_ROWS 256
+#define FEW_SLICE 128
+struct FewArgs {
+  const float *W, *x, *d;
+  float *dw, *dx, *partial, *bias_grad;
+  int k, units, slice, slices;
+  float beta, mult;
+};
+template <int N>
+__device__ __forceinline__ void few_derivs(const FewArgs& a, float (*ds)[N], int j0, int len) {
+  for (int i = threadIdx.x; i < len * N; i += 256) ds[i % len][i / len] = a.d[(size_t)(i / len) * a.units + j0 + i % len];
+  __syncthreads();
+}
+// rows `count` (1 to 4) of a group
+__device__ __forceinline__ void few_load(float (&v)[4], const float* p, int count) {
+  if (count == 4) { col_load<true>(v, p); return; }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < count ? p[e] : 0.f;
+}
+// dw = beta dw + mult x d^T, and the sums of d: a wavefront a block of rows, all four the same slice of units.
+template <int N>
+__global__ void __launch_bounds__(256) k_few_outer(FewArgs a) {
+  __shared__ float ds[FEW_SLICE][N];
+  const int lane = threadIdx.x & 63, j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
+  few_derivs<N>(a, ds, j0, len);
+  if (a.bias_grad && blockIdx.x == 0)
+    for (int j = threadIdx.x; j < len; j += 256) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < N; ++c) s += ds[j][c];
+      float* b = a.bias_grad + j0 + j;
+      *b = a.beta != 0.f ? __fmaf_rn(a.mult, s, a.beta * *b) : a.mult * s;
+    }
+  const int row = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) * FEW_ROWS + 4 * lane, count = a.k - row < 4 ? a.k - row : 4;
+  if (!a.dw || count <= 0) return;
+  float x[N][4];
+#pragma unroll
+  for (int c = 0; c < N; ++c) few_load(x[c], a.x + (size_t)c * a.k + row, count);
+  float* out = a.dw + (size_t)j0 * a.k + row;
+#pragma unroll 4
+  for (int j = 0; j < len; ++j, out += a.k) {
+    float y[4] = {0.f, 0.f, 0.f, 0.f}, old[4] = {0.f, 0.f, 0.f, 0.f};
+    if (a.beta != 0.f) few_load(old, out, count);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __fmaf_rn(x[c][e], ds[j][c], y[e]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = a.beta != 0.f ? __fmaf_rn(a.mult, y[e], a.beta * old[e]) : a.mult * y[e];
+    if (count == 4) {
+      col_store<true>(out, y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) out[e] = y[e];
+    }
+  }
+}
+// W d: the four wavefronts of a workgroup take every fourth unit of a slice for the same rows and meet in LDS; slices are added up by
+// k_few_finish.
+template <int N>
+__global__ void __launch_bounds__(256) k_few_rows(FewArgs a) {
+  __shared__ float ds[FEW_SLICE][N], part[4][N][FEW_ROWS];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
+  few_derivs<N>(a, ds, j0, len);
+  const int row = (int)blockIdx.x * FEW_ROWS + 4 * lane, count = a.k - row < 4 ? a.k - row : 4;
+  float acc[N][4];
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[c][e] = 0.f;
+  if (count > 0) {
+    const float* w = a.W + (size_t)j0 * a.k + row;
+    for (int j = wv; j < len; j += 32) {
+      float v[8][4];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j + 4 * u < len) few_load(v[u], w + (size_t)(j + 4 * u) * a.k, count);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j + 4 * u < len) {
+#pragma unroll
+          for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][e] = __fmaf_rn(v[u][e], ds[j + 4 * u][c], acc[c][e]);
+        }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wv][c][4 * lane + e] = acc[c][e];
+  __syncthreads();
+  const int r = blockIdx.x * FEW_ROWS + threadIdx.x;
+  if (r < a.k)
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const float s = (part[0][c][threadIdx.x] + part[1][c][threadIdx.x]) + (part[2][c][threadIdx.x] + part[3][c][threadIdx.x]);
+      (a.slices > 1 ? a.partial + ((size_t)blockIdx.y * N) * a.k : a.dx)[(size_t)c * a.k + r] = s;
+    }
+}
+// dx: n outputs of `slices` partial results, 64 a workgroup, whose wavefronts take every fourth slice.
+__global__ void __launch_bounds__(256) k_few_finish(const float* partial, float* dx, long long n, int slices) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const long long i = (long long)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (i < n)
+#pragma unroll 8
+    for (int q = wv; q < slices; q += 4) s += partial[q * n + i];
+  red[wv][lane] = s;
+  __syncthreads();
+  if (wv == 0 && i < n) dx[i] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+
+template <int N>
+static int few_columns(FewArgs a) {
+  const int cus = dn_num_cus(), blocks = (a.k + FEW_ROWS - 1) / FEW_ROWS;
+  if (a.dw || a.bias_grad) {
+    const int wgs = (blocks + 3) / 4;
+    a.slice = FEW_SLICE;
+    while (a.slice > 16 && (long long)wgs * ((a.units + a.slice - 1) / a.slice) < 8 * cus) a.slice >>= 1;
+    const int slices = (a.units + a.slice - 1) / a.slice;
+    if (slices > 65535) return ERROR_UNSUPPORTED;
+    hipLaunchKernelGGL(k_few_outer<N>, dim3((unsigned)wgs, (unsigned)slices), dim3(256), 0, dn_stream(), a);
+  }
+  if (a.dx) {
+    a.slice = FEW_SLICE;
+    while (a.slice > 32 && (long long)blocks * ((a.units + a.slice - 1) / a.slice) < 4 * cus) a.slice >>= 1;
+    a.slices = (a.units + a.slice - 1) / a.slice;
+    if (a.slices > 65535) return ERROR_UNSUPPORTED;
+    if (a.slices > 1) {
+      a.partial = (float*)dn_scratch((size_t)a.slices * N * a.k * sizeof(float));
+      if (!a.partial) return CUDA_ERROR;
+    }
+    hipLaunchKernelGGL(k_few_rows<N>, dim3((unsigned)blocks, (unsigned)a.slices), dim3(256), 0, dn_stream(), a);
+    if (a.slices > 1) {
+      const long long n = (long long)N * a.k;
+      hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, n, a.slices);
+    }
+  }
+  return dn_launch_status();
+}
+
 static inline bool apart(const cudamat* a, const cudamat* b) {
   return !a || !b || a->data_device + dn_len(a) <= b->data_device || b->data_device + dn_len(b) <= a->data_device;
 }
@@ -265,6 +412,13 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
   if (e) return e;
   const float *w = mat1->data_device, *x = mat2->data_device, *d = target->data_device;
   const bool wt = mat1->is_trans != 0, xt = mat2->is_trans != 0;
+  if (n >= 1 && n <= GATED_COLUMNS && wt && !xt && f > 0 && k > 0 && 2 * f <= 65535 * 16) {
+    const FewArgs a = {w, x, d, mat1_grad ? mat1_grad->data_device : nullptr, mat2_grad ? mat2_grad->data_device : nullptr, nullptr,
+                       bias_grad ? bias_grad->data_device : nullptr, k, 2 * f, 0, 1, beta, mult};
+#define FEW(N) case N: return few_columns<N>(a)
+    switch (n) { FEW(1); FEW(2); FEW(3); FEW(4); FEW(5); FEW(6); FEW(7); FEW(8); }
+#undef FEW
+  }
   // The sums go with the weights' gradient where a kernel takes both, and the two products, which have nothing to do with each
   // other, share a launch where their tiles do.
   DnRowSumJob job = {d, bias_grad ? bias_grad->data_device : nullptr, 2 * f, n, mult, beta, 0};

@@ -258,7 +258,7 @@ def test_gates_far_from_zero(cm):
         check(d, np.vstack([s, v]), np.vstack([se, ve + 1e-38]), act)
 
 
-@pytest.mark.parametrize("d,f,n", [(1, 1, 1), (5, 7, 1), (65, 63, 2), (100, 33, 30), (127, 129, 64), (500, 1000, 100), (333, 301, 257), (64, 520, 512), (256, 1024, 1024)])
+@pytest.mark.parametrize("d,f,n", [(1, 1, 1), (5, 7, 1), (65, 63, 2), (258, 300, 1), (1027, 70, 3), (2048, 2500, 4), (300, 33, 5), (513, 64, 6), (64, 1000, 7), (1000, 517, 8), (100, 33, 30), (127, 129, 64), (500, 1000, 100), (333, 301, 257), (64, 520, 512), (256, 1024, 1024)])
 @pytest.mark.parametrize("act", ACTS)
 def test_dot_gated_grad(cm, rng, d, f, n, act):
     w, x, dy = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d)), F(rng.standard_normal((d, n))), F(rng.standard_normal((f, n)))

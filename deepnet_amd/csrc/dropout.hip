@@ -34,8 +34,7 @@ k_counter_dropout(const float* mat, const float* residual, float* target, const 
     else { const DropGroup q = *reinterpret_cast<const DropGroup*>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
   };
   auto one = [&](float x, float r, uint32_t word) __attribute__((always_inline)) {
-    x = word >= border ? x : 0.f;
-    return RES ? __fmaf_rn(mult, x, r) : mult * x;
+    return word >= border ? (RES ? __fmaf_rn(mult, x, r) : mult * x) : (RES ? r : 0.f);
   };
   float x[4], r[4] = {0.f, 0.f, 0.f, 0.f};
   if (g < whole) {

@@ -627,7 +627,7 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
     for (int j = 0; j < i; ++j)
       if (!apart(out[i], out[j])) return ERROR_UNSUPPORTED;
   }
-  if (h <= 0 || w <= 0) return 0;
+  if (w <= 0) return 0;
   LogProbArgs a = {mat->data_device, DPTR(labels), DPTR(logp), DPTR(entropy), DPTR(log_z), DPTR(top), DPTR(top_labels), h, w, k, 1, h, nullptr, nullptr, nullptr};
   if (h >= 4 && h <= 1024) {
     const dim3 grid((unsigned)((w + 3) / 4));
@@ -644,6 +644,7 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   int segments = 2 * dn_num_cus() / (w < 2 * dn_num_cus() ? w : 2 * dn_num_cus());
   const int most[3] = {(h + LP_SEGMENT - 1) / LP_SEGMENT, 64, k ? LP_JOIN / k : 64};
   for (int m : most) segments = segments < m ? segments : m;
+  if (segments < 1) segments = 1;                         // (no rows: columns of nothing)
   if (segments > 1) {
     a.length = ((h + segments - 1) / segments + 3) / 4 * 4;
     a.segments = segments = (h + a.length - 1) / a.length;

@@ -248,9 +248,9 @@ __device__ __forceinline__ void norm_param_out(float* out, int i, float sum, flo
 
 template <int T, int NV, bool TAIL, bool STREAM>
 __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
-  constexpr int AHEAD = NV <= 2 ? 1 : 0;                   // columns on their way (none fit the registers of 1024 lanes beyond)
+  constexpr int AHEAD = NV <= 3 ? 1 : 0;                   // columns on their way (none fit the registers of 1024 lanes beyond)
   __shared__ float part[2][T ? 1 : 16][T ? 1 : 96];
-  __shared__ float meet[NV <= 2 ? 512 * NV * 8 : 1];
+  __shared__ float meet[NV <= 3 ? 512 * NV * 8 : 1];
   const int h = a.h, w = a.w, W = a.waves, lanes = T ? T : 64 * W, teams = blockDim.x / lanes;
   const int team = T ? threadIdx.x / (T ? T : 1) : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W, lane = threadIdx.x - team * lanes;
   ColGroups<NV, TAIL> at;
@@ -482,11 +482,21 @@ int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target
   if (h <= 0) return 0;
   if (h >= 4 && h <= NORM_COLS_MAX && w > 0 && w <= NORM_COLS_W) {
     NormGradArgs a = {deriv->data_device, mat->data_device, gain ? gain->data_device : nullptr, target->data_device, nullptr,
-                            gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, h <= 8192 ? (h + 511) / 512 : (h + 1023) / 1024, eps, beta, mult};
+                            gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, 0, eps, beta, mult};
     if (h <= 64) return norm_grad_launch<16, 1>(a);
     if (h <= 256) return norm_grad_launch<64, 1>(a);
     if (h <= 512) return norm_grad_launch<64, 2>(a);
-    if (h <= 8192) return norm_grad_launch<0, 2>(a);
+    if (h <= 8192) {
+      // Two groups a lane, or three where that gives a workgroup half as many teams again: more columns are on their way (us, two / three:
+      // 4098 x 4099 54.2 / 50.2, 6144 x 4096 66.8 / 62.3, 3000 x 8192 63.9 / 61.0, 700 x 20000 40.9 / 38.1; 2048 x 8192, four teams against
+      // five, 42.8 / 45.1).
+      const int two = (h + 511) / 512, three = (h + 767) / 768;
+      a.waves = two;
+      if (2 * (16 / three) < 3 * (16 / two)) return norm_grad_launch<0, 2>(a);
+      a.waves = three;
+      return norm_grad_launch<0, 3>(a);
+    }
+    a.waves = (h + 1023) / 1024;
     return norm_grad_launch<0, 4>(a);
   }
   float* stats = (float*)dn_scratch((size_t)(w > 0 ? w : 1) * 5 * sizeof(float));

@@ -341,6 +341,9 @@ def test_counter_dropout(cm, rng, h, w, skip):
         t = device(cm, r, skip)
         cm.counter_dropout(device(cm, x, skip), p, seed, stream=stream, step=step, mult=1.5, residual=t, target=t)
         assert np.array_equal(t.asarray(), y.asarray())
+    y = cm.counter_dropout(device(cm, x, skip), 0.5, seed, mult=-np.inf, residual=device(cm, r, skip)).asarray()       # any factor
+    keep = tok.dropout_keep((h, w), 0.5, seed)
+    assert np.array_equal(y[~keep], r[~keep]) and not np.isfinite(y[keep]).any()
     keep = tok.dropout_keep((h, w), 0.5, 7)                 # no step, first stream; what is dropped may be anything
     x[~keep] = [np.nan, np.inf, -np.inf][h % 3]
     y = cm.counter_dropout(device(cm, x, skip), 0.5, 7, mult=1.0).asarray()
@@ -473,7 +476,10 @@ def test_log_probs_gives_what_is_asked_for(cm, rng):
     cm.log_probs(X, top=t); cm.log_probs(X, top_labels=l)
     assert np.allclose(t.asarray(), o['top'], rtol=1e-5) and np.array_equal(l.asarray(), o['top_labels'])
     cm.log_probs(cm.empty((300, 0)), entropy=cm.empty((1, 0)))
-    cm.log_probs(cm.empty((0, 3)), entropy=cm.empty((1, 3)))
+    z, e, p = (cm.CUDAMatrix(F(np.full((1, 3), 9.0))) for _ in range(3))                  # no rows: no distribution
+    cm.log_probs(cm.empty((0, 3)), cm.CUDAMatrix(F(np.zeros((1, 3)))), p, e, z)
+    assert (z.asarray() == -np.inf).all() and (e.asarray() == 0).all() and (p.asarray() == 0).all()
+    cm.log_probs_grad(cm.empty((0, 3)), None, z)
 
 
 @pytest.mark.parametrize("h,w", LOGP_SHAPES)

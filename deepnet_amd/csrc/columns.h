@@ -25,7 +25,8 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // A column of h >= 4 floats as groups of four: group j starts at row 4 j, the last one at h - 4; the rows that it has in common with the
-// one before (`lap`, only where h is no multiple of 4) are that one's.
+// one before (`lap`, only where h is no multiple of 4) are that one's.  Loads are never behind a branch (a lane without a group reads the last
+// one): with them the compiler could not count what is on its way, and would wait for all of it.
 // STREAM: non-temporal accesses, for what is touched once.
 typedef float ColGroup __attribute__((ext_vector_type(4), aligned(4)));
 template <bool STREAM>
@@ -43,7 +44,8 @@ __device__ __forceinline__ void col_store(float* p, const float (&v)[4]) {
 }
 template <int NV, bool TAIL>
 struct ColGroups {
-  int row[NV];                  // first row of a lane's group, or -1 for none
+  int row[NV];                  // first row of a lane's group; of lanes that have none, the last group's
+  bool in[NV];                  // whether it has one
   int lap;                      // rows of the last group that are its neighbour's, for the lane that has it (TAIL)
   int last;                     // which of its groups that is, or -1
   __device__ __forceinline__ void init(int lane, int T, int h) {
@@ -51,9 +53,10 @@ struct ColGroups {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int r = 4 * (lane + k * T);
-      row[k] = r < h ? r : -1;
-      if (TAIL && r < h && r + 4 > h) { row[k] = h - 4; lap = r - (h - 4); last = k; }
+      in[k] = r < h;
+      row[k] = r + 4 <= h ? r : h - 4;
+      if (TAIL && r < h && r + 4 > h) { lap = r - (h - 4); last = k; }
     }
   }
-  __device__ __forceinline__ bool own(int k, int e) const { return !TAIL || k != last || e >= lap; }
+  __device__ __forceinline__ bool own(int k, int e) const { return in[k] && (!TAIL || k != last || e >= lap); }
 };

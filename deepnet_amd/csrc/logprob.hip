@@ -183,19 +183,12 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
   LogProbPart p = lp_none();
   float best = -INFINITY;
   int best_at = 0;
+  const int full = n4 >> 10;               // trips that every lane has four groups of: their loads are behind no branch, so that they can be counted
   auto load = [&](float (&v)[4][4], int it) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = tid + 256 * u + 1024 * it;
-      if (j < n4) col_load<STREAM>(v[u], c + 4 * j);
-      else v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
-    }
+    for (int u = 0; u < 4; ++u) col_load<STREAM>(v[u], c + 4 * (tid + 256 * u + 1024 * it));
   };
-  float v[4][4], next[4][4];
-  load(v, 0);
-  if (TOP && tid == 0) listed = won = 0;
-  for (int it = 0; it < trips; ++it) {
-    if (it + 1 < trips) load(next, it + 1);
+  auto take = [&](const float (&v)[4][4], int it) __attribute__((always_inline)) {
     float m = v[0][0];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -207,12 +200,35 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) lp_take(p, v[u][e]);
-    if (it + 1 < trips) {
+  };
+  // two trips are on their way in turn
+  float v[4][4], next[4][4];
+  if (TOP && tid == 0) listed = won = 0;
+  if (full > 0) load(v, 0);
+  int it = 0;
+  for (; it + 2 < full; it += 2) {
+    load(next, it + 1);
+    take(v, it);
+    load(v, it + 2);
+    take(next, it + 1);
+  }
+  if (it + 1 < full) {
+    load(next, it + 1);
+    take(v, it);
+    take(next, it + 1);
+  } else if (it < full) {
+    take(v, it);
+  }
+  if (trips > full || TOP) {
+    // the last one, which some lanes have fewer groups of (or, for the top list of a column of whole trips, the one that was taken last)
+    const int at = trips > full ? full : full - 1;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] = next[u][e];
+    for (int u = 0; u < 4; ++u) {
+      const int j = tid + 256 * u + 1024 * at;
+      v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
+      if (at >= 0 && j < n4) col_load<false>(v[u], c + 4 * j);
     }
+    if (trips > full) take(v, at);
   }
   const bool tail = tid < (n & 3);                         // the rows behind the last group: one a lane
   float tail_x = 0.f;
@@ -448,8 +464,8 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
   }
 }
 
-// ---- columns of 4 to 1024 rows by a wavefront, which holds them in registers
-template <int NV, bool TAIL, bool TOP>
+// ---- columns of 4 to 1024 rows (many of them: to 4095, without a top list) by a wavefront, which holds them in registers
+template <int NV, bool TAIL, bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned long long lists[TOP ? 4 : 1][TOP ? 256 * NV + 2 : 2];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = blockIdx.x * 4 + wv;
@@ -461,13 +477,15 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   float v[NV][4], m = -FLT_MAX;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    if (at.row[k] >= 0) col_load<false>(v[k], c + at.row[k]);
+    col_load<STREAM>(v[k], c + at.row[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (at.row[k] < 0 || !at.own(k, e)) v[k][e] = -INFINITY;
+      if (!at.own(k, e)) v[k][e] = -INFINITY;
       m = fmaxf(m, v[k][e]);
     }
-  }
   LogProbPart p = lp_none();
   p.m = lanes_sum<64, true>(m);
 #pragma unroll
@@ -479,7 +497,7 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   if (live && lane == 0) lp_finish(a, col, p, o, label);
   if (!TOP) return;
   unsigned long long best = 0;
-  auto key_of = [&](int k, int e) __attribute__((always_inline)) { return at.row[k] >= 0 && at.own(k, e) ? lp_key(v[k][e], at.row[k] + e) : 0ull; };
+  auto key_of = [&](int k, int e) __attribute__((always_inline)) { return at.own(k, e) ? lp_key(v[k][e], at.row[k] + e) : 0ull; };
   // the lane's greatest entry: the first that is its maximum, of nothing but -inf and NaN the first of all
   int first = -1;
   float most = -INFINITY;
@@ -491,7 +509,7 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   for (int k = NV - 1; k >= 0; --k)
 #pragma unroll
     for (int e = 3; e >= 0; --e)
-      if (at.row[k] >= 0 && at.own(k, e) && (v[k][e] == most || most == -INFINITY)) first = at.row[k] + e;
+      if (at.own(k, e) && (v[k][e] == most || most == -INFINITY)) first = at.row[k] + e;
   if (first >= 0) best = lp_key(most, first);
   // (a wavefront's own part of LDS, whose accesses are in order: the compiler has to keep them so)
   auto ordered = []() __attribute__((always_inline)) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
@@ -629,15 +647,27 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   if (w <= 0) return 0;
   LogProbArgs a = {mat->data_device, DPTR(labels), DPTR(logp), DPTR(entropy), DPTR(log_z), DPTR(top), DPTR(top_labels), h, w, k, 1, h, nullptr, nullptr, nullptr};
-  if (h >= 4 && h <= 1024) {
+  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
+  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
+  // Columns of up to 1024 rows by a wavefront each, and where there are enough of them for the chip those that are shorter than one trip of a
+  // workgroup (us, workgroup / wavefront: 2050 x 8192 26.3 / 16.9, 1500 x 20000 50.8 / 21.2; 4096 x 8192 23.0 / 23.9, 3001 x 1100 6.7 / 7.3).
+  if (h >= 4 && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
     const dim3 grid((unsigned)((w + 3) / 4));
-#define LP_WAVE(NV, TAIL) do { if (k) hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, true>), grid, dim3(256), 0, dn_stream(), a); \
-                               else hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, false>), grid, dim3(256), 0, dn_stream(), a); } while (0)
-    if (h <= 256) { if (h % 4) LP_WAVE(1, true); else LP_WAVE(1, false); }
-    else if (h <= 512) { if (h % 4) LP_WAVE(2, true); else LP_WAVE(2, false); }
-    else if (h % 4) LP_WAVE(4, true);
-    else LP_WAVE(4, false);
+#define LP_WAVE4(NV, TAIL, TOP, S) hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, TOP, S>), grid, dim3(256), 0, dn_stream(), a)
+#define LP_WAVE3(NV, TOP, S) do { if (h % 4) LP_WAVE4(NV, true, TOP, S); else LP_WAVE4(NV, false, TOP, S); } while (0)
+#define LP_WAVE(NV) do { if (k) LP_WAVE3(NV, true, false); else LP_WAVE3(NV, false, false); } while (0)
+#define LP_WAVES(NV) do { if (stream) LP_WAVE3(NV, false, true); else LP_WAVE3(NV, false, false); } while (0)
+    if (h <= 256) LP_WAVE(1);
+    else if (h <= 512) LP_WAVE(2);
+    else if (k) LP_WAVE3(4, true, false);
+    else if (h <= 1024) LP_WAVES(4);
+    else if (h <= 2048) LP_WAVES(8);
+    else if (h <= 3 * 1024) LP_WAVES(12);
+    else LP_WAVES(16);
+#undef LP_WAVES
 #undef LP_WAVE
+#undef LP_WAVE3
+#undef LP_WAVE4
     return dn_launch_status();
   }
   // few columns: segments of them, about two workgroups a CU, none shorter than LP_SEGMENT rows
@@ -656,8 +686,6 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   const long long blocks = (long long)w * segments;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
-  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
 #define LP_GO(TOP, S) hipLaunchKernelGGL((k_log_probs<TOP, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
   if (k) { if (stream) LP_GO(true, true); else LP_GO(true, false); }
   else if (stream) LP_GO(false, true);

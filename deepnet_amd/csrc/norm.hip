@@ -130,7 +130,7 @@ __device__ __forceinline__ NormSums norm_sums(const ColGroups<NV, TAIL>& at, flo
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[k][e] = at.row[k] >= 0 ? v[k][e] - mi : 0.f;
+      v[k][e] = v[k][e] - mi;
       const float x = at.own(k, e) ? v[k][e] : 0.f;
       o.d += x;
       o.sq = __fmaf_rn(x, x, o.sq);
@@ -194,10 +194,8 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
   for (int k = 0; k < NV; ++k) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) { gv[k][e] = 1.f; bv[k][e] = 0.f; x[k][e] = next[k][e] = 0.f; }
-    if (at.row[k] >= 0) {
-      if (gain) col_load<false>(gv[k], gain + at.row[k]);
-      if (bias) col_load<false>(bv[k], bias + at.row[k]);
-    }
+    if (gain) col_load<false>(gv[k], gain + at.row[k]);
+    if (bias) col_load<false>(bv[k], bias + at.row[k]);
   }
   const int stride = gridDim.x * TEAMS;
   int c = blockIdx.x * TEAMS + (T ? threadIdx.x / (T ? T : 1) : 0);
@@ -205,8 +203,7 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
   auto fetch = [&](float (&v)[NV][4], int col) __attribute__((always_inline)) {
     const float* p = mat + (size_t)col * h;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (at.row[k] >= 0) col_load<STREAM>(v[k], p + at.row[k]);
+    for (int k = 0; k < NV; ++k) col_load<STREAM>(v[k], p + at.row[k]);
   };
   fetch(x, c);
   for (;;) {
@@ -218,7 +215,7 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
     float* t = target + (size_t)c * h;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (at.row[k] >= 0) {
+      if (at.in[k]) {
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = __fmaf_rn(gv[k][e], (x[k][e] - d) * r, bv[k][e]);
@@ -266,28 +263,28 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
 #pragma unroll
       for (int q = 0; q < AHEAD; ++q) nx[q][k][e] = ny[q][k][e] = 0.f;
     }
-    if (at.row[k] >= 0 && a.gain) col_load<false>(gv[k], a.gain + at.row[k]);
+    if (a.gain) col_load<false>(gv[k], a.gain + at.row[k]);
   }
   const int stride = gridDim.x * teams;
   auto fetch = [&](float (&u)[NV][4], float (&v)[NV][4], int col) __attribute__((always_inline)) {
     const size_t o = (size_t)col * h;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (at.row[k] >= 0) {
-        col_load<STREAM>(u[k], a.mat + o + at.row[k]);
-        col_load<STREAM>(v[k], a.deriv + o + at.row[k]);
-      }
+    for (int k = 0; k < NV; ++k) {
+      col_load<STREAM>(u[k], a.mat + o + at.row[k]);
+      col_load<STREAM>(v[k], a.deriv + o + at.row[k]);
+    }
   };
   // every team of a workgroup makes the same number of trips; those beyond the last column count and store nothing
   int c = blockIdx.x * teams + team;
-  if (AHEAD && c < w) fetch(x, dy, c);
+  auto column = [&](int n) __attribute__((always_inline)) { return n < w ? n : w - 1; };      // (behind the last one: that one again, from the caches)
+  if (AHEAD) fetch(x, dy, column(c));
 #pragma unroll
-  for (int q = 0; q + 1 < AHEAD; ++q)
-    if (c + (q + 1) * stride < w) fetch(nx[q], ny[q], c + (q + 1) * stride);
+  for (int q = 0; q + 1 < AHEAD; ++q) fetch(nx[q], ny[q], column(c + (q + 1) * stride));
   for (int base = blockIdx.x * teams; base < w; base += stride) {
     const bool live = c < w;
-    const int n = c + AHEAD * stride;
-    if (n < w) { if (AHEAD) fetch(nx[AHEAD ? AHEAD - 1 : 0], ny[AHEAD ? AHEAD - 1 : 0], n); else fetch(x, dy, n); }
+    const int n = column(c + AHEAD * stride);
+    if (AHEAD) fetch(nx[AHEAD ? AHEAD - 1 : 0], ny[AHEAD ? AHEAD - 1 : 0], n);
+    else fetch(x, dy, n);
     const NormSums o = norm_sums<T, NV, TAIL, true>(at, x, gv, dy, part[T ? 0 : turn][T ? 0 : team], rows, inv_rows, inv_h, lane, W);
     turn ^= 1;
     const float d = o.d * inv_h, r = norm_rstd(o.sq, d, inv_h, a.eps);
@@ -296,7 +293,7 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
       float* t = a.target + (size_t)c * h;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (at.row[k] >= 0) {
+        if (at.in[k]) {
           float out[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -359,7 +356,7 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (at.row[k] >= 0 && at.own(k, e)) {
+        if (at.own(k, e)) {
           const int i = at.row[k] + e;
           if (gridDim.x > 1) { p[i] = sg[k][e]; p[h + i] = sb[k][e]; }
           else {

@@ -363,7 +363,8 @@ def test_counter_dropout_depends_on_seed_stream_and_step(cm):
 
 # ------------------------------------------------------------------ log probabilities
 
-LOGP_SHAPES = [(1, 1), (1, 5), (2, 3), (3, 300), (10, 128), (63, 5), (64, 3), (65, 7), (100, 40), (257, 9), (1000, 33), (1001, 5), (1024, 64), (2050, 3),
+LOGP_SHAPES = [(1, 1), (1, 5), (2, 3), (3, 300), (10, 128), (63, 5), (64, 3), (65, 7), (100, 40), (257, 9), (1000, 33), (1001, 5), (1024, 64), (2050, 3), (1500, 2100),
+              (2050, 2048), (3074, 2049),
                (4096, 17), (4099, 2), (8192, 3), (10007, 5), (16384, 40), (32003, 4), (50000, 1), (50001, 2), (128256, 1), (131072, 3), (300007, 1)]
 
 

@@ -60,3 +60,11 @@ struct ColGroups {
   }
   __device__ __forceinline__ bool own(int k, int e) const { return in[k] && (!TAIL || k != last || e >= lap); }
 };
+// Stores a lane's group k.  OWN: without the rows that are its neighbour's, where two wavefronts may come to different roundings of them.
+template <bool STREAM, bool OWN, int NV, bool TAIL>
+__device__ __forceinline__ void col_store_group(const ColGroups<NV, TAIL>& at, int k, float* column, const float (&v)[4]) {
+  if (!OWN || !TAIL || k != at.last) { col_store<STREAM>(column + at.row[k], v); return; }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e >= at.lap) column[at.row[k] + e] = v[e];
+}

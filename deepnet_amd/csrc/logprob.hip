@@ -576,7 +576,8 @@ template <int T, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs_grad(LogProbGradArgs a) {
   const int lane = threadIdx.x % T;
   const long long unit = (long long)blockIdx.x * (256 / T) + threadIdx.x / T;
-  const int col = (int)(T == 64 ? unit : unit / a.pieces), piece = T == 64 ? 0 : (int)(unit - (long long)col * a.pieces);
+  const long long col = T == 64 ? unit : unit / a.pieces;
+  const int piece = T == 64 ? 0 : (int)(unit - col * a.pieces);
   if (col >= a.w) return;
   const int row0 = piece * a.length, n = a.h - row0 < a.length ? a.h - row0 : a.length, n4 = n >> 2;
   const float* c = a.mat + (size_t)col * a.h + row0;
@@ -622,6 +623,7 @@ static int check_shape(const cudamat* m, int rows, int cols) {
   return m->size[0] == rows && m->size[1] == cols ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
 #define LP_SEGMENT 4096           // rows of one trip of a workgroup
+#define LP_WAVE_COLUMNS (1 << 30)  // columns that wavefronts take: they are counted in 31 bits, four a workgroup
 #define LP_JOIN 512               // keys that the last workgroup of a column ranks
 #define DPTR(m) ((m) ? (m)->data_device : nullptr)
 
@@ -651,7 +653,7 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
   // Columns of up to 1024 rows by a wavefront each, and where there are enough of them for the chip those that are shorter than one trip of a
   // workgroup (us, workgroup / wavefront: 2050 x 8192 26.3 / 16.9, 1500 x 20000 50.8 / 21.2; 4096 x 8192 23.0 / 23.9, 3001 x 1100 6.7 / 7.3).
-  if (h >= 4 && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
+  if (h >= 4 && w <= LP_WAVE_COLUMNS && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
     const dim3 grid((unsigned)((w + 3) / 4));
 #define LP_WAVE4(NV, TAIL, TOP, S) hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, TOP, S>), grid, dim3(256), 0, dn_stream(), a)
 #define LP_WAVE3(NV, TOP, S) do { if (h % 4) LP_WAVE4(NV, true, TOP, S); else LP_WAVE4(NV, false, TOP, S); } while (0)
@@ -660,9 +662,9 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
     if (h <= 256) LP_WAVE(1);
     else if (h <= 512) LP_WAVE(2);
     else if (k) LP_WAVE3(4, true, false);
-    else if (h <= 1024) LP_WAVES(4);
-    else if (h <= 2048) LP_WAVES(8);
-    else if (h <= 3 * 1024) LP_WAVES(12);
+    else if (h <= 4 * 256) LP_WAVES(4);
+    else if (h <= 8 * 256) LP_WAVES(8);
+    else if (h <= 12 * 256) LP_WAVES(12);
     else LP_WAVES(16);
 #undef LP_WAVES
 #undef LP_WAVE

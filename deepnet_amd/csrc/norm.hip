@@ -74,10 +74,10 @@ __global__ void __launch_bounds__(256) k_layer_norm_grad_rows(const float* deriv
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
   float sg = 0.f, sb = 0.f;
   if (i < h)
-    for (int c = wv; c < w; c += 4) {
-      const float* s = stats + (size_t)c * 5;
-      const float dy = deriv[(size_t)c * h + i];
-      sg += dy * (((mat[(size_t)c * h + i] - s[0]) - s[1]) * s[2]);
+    for (size_t c = wv; c < (size_t)w; c += 4) {
+      const float* s = stats + c * 5;
+      const float dy = deriv[c * h + i];
+      sg += dy * (((mat[c * h + i] - s[0]) - s[1]) * s[2]);
       sb += dy;
     }
   red[0][wv][lane] = sg; red[1][wv][lane] = sb;
@@ -219,7 +219,7 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = __fmaf_rn(gv[k][e], (x[k][e] - d) * r, bv[k][e]);
-        col_store<STREAM>(t + at.row[k], y);
+        col_store_group<STREAM, T == 0>(at, k, t, y);
       }
     if (n >= w) break;
     c = n;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
             sb[k][e] += dy[k][e];
             out[e] = r * (__fmaf_rn(gv[k][e], dy[k][e], -mg) - xh * mgx);
           }
-          col_store<STREAM>(t + at.row[k], out);
+          col_store_group<STREAM, T == 0>(at, k, t, out);
         }
     }
     c += stride;

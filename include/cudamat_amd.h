@@ -374,7 +374,8 @@ int counter_dropout(cudamat* mat, cudamat* residual, cudamat* target, cudamat* s
 int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cudamat* log_z, cudamat* top, cudamat* top_labels);
 /* target (may be mat) = derivative by mat of  sum over the columns of  logp_weight * logp + entropy_weight * entropy, from log_z and
  * entropy as log_probs returns them.  labels NULL: no first term; logp_weight NULL: ones; entropy and entropy_weight NULL (both): no second
- * term.  A column that is no token has no first term; a column of -infinity gives zeros. */
+ * term.  A column that is no token has no first term.  Entries of -infinity have probability 0, also in a column of nothing
+ * else: those get 0, the token's logp_weight. */
 int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_weight, cudamat* entropy, cudamat* entropy_weight,
                    cudamat* target);
 

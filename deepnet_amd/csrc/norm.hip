@@ -366,14 +366,19 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_cols(NormGradArgs a) {
         }
   }
 }
-// The sums of `parts` workgroups: 64 of the 2 h rows a workgroup, its 16 wavefronts take every sixteenth part.
+// The sums of `parts` workgroups: 64 of the 2 h rows a workgroup, its 16 wavefronts take every sixteenth part, eight on their way at once.
 __global__ void __launch_bounds__(1024) k_layer_norm_grad_finish(NormGradArgs a, int parts) {
   __shared__ float red[16][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, rows = 2 * a.h, i = blockIdx.x * 64 + lane;
+  const float* from = a.partial + (i < rows ? i : rows - 1);
   float s = 0.f;
-  if (i < rows)
-#pragma unroll 4
-    for (int p = wv; p < parts; p += 16) s += a.partial[(size_t)p * rows + i];
+  for (int p = wv; p < parts; p += 16 * 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = from[(size_t)(p + 16 * u < parts ? p + 16 * u : p) * rows];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += p + 16 * u < parts ? v[u] : 0.f;
+  }
   red[wv][lane] = s;
   __syncthreads();
   if (wv == 0 && i < rows) {
@@ -391,11 +396,13 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_finish(NormGradArgs a,
 template <int T, int NV>
 static void norm_launch(const float* mat, const float* gain, const float* bias, float* target, int h, int w, float eps, int waves = 4) {
   const int teams = T ? 256 / (T ? T : 1) : 1, nt = 64 * waves;
-  const bool tail = h % 4 != 0, stream = !tail && (long long)h * w >= DN_STREAM_MIN_ELEMS && dn_aligned16(mat) && dn_aligned16(target);
+  // (at any alignment: 4098 x 4099 32.7 -> 28.8 us, 1001 x 8000 14.7 -> 13.3)
+  const bool tail = h % 4 != 0, stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
   // as many workgroups as fit the CUs, or one for as many columns as makes them even
   const int groups = (w + teams - 1) / teams, most = dn_num_cus() * (2048 / nt), each = (groups + most - 1) / most;
   const dim3 grid((unsigned)((groups + each - 1) / each));
-  if (tail) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, true, false>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
+  if (tail && stream) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, true, true>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
+  else if (tail) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, true, false>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
   else if (stream) hipLaunchKernelGGL((k_layer_norm_cols<T, NV, false, true>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
   else hipLaunchKernelGGL((k_layer_norm_cols<T, NV, false, false>), grid, dim3(nt), 0, dn_stream(), mat, gain, bias, target, h, w, eps);
 }
@@ -403,7 +410,8 @@ static void norm_launch(const float* mat, const float* gain, const float* bias, 
 template <int T, int NV>
 static int norm_grad_launch(NormGradArgs a) {
   const int lanes = T ? T : 64 * a.waves, cus = dn_num_cus(), least = T == 16 ? 4 : 1;
-  // teams of a workgroup: all that fit, or fewer where that leaves CUs without one
+  // teams of a workgroup: all that fit, or fewer where that leaves CUs without one; a workgroup a CU (two of half the teams: 4098 x 4099 45.2 ->
+  // 51.4 us, 4096 x 8192 72.6 -> 76.2)
   int teams = 1024 / lanes;
   while (teams > least && (a.w + teams - 1) / teams < cus) teams = (teams + 1) / 2 > least ? (teams + 1) / 2 : least;
   int blocks = (a.w + teams - 1) / teams;
@@ -413,9 +421,11 @@ static int norm_grad_launch(NormGradArgs a) {
     a.partial = (float*)dn_scratch((size_t)blocks * 2 * a.h * sizeof(float));
     if (!a.partial) return CUDA_ERROR;
   }
-  const bool tail = a.h % 4 != 0, stream = !tail && (long long)a.h * a.w >= DN_STREAM_MIN_ELEMS && dn_aligned16(a.mat) && dn_aligned16(a.deriv) && dn_aligned16(a.target);
+  // (at any alignment: 4098 x 4099 46.4 -> 45.3 us, 1026 x 8192 29.3 -> 26.9)
+  const bool tail = a.h % 4 != 0, stream = (long long)a.h * a.w >= DN_STREAM_MIN_ELEMS;
   const dim3 grid((unsigned)blocks), block((unsigned)(teams * lanes));
-  if (tail) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, true, false>), grid, block, 0, dn_stream(), a);
+  if (tail && stream) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, true, true>), grid, block, 0, dn_stream(), a);
+  else if (tail) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, true, false>), grid, block, 0, dn_stream(), a);
   else if (stream) hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, false, true>), grid, block, 0, dn_stream(), a);
   else hipLaunchKernelGGL((k_layer_norm_grad_cols<T, NV, false, false>), grid, block, 0, dn_stream(), a);
   if (sums && blocks > 1)
@@ -454,6 +464,9 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, floa
     else if (h <= 256) norm_launch<64, 1>(x, g, b, t, h, w, eps);
     else if (h <= 512) norm_launch<64, 2>(x, g, b, t, h, w, eps);
     else if (h <= 1024) norm_launch<64, 4>(x, g, b, t, h, w, eps);
+    // Two groups a lane (us, two / four: 4096 x 8192 45.7 / 47.0, 6001 x 5000 44.0 / 46.2, 1026 x 8192 15.0 / 16.5; 3000 x 8192 39.6 / 38.6; a
+    // wavefront with eight takes 18.4 for 1026 x 8192), four where that is more than 16 wavefronts.
+    else if (h <= 8192) norm_launch<0, 2>(x, g, b, t, h, w, eps, (h + 511) / 512);
     else norm_launch<0, 4>(x, g, b, t, h, w, eps, (h + 1023) / 1024);
     return dn_launch_status();
   }
@@ -485,8 +498,8 @@ int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target
     if (h <= 512) return norm_grad_launch<64, 2>(a);
     if (h <= 8192) {
       // Two groups a lane, or three where that gives a workgroup half as many teams again: more columns are on their way (us, two / three:
-      // 4098 x 4099 54.2 / 50.2, 6144 x 4096 66.8 / 62.3, 3000 x 8192 63.9 / 61.0, 700 x 20000 40.9 / 38.1; 2048 x 8192, four teams against
-      // five, 42.8 / 45.1).
+      // 4098 x 4099 47.4 / 45.2, 1500 x 8192 33.9 / 33.4, 6144 x 4096 66.8 / 62.3, 700 x 20000 40.9 / 38.1; 6001 x 5000 74.6 / 75.1; 2048 x 8192, four
+      // teams against five, 42.8 / 45.1).
       const int two = (h + 511) / 512, three = (h + 767) / 768;
       a.waves = two;
       if (2 * (16 / three) < 3 * (16 / two)) return norm_grad_launch<0, 2>(a);

@@ -172,7 +172,7 @@ template <bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
   __shared__ LogProbPart parts[4];
   __shared__ __attribute__((aligned(16))) unsigned long long lane_keys[TOP ? 256 : 2], list[TOP ? LP_LIST + 2 : 2];
-  __shared__ int winners[TOP ? 256 : 1], wave_won[4], won, listed, last;
+  __shared__ int winners[TOP ? 256 : 1], wave_won[4], wave_like[4], won, listed, last;
   __shared__ unsigned least_order;
   __shared__ unsigned long long border_key;
   unsigned* const orders = reinterpret_cast<unsigned*>(lane_keys);
@@ -267,10 +267,13 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
         }
         __syncthreads();
       };
-      const unsigned long long above = __ballot(own > least_order);
-      if (tid % 64 == 0) wave_won[tid >> 6] = __popcll(above);
+      // (a masked stretch: of lanes that have nothing else than -inf, the first place is in the order of the lanes, so counting is enough)
+      const bool nothing = least_order == lp_order(-INFINITY);
+      const unsigned long long above = __ballot(own > least_order), alike = __ballot(own == least_order);
+      if (tid % 64 == 0) { wave_won[tid >> 6] = __popcll(above); wave_like[tid >> 6] = __popcll(alike); }
       __syncthreads();
-      if (wave_won[0] + wave_won[1] + wave_won[2] + wave_won[3] >= a.k) {          // (else the quads' border is the lanes' too)
+      const int over = wave_won[0] + wave_won[1] + wave_won[2] + wave_won[3];
+      if (over >= a.k) {                                   // (else the quads' border is the lanes' too)
         standing(own, greater, reach);
         if (own && greater < a.k && reach >= a.k) { least_order = own; won = reach; }
         __syncthreads();
@@ -293,8 +296,15 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
       if (tail && lp_order(tail_x) == own && (first >= n || lp_order(best) != own)) first = 4 * n4 + tid;
       const unsigned place = own == value ? (unsigned)~(row0 + first) : 0;
       if (tid == 0) border_key = (unsigned long long)value << 32;
-      standing(own > value ? 0xffffffffu : place, greater, reach);
-      if (!by_value && place && greater == a.k - 1) border_key |= place;
+      if (nothing && over < a.k) {
+        __syncthreads();
+        int before = over + lp_before(alike);
+        for (int i = 0; i < tid >> 6; ++i) before += wave_like[i];
+        if (place && before == a.k - 1) border_key |= place;
+      } else {
+        standing(own > value ? 0xffffffffu : place, greater, reach);
+        if (!by_value && place && greater == a.k - 1) border_key |= place;
+      }
       __syncthreads();
       border = border_key;
       in = ((unsigned long long)own << 32 | place) >= border && own;

@@ -389,6 +389,75 @@ __global__ void __launch_bounds__(1024) k_layer_norm_grad_finish(NormGradArgs a,
   }
 }
 
+// ------------------------------------------------------------------ columns of one to three rows
+// A lane a column: nothing is exchanged but the sums of gain and bias, at the end.  us, a workgroup a column before: 3 x 1000000 916 -> 8.0, its
+// gradients 57123 -> 15.2 (those of gain and bias went through one workgroup).
+template <int H>
+__device__ __forceinline__ NormSums norm_short(float (&x)[H], const float (&g)[H], const float (&dy)[H]) {
+#pragma clang fp contract(off)
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < H; ++i) s += x[i];
+  const float m = s / (float)H;
+  NormSums o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    x[i] -= m;
+    o.d += x[i];
+    o.sq = __fmaf_rn(x[i], x[i], o.sq);
+    o.g += g[i] * dy[i];
+    o.gx = __fmaf_rn(g[i] * dy[i], x[i], o.gx);
+  }
+  return o;
+}
+template <int H>
+__global__ void __launch_bounds__(256) k_layer_norm_short(const float* mat, const float* gain, const float* bias, float* target, int w, float eps) {
+  for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < (size_t)w; c += (size_t)gridDim.x * 256) {
+    float x[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) x[i] = mat[c * H + i];
+    const NormSums o = norm_short<H>(x, x, x);
+    const float d = o.d / (float)H, r = norm_rstd(o.sq, d, 1.f / (float)H, eps);
+#pragma unroll
+    for (int i = 0; i < H; ++i) target[c * H + i] = __fmaf_rn(gain ? gain[i] : 1.f, (x[i] - d) * r, bias ? bias[i] : 0.f);
+  }
+}
+template <int H>
+__global__ void __launch_bounds__(256) k_layer_norm_grad_short(NormGradArgs a) {
+  __shared__ float red[4][2 * H];
+  float g[H], sum[2 * H];
+#pragma unroll
+  for (int i = 0; i < H; ++i) { g[i] = a.gain ? a.gain[i] : 1.f; sum[i] = sum[H + i] = 0.f; }
+  for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < (size_t)a.w; c += (size_t)gridDim.x * 256) {
+    float x[H], dy[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) { x[i] = a.mat[c * H + i]; dy[i] = a.deriv[c * H + i]; }
+    const NormSums o = norm_short<H>(x, g, dy);
+    const float d = o.d / (float)H, r = norm_rstd(o.sq, d, 1.f / (float)H, a.eps), mg = o.g / (float)H, mgx = r * (o.gx - d * o.g) / (float)H;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float xh = (x[i] - d) * r;
+      sum[i] = __fmaf_rn(dy[i], xh, sum[i]);
+      sum[H + i] += dy[i];
+      a.target[c * H + i] = r * (__fmaf_rn(g[i], dy[i], -mg) - xh * mgx);
+    }
+  }
+  if (!a.gain_grad && !a.bias_grad) return;
+#pragma unroll
+  for (int i = 0; i < 2 * H; ++i) sum[i] = lanes_sum<64>(sum[i]);
+  if (threadIdx.x % 64 == 0) {
+#pragma unroll
+    for (int i = 0; i < 2 * H; ++i) red[threadIdx.x / 64][i] = sum[i];
+  }
+  __syncthreads();
+  const int i = threadIdx.x;
+  if (i >= 2 * H) return;
+  const float s = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+  float* out = i < H ? a.gain_grad : a.bias_grad;
+  if (gridDim.x > 1) a.partial[(size_t)blockIdx.x * 2 * H + i] = s;
+  else if (out) norm_param_out(out, i % H, s, a.beta, a.mult);
+}
+
 #define NORM_COLS_MAX 16384       // tallest columns that a team holds
 #define NORM_COLS_W (1 << 29)     // most of them (they are counted in 31 bits)
 
@@ -433,6 +502,21 @@ static int norm_grad_launch(NormGradArgs a) {
   return dn_launch_status();
 }
 
+template <int H>
+static int norm_grad_short(NormGradArgs a) {
+  // (columns of a lane: one, or as many as leave two workgroups a CU)
+  const long long groups = (a.w + 255ll) / 256, most = 2 * dn_num_cus();
+  const int blocks = (int)(groups < most ? groups : most);
+  const bool sums = a.gain_grad || a.bias_grad;
+  if (sums && blocks > 1) {
+    a.partial = (float*)dn_scratch((size_t)blocks * 2 * H * sizeof(float));
+    if (!a.partial) return CUDA_ERROR;
+  }
+  hipLaunchKernelGGL(k_layer_norm_grad_short<H>, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
+  if (sums && blocks > 1) hipLaunchKernelGGL(k_layer_norm_grad_finish, dim3(1), dim3(1024), 0, dn_stream(), a, blocks);
+  return dn_launch_status();
+}
+
 static inline bool apart(const cudamat* a, const cudamat* b) {
   return !a || !b || a->data_device + dn_len(a) <= b->data_device || b->data_device + dn_len(b) <= a->data_device;
 }
@@ -470,6 +554,16 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, floa
     else norm_launch<0, 4>(x, g, b, t, h, w, eps, (h + 1023) / 1024);
     return dn_launch_status();
   }
+  if (h < 4) {
+    const long long groups = (w + 255ll) / 256, most = 8 * dn_num_cus();
+    const dim3 grid((unsigned)(groups < most ? groups : most));
+    const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
+    float* t = target->data_device;
+    if (h == 1) hipLaunchKernelGGL(k_layer_norm_short<1>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
+    else if (h == 2) hipLaunchKernelGGL(k_layer_norm_short<2>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
+    else hipLaunchKernelGGL(k_layer_norm_short<3>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
+    return dn_launch_status();
+  }
   hipLaunchKernelGGL(k_layer_norm, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)mat->data_device,
                      (const float*)(gain ? gain->data_device : nullptr), (const float*)(bias ? bias->data_device : nullptr), target->data_device, h, eps);
   return dn_launch_status();
@@ -490,9 +584,12 @@ int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target
     if (!apart(m, gain_grad) || !apart(m, bias_grad)) return ERROR_UNSUPPORTED;
   if (!apart(gain_grad, bias_grad)) return ERROR_UNSUPPORTED;
   if (h <= 0) return 0;
-  if (h >= 4 && h <= NORM_COLS_MAX && w > 0 && w <= NORM_COLS_W) {
+  if (w > 0 && (h < 4 || (h <= NORM_COLS_MAX && w <= NORM_COLS_W))) {
     NormGradArgs a = {deriv->data_device, mat->data_device, gain ? gain->data_device : nullptr, target->data_device, nullptr,
                             gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, 0, eps, beta, mult};
+    if (h == 1) return norm_grad_short<1>(a);
+    if (h == 2) return norm_grad_short<2>(a);
+    if (h == 3) return norm_grad_short<3>(a);
     if (h <= 64) return norm_grad_launch<16, 1>(a);
     if (h <= 256) return norm_grad_launch<64, 1>(a);
     if (h <= 512) return norm_grad_launch<64, 2>(a);

@@ -40,6 +40,7 @@ void dn_close_group();
 void dn_set_group_open(bool on);
 void dn_set_group_hook(void (*f)());
 void dn_group_allow(bool on);               // whether a product may go to the group instead of the stream
+void dn_ring_first(bool on);                // whether products take the ring's tiles wherever they fit (and the bf16 ones are not faster)
 bool dn_group_take_sums(const struct DnRowSumJob* jobs, int n);   // row sums that join the open group; false: launch them
 // apply_rectified_linear_deriv(target, gate, target) of the target of a product of the open group joins it
 bool dn_group_take_gate(const float* target, const float* gate, int h, int w);

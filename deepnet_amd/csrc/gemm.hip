@@ -1161,6 +1161,8 @@ static inline bool side_jobs_fit(const GemmEpilogue& epi) {
 // of a workgroup; slabs (perhaps of a split reduction, summed by a second kernel)
 enum GemmKind { GEMM_EMPTY, GEMM_BOX, GEMM_SPLIT, GEMM_RING, GEMM_T16, GEMM_SMALL, GEMM_SLAB };
 struct GemmPlan { GemmKind kind; RingPlan ring; bool heavy; };
+static bool g_ring_first;            // dn_ring_first
+void dn_ring_first(bool on) { g_ring_first = on; }
 static GemmPlan gemm_plan(bool a_kc, bool b_kc, int M, int N, int K, const float* A, int lda, const float* B, int ldb, float beta) {
   const RingPlan no_ring = {-1, 0.};
   if (K <= 0) return GemmPlan{GEMM_EMPTY, no_ring, false};
@@ -1194,7 +1196,8 @@ static GemmPlan gemm_plan(bool a_kc, bool b_kc, int M, int N, int K, const float
   }
   // Reductions of more than 128 terms: k_gemm_ring, unless another kernel is expected to be faster (gemm_ring_plan).
   const size_t a_bytes = (size_t)lda * (a_kc ? M : K) * sizeof(float), b_bytes = (size_t)ldb * (b_kc ? N : K) * sizeof(float);
-  const RingPlan ring = K > BOX_K ? gemm_ring_plan(M, N, K, a_bytes, b_bytes, cus, a_vec && b_vec && !(a_kc && b_kc)) : no_ring;
+  const RingPlan ring = g_ring_first ? ring_plan(M, N, K, a_bytes, b_bytes, cus)
+                        : K > BOX_K  ? gemm_ring_plan(M, N, K, a_bytes, b_bytes, cus, a_vec && b_vec && !(a_kc && b_kc)) : no_ring;
   if (gemm_split_wins(M, N, K, beta != 0.f, a_bytes, b_bytes, ring, cus)) return GemmPlan{GEMM_SPLIT, no_ring, heavy};   // (no product that draws a sample)
   if (ring.cfg >= 0) return GemmPlan{GEMM_RING, ring, heavy};
   // Two K-contiguous operands whose rows lie a multiple of 1 KiB apart: the 16 x 16 block kernel

@@ -33,7 +33,9 @@ __device__ __forceinline__ bool gated_tile(const RingArgs& g, int& bx, int& by) 
   return true;
 }
 
-// On the bf16 matrix cores (split_tile.h).  Measured: see DESIGN's table and k_gated_ring.
+// On the bf16 matrix cores (split_tile.h), where the plain product would run there.  Bound as that is, by the rate of those cores at the clock that
+// the power limit leaves: 4096 -> 8192 units of 4096 columns 2.76 to 2.81 ms, 196 to 199 TFLOP/s of fp32 results (the product of 8192 x 8192 x
+// 8192 reaches 197); the product alone and a pass over the halves took 3.82.
 template <bool A_KC, bool B_KC>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2) k_gated_split(GatedArgs a) {
   constexpr int BM = SPLIT_BM, BN = SPLIT_BM, BK = SPLIT_BK, NT = SPLIT_THREADS, HALF = BM / 2;
@@ -58,7 +60,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2) k_gated_split(GatedArgs a) {
     if (m0 + i >= m_lo && n0 + c >= n_lo) gated_out(a.out, m0 + i, n0 + c, part[c * BM + i], part[c * BM + HALF + i]);
 }
 
-// On the tiles of the mid-sized products.
+// On the tiles of the mid-sized products.  Bound by the fp32 matrix cores: 1001 -> 1500 units of 300 columns, gelu, bias and halves kept,
+// 21.0 us (86 TFLOP/s; one 64 x 64 tile a CU takes 13.4 at the peak rate of a CU, the rest is its start and end), 20.0 without; the
+// other tiles 22.9 to 31.7.  2048 -> 1024 of 500 34.3 us, 122 TFLOP/s.
 template <int TB, int BM, int BN, int BK, bool A_KC, bool B_KC>
 __global__ void __launch_bounds__(RING_THREADS, 4) k_gated_ring(GatedArgs a) {
   using OA = GatedOperand<GatedRingTile<BM, BK, A_KC>>;
@@ -97,11 +101,18 @@ bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int
   const bool a_kc = a_trans, b_kc = !b_trans;
   if (f <= 0 || N <= 0 || K <= 0) return false;
   GemmPlan plan = gemm_plan(a_kc, b_kc, M, N, K, A, lda, B, ldb, 0.f);
-  // Strips of 9 to 15 columns, whose other kernels read the weights several times (2048 -> 5632 of 9 44.3 -> 22 us): the tile of 16 columns,
-  // where a column beyond the last one lies behind the operand's bytes.
-  if (N > 8 && N < 16 && f >= 16 && K > 128 && b_kc && (size_t)lda * (a_kc ? M : K) * sizeof(float) < (1ull << 31) &&
-      (size_t)16 * ldb * sizeof(float) < (1ull << 31))
-    plan = GemmPlan{GEMM_RING, RingPlan{4, 0.}, false};
+  // Where the product would run on a kernel without tiles like these, the ring's are taken all the same: no launch and no trip of the halves
+  // through memory behind it (us, product and pass / ring: 128 -> 2048 units of 2048 columns 39.8 / 32.1, 128 -> 512 of 128 7.9 / 4.0, 500 ->
+  // 1000 of 20 7.8 / 5.7, 2048 -> 5632 of 17 42.3 / 27.2, 4096 -> 512 of 64 19.6 / 13.9).
+  if (plan.kind != GEMM_SPLIT && plan.kind != GEMM_RING) {
+    const size_t a_bytes = (size_t)lda * (a_kc ? M : K) * sizeof(float), b_bytes = (size_t)ldb * (b_kc ? N : K) * sizeof(float);
+    const RingPlan ring = ring_plan(M, N, K, a_bytes, b_bytes, dn_num_cus());
+    if (ring.cfg >= 0) plan = GemmPlan{GEMM_RING, ring, false};
+    // Strips of 9 to 15 columns, whose other kernels read the weights several times (2048 -> 5632 of 9 44.3 -> 22 us): the tile of 16 columns,
+    // where a column beyond the last one lies behind the operand's bytes.
+    else if (N > 8 && N < 16 && f >= 16 && K >= 128 && b_kc && a_bytes < (1ull << 31) && (size_t)16 * ldb * sizeof(float) < (1ull << 31))
+      plan = GemmPlan{GEMM_RING, RingPlan{4, 0.}, false};
+  }
   GatedArgs a = {RingArgs{A, B, nullptr, (unsigned)((size_t)lda * (a_kc ? M : K) * sizeof(float)), (unsigned)((size_t)ldb * (b_kc ? N : K) * sizeof(float)),
                           lda, ldb, 0, M, N, K, 0, 0, 1.f, 0.f}, out};
   auto grid = [&](int half, int bn) {

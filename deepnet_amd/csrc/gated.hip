@@ -8,7 +8,10 @@ bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int
 // ------------------------------------------------------------------ up to eight columns
 // One to eight columns (single tokens of a few sequences) against weights whose rows are contiguous: bound by the weights' bytes.  A
 // wavefront (or the four of a workgroup, a quarter of the terms each, where there are few units) has R units, that is 2 R rows, for all
-// columns; its lanes take 16 bytes of every row at any 4-byte boundary, U pieces of 256 terms on their way at once.
+// columns; its lanes take 16 bytes of every row at any 4-byte boundary, U pieces of 256 terms on their way at once.  us, 2048 -> 5632 units (14.3 by
+// the bytes) of 1, 2, 4, 8 columns: 14.8 to 15.2, 16.6, 18.1, 22.6; 4096 -> 8192 of one 38.2, 7.0 TB/s (some of it from the caches); 2048 -> 512 of one
+// 3.6.  Two units a wavefront read the inputs half as often: 17.2 for one column, four and eight columns take 19.0 and 28.0 with one.  Weights read
+// with cached loads 16.6 for 14.9, loads of whole trips behind no branch 15.8 for 15.3.
 struct GatedColumnsArgs {
   const float *A, *B;
   int lda, ldb, K;
@@ -99,7 +102,10 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
 #define GATED_COLUMNS 8
 static int gated_columns(int n, const GatedColumnsArgs& a) {
   const int f = a.out.f;
-  const bool shared = f < 8 * dn_num_cus();        // (fewer than eight wavefronts a CU by themselves)
+  // A workgroup's wavefronts share a unit's terms where there are fewer than eight wavefronts a CU by themselves (us, by themselves / shared: 2048 -> 512
+  // units 4.3 / 3.6, 500 -> 1000 of four columns 4.65 / 4.2), and where up to four columns have more than a thousand terms (4096 -> 8192 42.3 /
+  // 38.2, 2048 -> 5632 15.8 / 15.2, of three 18.6 / 16.8; 1001 -> 3000 5.9 / 6.9, 500 -> 3000 of four 5.9 / 6.7, 2048 -> 5632 of eight 22.6 / 26.9).
+  const bool shared = f < 8 * dn_num_cus() || (n <= 4 && a.K > 1024);
 #define GATED_COLS(N, R, U)                                                                                                       \
   case N:                                                                                                                         \
     if (shared) hipLaunchKernelGGL((k_gated_columns<N, R, U, true>), dim3((unsigned)((f + R - 1) / R)), dim3(256), 0, dn_stream(), a); \
@@ -120,14 +126,17 @@ static int gated_columns(int n, const GatedColumnsArgs& a) {
 }
 
 // ------------------------------------------------------------------ a pass over the halves
-// A wavefront takes up to G groups of four rows a lane of a piece of one column; the rows behind the last group go one a lane.
+// A wavefront takes 256 rows of one column or fewer, four a lane; the rows behind the last group go one a lane.  Bound by the bytes, 20 a unit and
+// column backward and 12 forward: 4096 units of 2048 columns backward 30 to 32 us, 5.2 to
+// 5.6 TB/s.  (Four groups a lane on their way at once: 4096 units of 1000 columns
+// with 256 inputs, all of the backward pass, 92.4 us for 90.3, of 100 columns 48.3 for 45.7, of one with 2048 inputs 37.2 for 34.7.)
 struct GatePass {
   const float *deriv, *pre;
   float* target;
   int f, w, act, pieces, length;
 };
 // GRAD: target (2 f rows, may be pre) = the derivatives by the halves; else target = act(gate) * up.
-template <int G, bool GRAD, bool STREAM>
+template <bool GRAD, bool STREAM>
 __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
   const int lane = threadIdx.x & 63;
   const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -147,31 +156,15 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
       to_gate = gate_act(gate, a.act) * up;
     }
   };
-  float x[G][4], y[G][4], z[G][4];
+  if (lane < n4) {
+    float x[4], y[4], z[4], p[4], q[4];
+    col_load<STREAM>(x, g + 4 * lane);
+    col_load<STREAM>(y, g + a.f + 4 * lane);
+    if (GRAD) col_load<STREAM>(z, d + 4 * lane);
 #pragma unroll
-  for (int u = 0; u < G; ++u) {
-    const int j = lane + 64 * u;
-    if (j < n4) {
-      col_load<STREAM>(x[u], g + 4 * j);
-      col_load<STREAM>(y[u], g + a.f + 4 * j);
-      if (GRAD) col_load<STREAM>(z[u], d + 4 * j);
-    }
-  }
-#pragma unroll 1
-  for (int u = 0; u < G; ++u) {
-    const int j = lane + 64 * u;
-    if (j < n4) {
-      float p[4], q[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) one(x[0][e], y[0][e], GRAD ? z[0][e] : 0.f, p[e], q[e]);
-      col_store<STREAM>(t + 4 * j, p);
-      if (GRAD) col_store<STREAM>(t + a.f + 4 * j, q);
-    }
-    // (one copy of the code for the groups: they move up)
-#pragma unroll
-    for (int k = 0; k + 1 < G; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { x[k][e] = x[k + 1][e]; y[k][e] = y[k + 1][e]; if (GRAD) z[k][e] = z[k + 1][e]; }
+    for (int e = 0; e < 4; ++e) one(x[e], y[e], GRAD ? z[e] : 0.f, p[e], q[e]);
+    col_store<STREAM>(t + 4 * lane, p);
+    if (GRAD) col_store<STREAM>(t + a.f + 4 * lane, q);
   }
   if (lane < (n & 3)) {
     const int i = 4 * n4 + lane;
@@ -183,23 +176,20 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
 }
 template <bool GRAD>
 static int gate_pass(const float* deriv, const float* pre, float* target, int f, int w, int act) {
-  // four groups a lane, or one where that makes less than two wavefronts for every SIMD
-  const bool wide = (long long)w * ((f + 1023) / 1024) >= 8 * dn_num_cus();
-  const int most = wide ? 1024 : 256, pieces = (f + most - 1) / most;
+  const int pieces = (f + 255) / 256;
   const GatePass a = {deriv, pre, target, f, w, act, pieces, ((f + pieces - 1) / pieces + 3) / 4 * 4};
   const long long blocks = ((long long)w * pieces + 3) / 4;
   if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  const bool stream = (long long)f * w >= DN_STREAM_MIN_ELEMS;
-#define GATE_GO(G, S) hipLaunchKernelGGL((k_gate_pass<G, GRAD, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
-  if (wide) { if (stream) GATE_GO(4, true); else GATE_GO(4, false); }
-  else GATE_GO(1, false);
-#undef GATE_GO
+  if ((long long)f * w >= DN_STREAM_MIN_ELEMS) hipLaunchKernelGGL((k_gate_pass<GRAD, true>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
+  else hipLaunchKernelGGL((k_gate_pass<GRAD, false>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
   return dn_launch_status();
 }
 
 // ------------------------------------------------------------------ the backward products of up to eight columns
 // Both are bound by the weights' bytes: their gradient mult d x^T is written (k rows, 2 f columns), the inputs' gradient W d reads them.  A
-// wavefront has 256 rows, four a lane at any 4-byte boundary; the derivatives d of a slice of the 2 f units wait in LDS.
+// wavefront has 256 rows, four a lane at any 4-byte boundary; the derivatives d of a slice of the 2 f units wait in LDS.  2048 -> 4096 units, one
+// column: 34.6 us in all (20.8 by the bytes): 13 the weights' gradient, 14 the inputs', 3 k_few_finish, 2 the pass over the halves; eight
+// columns 41.2.
 #define FEW_ROWS 256
 #define FEW_SLICE 128
 struct FewArgs {
@@ -319,6 +309,8 @@ template <int N>
 static int few_columns(FewArgs a) {
   const int cus = dn_num_cus(), blocks = (a.k + FEW_ROWS - 1) / FEW_ROWS;
   if (a.dw || a.bias_grad) {
+    // (slices as short as give eight workgroups a CU, below four: with the longest for all, 2048 -> 4096 units of one column 47.6 us for 34.7, 500 ->
+    // 500 38.2 for 13.6)
     const int wgs = (blocks + 3) / 4;
     a.slice = FEW_SLICE;
     while (a.slice > 16 && (long long)wgs * ((a.units + a.slice - 1) / a.slice) < 8 * cus) a.slice >>= 1;

@@ -167,7 +167,11 @@ __device__ __forceinline__ unsigned lp_order(float x) { return (unsigned)(lp_key
 // (a mask, a constant column), by their places too, lane by lane.
 #define LP_LIST 2048               // candidates that a workgroup holds
 
-// ---- columns (or segments of them) by a workgroup of 256 lanes, four 16-byte groups a lane in flight
+// ---- columns (or segments of them) by a workgroup of 256 lanes, eight 16-byte groups a lane on their way
+// Bound by the bytes, 4 an entry: 32768 x 2048 41.8 to 42.2 us, 6.4 TB/s (copy rate: 41.6), 32003 x 2048 43.2; the exponentials take 0.8 of the
+// vector unit's time.  Few columns are split, so that the chip reads them at once: 50000 x 4 in 52 workgroups 4.8 us.  Top lists are found in
+// the same pass, after it: 32000 x 1024 with 20 best 38.2 us (20.3 by the bytes), 50000 x 4 10.0, a chain of some ten trips to LDS and three to
+// memory, whose steps take 0.4 to 1.4 us each.
 template <bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
   __shared__ LogProbPart parts[4];
@@ -475,6 +479,7 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
 }
 
 // ---- columns of 4 to 1024 rows (many of them: to 4095, without a top list) by a wavefront, which holds them in registers
+// Bound by the bytes: 1024 x 20000 15.6 us, 5.3 TB/s (with 20 best 40.7: by the vector instructions of the list), 2050 x 8192 14.6.
 template <int NV, bool TAIL, bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned long long lists[TOP ? 4 : 1][TOP ? 256 * NV + 2 : 2];
@@ -576,7 +581,8 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
 
 // target = logp_weight (onehot(label) - p) - entropy_weight p (log p + entropy), log p = mat - log_z, p = e^(log p): one pass.  A unit of 64
 // lanes (columns of up to 1024 rows) or 256 (pieces of 4096) takes up to 16 rows a lane of one column; the rows behind the last group of
-// four go one a lane, so that target may be mat (no row is read by one lane when another may have written it).
+// four go one a lane, so that target may be mat (no row is read by one lane when another may have written it).  8 bytes an entry: 32768 x
+// 1000 45.5 us, 5.8 TB/s (copy rate: 40.6), 32003 x 1000 47.5, 1000 x 20000 31.6.
 struct LogProbGradArgs {
   const float *mat, *labels, *log_z, *logp_weight, *entropy, *entropy_weight;
   float* target;
@@ -659,7 +665,7 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   if (w <= 0) return 0;
   LogProbArgs a = {mat->data_device, DPTR(labels), DPTR(logp), DPTR(entropy), DPTR(log_z), DPTR(top), DPTR(top_labels), h, w, k, 1, h, nullptr, nullptr, nullptr};
-  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
+  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4; 500 x 40000 21.5 -> 20.1)
   const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
   // Columns of up to 1024 rows by a wavefront each, and where there are enough of them for the chip those that are shorter than one trip of a
   // workgroup (us, workgroup / wavefront: 2050 x 8192 26.3 / 16.9, 1500 x 20000 50.8 / 21.2; 4096 x 8192 23.0 / 23.9, 3001 x 1100 6.7 / 7.3).
@@ -667,17 +673,17 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
     const dim3 grid((unsigned)((w + 3) / 4));
 #define LP_WAVE4(NV, TAIL, TOP, S) hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, TOP, S>), grid, dim3(256), 0, dn_stream(), a)
 #define LP_WAVE3(NV, TOP, S) do { if (h % 4) LP_WAVE4(NV, true, TOP, S); else LP_WAVE4(NV, false, TOP, S); } while (0)
-#define LP_WAVE(NV) do { if (k) LP_WAVE3(NV, true, false); else LP_WAVE3(NV, false, false); } while (0)
 #define LP_WAVES(NV) do { if (stream) LP_WAVE3(NV, false, true); else LP_WAVE3(NV, false, false); } while (0)
-    if (h <= 256) LP_WAVE(1);
-    else if (h <= 512) LP_WAVE(2);
+    if (k && h <= 256) LP_WAVE3(1, true, false);
+    else if (k && h <= 512) LP_WAVE3(2, true, false);
     else if (k) LP_WAVE3(4, true, false);
+    else if (h <= 256) LP_WAVES(1);
+    else if (h <= 512) LP_WAVES(2);
     else if (h <= 4 * 256) LP_WAVES(4);
     else if (h <= 8 * 256) LP_WAVES(8);
     else if (h <= 12 * 256) LP_WAVES(12);
     else LP_WAVES(16);
 #undef LP_WAVES
-#undef LP_WAVE
 #undef LP_WAVE3
 #undef LP_WAVE4
     return dn_launch_status();

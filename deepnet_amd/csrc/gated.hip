@@ -1,6 +1,7 @@
 // Gated products act(G) * U of the two halves of one product, and their backward pass (no counterpart in cudamat.cu).
 #include "columns.h"
 #include "gated_act.h"
+#include <type_traits>
 
 int dn_row_sums(const float* M, int h, int w, float* y, float alpha, float beta);
 bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int lda, const float* B, int ldb, const GatedOut& out, int* err);
@@ -186,35 +187,29 @@ static int gate_pass(const float* deriv, const float* pre, float* target, int f,
 }
 
 // ------------------------------------------------------------------ the backward products of up to eight columns
-// Both are bound by the weights' bytes: their gradient mult d x^T is written (k rows, 2 f columns), the inputs' gradient W d reads them.  A
-// wavefront has 256 rows, four a lane at any 4-byte boundary; the derivatives d of a slice of the 2 f units wait in LDS.  2048 -> 4096 units, one
-// column: 34.6 us in all (20.8 by the bytes): 13 the weights' gradient, 14 the inputs', 3 k_few_finish, 2 the pass over the halves; eight
-// columns 41.2.
+// Both are bound by the weights' bytes: their gradient mult x d^T (k rows, 2 f columns) is written, the inputs' gradient W d reads them.  One kernel
+// does both, so that reads and writes share the memory's time.  A wavefront has 256 rows, four a lane at any 4-byte boundary, and every fourth
+// unit of a slice of the 2 f; the derivatives d of the slice wait in LDS.  The four meet in LDS for W d, the slices' parts are added up by
+// k_few_finish.  2048 -> 4096 units, one column: 31.7 us in all (20.8 by the bytes), of which k_few_finish
+// is 3 and the pass over the halves 2; eight 34.6, 500 -> 500 of one 9.4.  In a kernel each: 34.7, 41.2, 13.6.  Eight units are on their way at once
+// (four: 39.1, 44.7, sixteen: 31.5, 36.3).
 #define FEW_ROWS 256
 #define FEW_SLICE 128
+#define FEW_AHEAD 8
 struct FewArgs {
   const float *W, *x, *d;
   float *dw, *dx, *partial, *bias_grad;
   int k, units, slice, slices;
   float beta, mult;
 };
-template <int N>
-__device__ __forceinline__ void few_derivs(const FewArgs& a, float (*ds)[N], int j0, int len) {
+// DX: dx = W d.  DW: dw = mult x d^T, with ADD + beta dw.  The sums of d to bias_grad, where that is given, by the first block of rows.
+template <int N, bool DX, bool DW, bool ADD>
+__global__ void __launch_bounds__(256) k_few(FewArgs a) {
+  __shared__ float ds[FEW_SLICE][N], part[DX ? 4 : 1][N][DX ? FEW_ROWS : 1];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
   for (int i = threadIdx.x; i < len * N; i += 256) ds[i % len][i / len] = a.d[(size_t)(i / len) * a.units + j0 + i % len];
   __syncthreads();
-}
-// rows `count` (1 to 4) of a group
-__device__ __forceinline__ void few_load(float (&v)[4], const float* p, int count) {
-  if (count == 4) { col_load<true>(v, p); return; }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = e < count ? p[e] : 0.f;
-}
-// dw = beta dw + mult x d^T, and the sums of d: a wavefront a block of rows, all four the same slice of units.
-template <int N>
-__global__ void __launch_bounds__(256) k_few_outer(FewArgs a) {
-  __shared__ float ds[FEW_SLICE][N];
-  const int lane = threadIdx.x & 63, j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
-  few_derivs<N>(a, ds, j0, len);
   if (a.bias_grad && blockIdx.x == 0)
     for (int j = threadIdx.x; j < len; j += 256) {
       float s = 0.f;
@@ -223,71 +218,65 @@ __global__ void __launch_bounds__(256) k_few_outer(FewArgs a) {
       float* b = a.bias_grad + j0 + j;
       *b = a.beta != 0.f ? __fmaf_rn(a.mult, s, a.beta * *b) : a.mult * s;
     }
-  const int row = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) * FEW_ROWS + 4 * lane, count = a.k - row < 4 ? a.k - row : 4;
-  if (!a.dw || count <= 0) return;
-  float x[N][4];
+  // a group over the last row moves back; of the rows that it shares with its neighbour it stores none
+  const int first = (int)blockIdx.x * FEW_ROWS + 4 * lane, row = first + 4 <= a.k ? first : a.k - 4, lap = first - row;
+  float x[N][4], acc[N][4];
 #pragma unroll
-  for (int c = 0; c < N; ++c) few_load(x[c], a.x + (size_t)c * a.k + row, count);
-  float* out = a.dw + (size_t)j0 * a.k + row;
-#pragma unroll 4
-  for (int j = 0; j < len; ++j, out += a.k) {
-    float y[4] = {0.f, 0.f, 0.f, 0.f}, old[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.beta != 0.f) few_load(old, out, count);
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = __fmaf_rn(x[c][e], ds[j][c], y[e]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = a.beta != 0.f ? __fmaf_rn(a.mult, y[e], a.beta * old[e]) : a.mult * y[e];
-    if (count == 4) {
-      col_store<true>(out, y);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) out[e] = y[e];
-    }
-  }
-}
-// W d: the four wavefronts of a workgroup take every fourth unit of a slice for the same rows and meet in LDS; slices are added up by
-// k_few_finish.
-template <int N>
-__global__ void __launch_bounds__(256) k_few_rows(FewArgs a) {
-  __shared__ float ds[FEW_SLICE][N], part[4][N][FEW_ROWS];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
-  few_derivs<N>(a, ds, j0, len);
-  const int row = (int)blockIdx.x * FEW_ROWS + 4 * lane, count = a.k - row < 4 ? a.k - row : 4;
-  float acc[N][4];
-#pragma unroll
-  for (int c = 0; c < N; ++c)
+  for (int c = 0; c < N; ++c) {
+    if (DW) col_load<false>(x[c], a.x + (size_t)c * a.k + row);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[c][e] = 0.f;
-  if (count > 0) {
-    const float* w = a.W + (size_t)j0 * a.k + row;
-    for (int j = wv; j < len; j += 32) {
-      float v[8][4];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (j + 4 * u < len) few_load(v[u], w + (size_t)(j + 4 * u) * a.k, count);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (j + 4 * u < len) {
-#pragma unroll
-          for (int c = 0; c < N; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c][e] = __fmaf_rn(v[u][e], ds[j + 4 * u][c], acc[c][e]);
-        }
-    }
   }
+  const size_t at = (size_t)j0 * a.k + row;
+  auto trip = [&](int j, auto units) __attribute__((always_inline)) {
+    constexpr int U = decltype(units)::value;
+    float v[U][4], old[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t o = at + (size_t)(j + 4 * u) * a.k;
+      if (DX) col_load<true>(v[u], a.W + o);
+      if (ADD) col_load<true>(old[u], a.dw + o);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const float d = ds[j + 4 * u][c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (DX) acc[c][e] = __fmaf_rn(v[u][e], d, acc[c][e]);
+          if (DW) y[e] = __fmaf_rn(x[c][e], d, y[e]);
+        }
+      }
+      if (!DW) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = ADD ? __fmaf_rn(a.mult, y[e], a.beta * old[u][e]) : a.mult * y[e];
+      float* out = a.dw + at + (size_t)(j + 4 * u) * a.k;
+      if (lap == 0) {
+        col_store<true>(out, y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e >= lap) out[e] = y[e];
+      }
+    }
+  };
+  int j = wv;
+  for (; j + 4 * (FEW_AHEAD - 1) < len; j += 4 * FEW_AHEAD) trip(j, std::integral_constant<int, FEW_AHEAD>());
+  for (; j < len; j += 4) trip(j, std::integral_constant<int, 1>());
+  if (!DX) return;
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wv][c][4 * lane + e] = acc[c][e];
+    for (int e = 0; e < 4; ++e)
+      if (e >= lap) part[wv][c][row + e - (int)blockIdx.x * FEW_ROWS] = acc[c][e];
   __syncthreads();
   const int r = blockIdx.x * FEW_ROWS + threadIdx.x;
   if (r < a.k)
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const float s = (part[0][c][threadIdx.x] + part[1][c][threadIdx.x]) + (part[2][c][threadIdx.x] + part[3][c][threadIdx.x]);
+      const float s = (part[0][c][threadIdx.x] + part[DX ? 1 : 0][c][threadIdx.x]) + (part[DX ? 2 : 0][c][threadIdx.x] + part[DX ? 3 : 0][c][threadIdx.x]);
       (a.slices > 1 ? a.partial + ((size_t)blockIdx.y * N) * a.k : a.dx)[(size_t)c * a.k + r] = s;
     }
 }
@@ -305,33 +294,30 @@ __global__ void __launch_bounds__(256) k_few_finish(const float* partial, float*
   if (wv == 0 && i < n) dx[i] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
+// At least four rows; units of 65535 slices of 32 at most.
 template <int N>
 static int few_columns(FewArgs a) {
   const int cus = dn_num_cus(), blocks = (a.k + FEW_ROWS - 1) / FEW_ROWS;
-  if (a.dw || a.bias_grad) {
-    // (slices as short as give eight workgroups a CU, below four: with the longest for all, 2048 -> 4096 units of one column 47.6 us for 34.7, 500 ->
-    // 500 38.2 for 13.6)
-    const int wgs = (blocks + 3) / 4;
-    a.slice = FEW_SLICE;
-    while (a.slice > 16 && (long long)wgs * ((a.units + a.slice - 1) / a.slice) < 8 * cus) a.slice >>= 1;
-    const int slices = (a.units + a.slice - 1) / a.slice;
-    if (slices > 65535) return ERROR_UNSUPPORTED;
-    hipLaunchKernelGGL(k_few_outer<N>, dim3((unsigned)wgs, (unsigned)slices), dim3(256), 0, dn_stream(), a);
+  // Slices as short as give two workgroups a CU (2048 -> 4096 units of one and of eight columns, us: one workgroup 41.6, 45.8, two 31.7, 34.6, four
+  // 37.5, 40.4, eight 31.0, 38.9).
+  a.slice = FEW_SLICE;
+  while (a.slice > 32 && (long long)blocks * ((a.units + a.slice - 1) / a.slice) < 2 * cus) a.slice >>= 1;
+  a.slices = (a.units + a.slice - 1) / a.slice;
+  if (a.dx && a.slices > 1) {
+    a.partial = (float*)dn_scratch((size_t)a.slices * N * a.k * sizeof(float));
+    if (!a.partial) return CUDA_ERROR;
   }
-  if (a.dx) {
-    a.slice = FEW_SLICE;
-    while (a.slice > 32 && (long long)blocks * ((a.units + a.slice - 1) / a.slice) < 4 * cus) a.slice >>= 1;
-    a.slices = (a.units + a.slice - 1) / a.slice;
-    if (a.slices > 65535) return ERROR_UNSUPPORTED;
-    if (a.slices > 1) {
-      a.partial = (float*)dn_scratch((size_t)a.slices * N * a.k * sizeof(float));
-      if (!a.partial) return CUDA_ERROR;
-    }
-    hipLaunchKernelGGL(k_few_rows<N>, dim3((unsigned)blocks, (unsigned)a.slices), dim3(256), 0, dn_stream(), a);
-    if (a.slices > 1) {
-      const long long n = (long long)N * a.k;
-      hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, n, a.slices);
-    }
+  const dim3 grid((unsigned)blocks, (unsigned)a.slices);
+#define FEW_GO(DX, DW, ADD) hipLaunchKernelGGL((k_few<N, DX, DW, ADD>), grid, dim3(256), 0, dn_stream(), a)
+  const bool add = a.beta != 0.f;
+  if (a.dw && a.dx) { if (add) FEW_GO(true, true, true); else FEW_GO(true, true, false); }
+  else if (a.dw) { if (add) FEW_GO(false, true, true); else FEW_GO(false, true, false); }
+  else if (a.dx) FEW_GO(true, false, false);
+  else if (a.bias_grad) FEW_GO(false, false, false);
+#undef FEW_GO
+  if (a.dx && a.slices > 1) {
+    const long long n = (long long)N * a.k;
+    hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, n, a.slices);
   }
   return dn_launch_status();
 }
@@ -404,7 +390,7 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
   if (e) return e;
   const float *w = mat1->data_device, *x = mat2->data_device, *d = target->data_device;
   const bool wt = mat1->is_trans != 0, xt = mat2->is_trans != 0;
-  if (n >= 1 && n <= GATED_COLUMNS && wt && !xt && f > 0 && k > 0 && 2 * f <= 65535 * 16) {
+  if (n >= 1 && n <= GATED_COLUMNS && wt && !xt && f > 0 && k >= 4 && 2 * f <= 65535 * 32) {
     const FewArgs a = {w, x, d, mat1_grad ? mat1_grad->data_device : nullptr, mat2_grad ? mat2_grad->data_device : nullptr, nullptr,
                        bias_grad ? bias_grad->data_device : nullptr, k, 2 * f, 0, 1, beta, mult};
 #define FEW(N) case N: return few_columns<N>(a)

@@ -307,6 +307,32 @@ def test_dot_gated_grad(cm, rng, d, f, n, act):
     check(db.asarray(), 0.5 - 2.0 * wdb, 2 * edb + 3 * U * (1 + 2 * np.abs(wdb)), 'scaled')
 
 
+@pytest.mark.parametrize("d,f,n", [(4, 3, 1), (5, 30, 8), (258, 130, 3), (1030, 700, 8), (2051, 100, 1), (300, 64, 64), (3, 9, 2)])
+def test_dot_gated_grad_of_one_operand_alone_and_accumulated(cm, rng, d, f, n):
+    """Which gradients are asked for does not change them; all of them accumulated."""
+    w, x, dy = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d)), F(rng.standard_normal((d, n))), F(rng.standard_normal((f, n)))
+    W, X, PRE, DY = cm.CUDAMatrix(w), cm.CUDAMatrix(x), cm.CUDAMatrix(F(rng.standard_normal((2 * f, n)))), cm.CUDAMatrix(dy)
+    def run(names, old=np.nan, **scales):
+        t, out = cm.empty((2 * f, n)), dict(m1_grad=(d, 2 * f), m2_grad=(d, n), bias_grad=(2 * f, 1))
+        out = {k: cm.CUDAMatrix(F(np.full(out[k], old))) for k in names}
+        cm.dot_gated_grad(DY, W.T, X, PRE, target=t, **out, **scales)
+        return t.asarray().astype(np.float64), {k: m.asarray().copy() for k, m in out.items()}
+    t, every = run(('m1_grad', 'm2_grad', 'bias_grad'))
+    at, chains = np.abs(t), U * (n / 4 + 24)
+    edw, edb = chains * (np.abs(x.astype(np.float64)) @ at.T), chains * at.sum(axis=1, keepdims=True)
+    edx = U * (f / 2 + 24) * (np.abs(w.astype(np.float64)) @ at)
+    wdw, wdx, wdb = x.astype(np.float64) @ t.T, w.astype(np.float64) @ t, t.sum(axis=1, keepdims=True)
+    for names in (('m1_grad',), ('m2_grad',), ('bias_grad',), ('m1_grad', 'm2_grad'), ('m2_grad', 'bias_grad'), tuple(every)):
+        _, got = run(names)
+        for k, want, bound in (('m1_grad', wdw, edw), ('m2_grad', wdx, edx), ('bias_grad', wdb, edb)):
+            if k in names:
+                check(got[k], want, bound, (names, k))
+    _, got = run(tuple(every), old=3.0, beta=0.5, mult=-2.0)
+    check(got['m1_grad'], 1.5 - 2 * wdw, 2 * edw + 3 * U * (1.5 + 2 * np.abs(wdw)), 'added')
+    check(got['m2_grad'], wdx, edx, 'not added')
+    check(got['bias_grad'], 1.5 - 2 * wdb, 2 * edb + 3 * U * (1.5 + 2 * np.abs(wdb)), 'added')
+
+
 def test_dot_gated_grad_of_operands_stored_either_way(cm, rng):
     d, f, n = 70, 33, 20
     w, x, dy = F(rng.standard_normal((d, 2 * f))), F(rng.standard_normal((d, n))), F(rng.standard_normal((f, n)))

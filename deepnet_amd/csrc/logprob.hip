@@ -138,6 +138,16 @@ __device__ __forceinline__ unsigned lp_quad_max(unsigned v) {
   const unsigned b = (unsigned)lane_move_int<0x4E>((int)v);
   return b > v ? b : v;
 }
+// The k-th greatest of a wavefront's values (which has as many), bit by bit: the greatest number that k of them reach.
+__device__ __forceinline__ unsigned lp_kth(unsigned value, int k) {
+  unsigned r = 0;
+#pragma unroll 4
+  for (int b = 31; b >= 0; --b) {
+    const unsigned t = r | 1u << b;
+    if (__popcll(__ballot(value >= t)) >= k) r = t;
+  }
+  return r;
+}
 // Lanes before this one that are in the mask.
 __device__ __forceinline__ int lp_before(unsigned long long mask) {
   return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
@@ -479,16 +489,19 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
 }
 
 // ---- columns of 4 to 1024 rows (many of them: to 4095, without a top list) by a wavefront, which holds them in registers
-// Bound by the bytes: 1024 x 20000 15.6 us, 5.3 TB/s (with 20 best 40.7: by the vector instructions of the list), 2050 x 8192 14.6.
-template <int NV, bool TAIL, bool TOP, bool STREAM>
+// Bound by the bytes: 1024 x 20000 15.5 us, 5.3 TB/s (with 20 best 38.4: by the vector instructions of the list), 2050 x 8192 14.6, 256 x 80000
+// 15.2, 100 x 200000 22.3; 100 x 8192 with 20 best 11.9.  The results of a column take a hundred instructions in 64 bits, which four columns share.
+// T: the lanes of a column, 64 or (up to 512 rows without a top list) 16, four columns a wavefront.
+template <int T, int NV, bool TAIL, bool TOP, bool STREAM>
 __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
+  static_assert(T == 64 || !TOP, "a wavefront finds a list");
   __shared__ __attribute__((aligned(16))) unsigned long long lists[TOP ? 4 : 1][TOP ? 256 * NV + 2 : 2];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = blockIdx.x * 4 + wv;
+  const int lane = threadIdx.x % T, wv = threadIdx.x >> 6, col = blockIdx.x * (256 / T) + threadIdx.x / T;
   const bool live = col < a.w;
   const float* c = a.mat + (size_t)(live ? col : 0) * a.h;
   const LogProbLabel label = lp_label(a, live ? col : 0);
   ColGroups<NV, TAIL> at;
-  at.init(lane, 64, a.h);
+  at.init(lane, T, a.h);
   float v[NV][4], m = -FLT_MAX;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -502,12 +515,12 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
       m = fmaxf(m, v[k][e]);
     }
   LogProbPart p = lp_none();
-  p.m = lanes_sum<64, true>(m);
+  p.m = lanes_sum<T, true>(m);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) lp_take(p, v[k][e]);
-  p = LogProbPart{p.m, (int)lanes_sum<64>((float)p.count), lanes_sum<64>(p.r), lanes_sum<64>(p.t)};
+  p = LogProbPart{p.m, (int)lanes_sum<T>((float)p.count), lanes_sum<T>(p.r), lanes_sum<T>(p.t)};
   const LogProbResult o = lp_result(p);
   if (live && lane == 0) lp_finish(a, col, p, o, label);
   if (!TOP) return;
@@ -529,36 +542,14 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
   // (a wavefront's own part of LDS, whose accesses are in order: the compiler has to keep them so)
   auto ordered = []() __attribute__((always_inline)) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
   unsigned long long* list = lists[wv];
-  unsigned* const orders = reinterpret_cast<unsigned*>(list);
   const unsigned order = (unsigned)(best >> 32);
-  orders[lane] = order;
-  ordered();
-  int greater, reach;
-  auto stand = [&](unsigned value) __attribute__((always_inline)) {
-    greater = reach = 0;
-#pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(orders + i);
-      greater += (q.x > value ? 1 : 0) + (q.y > value ? 1 : 0) + (q.z > value ? 1 : 0) + (q.w > value ? 1 : 0);
-      reach += (q.x >= value ? 1 : 0) + (q.y >= value ? 1 : 0) + (q.z >= value ? 1 : 0) + (q.w >= value ? 1 : 0);
-    }
-  };
-  stand(order);
-  const unsigned long long kth = __ballot(order && greater < a.k && reach >= a.k);          // the k-th maximum, or several that are alike
-  ordered();
   unsigned long long border = 1;
-  if (kth) {
-    const int first_kth = __builtin_ctzll(kth);
-    border = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)order, first_kth) << 32;
-    if (__builtin_amdgcn_readlane(reach, first_kth) != a.k) {
-      // several are alike at the border: of those the first places
-      const unsigned value = (unsigned)(border >> 32), standing = order > value ? 0xffffffffu : order == value ? (unsigned)best : 0;
-      orders[lane] = standing;
-      ordered();
-      stand(standing);
-      border |= (unsigned)__builtin_amdgcn_readlane((int)standing, __builtin_ctzll(__ballot(standing && greater < a.k && reach >= a.k)));
-      ordered();
-    }
+  if (__popcll(__ballot(order != 0)) >= a.k) {             // the k-th of the lanes' maxima, or several that are alike
+    const unsigned value = lp_kth(order, a.k);
+    const int above = __popcll(__ballot(order > value));
+    border = (unsigned long long)value << 32;
+    // several are alike at the border: of those the first places
+    if (__popcll(__ballot(order >= value)) != a.k) border |= lp_kth(order == value ? (unsigned)best : 0, a.k - above);
   }
   const float least = border > 1 ? lp_key_value(border) : -INFINITY;
   int count = 0;
@@ -665,24 +656,28 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
   }
   if (w <= 0) return 0;
   LogProbArgs a = {mat->data_device, DPTR(labels), DPTR(logp), DPTR(entropy), DPTR(log_z), DPTR(top), DPTR(top_labels), h, w, k, 1, h, nullptr, nullptr, nullptr};
-  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4; 500 x 40000 21.5 -> 20.1)
+  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
   const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
   // Columns of up to 1024 rows by a wavefront each, and where there are enough of them for the chip those that are shorter than one trip of a
   // workgroup (us, workgroup / wavefront: 2050 x 8192 26.3 / 16.9, 1500 x 20000 50.8 / 21.2; 4096 x 8192 23.0 / 23.9, 3001 x 1100 6.7 / 7.3).
+  // Up to 512 rows four columns a wavefront (us, one / four: 100 x 200000 67.8 / 22.3, 256 x 80000 30.3 / 15.2, 500 x 40000 20.0 / 15.7, 1024 x
+  // 20000 15.5 / 19.9).
   if (h >= 4 && w <= LP_WAVE_COLUMNS && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
-    const dim3 grid((unsigned)((w + 3) / 4));
-#define LP_WAVE4(NV, TAIL, TOP, S) hipLaunchKernelGGL((k_log_probs_wave<NV, TAIL, TOP, S>), grid, dim3(256), 0, dn_stream(), a)
-#define LP_WAVE3(NV, TOP, S) do { if (h % 4) LP_WAVE4(NV, true, TOP, S); else LP_WAVE4(NV, false, TOP, S); } while (0)
-#define LP_WAVES(NV) do { if (stream) LP_WAVE3(NV, false, true); else LP_WAVE3(NV, false, false); } while (0)
-    if (k && h <= 256) LP_WAVE3(1, true, false);
-    else if (k && h <= 512) LP_WAVE3(2, true, false);
-    else if (k) LP_WAVE3(4, true, false);
-    else if (h <= 256) LP_WAVES(1);
-    else if (h <= 512) LP_WAVES(2);
-    else if (h <= 4 * 256) LP_WAVES(4);
-    else if (h <= 8 * 256) LP_WAVES(8);
-    else if (h <= 12 * 256) LP_WAVES(12);
-    else LP_WAVES(16);
+#define LP_WAVE4(T, NV, TAIL, TOP, S) \
+  hipLaunchKernelGGL((k_log_probs_wave<T, NV, TAIL, TOP, S>), dim3((unsigned)((w + 256 / T - 1) / (256 / T))), dim3(256), 0, dn_stream(), a)
+#define LP_WAVE3(T, NV, TOP, S) do { if (h % 4) LP_WAVE4(T, NV, true, TOP, S); else LP_WAVE4(T, NV, false, TOP, S); } while (0)
+#define LP_WAVES(T, NV) do { if (stream) LP_WAVE3(T, NV, false, true); else LP_WAVE3(T, NV, false, false); } while (0)
+    if (k && h <= 256) LP_WAVE3(64, 1, true, false);
+    else if (k && h <= 512) LP_WAVE3(64, 2, true, false);
+    else if (k) LP_WAVE3(64, 4, true, false);
+    else if (h <= 64) LP_WAVES(16, 1);
+    else if (h <= 128) LP_WAVES(16, 2);
+    else if (h <= 256) LP_WAVES(16, 4);
+    else if (h <= 512) LP_WAVES(16, 8);
+    else if (h <= 4 * 256) LP_WAVES(64, 4);
+    else if (h <= 8 * 256) LP_WAVES(64, 8);
+    else if (h <= 12 * 256) LP_WAVES(64, 12);
+    else LP_WAVES(64, 16);
 #undef LP_WAVES
 #undef LP_WAVE3
 #undef LP_WAVE4

@@ -186,20 +186,21 @@ static int gate_pass(const float* deriv, const float* pre, float* target, int f,
   return dn_launch_status();
 }
 
-// ------------------------------------------------------------------ the backward products of up to eight columns
+// ------------------------------------------------------------------ the backward products of up to sixteen columns
 // Both are bound by the weights' bytes: their gradient mult x d^T (k rows, 2 f columns) is written, the inputs' gradient W d reads them.  One kernel
 // does both, so that reads and writes share the memory's time.  A wavefront has 256 rows, four a lane at any 4-byte boundary, and every fourth
 // unit of a slice of the 2 f; the derivatives d of the slice wait in LDS.  The four meet in LDS for W d, the slices' parts are added up by
 // k_few_finish.  2048 -> 4096 units, one column: 31.7 us in all (20.8 by the bytes), of which k_few_finish
 // is 3 and the pass over the halves 2; eight 34.6, 500 -> 500 of one 9.4.  In a kernel each: 34.7, 41.2, 13.6.  Eight units are on their way at once
-// (four: 39.1, 44.7, sixteen: 31.5, 36.3).
+// (four: 39.1, 44.7, sixteen: 31.5, 36.3), four from nine columns on: sixteen 39.1 (eight 48.1; the two products by k_gemm's kernels 51.9), twelve 36.5
+// (37.3; 51.5), 4096 -> 8192 of sixteen 140.6 (168.8; 154.9).
 #define FEW_ROWS 256
 #define FEW_SLICE 128
-#define FEW_AHEAD 8
+#define FEW_COLUMNS 16
 struct FewArgs {
   const float *W, *x, *d;
   float *dw, *dx, *partial, *bias_grad;
-  int k, units, slice, slices;
+  int n, k, units, slice, slices;       // n: columns (N may be one more: it counts as zeros)
   float beta, mult;
 };
 // DX: dx = W d.  DW: dw = mult x d^T, with ADD + beta dw.  The sums of d to bias_grad, where that is given, by the first block of rows.
@@ -208,7 +209,10 @@ __global__ void __launch_bounds__(256) k_few(FewArgs a) {
   __shared__ float ds[FEW_SLICE][N], part[DX ? 4 : 1][N][DX ? FEW_ROWS : 1];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j0 = blockIdx.y * a.slice, len = a.units - j0 < a.slice ? a.units - j0 : a.slice;
-  for (int i = threadIdx.x; i < len * N; i += 256) ds[i % len][i / len] = a.d[(size_t)(i / len) * a.units + j0 + i % len];
+  for (int i = threadIdx.x; i < len * N; i += 256) {
+    const int c = i / len, j = i - c * len;
+    ds[j][c] = c < a.n ? a.d[(size_t)c * a.units + j0 + j] : 0.f;
+  }
   __syncthreads();
   if (a.bias_grad && blockIdx.x == 0)
     for (int j = threadIdx.x; j < len; j += 256) {
@@ -223,10 +227,15 @@ __global__ void __launch_bounds__(256) k_few(FewArgs a) {
   float x[N][4], acc[N][4];
 #pragma unroll
   for (int c = 0; c < N; ++c) {
-    if (DW) col_load<false>(x[c], a.x + (size_t)c * a.k + row);
+    if (DW) {
+      col_load<false>(x[c], a.x + (size_t)(c < a.n ? c : a.n - 1) * a.k + row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[c][e] = c < a.n ? x[c][e] : 0.f;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[c][e] = 0.f;
   }
+  constexpr int AHEAD = N > 8 ? 4 : 8;
   const size_t at = (size_t)j0 * a.k + row;
   auto trip = [&](int j, auto units) __attribute__((always_inline)) {
     constexpr int U = decltype(units)::value;
@@ -263,7 +272,7 @@ __global__ void __launch_bounds__(256) k_few(FewArgs a) {
     }
   };
   int j = wv;
-  for (; j + 4 * (FEW_AHEAD - 1) < len; j += 4 * FEW_AHEAD) trip(j, std::integral_constant<int, FEW_AHEAD>());
+  for (; j + 4 * (AHEAD - 1) < len; j += 4 * AHEAD) trip(j, std::integral_constant<int, AHEAD>());
   for (; j < len; j += 4) trip(j, std::integral_constant<int, 1>());
   if (!DX) return;
 #pragma unroll
@@ -276,8 +285,9 @@ __global__ void __launch_bounds__(256) k_few(FewArgs a) {
   if (r < a.k)
 #pragma unroll
     for (int c = 0; c < N; ++c) {
+      if (c >= a.n) break;
       const float s = (part[0][c][threadIdx.x] + part[DX ? 1 : 0][c][threadIdx.x]) + (part[DX ? 2 : 0][c][threadIdx.x] + part[DX ? 3 : 0][c][threadIdx.x]);
-      (a.slices > 1 ? a.partial + ((size_t)blockIdx.y * N) * a.k : a.dx)[(size_t)c * a.k + r] = s;
+      (a.slices > 1 ? a.partial + (size_t)blockIdx.y * a.n * a.k : a.dx)[(size_t)c * a.k + r] = s;
     }
 }
 // dx: n outputs of `slices` partial results, 64 a workgroup, whose wavefronts take every fourth slice.
@@ -304,7 +314,7 @@ static int few_columns(FewArgs a) {
   while (a.slice > 32 && (long long)blocks * ((a.units + a.slice - 1) / a.slice) < 2 * cus) a.slice >>= 1;
   a.slices = (a.units + a.slice - 1) / a.slice;
   if (a.dx && a.slices > 1) {
-    a.partial = (float*)dn_scratch((size_t)a.slices * N * a.k * sizeof(float));
+    a.partial = (float*)dn_scratch((size_t)a.slices * a.n * a.k * sizeof(float));
     if (!a.partial) return CUDA_ERROR;
   }
   const dim3 grid((unsigned)blocks, (unsigned)a.slices);
@@ -316,7 +326,7 @@ static int few_columns(FewArgs a) {
   else if (a.bias_grad) FEW_GO(false, false, false);
 #undef FEW_GO
   if (a.dx && a.slices > 1) {
-    const long long n = (long long)N * a.k;
+    const long long n = (long long)a.n * a.k;
     hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, n, a.slices);
   }
   return dn_launch_status();
@@ -390,11 +400,11 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
   if (e) return e;
   const float *w = mat1->data_device, *x = mat2->data_device, *d = target->data_device;
   const bool wt = mat1->is_trans != 0, xt = mat2->is_trans != 0;
-  if (n >= 1 && n <= GATED_COLUMNS && wt && !xt && f > 0 && k >= 4 && 2 * f <= 65535 * 32) {
+  if (n >= 1 && n <= FEW_COLUMNS && wt && !xt && f > 0 && k >= 4 && 2 * f <= 65535 * 32) {
     const FewArgs a = {w, x, d, mat1_grad ? mat1_grad->data_device : nullptr, mat2_grad ? mat2_grad->data_device : nullptr, nullptr,
-                       bias_grad ? bias_grad->data_device : nullptr, k, 2 * f, 0, 1, beta, mult};
+                       bias_grad ? bias_grad->data_device : nullptr, n, k, 2 * f, 0, 1, beta, mult};
 #define FEW(N) case N: return few_columns<N>(a)
-    switch (n) { FEW(1); FEW(2); FEW(3); FEW(4); FEW(5); FEW(6); FEW(7); FEW(8); }
+    switch (n <= 8 ? n : (n + 1) / 2 * 2) { FEW(1); FEW(2); FEW(3); FEW(4); FEW(5); FEW(6); FEW(7); FEW(8); FEW(10); FEW(12); FEW(14); FEW(16); }
 #undef FEW
   }
   // The sums go with the weights' gradient where a kernel takes both, and the two products, which have nothing to do with each

@@ -307,7 +307,7 @@ def test_dot_gated_grad(cm, rng, d, f, n, act):
     check(db.asarray(), 0.5 - 2.0 * wdb, 2 * edb + 3 * U * (1 + 2 * np.abs(wdb)), 'scaled')
 
 
-@pytest.mark.parametrize("d,f,n", [(4, 3, 1), (5, 30, 8), (258, 130, 3), (1030, 700, 8), (2051, 100, 1), (300, 64, 64), (3, 9, 2)])
+@pytest.mark.parametrize("d,f,n", [(4, 3, 1), (5, 30, 8), (258, 130, 3), (1030, 700, 8), (2051, 100, 1), (300, 64, 64), (3, 9, 2), (7, 20, 9), (300, 260, 13), (1027, 130, 16)])
 def test_dot_gated_grad_of_one_operand_alone_and_accumulated(cm, rng, d, f, n):
     """Which gradients are asked for does not change them; all of them accumulated."""
     w, x, dy = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d)), F(rng.standard_normal((d, n))), F(rng.standard_normal((f, n)))

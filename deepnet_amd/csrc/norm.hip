@@ -239,7 +239,7 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
 // the deviations come from one round.  The gradients of gain and bias stay in the lanes that have their rows, for all columns of
 // the workgroup; its teams meet in LDS at the end, and a second kernel adds up the workgroups (a single one finishes by itself).  12 bytes an
 // entry: 4096 x 8192 72.8 us, 5.5 TB/s (copy rate: 62.4), of which the second kernel is 4.2; 1024 x 16384 38.9, 4098 x 4099 45.2 (31.2), 1024 x 4
-// 7.2 (two launches).  A workgroup's teams go in step from barrier to barrier, vector instructions issue in half of the cycles.
+// 5.1.  A workgroup's teams go in step from barrier to barrier, vector instructions issue in half of the cycles.
 struct NormGradArgs {
   const float *deriv, *mat, *gain;
   float *target, *partial, *gain_grad, *bias_grad;
@@ -489,10 +489,14 @@ static int norm_grad_launch(NormGradArgs a) {
   // teams of a workgroup: all that fit, or fewer where that leaves CUs without one; a workgroup a CU (two of half the teams: 4098 x 4099 45.2 ->
   // 51.4 us, 4096 x 8192 72.6 -> 76.2)
   int teams = 1024 / lanes;
-  while (teams > least && (a.w + teams - 1) / teams < cus) teams = (teams + 1) / 2 > least ? (teams + 1) / 2 : least;
+  // What one workgroup does in a trip (two, of teams within a wavefront) it does alone, without a launch for the sums (us, two launches / one: 1024 x 4
+  // 7.1 / 5.1, 1024 x 8 7.4 / 6.7, 256 x 16 7.1 / 4.3, 256 x 32 7.4 / 5.4, 64 x 64 7.3 / 4.2; two trips of larger teams 1024 x 16 7.5 / 8.7).
+  const bool sums = a.gain_grad || a.bias_grad, alone = sums && a.w <= (T ? 2 : 1) * teams;
+  if (alone && a.w < teams) teams = (a.w + least - 1) / least * least;       // (whole wavefronts)
+  while (!alone && teams > least && (a.w + teams - 1) / teams < cus) teams = (teams + 1) / 2 > least ? (teams + 1) / 2 : least;
   int blocks = (a.w + teams - 1) / teams;
+  if (alone) blocks = 1;
   if (blocks > cus) blocks = cus;
-  const bool sums = a.gain_grad || a.bias_grad;
   if (sums && blocks > 1) {
     a.partial = (float*)dn_scratch((size_t)blocks * 2 * a.h * sizeof(float));
     if (!a.partial) return CUDA_ERROR;

@@ -129,7 +129,7 @@ def grad_bounds(dy, x, gain):
     return dx, U * rows * (dya * (xa + 1)).sum(axis=1, keepdims=True), U * (w / 4 + 24) * dya.sum(axis=1, keepdims=True)
 
 
-@pytest.mark.parametrize("h,w", NORM_SHAPES + [(1, 70000), (2, 400), (3, 200001), (4, 30001), (1000, 700), (516, 2049), (4098, 130)])
+@pytest.mark.parametrize("h,w", NORM_SHAPES + [(64, 127), (33, 128), (64, 129), (256, 31), (200, 32), (200, 33), (1024, 8), (1024, 9), (700, 5), (1, 70000), (2, 400), (3, 200001), (4, 30001), (1000, 700), (516, 2049), (4098, 130)])
 @pytest.mark.parametrize("skip", [0, 1])
 def test_layer_norm_grad(cm, rng, h, w, skip):
     x, gain, _ = norm_inputs(rng, h, w)

@@ -15,7 +15,7 @@ bool dn_gemm_gated(bool a_trans, bool b_trans, int N, int K, const float* A, int
 // with cached loads 16.6 for 14.9, loads of whole trips behind no branch 15.8 for 15.3.
 struct GatedColumnsArgs {
   const float *A, *B;
-  int lda, ldb, K;
+  int lda, ldb, K, n;
   GatedOut out;
 };
 template <int N, int R, int U, bool SHARED>
@@ -24,6 +24,9 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), f = a.out.f;
   const int unit0 = (SHARED ? (int)blockIdx.x : (int)blockIdx.x * 4 + wv) * R, n4 = a.K >> 2;
   if (!SHARED && unit0 >= f) return;
+  // (columns of the group: the last one moves back and leaves the same results for those that it shares)
+  const int col0 = (int)(blockIdx.y + 1) * N <= a.n ? (int)blockIdx.y * N : a.n - N;
+  const float* B = a.B + (size_t)col0 * a.ldb;
   // (units beyond the last one repeat it and store nothing)
   const float* row[2 * R];
 #pragma unroll
@@ -51,7 +54,7 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
 #pragma unroll
       for (int c = 0; c < N; ++c) {
         x[u][c][0] = x[u][c][1] = x[u][c][2] = x[u][c][3] = 0.f;
-        if (j < n4) col_load<false>(x[u][c], a.B + (size_t)c * a.ldb + 4 * j);
+        if (j < n4) col_load<false>(x[u][c], B + (size_t)c * a.ldb + 4 * j);
       }
     }
 #pragma unroll
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
 #pragma unroll
     for (int r = 0; r < 2 * R; ++r)
 #pragma unroll
-      for (int c = 0; c < N; ++c) acc[r][c] = __fmaf_rn(row[r][k], a.B[(size_t)c * a.ldb + k], acc[r][c]);
+      for (int c = 0; c < N; ++c) acc[r][c] = __fmaf_rn(row[r][k], B[(size_t)c * a.ldb + k], acc[r][c]);
   }
 #pragma unroll
   for (int r = 0; r < 2 * R; ++r)
@@ -97,20 +100,22 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
       g = lane == r * N + c ? acc[2 * r][c] : g;
       u = lane == r * N + c ? acc[2 * r + 1][c] : u;
     }
-  if (lane < R * N && unit0 + lane / N < f) gated_out(a.out, unit0 + lane / N, lane % N, g, u);
+  if (lane < R * N && unit0 + lane / N < f) gated_out(a.out, unit0 + lane / N, col0 + lane % N, g, u);
 }
 
 #define GATED_COLUMNS 8
-static int gated_columns(int n, const GatedColumnsArgs& a) {
-  const int f = a.out.f;
-  // A workgroup's wavefronts share a unit's terms where there are fewer than eight wavefronts a CU by themselves (us, by themselves / shared: 2048 -> 512
-  // units 4.3 / 3.6, 500 -> 1000 of four columns 4.65 / 4.2), and where up to four columns have more than a thousand terms (4096 -> 8192 42.3 /
-  // 38.2, 2048 -> 5632 15.8 / 15.2, of three 18.6 / 16.8; 1001 -> 3000 5.9 / 6.9, 500 -> 3000 of four 5.9 / 6.7, 2048 -> 5632 of eight 22.6 / 26.9).
-  const bool shared = f < 8 * dn_num_cus() || (n <= 4 && a.K > 1024);
+// More than eight: in groups of as many, all in one grid.
+static int gated_columns(const GatedColumnsArgs& a) {
+  const int f = a.out.f, groups = (a.n + GATED_COLUMNS - 1) / GATED_COLUMNS, n = (a.n + groups - 1) / groups;
+  // A workgroup's wavefronts share a unit's terms, if there are more than one holds (200 -> 1500 units of eight columns 6.6 us shared, 4.8 not), where there
+  // are fewer than eight wavefronts a CU by themselves (us, by themselves / shared: 2048 -> 512 4.3 / 3.6, 500 -> 1000 of four 4.65 / 4.2), and
+  // where up to four columns have more than a thousand terms (4096 -> 8192 42.3 / 38.2, 2048 -> 5632 15.8 / 15.2, of three 18.6 / 16.8; 1001 ->
+  // 3000 5.9 / 6.9, 500 -> 3000 of four 5.9 / 6.7, 2048 -> 5632 of eight 22.6 / 26.9).
+  const bool shared = a.K > 256 && (f < 8 * dn_num_cus() || (n <= 4 && a.K > 1024));
 #define GATED_COLS(N, R, U)                                                                                                       \
   case N:                                                                                                                         \
-    if (shared) hipLaunchKernelGGL((k_gated_columns<N, R, U, true>), dim3((unsigned)((f + R - 1) / R)), dim3(256), 0, dn_stream(), a); \
-    else hipLaunchKernelGGL((k_gated_columns<N, R, U, false>), dim3((unsigned)((f + 4 * R - 1) / (4 * R))), dim3(256), 0, dn_stream(), a);  \
+    if (shared) hipLaunchKernelGGL((k_gated_columns<N, R, U, true>), dim3((unsigned)((f + R - 1) / R), (unsigned)groups), dim3(256), 0, dn_stream(), a); \
+    else hipLaunchKernelGGL((k_gated_columns<N, R, U, false>), dim3((unsigned)((f + 4 * R - 1) / (4 * R)), (unsigned)groups), dim3(256), 0, dn_stream(), a);  \
     break
   switch (n) {
     GATED_COLS(1, 1, 4);
@@ -360,10 +365,14 @@ int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cuda
   if (count <= 0) return 0;
   const bool ta = mat1->is_trans != 0, tb = mat2->is_trans != 0;
   const GatedOut out = {bias ? bias->data_device : nullptr, target->data_device, pre ? pre->data_device : nullptr, f, act};
-  if (n <= GATED_COLUMNS && ta && !tb && k > 0)
-    return gated_columns(n, GatedColumnsArgs{mat1->data_device, mat2->data_device, mat1->size[0], mat2->size[0], k, out});
+  const GatedColumnsArgs columns = {mat1->data_device, mat2->data_device, mat1->size[0], mat2->size[0], k, n, out};
+  if (n <= GATED_COLUMNS && ta && !tb && k > 0) return gated_columns(columns);
   int done = 0;
   if (n > 1 && dn_gemm_gated(ta, tb, n, k, mat1->data_device, mat1->size[0], mat2->data_device, mat2->size[0], out, &done)) return done;
+  // Up to two groups of such columns with few terms, which no tile fits, as long as the sums over the lanes take less than a second launch (us, two
+  // launches / so: 71 -> 160 units of 10 columns 7.9 / 3.9, 100 -> 1000 of 16 7.6 / 4.5, 64 -> 4096 of 9 8.4 / 5.4; 120 -> 4000 of 16 8.0 / 8.7, 64 -> 8000
+  // of 16 7.7 / 13.6).
+  if (n <= 2 * GATED_COLUMNS && ta && !tb && k > 0 && k < 128 && count <= 40000) return gated_columns(columns);
   // other products: the halves, then a pass over them
   cudamat both = *target;
   both.size[0] = 2 * f;

@@ -218,7 +218,8 @@ GATED_SHAPES = [(1, 1, 1), (1, 3, 2), (3, 1, 5), (5, 7, 1), (64, 64, 1), (65, 63
                 (500, 1000, 9), (256, 64, 16), (1001, 517, 1), (1000, 130, 17), (64, 512, 64), (333, 301, 65), (1024, 640, 33),
                 (200, 700, 300), (2048, 300, 5), (300, 700, 9), (1001, 33, 13), (260, 5000, 15), (129, 16, 11), (2049, 128, 2), (4100, 70, 1), (64, 128, 128), (40, 256, 384), (256, 1024, 512),
                 (1001, 1500, 300), (520, 1030, 777), (31, 2048, 1024), (512, 2050, 1030), (32, 32, 64), (33, 35, 67), (63, 100, 500), (70, 300, 40),
-                (64, 1000, 33), (130, 40, 31), (128, 17, 20), (1001, 257, 65)]
+                (64, 1000, 33), (130, 40, 31), (128, 17, 20), (1001, 257, 65), (71, 160, 10), (40, 33, 9),
+                (127, 64, 31), (5, 7, 13), (100, 1000, 20), (97, 2100, 25), (3, 2, 32)]
 
 
 @pytest.mark.parametrize("d,f,n", GATED_SHAPES)

@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(256) k_log_probs(LogProbArgs a) {
         for (int i = 0; i < tid >> 6; ++i) before += wave_like[i];
         if (place && before == a.k - 1) border_key |= place;
       } else {
-        standing(own > value ? 0xffffffffu : place, greater, reach);
+        // (places without their top bit, which is set in all of them: lanes above the border are above row 0's place too)
+        standing(own > value ? 0xffffffffu : place & 0x7fffffffu, greater, reach);
         if (!by_value && place && greater == a.k - 1) border_key |= place;
       }
       __syncthreads();

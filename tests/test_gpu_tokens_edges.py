@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from test_gpu_tokens import F, check_log_probs
 
 pytestmark = pytest.mark.gpu
 

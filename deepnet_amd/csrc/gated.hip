@@ -357,9 +357,10 @@ int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cuda
       (pre && (pre->size[0] != 2 * f || pre->size[1] != n)))
     return ERROR_INCOMPATIBLE_DIMENSIONS;
   if (int e = check_column(bias, 2 * f)) return e;
-  cudamat* in[4] = {mat1, mat2, bias, pre};
+  cudamat* in[3] = {mat1, mat2, bias};
   for (cudamat* m : in)
-    if (!apart(m, target) || (m != pre && !apart(m, pre))) return ERROR_UNSUPPORTED;
+    if (!apart(m, target) || !apart(m, pre)) return ERROR_UNSUPPORTED;       // (the same handle in two places too)
+  if (!apart(pre, target)) return ERROR_UNSUPPORTED;
   if (act < GATE_LINEAR || act > GATE_GELU) return ERROR_UNSUPPORTED;
   const long long count = (long long)f * n;
   if (count <= 0) return 0;

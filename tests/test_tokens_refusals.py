@@ -1,0 +1,33 @@
+"""What the operators on columns of tokens refuse, beside test_oracle_tokens.py: the same matrix in two places of a call.  Handles only, no
+memory is touched."""
+import ctypes as ct
+
+import pytest
+
+from test_oracle_tokens import UNSUPPORTED, Space, handle
+
+
+@pytest.fixture
+def lib():
+    from deepnet_amd import cudamat
+    return cudamat._cudamat
+
+
+@pytest.fixture
+def new():
+    from deepnet_amd import cudamat
+    return Space(cudamat)
+
+
+def test_dot_gated_keeps_its_halves_apart_from_what_it_reads(lib, new):
+    """pre where an operand of the same shape is: the very same handle, another one of its memory, a part of it."""
+    f = 6
+    at = lambda m: ct.addressof(m.contents.data_device.contents)
+    w, x, b, y = new(2 * f, 2 * f, trans=1), new(2 * f, 3), new(2 * f, 1), new(f, 3)
+    for pre in (x, handle(new.cm, 2 * f, 3, at(x)), handle(new.cm, 2 * f, 3, at(x) + 16), handle(new.cm, 2 * f, 3, at(w) + 64)):
+        assert lib.dot_gated(w, x, b, y, pre, 4) == UNSUPPORTED
+    # one column: the bias has the shape of pre too; weights of as many columns as cases
+    x, y = new(2 * f, 1), new(f, 1)
+    assert lib.dot_gated(w, x, b, y, b, 4) == UNSUPPORTED
+    w, x, y = new(2 * f, 2 * f), new(2 * f, 2 * f), new(f, 2 * f)
+    assert lib.dot_gated(w, x, b, y, w, 4) == UNSUPPORTED

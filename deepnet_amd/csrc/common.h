@@ -84,6 +84,10 @@ int dn_gemm_pair_sums(bool a_trans, bool b_trans, int M, int N, int K, float alp
                       const DnRowSumJob* jobs, int njobs);
 bool dn_capturing();
 
+// Most workgroups of 256 lanes that one launch takes (HIP launches fewer than 2^32 work items in a dimension).  Calls that need more are
+// queued as several launches.
+#define DN_MAX_GROUPS ((1ll << 24) - 1)
+
 // Records the launch status of the kernel just queued; returns CUDA_ERROR or 0.
 static inline int dn_launch_status() {
   return hipPeekAtLastError() == hipSuccess ? 0 : CUDA_ERROR;

@@ -635,35 +635,14 @@ static int check_shape(const cudamat* m, int rows, int cols) {
 #define LP_JOIN 512               // keys that the last workgroup of a column ranks
 #define DPTR(m) ((m) ? (m)->data_device : nullptr)
 
-extern "C" {
-
-int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cudamat* log_z, cudamat* top, cudamat* top_labels) {
-  const int h = mat->size[0], w = mat->size[1];
-  if (!mat->on_device) return ERROR_NOT_ON_DEVICE;
-  if (mat->is_trans) return ERROR_TRANSPOSED;
-  cudamat* row[4] = {labels, logp, entropy, log_z};
-  for (cudamat* m : row)
-    if (int e = check_shape(m, 1, w)) return e;
-  const int k = top ? top->size[0] : top_labels ? top_labels->size[0] : 0;
-  if (int e = check_shape(top, k, w)) return e;
-  if (int e = check_shape(top_labels, k, w)) return e;
-  if (k > h || (logp && !labels)) return ERROR_INCOMPATIBLE_DIMENSIONS;
-  if (k > LOG_PROBS_MAX_TOP || h > (1 << 24)) return ERROR_UNSUPPORTED;     // (whole numbers as floats)
-  cudamat* out[5] = {logp, entropy, log_z, top, top_labels};
-  for (int i = 0; i < 5; ++i) {
-    if (!apart(out[i], mat) || !apart(out[i], labels)) return ERROR_UNSUPPORTED;
-    for (int j = 0; j < i; ++j)
-      if (!apart(out[i], out[j])) return ERROR_UNSUPPORTED;
-  }
-  if (w <= 0) return 0;
-  LogProbArgs a = {mat->data_device, DPTR(labels), DPTR(logp), DPTR(entropy), DPTR(log_z), DPTR(top), DPTR(top_labels), h, w, k, 1, h, nullptr, nullptr, nullptr};
-  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
-  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
+// The columns of one launch.
+static int log_probs_launch(LogProbArgs a, bool stream) {
+  const int h = a.h, w = a.w, k = a.k;
   // Columns of up to 1024 rows by a wavefront each, and where there are enough of them for the chip those that are shorter than one trip of a
   // workgroup (us, workgroup / wavefront: 2050 x 8192 26.3 / 16.9, 1500 x 20000 50.8 / 21.2; 4096 x 8192 23.0 / 23.9, 3001 x 1100 6.7 / 7.3).
   // Up to 512 rows four columns a wavefront (us, one / four: 100 x 200000 67.8 / 22.3, 256 x 80000 30.3 / 15.2, 500 x 40000 20.0 / 15.7, 1024 x
   // 20000 15.5 / 19.9).
-  if (h >= 4 && w <= LP_WAVE_COLUMNS && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
+  if (h >= 4 && (h <= 1024 || (h < LP_SEGMENT && !k && w >= 8 * dn_num_cus()))) {
 #define LP_WAVE4(T, NV, TAIL, TOP, S) \
   hipLaunchKernelGGL((k_log_probs_wave<T, NV, TAIL, TOP, S>), dim3((unsigned)((w + 256 / T - 1) / (256 / T))), dim3(256), 0, dn_stream(), a)
 #define LP_WAVE3(T, NV, TOP, S) do { if (h % 4) LP_WAVE4(T, NV, true, TOP, S); else LP_WAVE4(T, NV, false, TOP, S); } while (0)
@@ -698,14 +677,47 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
     if (!a.keys || !a.arrived) return CUDA_ERROR;
     a.parts = (float*)(a.keys + parts * k);
   }
-  const long long blocks = (long long)w * segments;
-  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-#define LP_GO(TOP, S) hipLaunchKernelGGL((k_log_probs<TOP, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
+#define LP_GO(TOP, S) hipLaunchKernelGGL((k_log_probs<TOP, S>), dim3((unsigned)(w * segments)), dim3(256), 0, dn_stream(), a)
   if (k) { if (stream) LP_GO(true, true); else LP_GO(true, false); }
   else if (stream) LP_GO(false, true);
   else LP_GO(false, false);
 #undef LP_GO
   return dn_launch_status();
+}
+
+extern "C" {
+
+int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cudamat* log_z, cudamat* top, cudamat* top_labels) {
+  const int h = mat->size[0], w = mat->size[1];
+  if (!mat->on_device) return ERROR_NOT_ON_DEVICE;
+  if (mat->is_trans) return ERROR_TRANSPOSED;
+  cudamat* row[4] = {labels, logp, entropy, log_z};
+  for (cudamat* m : row)
+    if (int e = check_shape(m, 1, w)) return e;
+  const int k = top ? top->size[0] : top_labels ? top_labels->size[0] : 0;
+  if (int e = check_shape(top, k, w)) return e;
+  if (int e = check_shape(top_labels, k, w)) return e;
+  if (k > h || (logp && !labels)) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (k > LOG_PROBS_MAX_TOP || h > (1 << 24)) return ERROR_UNSUPPORTED;     // (whole numbers as floats)
+  cudamat* out[5] = {logp, entropy, log_z, top, top_labels};
+  for (int i = 0; i < 5; ++i) {
+    if (!apart(out[i], mat) || !apart(out[i], labels)) return ERROR_UNSUPPORTED;
+    for (int j = 0; j < i; ++j)
+      if (!apart(out[i], out[j])) return ERROR_UNSUPPORTED;
+  }
+  if (w <= 0) return 0;
+  // (at any alignment: 32003 x 2048 50.6 -> 46.9 us; 32768 x 2048 51.5 -> 45.4)
+  const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
+  // Columns of up to 1024 rows go four or sixteen to a workgroup, others one.  Even ranges, so that all take the same kernel.
+  const long long most = h >= 4 && h <= 1024 ? 4 * DN_MAX_GROUPS : DN_MAX_GROUPS, launches = (w + most - 1) / most, each = (w + launches - 1) / launches;
+  for (long long c0 = 0; c0 < w; c0 += each) {
+    const int n = (int)(w - c0 < each ? w - c0 : each);
+    auto from = [c0](float* p, int rows) { return p ? p + c0 * rows : nullptr; };
+    const LogProbArgs a = {mat->data_device + c0 * h, from(DPTR(labels), 1), from(DPTR(logp), 1), from(DPTR(entropy), 1), from(DPTR(log_z), 1),
+                           from(DPTR(top), k), from(DPTR(top_labels), k), h, n, k, 1, h, nullptr, nullptr, nullptr};
+    if (int e = log_probs_launch(a, stream)) return e;
+  }
+  return 0;
 }
 
 int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_weight, cudamat* entropy, cudamat* entropy_weight,

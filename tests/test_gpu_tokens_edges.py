@@ -33,3 +33,49 @@ def test_log_probs_of_a_mask_that_leaves_one_entry_fewer_than_asked_for(cm, h, w
         got = {name: m.asarray()[:, few] for name, m in out.items()}
         assert not np.isnan(out['top_labels'].asarray()).any(), (h, w, k)
         check_log_probs(x[:, few], labels[:, few], k, got)
+
+
+# ------------------------------------------------------------------ more columns than one launch takes
+
+def ends(mat, n):
+    """The first, and the last n columns, where a call of more than one launch joins, and those around the middle."""
+    w = mat.shape[1]
+    return [mat.slice(a, a + n).asarray().copy() for a in (0, (w - n) // 2, w - n)]
+
+
+def wide(cm, rng, h, w, n):
+    """h x w with random columns at the places of `ends`, and those (the rest is constant)."""
+    big = cm.empty((h, w))
+    big.assign(0.125)
+    parts = [F(rng.standard_normal((h, n))) for _ in range(3)]
+    for a, p in zip((0, (w - n) // 2, w - n), parts):
+        src = cm.CUDAMatrix(p)
+        big.slice(a, a + n).assign(src)
+        src.free_device_memory()
+    return big, parts
+
+
+def release(*mats):
+    for m in mats:
+        m.free_device_memory()
+
+
+@pytest.mark.parametrize("h,w,k", [(1, (1 << 24) + 5, 1), (2, (1 << 24) + 3, 0), (3, (1 << 25) + 7, 2), (4, (1 << 26) + 5, 1), (10, (1 << 26) + 5, 0)])
+def test_log_probs_of_more_columns_than_a_launch_takes(cm, rng, h, w, k):
+    n = 40
+    big, parts = wide(cm, rng, h, w, n)
+    labels = cm.empty((1, w))
+    labels.assign(float(h - 1))
+    out = {name: cm.empty((1, w)) for name in ('logp', 'entropy', 'log_z')}
+    if k:
+        out.update(top=cm.empty((k, w)), top_labels=cm.empty((k, w)))
+    for m in out.values():
+        m.assign(np.nan)
+    cm.log_probs(big, labels, **out)
+    got = {name: ends(m, n) for name, m in out.items()}
+    for i, p in enumerate(parts):
+        check_log_probs(p, F(np.full((1, n), h - 1)), k, {name: g[i] for name, g in got.items()})
+    # every column of the rest has the same result, and has been written
+    rest = out['log_z'].slice(n, (w - n) // 2).asarray()
+    assert (rest == rest[0, 0]).all() and abs(rest[0, 0] - (0.125 + np.log(h))) < 1e-6
+    release(big, labels, *out.values())

@@ -736,18 +736,23 @@ int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_
   if (h <= 0 || w <= 0) return 0;
   const bool wave = h <= 1024;
   const int pieces = wave ? 1 : (h + 4095) / 4096;
-  const LogProbGradArgs a = {mat->data_device, DPTR(labels), log_z->data_device, DPTR(logp_weight), DPTR(entropy), DPTR(entropy_weight),
-                             target->data_device, h, w, pieces, wave ? h : ((h + pieces - 1) / pieces + 3) / 4 * 4};
-  const long long blocks = wave ? (w + 3ll) / 4 : (long long)w * a.pieces;
-  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
   // (at any alignment: 32003 x 1000 51.7 -> 47.7 us)
   const bool stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
-#define LP_GRAD(T, S) hipLaunchKernelGGL((k_log_probs_grad<T, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a)
-  if (wave) { if (stream) LP_GRAD(64, true); else LP_GRAD(64, false); }
-  else if (stream) LP_GRAD(256, true);
-  else LP_GRAD(256, false);
+  const long long most = wave ? 4 * DN_MAX_GROUPS : DN_MAX_GROUPS / pieces;            // columns of one launch
+  for (long long c0 = 0; c0 < w; c0 += most) {
+    const int n = (int)(w - c0 < most ? w - c0 : most);
+    auto from = [c0](const cudamat* m) { return m ? m->data_device + c0 : nullptr; };
+    const LogProbGradArgs a = {mat->data_device + c0 * h, from(labels), from(log_z), from(logp_weight), from(entropy), from(entropy_weight),
+                               target->data_device + c0 * h, h, n, pieces, wave ? h : ((h + pieces - 1) / pieces + 3) / 4 * 4};
+    const unsigned blocks = wave ? (unsigned)((n + 3ll) / 4) : (unsigned)n * (unsigned)pieces;
+#define LP_GRAD(T, S) hipLaunchKernelGGL((k_log_probs_grad<T, S>), dim3(blocks), dim3(256), 0, dn_stream(), a)
+    if (wave) { if (stream) LP_GRAD(64, true); else LP_GRAD(64, false); }
+    else if (stream) LP_GRAD(256, true);
+    else LP_GRAD(256, false);
 #undef LP_GRAD
-  return dn_launch_status();
+    if (int e = dn_launch_status()) return e;
+  }
+  return 0;
 }
 
 }  // extern "C"

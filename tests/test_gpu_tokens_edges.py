@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from test_gpu_tokens import F, check_log_probs
+from oracle import token_oracle as tok
+from test_gpu_tokens import F, U, check, check_log_probs
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +80,26 @@ def test_log_probs_of_more_columns_than_a_launch_takes(cm, rng, h, w, k):
     rest = out['log_z'].slice(n, (w - n) // 2).asarray()
     assert (rest == rest[0, 0]).all() and abs(rest[0, 0] - (0.125 + np.log(h))) < 1e-6
     release(big, labels, *out.values())
+
+
+@pytest.mark.parametrize("h,w", [(1, (1 << 26) + 5), (7, (1 << 26) + 33), (1025, (1 << 24) + 9)])
+def test_log_probs_grad_of_more_columns_than_a_launch_takes(cm, rng, h, w):
+    """In place.  Bound: log p is off by 2 u |log p| (x - log_z, and what exp2 takes), p by that and 3 u of it; every product and sum adds u of
+    its terms, the entropy term has log p twice."""
+    n = 40
+    big, parts = wide(cm, rng, h, w, n)
+    rows = dict(labels=h - 1.0, log_z=1.0 + np.log(h), logp_weight=-0.75, entropy=0.5, entropy_weight=0.25)
+    M = {}
+    for name, v in rows.items():
+        M[name] = cm.empty((1, w))
+        M[name].assign(v)
+    cm.log_probs_grad(big, M['labels'], M['log_z'], M['logp_weight'], M['entropy'], M['entropy_weight'])
+    row = {name: np.full((1, n), np.float32(v)) for name, v in rows.items()}
+    for p, got in zip(parts, ends(big, n)):
+        want = tok.log_probs_grad(p, row['labels'], row['log_z'], row['logp_weight'], row['entropy'], row['entropy_weight'])
+        lp = p.astype(np.float64) - row['log_z']
+        perr = np.exp(lp) * (2 * np.abs(lp) + 3)
+        check(got, want, U * (0.75 * (perr + 2 + 2 * np.exp(lp)) + 0.25 * (perr * (np.abs(lp) + 0.5) + np.exp(lp) * (2 * np.abs(lp) + 1)) + 2 * np.abs(want)))
+    rest = big.slice(n, n + 1000).asarray()
+    assert (big.slice((w + n) // 2, (w + n) // 2 + 1000).asarray() == rest[:, :1]).all() and (rest != 0.125).all()
+    release(big, *M.values())

@@ -151,15 +151,20 @@ static int launch_ew(const float* a, const float* b, float* t, long long n, F f)
   const bool same_phase = (NIN < 1 || head_of(a) == ht) && (NIN < 2 || head_of(b) == ht) &&
                           ((reinterpret_cast<uintptr_t>(t) & 3u) == 0);
   if (same_phase) {
-    const int head = (int)(ht < n ? ht : n);
-    const long long n4 = (n - head) / 4;
-    long long blocks = (n4 + EW_THREADS - 1) / EW_THREADS;
-    if (blocks < 1) blocks = 1;
-    if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-    if (n >= DN_STREAM_MIN_ELEMS)
-      hipLaunchKernelGGL((k_ew<NIN, true, F>), dim3((unsigned)blocks), dim3(EW_THREADS), 0, dn_stream(), a, b, t, n, head, n4, f);
-    else
-      hipLaunchKernelGGL((k_ew<NIN, false, F>), dim3((unsigned)blocks), dim3(EW_THREADS), 0, dn_stream(), a, b, t, n, head, n4, f);
+    // (what a launch takes at once is whole groups of four, so each part begins at the phase of the first)
+    const long long part = 4ll * EW_THREADS * DN_MAX_GROUPS;
+    for (long long o = 0; o < n; o += part) {
+      const long long len = n - o < part ? n - o : part;
+      const float *ao = NIN >= 1 ? a + o : a, *bo = NIN >= 2 ? b + o : b;
+      const int head = (int)(ht < len ? ht : len);
+      const long long n4 = (len - head) / 4;
+      long long blocks = (n4 + EW_THREADS - 1) / EW_THREADS;
+      if (blocks < 1) blocks = 1;
+      if (n >= DN_STREAM_MIN_ELEMS)
+        hipLaunchKernelGGL((k_ew<NIN, true, F>), dim3((unsigned)blocks), dim3(EW_THREADS), 0, dn_stream(), ao, bo, t + o, len, head, n4, f);
+      else
+        hipLaunchKernelGGL((k_ew<NIN, false, F>), dim3((unsigned)blocks), dim3(EW_THREADS), 0, dn_stream(), ao, bo, t + o, len, head, n4, f);
+    }
   } else {
     long long blocks = (n + EW_THREADS - 1) / EW_THREADS;
     const long long cap = (long long)cus * 32;

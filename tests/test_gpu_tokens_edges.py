@@ -103,3 +103,17 @@ def test_log_probs_grad_of_more_columns_than_a_launch_takes(cm, rng, h, w):
     rest = big.slice(n, n + 1000).asarray()
     assert (big.slice((w + n) // 2, (w + n) // 2 + 1000).asarray() == rest[:, :1]).all() and (rest != 0.125).all()
     release(big, *M.values())
+
+
+def test_elementwise_calls_of_more_entries_than_a_launch_takes(cm):
+    """2^34 entries and some, four a lane: all of them are written."""
+    h, w = 1 << 17, (1 << 17) + 3
+    big = cm.empty((h, w))
+    big.assign(0.0)
+    big.assign(-1.5)
+    for c in (0, 1, w // 2, (1 << 17) - 1, 1 << 17, w - 1):
+        assert (big.slice(c, c + 1).asarray() == -1.5).all(), c
+    big.add(2.0)
+    for c in (0, 1, w // 2, (1 << 17) - 1, 1 << 17, w - 1):
+        assert (big.slice(c, c + 1).asarray() == 0.5).all(), c
+    release(big)

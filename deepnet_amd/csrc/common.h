@@ -88,8 +88,24 @@ bool dn_capturing();
 // queued as several launches.
 #define DN_MAX_GROUPS ((1ll << 24) - 1)
 
-// Records the launch status of the kernel just queued; returns CUDA_ERROR or 0.
+// Of a grid of 2^32 work items or more in a dimension the runtime launches a part and reports no error (assign_scalar of 1025 x 16777225 set the
+// first 16373 columns), so such launches are left out, and dn_launch_status() says so.
+extern bool g_dn_launch_left_out;
+static inline bool dn_launch_fits(dim3 grid, dim3 block) {
+  const uint64_t end = 1ull << 32;
+  if ((uint64_t)grid.x * block.x < end && (uint64_t)grid.y * block.y < end && (uint64_t)grid.z * block.z < end) return true;
+  g_dn_launch_left_out = true;
+  return false;
+}
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)                                        \
+  do {                                                                                                   \
+    if (dn_launch_fits(grid, block)) (kernel)<<<(grid), (block), (lds), (stream)>>>(__VA_ARGS__);        \
+  } while (0)
+
+// The launch status of the kernel just queued: 0, CUDA_ERROR, or ERROR_UNSUPPORTED where one was left out.
 static inline int dn_launch_status() {
+  if (g_dn_launch_left_out) { g_dn_launch_left_out = false; return ERROR_UNSUPPORTED; }
   return hipPeekAtLastError() == hipSuccess ? 0 : CUDA_ERROR;
 }
 

@@ -21,6 +21,8 @@ int dn_num_cus() {
   return g_num_cus;
 }
 
+bool g_dn_launch_left_out = false;
+
 // ------------------------------------------------------------------ launch stream and graph capture
 static hipStream_t g_stream = nullptr;     // nullptr: the NULL stream
 static bool g_capturing = false;

@@ -117,3 +117,16 @@ def test_elementwise_calls_of_more_entries_than_a_launch_takes(cm):
     for c in (0, 1, w // 2, (1 << 17) - 1, 1 << 17, w - 1):
         assert (big.slice(c, c + 1).asarray() == 0.5).all(), c
     release(big)
+
+
+def test_a_call_without_a_launch_is_an_error_and_the_next_one_is_none(cm):
+    """normlimit takes four columns a workgroup in one launch: 2^26 of them are refused and left as they are."""
+    wide_one, row = cm.empty((4, 1 << 26)), cm.empty((4, 1000))
+    wide_one.assign(3.0)
+    row.assign(3.0)
+    with pytest.raises(cm.CUDAMatException):
+        wide_one.norm_limit(1.0, axis=0)
+    assert (wide_one.slice(0, 1000).asarray() == 3.0).all() and (wide_one.slice((1 << 26) - 1000, 1 << 26).asarray() == 3.0).all()
+    row.norm_limit(1.0, axis=0)
+    assert np.allclose(row.asarray(), 0.5, rtol=1e-6)
+    release(wide_one, row)

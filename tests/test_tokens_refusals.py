@@ -31,3 +31,15 @@ def test_dot_gated_keeps_its_halves_apart_from_what_it_reads(lib, new):
     assert lib.dot_gated(w, x, b, y, b, 4) == UNSUPPORTED
     w, x, y = new(2 * f, 2 * f), new(2 * f, 2 * f), new(f, 2 * f)
     assert lib.dot_gated(w, x, b, y, w, 4) == UNSUPPORTED
+
+
+def test_a_grid_that_no_launch_takes_is_refused(lib, new):
+    """2^24 workgroups of 256 lanes: the calls that do not split such a grid say so, where a part of it would run."""
+    w = 1 << 26
+    x, y, row = new(4, w), new(4, w), new(1, w)
+    apart = handle(new.cm, 4, w, 1 << 40)
+    assert lib.normlimit_by_axis(x, apart, 0, ct.c_float(1.0)) == UNSUPPORTED
+    assert lib.max_by_axis(x, row, 0) == UNSUPPORTED
+    # (a copy between places of another alignment takes an entry a lane; its error is the reference's one for copies)
+    a, b = handle(new.cm, 1 << 16, 1 << 16, 1 << 40), handle(new.cm, 1 << 16, 1 << 16, (1 << 41) + 4)
+    assert lib.copy_on_device(a, b) != 0

@@ -17,12 +17,13 @@ struct GatedColumnsArgs {
   const float *A, *B;
   int lda, ldb, K, n;
   GatedOut out;
+  int first;                       // unit that the launch begins at
 };
 template <int N, int R, int U, bool SHARED>
 __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
   __shared__ float part[SHARED ? 4 : 1][2 * R * N];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), f = a.out.f;
-  const int unit0 = (SHARED ? (int)blockIdx.x : (int)blockIdx.x * 4 + wv) * R, n4 = a.K >> 2;
+  const int unit0 = a.first + (SHARED ? (int)blockIdx.x : (int)blockIdx.x * 4 + wv) * R, n4 = a.K >> 2;
   if (!SHARED && unit0 >= f) return;
   // (columns of the group: the last one moves back and leaves the same results for those that it shares)
   const int col0 = (int)(blockIdx.y + 1) * N <= a.n ? (int)blockIdx.y * N : a.n - N;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(256) k_gated_columns(GatedColumnsArgs a) {
 
 #define GATED_COLUMNS 8
 // More than eight: in groups of as many, all in one grid.
-static int gated_columns(const GatedColumnsArgs& a) {
+static int gated_columns(GatedColumnsArgs a) {
   const int f = a.out.f, groups = (a.n + GATED_COLUMNS - 1) / GATED_COLUMNS, n = (a.n + groups - 1) / groups;
   // A workgroup's wavefronts share a unit's terms, if there are more than one holds (200 -> 1500 units of eight columns 6.6 us shared, 4.8 not), where there
   // are fewer than eight wavefronts a CU by themselves (us, by themselves / shared: 2048 -> 512 4.3 / 3.6, 500 -> 1000 of four 4.65 / 4.2), and
@@ -115,7 +116,12 @@ static int gated_columns(const GatedColumnsArgs& a) {
 #define GATED_COLS(N, R, U)                                                                                                       \
   case N:                                                                                                                         \
     if (shared) hipLaunchKernelGGL((k_gated_columns<N, R, U, true>), dim3((unsigned)((f + R - 1) / R), (unsigned)groups), dim3(256), 0, dn_stream(), a); \
-    else hipLaunchKernelGGL((k_gated_columns<N, R, U, false>), dim3((unsigned)((f + 4 * R - 1) / (4 * R)), (unsigned)groups), dim3(256), 0, dn_stream(), a);  \
+    else                                                                                                                          \
+      for (long long i0 = 0; i0 < f; i0 += 4 * R * DN_MAX_GROUPS) {                                                               \
+        const long long units = f - i0 < 4 * R * DN_MAX_GROUPS ? f - i0 : 4 * R * DN_MAX_GROUPS;                                  \
+        a.first = (int)i0;                                                                                                        \
+        hipLaunchKernelGGL((k_gated_columns<N, R, U, false>), dim3((unsigned)((units + 4 * R - 1) / (4 * R)), (unsigned)groups), dim3(256), 0, dn_stream(), a); \
+      }                                                                                                                           \
     break
   switch (n) {
     GATED_COLS(1, 1, 4);
@@ -183,11 +189,15 @@ __global__ void __launch_bounds__(256) k_gate_pass(GatePass a) {
 template <bool GRAD>
 static int gate_pass(const float* deriv, const float* pre, float* target, int f, int w, int act) {
   const int pieces = (f + 255) / 256;
-  const GatePass a = {deriv, pre, target, f, w, act, pieces, ((f + pieces - 1) / pieces + 3) / 4 * 4};
-  const long long blocks = ((long long)w * pieces + 3) / 4;
-  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
-  if ((long long)f * w >= DN_STREAM_MIN_ELEMS) hipLaunchKernelGGL((k_gate_pass<GRAD, true>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
-  else hipLaunchKernelGGL((k_gate_pass<GRAD, false>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
+  const bool stream = (long long)f * w >= DN_STREAM_MIN_ELEMS;
+  const long long most = 4 * DN_MAX_GROUPS / pieces;         // columns of one launch
+  for (long long c0 = 0; c0 < w; c0 += most) {
+    const int n = (int)(w - c0 < most ? w - c0 : most);
+    const GatePass a = {GRAD ? deriv + c0 * f : nullptr, pre + 2 * c0 * f, target + (GRAD ? 2 : 1) * c0 * f, f, n, act, pieces, ((f + pieces - 1) / pieces + 3) / 4 * 4};
+    const unsigned blocks = (unsigned)(((long long)n * pieces + 3) / 4);
+    if (stream) hipLaunchKernelGGL((k_gate_pass<GRAD, true>), dim3(blocks), dim3(256), 0, dn_stream(), a);
+    else hipLaunchKernelGGL((k_gate_pass<GRAD, false>), dim3(blocks), dim3(256), 0, dn_stream(), a);
+  }
   return dn_launch_status();
 }
 
@@ -295,11 +305,11 @@ __global__ void __launch_bounds__(256) k_few(FewArgs a) {
       (a.slices > 1 ? a.partial + (size_t)blockIdx.y * a.n * a.k : a.dx)[(size_t)c * a.k + r] = s;
     }
 }
-// dx: n outputs of `slices` partial results, 64 a workgroup, whose wavefronts take every fourth slice.
-__global__ void __launch_bounds__(256) k_few_finish(const float* partial, float* dx, long long n, int slices) {
+// dx: n outputs of `slices` partial results, from `first` on, 64 a workgroup, whose wavefronts take every fourth slice.
+__global__ void __launch_bounds__(256) k_few_finish(const float* partial, float* dx, long long first, long long n, int slices) {
   __shared__ float red[4][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const long long i = (long long)blockIdx.x * 64 + lane;
+  const long long i = first + (long long)blockIdx.x * 64 + lane;
   float s = 0.f;
   if (i < n)
 #pragma unroll 8
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(256) k_few_finish(const float* partial, float*
   if (wv == 0 && i < n) dx[i] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
-// At least four rows; units of 65535 slices of 32 at most.
+// At least four rows and 2^30 at most (they are counted in 31 bits); units of 65535 slices of 32 at most.
 template <int N>
 static int few_columns(FewArgs a) {
   const int cus = dn_num_cus(), blocks = (a.k + FEW_ROWS - 1) / FEW_ROWS;
@@ -332,7 +342,10 @@ static int few_columns(FewArgs a) {
 #undef FEW_GO
   if (a.dx && a.slices > 1) {
     const long long n = (long long)a.n * a.k;
-    hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, n, a.slices);
+    for (long long i0 = 0; i0 < n; i0 += 64 * DN_MAX_GROUPS) {
+      const long long count = n - i0 < 64 * DN_MAX_GROUPS ? n - i0 : 64 * DN_MAX_GROUPS;
+      hipLaunchKernelGGL(k_few_finish, dim3((unsigned)((count + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)a.partial, a.dx, i0, n, a.slices);
+    }
   }
   return dn_launch_status();
 }
@@ -366,7 +379,7 @@ int dot_gated(cudamat* mat1, cudamat* mat2, cudamat* bias, cudamat* target, cuda
   if (count <= 0) return 0;
   const bool ta = mat1->is_trans != 0, tb = mat2->is_trans != 0;
   const GatedOut out = {bias ? bias->data_device : nullptr, target->data_device, pre ? pre->data_device : nullptr, f, act};
-  const GatedColumnsArgs columns = {mat1->data_device, mat2->data_device, mat1->size[0], mat2->size[0], k, n, out};
+  const GatedColumnsArgs columns = {mat1->data_device, mat2->data_device, mat1->size[0], mat2->size[0], k, n, out, 0};
   if (n <= GATED_COLUMNS && ta && !tb && k > 0) return gated_columns(columns);
   int done = 0;
   if (n > 1 && dn_gemm_gated(ta, tb, n, k, mat1->data_device, mat1->size[0], mat2->data_device, mat2->size[0], out, &done)) return done;
@@ -410,7 +423,7 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
   if (e) return e;
   const float *w = mat1->data_device, *x = mat2->data_device, *d = target->data_device;
   const bool wt = mat1->is_trans != 0, xt = mat2->is_trans != 0;
-  if (n >= 1 && n <= FEW_COLUMNS && wt && !xt && f > 0 && k >= 4 && 2 * f <= 65535 * 32) {
+  if (n >= 1 && n <= FEW_COLUMNS && wt && !xt && f > 0 && k >= 4 && k <= 1 << 30 && 2 * f <= 65535 * 32) {
     const FewArgs a = {w, x, d, mat1_grad ? mat1_grad->data_device : nullptr, mat2_grad ? mat2_grad->data_device : nullptr, nullptr,
                        bias_grad ? bias_grad->data_device : nullptr, n, k, 2 * f, 0, 1, beta, mult};
 #define FEW(N) case N: return few_columns<N>(a)

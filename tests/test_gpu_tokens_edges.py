@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from oracle import token_oracle as tok
-from test_gpu_tokens import F, U, check, check_log_probs
+from test_gpu_tokens import F, U, act_bounds, check, check_log_probs
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,40 @@ def test_a_call_without_a_launch_is_an_error_and_the_next_one_is_none(cm):
     row.norm_limit(1.0, axis=0)
     assert np.allclose(row.asarray(), 0.5, rtol=1e-6)
     release(wide_one, row)
+
+
+@pytest.mark.parametrize("f,w,acts", [(1, (1 << 26) + 5, ('silu',)), (3, (1 << 26) + 7, ('relu',))])
+def test_the_halves_of_more_columns_than_a_launch_takes(cm, rng, f, w, acts):
+    """The pass over the halves, backward, in the place of pre."""
+    n = 40
+    for act in acts:
+        dy, dys = wide(cm, rng, f, w, n)
+        pre, pres = wide(cm, rng, 2 * f, w, n)
+        m1, m2 = cm.empty((2 * f, 1)), cm.empty((1, w))                     # (their values are not read: no gradient of theirs is asked for)
+        assert cm.dot_gated_grad(dy, m1, m2, pre, act=act) is pre
+        for d, p, got in zip(dys, pres, ends(pre, n)):
+            want = tok.gate_grad(d, p, act)
+            ve, se = act_bounds(act, p[:f].astype(np.float64), 0.0)
+            ad, au = np.abs(d.astype(np.float64)), np.abs(p[f:].astype(np.float64))
+            check(got, want, np.vstack([ad * au * se, ad * ve]) + 4 * U * np.abs(want))
+        rest = pre.slice(n, n + 500).asarray()
+        assert (pre.slice((w + n) // 2, (w + n) // 2 + 500).asarray() == rest[:, :1]).all() and (rest != 0.125).all()
+        release(dy, pre, m1, m2)
+
+
+def test_dot_gated_of_more_units_than_a_launch_takes(cm, rng):
+    """One column and one term: products of two numbers."""
+    f, n = (1 << 26) + 5, 40
+    w, parts = wide(cm, rng, 1, 2 * f, n)
+    gate, up = w.slice(0, n).asarray().copy(), w.slice(2 * f - n, 2 * f).asarray().copy()
+    x, y = cm.CUDAMatrix(F([[1.5]])), cm.empty((f, 1))
+    y.assign(np.nan)
+    cm.dot_gated(w.T, x, target=y, act='relu')
+    y.reshape((1, f))
+    at = w.slice(f, f + n).asarray().astype(np.float64)
+    got, last = y.slice(0, n).asarray(), y.slice(f - n, f).asarray()
+    check(got, np.maximum(1.5 * gate, 0) * 1.5 * at, 4 * U * np.abs(2.25 * gate * at))
+    g = 1.5 * w.slice(f - n, f).asarray().astype(np.float64)
+    check(last, np.maximum(g, 0) * 1.5 * up, 4 * U * np.abs(g * 1.5 * up))
+    assert not np.isnan(y.asarray()).any()
+    release(w, x, y)

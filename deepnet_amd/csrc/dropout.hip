@@ -18,16 +18,16 @@ __device__ __forceinline__ void philox10(uint32_t (&c)[4], PhiloxKey k) {
 }
 
 // Entry i of the matrix (column-major) is dropped when word i % 4 of counter (i / 4, i / 4 >> 32, bits of the step,
-// stream) is below border.  target may be mat or residual.  A lane has one counter and its four entries, 16 bytes at any 4-byte
+// stream) is below border; a launch begins at counter `first`.  target may be mat or residual.  A lane has one counter and its four entries, 16 bytes at any 4-byte
 // boundary that are on their way while the generator runs.  Bound by the bytes: 4096 x 8192 onto a residual 62.4 us, 6.46 TB/s, what a
 // copy reaches; 42.3 us without, 4097 x 4097 32.1.  Two, four, eight counters a lane: 64.0, 66.9, 68.7 us.  The generator is hidden: with
 // seven of its rounds instead of ten, four counters a lane take 66.4.
 struct __attribute__((packed, aligned(4))) DropGroup { float x, y, z, w; };
 template <bool RES, bool STREAM>
 __global__ void __launch_bounds__(256)
-k_counter_dropout(const float* mat, const float* residual, float* target, const float* step, long long n, uint64_t border, float mult,
-                  uint32_t stream, PhiloxKey key) {
-  const long long g = (long long)blockIdx.x * 256 + threadIdx.x, whole = n >> 2;
+k_counter_dropout(const float* mat, const float* residual, float* target, const float* step, long long first, long long n, uint64_t border,
+                  float mult, uint32_t stream, PhiloxKey key) {
+  const long long g = first + (long long)blockIdx.x * 256 + threadIdx.x, whole = n >> 2;
   if (4 * g >= n) return;
   auto load = [](float (&v)[4], const float* p) __attribute__((always_inline)) {
     if (STREAM) { const float4 q = dn_ld4<true>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
@@ -71,16 +71,19 @@ extern "C" int counter_dropout(cudamat* mat, cudamat* residual, cudamat* target,
     return ERROR_UNSUPPORTED;
   const long long n = dn_len(mat);
   if (n <= 0) return 0;
-  const long long blocks = ((n + 3) / 4 + 255) / 256;
-  if (blocks > 0x7fffffffll) return ERROR_UNSUPPORTED;
   const float *x = mat->data_device, *r = residual ? residual->data_device : nullptr, *s = step ? step->data_device : nullptr;
   float* t = target->data_device;
   const bool wide = n >= DN_STREAM_MIN_ELEMS && dn_aligned16(x) && dn_aligned16(t) && dn_aligned16(r);
   const uint64_t border = (uint64_t)((double)dropprob * 4294967296.0);
-#define DROP_GO(R, S) hipLaunchKernelGGL((k_counter_dropout<R, S>), dim3((unsigned)blocks), dim3(256), 0, dn_stream(), x, r, t, s, n, border, mult, stream, PhiloxKey{seed_lo, seed_hi})
-  if (r) { if (wide) DROP_GO(true, true); else DROP_GO(true, false); }
-  else if (wide) DROP_GO(false, true);
-  else DROP_GO(false, false);
+  const long long counters = (n + 3) / 4;
+  for (long long first = 0; first < counters; first += 256 * DN_MAX_GROUPS) {
+    const long long blocks = (counters - first + 255) / 256;
+    const dim3 grid((unsigned)(blocks < DN_MAX_GROUPS ? blocks : DN_MAX_GROUPS));
+#define DROP_GO(R, S) hipLaunchKernelGGL((k_counter_dropout<R, S>), grid, dim3(256), 0, dn_stream(), x, r, t, s, first, n, border, mult, stream, PhiloxKey{seed_lo, seed_hi})
+    if (r) { if (wide) DROP_GO(true, true); else DROP_GO(true, false); }
+    else if (wide) DROP_GO(false, true);
+    else DROP_GO(false, false);
+  }
 #undef DROP_GO
   return dn_launch_status();
 }

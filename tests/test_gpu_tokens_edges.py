@@ -167,3 +167,17 @@ def test_dot_gated_of_more_units_than_a_launch_takes(cm, rng):
     check(last, np.maximum(g, 0) * 1.5 * up, 4 * U * np.abs(g * 1.5 * up))
     assert not np.isnan(y.asarray()).any()
     release(w, x, y)
+
+
+def test_counter_dropout_of_more_entries_than_a_launch_takes(cm, rng):
+    """2^34 entries and some, in place: counters go on past 2^32."""
+    h, w, n = 1 << 17, (1 << 17) + 3, 2
+    big, parts = wide(cm, rng, h, w, n)
+    cm.counter_dropout(big, 0.25, 77, stream=5, mult=2.0)
+    for a, p, got in zip((0, (w - n) // 2, w - n), parts, ends(big, n)):
+        keep = tok.dropout_keep((h, n), 0.25, 77, stream=5, first=h * a, count=h * n).reshape((h, n), order='F')
+        assert np.array_equal(got, np.where(keep, 2 * p, np.float32(0))), a
+    for c in ((1 << 17) - 2, (1 << 17) - 1, 1 << 17):                   # (where the second launch begins)
+        keep = tok.dropout_keep((h, 1), 0.25, 77, stream=5, first=h * c, count=h).reshape((h, 1))
+        assert np.array_equal(big.slice(c, c + 1).asarray(), np.where(keep, np.float32(0.25), np.float32(0))) or c >= w - n, c
+    release(big)

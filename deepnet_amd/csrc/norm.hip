@@ -20,7 +20,7 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float (*red)[4]) {
 
 // ------------------------------------------------------------------ columns that no team holds
 // A workgroup a column, three passes over it (the later ones from the caches): more than 16384 rows, where a lane would have to hold more than
-// 16, and more than 2^29 columns.  20000 x 1000 106 us (1.5 TB/s), its gradients 257: waits for each pass's loads and its meeting.
+// 16.  20000 x 1000 106 us (1.5 TB/s), its gradients 257: waits for each pass's loads and its meeting.
 // The mean as a pair m + d (m the rounded sum's, d what the deviations from m still sum to) and 1 / sqrt(variance + eps):
 // deviations are taken from m, so that a mean far from zero costs no digits of the variance.
 struct NormStats { float m, d, r; };
@@ -466,7 +466,10 @@ __global__ void __launch_bounds__(256) k_layer_norm_grad_short(NormGradArgs a) {
 }
 
 #define NORM_COLS_MAX 16384       // tallest columns that a team holds
-#define NORM_COLS_W (1 << 29)     // most of them (they are counted in 31 bits)
+#define NORM_COLS_W (1 << 29)     // most of them in a launch (they are counted in 31 bits)
+#define NORM_ROWS_MAX ((1 << 30) - 1)
+// Columns of one launch; those of up to three rows are counted in 64 bits.
+static inline long long norm_launch_columns(int h) { return h < 4 ? 0x7fffffffll : h <= NORM_COLS_MAX ? NORM_COLS_W : DN_MAX_GROUPS; }
 
 // waves: of the workgroup, where that is a team
 template <int T, int NV>
@@ -541,20 +544,9 @@ static int check_vector(const cudamat* v, int h) {
   return v->size[0] == h && v->size[1] == 1 ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
 
-extern "C" {
-
-int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, float eps) {
-  const int h = mat->size[0], w = mat->size[1];
-  if (!mat->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
-  if (mat->is_trans || target->is_trans) return ERROR_TRANSPOSED;
-  if (target->size[0] != h || target->size[1] != w) return ERROR_INCOMPATIBLE_DIMENSIONS;
-  if (int e = check_vector(gain, h)) return e;
-  if (int e = check_vector(bias, h)) return e;
-  if (!(eps >= 0.f) || !same_or_apart(mat, target) || !apart(gain, target) || !apart(bias, target)) return ERROR_UNSUPPORTED;
-  if (h <= 0 || w <= 0) return 0;
-  if (h >= 4 && h <= NORM_COLS_MAX && w <= NORM_COLS_W) {
-    const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
-    float* t = target->data_device;
+// What one launch takes of the columns.
+static int norm_columns(const float* x, const float* g, const float* b, float* t, int h, int w, float eps) {
+  if (h >= 4 && h <= NORM_COLS_MAX) {
     // Teams of 16 lanes up to 64 rows, a wavefront up to 1024 (us, against the next larger team: 64 x 100000 11.0 / 23.9, 60 x 300 3.3 / 4.2, 700 x
     // 20000 22.3 / 24.0, 1024 x 16384 24.1 / 24.4; gradients 64 x 100000 19.1 / 38.3).
     if (h <= 64) norm_launch<16, 1>(x, g, b, t, h, w, eps);
@@ -570,36 +562,18 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, floa
   if (h < 4) {
     const long long groups = (w + 255ll) / 256, most = 8 * dn_num_cus();
     const dim3 grid((unsigned)(groups < most ? groups : most));
-    const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
-    float* t = target->data_device;
     if (h == 1) hipLaunchKernelGGL(k_layer_norm_short<1>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
     else if (h == 2) hipLaunchKernelGGL(k_layer_norm_short<2>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
     else hipLaunchKernelGGL(k_layer_norm_short<3>, grid, dim3(256), 0, dn_stream(), x, g, b, t, w, eps);
     return dn_launch_status();
   }
-  hipLaunchKernelGGL(k_layer_norm, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)mat->data_device,
-                     (const float*)(gain ? gain->data_device : nullptr), (const float*)(bias ? bias->data_device : nullptr), target->data_device, h, eps);
+  hipLaunchKernelGGL(k_layer_norm, dim3((unsigned)w), dim3(256), 0, dn_stream(), x, g, b, t, h, eps);
   return dn_launch_status();
 }
 
-int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target, cudamat* gain_grad, cudamat* bias_grad, float eps,
-                    float beta, float mult) {
-  const int h = mat->size[0], w = mat->size[1];
-  if (!deriv->on_device || !mat->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
-  if (deriv->is_trans || mat->is_trans || target->is_trans) return ERROR_TRANSPOSED;
-  if (deriv->size[0] != h || deriv->size[1] != w || target->size[0] != h || target->size[1] != w) return ERROR_INCOMPATIBLE_DIMENSIONS;
-  cudamat* vec[3] = {gain, gain_grad, bias_grad};
-  for (cudamat* v : vec)
-    if (int e = check_vector(v, h)) return e;
-  if (!(eps >= 0.f) || !same_or_apart(deriv, target) || !same_or_apart(mat, target) || !apart(gain, target)) return ERROR_UNSUPPORTED;
-  cudamat* in[4] = {deriv, mat, gain, target};
-  for (cudamat* m : in)
-    if (!apart(m, gain_grad) || !apart(m, bias_grad)) return ERROR_UNSUPPORTED;
-  if (!apart(gain_grad, bias_grad)) return ERROR_UNSUPPORTED;
-  if (h <= 0) return 0;
-  if (w > 0 && (h < 4 || (h <= NORM_COLS_MAX && w <= NORM_COLS_W))) {
-    NormGradArgs a = {deriv->data_device, mat->data_device, gain ? gain->data_device : nullptr, target->data_device, nullptr,
-                            gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, 0, eps, beta, mult};
+static int norm_grad_columns(NormGradArgs a) {
+  const int h = a.h, w = a.w;
+  if (w > 0 && h <= NORM_COLS_MAX) {
     if (h == 1) return norm_grad_short<1>(a);
     if (h == 2) return norm_grad_short<2>(a);
     if (h == 3) return norm_grad_short<3>(a);
@@ -621,18 +595,60 @@ int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target
   }
   float* stats = (float*)dn_scratch((size_t)(w > 0 ? w : 1) * 5 * sizeof(float));
   if (!stats) return CUDA_ERROR;
-  const float* gp = gain ? gain->data_device : nullptr;
-  if (w > 0)
-    hipLaunchKernelGGL(k_layer_norm_grad_stats, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)deriv->data_device,
-                       (const float*)mat->data_device, gp, stats, h, eps);
-  if (gain_grad || bias_grad)
-    hipLaunchKernelGGL(k_layer_norm_grad_rows, dim3((unsigned)((h + 63) / 64)), dim3(256), 0, dn_stream(), (const float*)deriv->data_device,
-                       (const float*)mat->data_device, (const float*)stats, gain_grad ? gain_grad->data_device : nullptr,
-                       bias_grad ? bias_grad->data_device : nullptr, h, w, beta, mult);
-  if (w > 0)
-    hipLaunchKernelGGL(k_layer_norm_grad_inputs, dim3((unsigned)w), dim3(256), 0, dn_stream(), (const float*)deriv->data_device,
-                       (const float*)mat->data_device, gp, (const float*)stats, target->data_device, h);
+  if (w > 0) hipLaunchKernelGGL(k_layer_norm_grad_stats, dim3((unsigned)w), dim3(256), 0, dn_stream(), a.deriv, a.mat, a.gain, stats, h, a.eps);
+  if (a.gain_grad || a.bias_grad)
+    hipLaunchKernelGGL(k_layer_norm_grad_rows, dim3((unsigned)((h + 63) / 64)), dim3(256), 0, dn_stream(), a.deriv, a.mat, (const float*)stats, a.gain_grad,
+                       a.bias_grad, h, w, a.beta, a.mult);
+  if (w > 0) hipLaunchKernelGGL(k_layer_norm_grad_inputs, dim3((unsigned)w), dim3(256), 0, dn_stream(), a.deriv, a.mat, a.gain, (const float*)stats, a.target, h);
   return dn_launch_status();
+}
+
+extern "C" {
+
+int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, float eps) {
+  const int h = mat->size[0], w = mat->size[1];
+  if (!mat->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
+  if (mat->is_trans || target->is_trans) return ERROR_TRANSPOSED;
+  if (target->size[0] != h || target->size[1] != w) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (int e = check_vector(gain, h)) return e;
+  if (int e = check_vector(bias, h)) return e;
+  if (!(eps >= 0.f) || !same_or_apart(mat, target) || !apart(gain, target) || !apart(bias, target)) return ERROR_UNSUPPORTED;
+  if (h > NORM_ROWS_MAX) return ERROR_UNSUPPORTED;         // (rows are counted in 31 bits, 256 at a time)
+  if (h <= 0 || w <= 0) return 0;
+  const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
+  const long long most = norm_launch_columns(h);
+  for (long long c0 = 0; c0 < w; c0 += most)
+    if (int e = norm_columns(x + c0 * h, g, b, target->data_device + c0 * h, h, (int)(w - c0 < most ? w - c0 : most), eps)) return e;
+  return 0;
+}
+
+int layer_norm_grad(cudamat* deriv, cudamat* mat, cudamat* gain, cudamat* target, cudamat* gain_grad, cudamat* bias_grad, float eps,
+                    float beta, float mult) {
+  const int h = mat->size[0], w = mat->size[1];
+  if (!deriv->on_device || !mat->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
+  if (deriv->is_trans || mat->is_trans || target->is_trans) return ERROR_TRANSPOSED;
+  if (deriv->size[0] != h || deriv->size[1] != w || target->size[0] != h || target->size[1] != w) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  cudamat* vec[3] = {gain, gain_grad, bias_grad};
+  for (cudamat* v : vec)
+    if (int e = check_vector(v, h)) return e;
+  if (!(eps >= 0.f) || !same_or_apart(deriv, target) || !same_or_apart(mat, target) || !apart(gain, target)) return ERROR_UNSUPPORTED;
+  cudamat* in[4] = {deriv, mat, gain, target};
+  for (cudamat* m : in)
+    if (!apart(m, gain_grad) || !apart(m, bias_grad)) return ERROR_UNSUPPORTED;
+  if (!apart(gain_grad, bias_grad)) return ERROR_UNSUPPORTED;
+  if (h > NORM_ROWS_MAX) return ERROR_UNSUPPORTED;
+  if (h <= 0) return 0;
+  NormGradArgs a = {deriv->data_device, mat->data_device, gain ? gain->data_device : nullptr, target->data_device, nullptr,
+                    gain_grad ? gain_grad->data_device : nullptr, bias_grad ? bias_grad->data_device : nullptr, h, w, 0, eps, beta, mult};
+  const long long most = norm_launch_columns(h);
+  for (long long c0 = 0;;) {
+    a.w = (int)(w - c0 < most ? w - c0 : most);
+    if (int e = norm_grad_columns(a)) return e;
+    c0 += most;
+    if (c0 >= w) return 0;
+    a.deriv += most * h; a.mat += most * h; a.target += most * h;
+    a.beta = 1.f;                                          // (the gradients of gain and bias go on from what these columns left)
+  }
 }
 
 }  // extern "C"

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from oracle import token_oracle as tok
-from test_gpu_tokens import F, U, act_bounds, check, check_log_probs
+from test_gpu_tokens import F, U, act_bounds, check, check_log_probs, grad_bounds, norm_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,35 @@ def test_counter_dropout_of_more_entries_than_a_launch_takes(cm, rng):
         keep = tok.dropout_keep((h, 1), 0.25, 77, stream=5, first=h * c, count=h).reshape((h, 1))
         assert np.array_equal(big.slice(c, c + 1).asarray(), np.where(keep, np.float32(0.25), np.float32(0))) or c >= w - n, c
     release(big)
+
+
+@pytest.mark.parametrize("h", [3, 4])
+def test_layer_norm_of_more_columns_than_a_launch_takes(cm, rng, h):
+    """2^29 columns and some, forward and backward in place; constant columns give the bias, and add nothing to the gain's gradient."""
+    w, n = (1 << 29) + 37, 40
+    big, parts = wide(cm, rng, h, w, n)
+    gain, bias = F(1 + 0.3 * rng.standard_normal((h, 1))), F(rng.standard_normal((h, 1)))
+    G, B = cm.CUDAMatrix(gain), cm.CUDAMatrix(bias)
+    cm.layer_norm(big, G, B)
+    for p, got in zip(parts, ends(big, n)):
+        want = tok.layer_norm(p, gain, bias)
+        check(got, want, norm_bound(p, gain, want))
+    for c in (n, (1 << 29) - 500, w // 2 + n):
+        assert (big.slice(c, c + 400).asarray() == bias).all(), c
+    release(big)
+    x, xs = wide(cm, rng, h, w, n)
+    dy, dys = wide(cm, rng, h, w, n)
+    gg, gb = cm.empty((h, 1)), cm.empty((h, 1))
+    gg.assign(2.0)
+    gb.assign(2.0)
+    cm.layer_norm_grad(dy, x, G, gain_grad=gg, bias_grad=gb, mult=0.5, beta=3.0)
+    wg, wb, eg, eb = 6.0, 6.0 + 0.5 * 0.125 * (w - 3 * n), 0.0, 0.125 * (w - 3 * n)
+    for p, d, got in zip(xs, dys, ends(dy, n)):
+        dx, dg, db = tok.layer_norm_grad(d, p, gain)
+        ex, e1, e2 = grad_bounds(d, p, gain)
+        check(got, dx, ex)
+        wg, wb, eg, eb = wg + 0.5 * dg, wb + 0.5 * db, eg + e1, eb + np.abs(d.astype(np.float64)).sum(axis=1, keepdims=True)
+    # (a lane adds up every 16384th column or fewer)
+    check(gg.asarray(), wg, 0.5 * eg + 4 * U * (np.abs(wg) + 6))
+    check(gb.asarray(), wb, U * (w / 16384 + 100) * 0.5 * eb + 4 * U * (np.abs(wb) + 6))
+    release(x, dy, gg, gb, G, B)

@@ -43,3 +43,10 @@ def test_a_grid_that_no_launch_takes_is_refused(lib, new):
     # (a copy between places of another alignment takes an entry a lane; its error is the reference's one for copies)
     a, b = handle(new.cm, 1 << 16, 1 << 16, 1 << 40), handle(new.cm, 1 << 16, 1 << 16, (1 << 41) + 4)
     assert lib.copy_on_device(a, b) != 0
+
+
+def test_layer_norm_of_columns_that_it_cannot_count_is_refused(lib, new):
+    h = 1 << 30
+    x, y, dy = (handle(new.cm, h, 1, (i + 1) << 40) for i in range(3))
+    assert lib.layer_norm(x, None, None, y, 1e-5) == UNSUPPORTED
+    assert lib.layer_norm_grad(dy, x, None, y, None, None, 1e-5, 0.0, 1.0) == UNSUPPORTED

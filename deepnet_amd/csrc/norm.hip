@@ -3,8 +3,9 @@
 #include <math.h>
 
 // Sums over the 256 lanes of a workgroup; every lane gets them.  `red` is free again after the next barrier.
-template <int N>
-__device__ __forceinline__ void block_sums(float (&v)[N], float (*red)[4]) {
+__device__ __forceinline__ double wave_sum(double v) { return wave_sum_d(v); }
+template <int N, typename V>
+__device__ __forceinline__ void block_sums(V (&v)[N], V (*red)[4]) {
   const int wv = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
@@ -21,15 +22,18 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float (*red)[4]) {
 // ------------------------------------------------------------------ columns that no team holds
 // A workgroup a column, three passes over it (the later ones from the caches): more than 16384 rows, where a lane would have to hold more than
 // 16.  20000 x 1000 106 us (1.5 TB/s), its gradients 257: waits for each pass's loads and its meeting.
-// The mean as a pair m + d (m the rounded sum's, d what the deviations from m still sum to) and 1 / sqrt(variance + eps):
-// deviations are taken from m, so that a mean far from zero costs no digits of the variance.
+// The mean as a pair m + d (m rounded to fp32, d what the deviations from m still sum to) and 1 / sqrt(variance + eps):
+// deviations are taken from m, so that a mean far from zero costs no digits of the variance.  That takes an m that is off by its own rounding only:
+// a lane adds up h / 256 entries, and in 32 bits m was off by so much (1000003 equal entries of 98765.4: by 2.8) that d^2 outweighed
+// the variance and what was left of it could be below zero.
 struct NormStats { float m, d, r; };
 __device__ __forceinline__ NormStats norm_stats(const float* c, int h, float eps, float (*red)[4]) {
+  __shared__ double sums[1][4];
   NormStats s;
-  float one[1] = {0.f};
-  for (int i = threadIdx.x; i < h; i += 256) one[0] += c[i];
-  block_sums(one, red);
-  s.m = one[0] / (float)h;
+  double one[1] = {0.0};
+  for (int i = threadIdx.x; i < h; i += 256) one[0] += (double)c[i];
+  block_sums(one, sums);
+  s.m = (float)(one[0] / (double)h);
   float two[2] = {0.f, 0.f};
   for (int i = threadIdx.x; i < h; i += 256) {
     const float x = c[i] - s.m;
@@ -38,7 +42,8 @@ __device__ __forceinline__ NormStats norm_stats(const float* c, int h, float eps
   }
   block_sums(two, red);
   s.d = two[0] / (float)h;
-  s.r = 1.f / sqrtf(two[1] / (float)h - s.d * s.d + eps);
+  const float var = two[1] / (float)h - s.d * s.d;
+  s.r = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);        // (NaN stays)
   return s;
 }
 

@@ -213,3 +213,29 @@ def test_layer_norm_of_more_columns_than_a_launch_takes(cm, rng, h):
     check(gg.asarray(), wg, 0.5 * eg + 4 * U * (np.abs(wg) + 6))
     check(gb.asarray(), wb, U * (w / 16384 + 100) * 0.5 * eb + 4 * U * (np.abs(wb) + 6))
     release(x, dy, gg, gb, G, B)
+
+
+# ------------------------------------------------------------------ tall columns
+
+@pytest.mark.parametrize("h", [16390, 20000, 100000, 1000003])
+def test_layer_norm_of_tall_columns_far_from_zero(cm, h):
+    """Columns that are constant give the bias, whatever their value (the sum of equal entries is exact in 64 bits, and so is its quotient by
+    their number): nothing is NaN.  Entries that differ by a few steps of fp32: the mean is taken as m + d with |d| of half a step of m, so the
+    variance is off by chain u of itself and d^2, which is no more than twice it here."""
+    rng = np.random.default_rng(h)
+    values = [3.0, 98765.4, -1000000.3, 7.7e7, 1e9, 3e38, -1e-30]
+    x = F(np.repeat(F([values]), h, axis=0))
+    steps = F(98765.4 + 2.0 ** -7 * rng.integers(-2, 3, (h, 1)))
+    dy, gain, bias = F(rng.standard_normal((h, 8))), F(1 + 0.3 * rng.standard_normal((h, 1))), F(rng.standard_normal((h, 1)))
+    x = F(np.hstack([x, steps]))
+    y = cm.layer_norm(cm.CUDAMatrix(x), cm.CUDAMatrix(gain), cm.CUDAMatrix(bias), target=cm.empty(x.shape)).asarray()
+    assert np.array_equal(y[:, :7], np.repeat(bias, 7, axis=1))
+    want = tok.layer_norm(x[:, 7:], gain, bias)
+    check(y[:, 7:], want, 3 * norm_bound(x[:, 7:], gain, want))
+    G, dx, gg, gb = cm.CUDAMatrix(gain), cm.empty(x.shape), cm.empty((h, 1)), cm.empty((h, 1))
+    cm.layer_norm_grad(cm.CUDAMatrix(dy), cm.CUDAMatrix(x), G, target=dx, gain_grad=gg, bias_grad=gb)
+    want, wg, wb = tok.layer_norm_grad(dy, np.hstack([np.repeat(F([[3.0]]), 7, axis=1) * np.ones((h, 1)), x[:, 7:]]), gain)
+    ex, eg, eb = grad_bounds(dy, F(np.hstack([np.full((h, 7), 3.0), x[:, 7:]])), gain)
+    check(dx.asarray(), want, 3 * ex)
+    check(gg.asarray(), wg, 3 * eg)
+    check(gb.asarray(), wb, eb)

@@ -40,7 +40,6 @@ void dn_close_group();
 void dn_set_group_open(bool on);
 void dn_set_group_hook(void (*f)());
 void dn_group_allow(bool on);               // whether a product may go to the group instead of the stream
-void dn_ring_first(bool on);                // whether products take the ring's tiles wherever they fit (and the bf16 ones are not faster)
 bool dn_group_take_sums(const struct DnRowSumJob* jobs, int n);   // row sums that join the open group; false: launch them
 // apply_rectified_linear_deriv(target, gate, target) of the target of a product of the open group joins it
 bool dn_group_take_gate(const float* target, const float* gate, int h, int w);
@@ -77,8 +76,9 @@ int dn_row_sum_job_kind(const float* M, int h, int w);    // 0: not as a job, 1:
 int dn_row_sum_jobs(const DnRowSumJob* jobs, int n);
 int dn_gemm(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb,
             float beta, float* C, int ldc);
+// ring_first: the product takes the ring's tiles wherever they fit (and the bf16 ones are not faster)
 int dn_gemm_sums(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb,
-                 float beta, float* C, int ldc, const DnRowSumJob* jobs, int njobs);
+                 float beta, float* C, int ldc, const DnRowSumJob* jobs, int njobs, bool ring_first = false);
 int dn_gemm_pair_sums(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B,
                       int ldb, float beta, float alpha2, const float* A2, int lda2, const float* B2, int ldb2, float* C, int ldc,
                       const DnRowSumJob* jobs, int njobs);

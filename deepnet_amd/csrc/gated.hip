@@ -439,17 +439,16 @@ int dot_gated_grad(cudamat* deriv, cudamat* mat1, cudamat* mat2, cudamat* pre, c
   // From 64 columns on, on the ring's tiles where they fit: the two products share a launch then (us, by the plain products' rules / so: 1001 -> 1500
   // units of 300 columns 68.9 / 52.8, 256 -> 256 of 64 12.0 / 8.8, 100 -> 500 of 100 12.3 / 10.8, 2048 -> 4096 of 100 101.9 / 104.5; 2048 -> 4096 of
   // 20 56.7 / 71.9, 500 -> 2000 of 50 23.7 / 26.1).
-  dn_ring_first(n >= 64);
+  const bool ring_first = n >= 64;
   // by op(mat1): d op(mat2)^T; where mat1 is stored transposed, so is that
   if (mat1_grad && f > 0 && k > 0) {
-    e = wt ? dn_gemm_sums(xt, true, k, 2 * f, n, mult, x, mat2->size[0], d, 2 * f, beta, mat1_grad->data_device, k, &job, kind ? 1 : 0)
-           : dn_gemm_sums(false, !xt, 2 * f, k, n, mult, d, 2 * f, x, mat2->size[0], beta, mat1_grad->data_device, 2 * f, &job, kind ? 1 : 0);
+    e = wt ? dn_gemm_sums(xt, true, k, 2 * f, n, mult, x, mat2->size[0], d, 2 * f, beta, mat1_grad->data_device, k, &job, kind ? 1 : 0, ring_first)
+           : dn_gemm_sums(false, !xt, 2 * f, k, n, mult, d, 2 * f, x, mat2->size[0], beta, mat1_grad->data_device, 2 * f, &job, kind ? 1 : 0, ring_first);
   }
   // by op(mat2): op(mat1)^T d
   if (!e && mat2_grad && k > 0 && n > 0)
-    e = xt ? dn_gemm(true, wt, n, k, 2 * f, 1.f, d, 2 * f, w, mat1->size[0], 0.f, mat2_grad->data_device, n)
-           : dn_gemm(!wt, false, k, n, 2 * f, 1.f, w, mat1->size[0], d, 2 * f, 0.f, mat2_grad->data_device, k);
-  dn_ring_first(false);
+    e = xt ? dn_gemm_sums(true, wt, n, k, 2 * f, 1.f, d, 2 * f, w, mat1->size[0], 0.f, mat2_grad->data_device, n, nullptr, 0, ring_first)
+           : dn_gemm_sums(!wt, false, k, n, 2 * f, 1.f, w, mat1->size[0], d, 2 * f, 0.f, mat2_grad->data_device, k, nullptr, 0, ring_first);
   dn_group_allow(false);
   dn_close_group();
   if (!e && bias_grad && !kind) e = dn_row_sums(d, 2 * f, n, bias_grad->data_device, mult, beta);

@@ -1161,9 +1161,8 @@ static inline bool side_jobs_fit(const GemmEpilogue& epi) {
 // of a workgroup; slabs (perhaps of a split reduction, summed by a second kernel)
 enum GemmKind { GEMM_EMPTY, GEMM_BOX, GEMM_SPLIT, GEMM_RING, GEMM_T16, GEMM_SMALL, GEMM_SLAB };
 struct GemmPlan { GemmKind kind; RingPlan ring; bool heavy; };
-static bool g_ring_first;            // dn_ring_first
-void dn_ring_first(bool on) { g_ring_first = on; }
-static GemmPlan gemm_plan(bool a_kc, bool b_kc, int M, int N, int K, const float* A, int lda, const float* B, int ldb, float beta) {
+static GemmPlan gemm_plan(bool a_kc, bool b_kc, int M, int N, int K, const float* A, int lda, const float* B, int ldb, float beta,
+                          bool ring_first = false) {
   const RingPlan no_ring = {-1, 0.};
   if (K <= 0) return GemmPlan{GEMM_EMPTY, no_ring, false};
   const int cus = dn_num_cus();
@@ -1196,8 +1195,8 @@ static GemmPlan gemm_plan(bool a_kc, bool b_kc, int M, int N, int K, const float
   }
   // Reductions of more than 128 terms: k_gemm_ring, unless another kernel is expected to be faster (gemm_ring_plan).
   const size_t a_bytes = (size_t)lda * (a_kc ? M : K) * sizeof(float), b_bytes = (size_t)ldb * (b_kc ? N : K) * sizeof(float);
-  const RingPlan ring = g_ring_first ? ring_plan(M, N, K, a_bytes, b_bytes, cus)
-                        : K > BOX_K  ? gemm_ring_plan(M, N, K, a_bytes, b_bytes, cus, a_vec && b_vec && !(a_kc && b_kc)) : no_ring;
+  const RingPlan ring = ring_first ? ring_plan(M, N, K, a_bytes, b_bytes, cus)
+                        : K > BOX_K ? gemm_ring_plan(M, N, K, a_bytes, b_bytes, cus, a_vec && b_vec && !(a_kc && b_kc)) : no_ring;
   if (gemm_split_wins(M, N, K, beta != 0.f, a_bytes, b_bytes, ring, cus)) return GemmPlan{GEMM_SPLIT, no_ring, heavy};   // (no product that draws a sample)
   if (ring.cfg >= 0) return GemmPlan{GEMM_RING, ring, heavy};
   // Two K-contiguous operands whose rows lie a multiple of 1 KiB apart: the 16 x 16 block kernel
@@ -1276,7 +1275,7 @@ static bool group_apart(const GroupRange& r, bool writes_only, int skip = -1) {
 }
 
 static int gemm(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb, float beta,
-                float* C, int ldc, GemmEpilogue epi = g_no_epilogue, bool* fused = nullptr, bool* sampled = nullptr);
+                float* C, int ldc, GemmEpilogue epi = g_no_epilogue, bool* fused = nullptr, bool* sampled = nullptr, bool ring_first = false);
 
 // The products on the ring and the sums that go with them.
 static void group_launch_ring(const GroupJob* const* jobs, int n, const RowSumJobs& sums, int blocks) {
@@ -1341,6 +1340,7 @@ static void group_close() {
     if (o.plan.kind == GEMM_RING) continue;
     g_side_jobs = &J;
     g_side_blocks = blocks;
+    // (planned anew, without ring_first: none of the ring's tiles fits it either way)
     gemm(o.a_kc, !o.b_kc, o.g.M, o.g.N, o.g.K, o.g.alpha, o.g.A, o.g.lda, o.g.B, o.g.ldb, o.g.beta, o.g.C, o.g.ldc, o.epi);
     blocks = g_side_blocks;             // (0 where the launch took them along)
   }
@@ -1429,13 +1429,13 @@ bool dn_group_take_gate(const float* target, const float* gate, int h, int w) {
 // epi: what to append to each output (bias / activation); *fused tells the caller whether
 // the launch could carry it (the split-K and empty-K paths cannot).
 static int gemm(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb, float beta,
-                float* C, int ldc, GemmEpilogue epi, bool* fused, bool* sampled) {
+                float* C, int ldc, GemmEpilogue epi, bool* fused, bool* sampled, bool ring_first) {
   if (fused) *fused = false;
   if (sampled) *sampled = false;
   if (M <= 0 || N <= 0) return 0;
   const int cus = dn_num_cus();
   const bool a_kc = a_trans, b_kc = !b_trans;
-  const GemmPlan plan = gemm_plan(a_kc, b_kc, M, N, K, A, lda, B, ldb, beta);
+  const GemmPlan plan = gemm_plan(a_kc, b_kc, M, N, K, A, lda, B, ldb, beta, ring_first);
   if (plan.kind == GEMM_EMPTY) {
     size_t total = (size_t)M * N;
     unsigned blocks = (unsigned)((total + 255) / 256 < (size_t)cus * 8 ? (total + 255) / 256 : (size_t)cus * 8);
@@ -1595,7 +1595,7 @@ static int gemm(bool a_trans, bool b_trans, int M, int N, int K, float alpha, co
 // C = beta*C + alpha*op(A)*op(B) and the sums of `jobs`, which touch nothing the product reads or writes:
 // one launch where the product's kernel can take the sums along, otherwise the product, then the sums.
 int dn_gemm_sums(bool a_trans, bool b_trans, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb,
-                 float beta, float* C, int ldc, const DnRowSumJob* jobs, int njobs) {
+                 float beta, float* C, int ldc, const DnRowSumJob* jobs, int njobs, bool ring_first) {
   RowSumJobs J = {};
   const int jblocks = njobs > 0 ? rows_sum_jobs_table(jobs, njobs, &J) : 0;
   if (jblocks < 0) return ERROR_GENERIC;
@@ -1604,7 +1604,7 @@ int dn_gemm_sums(bool a_trans, bool b_trans, int M, int N, int K, float alpha, c
   g_side_blocks = jblocks;
   g_side_list = jobs;
   g_side_count = njobs;
-  const int e = gemm(a_trans, b_trans, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc);
+  const int e = gemm(a_trans, b_trans, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc, g_no_epilogue, nullptr, nullptr, ring_first);
   const bool taken = g_side_blocks == 0;
   g_side_jobs = nullptr;
   g_side_list = nullptr;

@@ -239,3 +239,22 @@ def test_layer_norm_of_tall_columns_far_from_zero(cm, h):
     check(dx.asarray(), want, 3 * ex)
     check(gg.asarray(), wg, 3 * eg)
     check(gb.asarray(), wb, eb)
+
+
+# ------------------------------------------------------------------ what else is queued
+
+@pytest.mark.parametrize("m,n,k", [(500, 100, 100), (256, 256, 64), (300, 200, 120), (1000, 64, 128)])
+def test_a_product_that_waits_keeps_its_kernel_beside_a_gated_gradient(cm, rng, m, n, k):
+    """dot may hold its launch back until the next call; the gradient's own choice of tiles (64 columns, no units: nothing but the fill of
+    m2_grad is launched) is not for it."""
+    a, b = cm.CUDAMatrix(F(rng.standard_normal((k, m)))), cm.CUDAMatrix(F(rng.standard_normal((k, n))))
+    want, got = cm.empty((m, n)), cm.empty((m, n))
+    cm.dot(a.T, b, target=want)
+    want = want.asarray().copy()
+    w, x, dx, dy, pre = cm.empty((7, 0)), cm.empty((7, 64)), cm.empty((7, 64)), cm.empty((0, 64)), cm.empty((0, 64))
+    dx.assign(5.0)
+    wt, at = w.T, a.T
+    cm.cuda_sync_threads()
+    cm.dot(at, b, target=got)
+    cm.dot_gated_grad(dy, wt, x, pre, m2_grad=dx)
+    assert np.array_equal(got.asarray(), want) and not dx.asarray().any()

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from oracle import token_oracle as tok
-from test_gpu_tokens import F, U, act_bounds, check, check_log_probs, grad_bounds, norm_bound
+from test_gpu_tokens import F, U, act_bounds, bits, check, check_log_probs, device, gated_check, grad_bounds, neighbours_untouched, norm_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -258,3 +258,195 @@ def test_a_product_that_waits_keeps_its_kernel_beside_a_gated_gradient(cm, rng, 
     cm.dot(at, b, target=got)
     cm.dot_gated_grad(dy, wt, x, pre, m2_grad=dx)
     assert np.array_equal(got.asarray(), want) and not dx.asarray().any()
+
+
+# ------------------------------------------------------------------ offsets beyond 2^31 entries, at ordinary heights
+
+@pytest.mark.parametrize("h", [64, 1023, 2050])
+def test_columns_beyond_two_to_the_31_entries(cm, rng, h):
+    """The kernels that hold columns in registers (16 lanes, a wavefront, a workgroup), in place: the last columns against the definitions."""
+    w, n = (1 << 31) // h + 200, 40
+    gain, bias = F(1 + 0.3 * rng.standard_normal((h, 1))), F(rng.standard_normal((h, 1)))
+    G, B = cm.CUDAMatrix(gain), cm.CUDAMatrix(bias)
+    big, parts = wide(cm, rng, h, w, n)
+    cm.layer_norm(big, G, B)
+    for p, got in zip(parts, ends(big, n)):
+        want = tok.layer_norm(p, gain, bias)
+        check(got, want, norm_bound(p, gain, want))
+    release(big)
+    x, xs = wide(cm, rng, h, w, n)
+    labels, rows = cm.empty((1, w)), {name: cm.empty((1, w)) for name in ('logp', 'entropy', 'log_z')}
+    labels.assign(h - 3.0)
+    cm.log_probs(x, labels, **rows)
+    got = {name: ends(m, n) for name, m in rows.items()}
+    for i, p in enumerate(xs):
+        check_log_probs(p, F(np.full((1, n), h - 3)), 0, {name: g[i] for name, g in got.items()})
+    dy, dys = wide(cm, rng, h, w, n)
+    gg, gb = cm.empty((h, 1)), cm.empty((h, 1))
+    cm.layer_norm_grad(dy, x, G, gain_grad=gg, bias_grad=gb)
+    wg, eg = 0.0, 0.0
+    for p, d, got in zip(xs, dys, ends(dy, n)):
+        dx, dg, _ = tok.layer_norm_grad(d, p, gain)
+        ex, e1, _ = grad_bounds(d, p, gain)
+        check(got, dx, ex)
+        wg, eg = wg + dg, eg + e1
+    check(gg.asarray(), wg, eg + 4 * U * np.abs(wg))                    # (constant columns of 0.125 add nothing)
+    lw = F(np.full((1, n), -1.0))
+    ones = cm.empty((1, w))
+    ones.assign(-1.0)
+    log_z = [z.astype(np.float64) for z in ends(rows['log_z'], n)]
+    cm.log_probs_grad(x, labels, rows['log_z'], ones)
+    for p, z, got in zip(xs, log_z, ends(x, n)):
+        want = tok.log_probs_grad(p, np.full((1, n), h - 3.0), z, lw)
+        lp = p.astype(np.float64) - z
+        check(got, want, U * (np.exp(lp) * (2 * np.abs(lp) + 4) + 2 * np.abs(want) + np.exp(lp)))
+    release(x, dy, labels, ones, gg, gb, G, B, *rows.values())
+
+
+def test_halves_and_results_beyond_two_to_the_31_entries(cm, rng):
+    """pre of 2 f rows passes 2^31 entries at half the columns: the pass over the halves, and the stores of a gated product on tiles."""
+    f, n = 1000, 40
+    w = (1 << 31) // (2 * f) + 200
+    dy, dys = wide(cm, rng, f, w, n)
+    pre, pres = wide(cm, rng, 2 * f, w, n)
+    m1, m2 = cm.empty((2 * f, 1)), cm.empty((1, w))
+    cm.dot_gated_grad(dy, m1, m2, pre, act='relu')
+    for d, p, got in zip(dys, pres, ends(pre, n)):
+        want = tok.gate_grad(d, p, 'relu')
+        check(got, want, 4 * U * np.abs(want))
+    release(dy, m1, m2)
+    d = 32
+    wt = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d))
+    x, xs = wide(cm, rng, d, w, n)
+    y = cm.empty((f, w))
+    cm.dot_gated(cm.CUDAMatrix(wt).T, x, target=y, pre=pre, act='silu')
+    for p, got, halves in zip(xs, ends(y, n), ends(pre, n)):
+        gated_check(cm, wt, p, None, 'silu', got, halves)
+    release(x, y, pre)
+
+
+# ------------------------------------------------------------------ operands stored either way, anywhere
+
+@pytest.mark.parametrize("d,f,n", [(70, 33, 1), (70, 33, 9), (257, 130, 20), (64, 100, 65), (130, 70, 300), (256, 256, 256)])
+@pytest.mark.parametrize("skip", [0, 1, 3])
+def test_dot_gated_grad_of_operands_stored_either_way_with_sums(cm, rng, d, f, n, skip):
+    """Weights and inputs stored either way, every operand and result off a 16-byte boundary, the gradients accumulated and scaled, that of the
+    bias among them.  The halves' derivatives are read back, so the bounds are those of the products and sums."""
+    w, x, dy = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d)), F(rng.standard_normal((d, n))), F(rng.standard_normal((f, n)))
+    pre, old = F(rng.standard_normal((2 * f, n))), F(rng.standard_normal((d, 2 * f)))
+    aw, ax = np.abs(w.astype(np.float64)), np.abs(x.astype(np.float64))
+    for wt in (False, True):
+        for xt in (False, True):
+            W, X = device(cm, w if wt else w.T, skip), device(cm, x.T if xt else x, skip)
+            dw, dx, db = device(cm, old if wt else old.T, skip), device(cm, np.full(X.shape, np.nan), skip), device(cm, np.full((2 * f, 1), 2.0), skip)
+            t = device(cm, np.zeros((2 * f, n)), skip)
+            cm.dot_gated_grad(device(cm, dy, skip), W.T if wt else W, X.T if xt else X, device(cm, pre, skip), target=t, m1_grad=dw, m2_grad=dx,
+                              bias_grad=db, mult=-0.5, beta=0.25)
+            got = t.asarray().astype(np.float64)
+            ve, se = act_bounds('silu', pre[:f].astype(np.float64), 0.0)
+            ad, au = np.abs(dy.astype(np.float64)), np.abs(pre[f:].astype(np.float64))
+            check(got, tok.gate_grad(dy, pre, 'silu'), np.vstack([ad * au * se, ad * ve]) + 4 * U * np.abs(got), ('halves', wt, xt))
+            at, c = np.abs(got), U * (n / 4 + 24)
+            wdw, wdx, wdb = x.astype(np.float64) @ got.T, w.astype(np.float64) @ got, got.sum(axis=1, keepdims=True)
+            want = 0.25 * old - 0.5 * wdw
+            check(dw.asarray() if wt else dw.asarray().T, want, 0.5 * c * (ax @ at.T) + 3 * U * (0.25 * np.abs(old) + np.abs(wdw)), ('weights', wt, xt))
+            check(dx.asarray().T if xt else dx.asarray(), wdx, U * (f / 2 + 24) * (aw @ at), ('inputs', wt, xt))
+            check(db.asarray(), 0.5 - 0.5 * wdb, 0.5 * c * at.sum(axis=1, keepdims=True) + 3 * U * (0.5 + np.abs(wdb)), ('bias', wt, xt))
+            for m in (W, X, dw, dx, db, t):
+                neighbours_untouched(m, skip)
+
+
+def test_an_infinite_column_of_a_gated_product_is_in_all_of_its_results(cm, rng):
+    """Sigmoid gates: 0 or 1 times an infinity, or 0 times one (NaN); no result of that column is finite."""
+    for d, f, n in ((64, 40, 6), (300, 700, 300), (1024, 1500, 1500), (64, 40, 11), (2048, 30, 6), (100, 60, 16), (512, 2050, 40)):
+        w, x = F(rng.standard_normal((d, 2 * f)) / np.sqrt(d)), F(rng.standard_normal((d, n)))
+        x[5, 4] = np.inf
+        y = cm.dot_gated(cm.CUDAMatrix(w).T, cm.CUDAMatrix(x), act='sigmoid').asarray()
+        ok = w[5, :f] > 0                                   # (a gate of 0 leaves the sign of 0 times infinity: NaN; one of 1 the infinity)
+        want = np.where(ok, np.where(w[5, f:] > 0, np.inf, -np.inf), np.nan)
+        assert not np.isfinite(y[:, 4]).any() and np.array_equal(y[:, 4], want, equal_nan=True), (d, f, n)
+        cols = [c for c in range(n) if c != 4]
+        gated_check(cm, w, x[:, cols], None, 'sigmoid', y[:, cols], None)
+
+
+# ------------------------------------------------------------------ lists of anything
+
+def any_column(rng, h):
+    """Entries with ties, masks of one kind or several, NaN and infinities in places of any number."""
+    kind = rng.integers(7)
+    x = rng.standard_normal(h)
+    if kind == 1:
+        x = np.round(x)
+    elif kind >= 2:
+        x = np.full(h, rng.choice([-1e9, np.finfo(np.float32).min, -np.inf, 0.0, -0.0]))
+        at = rng.choice(h, min(h, int(rng.choice([0, 1, 3, 4, 5, 19, 20, 63, 64, 65, 300]))), replace=False)
+        x[at] = 2.0 if kind == 3 else rng.standard_normal(at.size)
+        if kind == 4:
+            x[rng.integers(0, h, 30)] = np.nan
+        elif kind == 5:
+            a, b = np.sort(rng.integers(0, h + 1, 2))
+            x[a:b] = -np.inf
+        elif kind == 6:
+            x[rng.integers(0, h, 3)] = rng.choice([np.inf, 0.0, -0.0])
+    return x
+
+
+@pytest.mark.parametrize("h,w", [(4, 64), (37, 64), (257, 64), (1000, 64), (1024, 64), (1025, 64), (1027, 64), (4095, 64), (4099, 64), (9001, 64), (9001, 600), (30000, 40), (70003, 9)])
+@pytest.mark.parametrize("k", [1, 2, 4, 5, 20, 63, 64])
+def test_lists_of_any_columns(cm, h, w, k):
+    k = min(k, h)
+    rng = np.random.default_rng(100 * h + k)
+    few = min(w, 64)
+    x = F(np.stack([any_column(rng, h) for _ in range(few)], axis=1))
+    if w > few:
+        x = F(np.tile(x, (1, w // few + 1))[:, :w])
+    labels = F(rng.integers(-1, h, (1, w)))
+    names = dict(logp=(1, w), entropy=(1, w), log_z=(1, w), top=(k, w), top_labels=(k, w))
+    out = {name: cm.CUDAMatrix(F(np.full(shape, 7.0))) for name, shape in names.items()}
+    cm.log_probs(cm.CUDAMatrix(x), cm.CUDAMatrix(labels), **out)
+    check_log_probs(x[:, -few:], labels[:, -few:], k, {name: m.asarray()[:, -few:] for name, m in out.items()})
+
+
+# ------------------------------------------------------------------ recordings that share workspaces
+
+def test_two_recordings_of_calls_with_workspaces(cm, rng):
+    """Columns in segments, sums of several workgroups, gradients of few and of many columns: two graphs of different sizes, replayed in turn
+    with eager calls of a third size between them, each with the bits of the calls by themselves."""
+    class Set(object):
+        def __init__(self, v, c, d, f, n):
+            D = lambda *s: cm.CUDAMatrix(F(rng.standard_normal(s)))
+            self.x, self.labels, self.top = D(v, c), cm.CUDAMatrix(F(rng.integers(0, v, (1, c)))), 5
+            self.rows, self.lists = [cm.empty((1, c)) for _ in range(3)], [cm.empty((5, c)) for _ in range(2)]
+            self.dy, self.h, self.g = D(d, 700), D(d, 700), D(d, 1)
+            self.dh, self.gg, self.gb = cm.empty((d, 700)), cm.empty((d, 1)), cm.empty((d, 1))
+            self.w, self.in_, self.dg, self.pre = D(d, 2 * f), D(d, n), D(f, n), D(2 * f, n)
+            self.t, self.dw, self.dx, self.db, self.y = cm.empty((2 * f, n)), cm.empty((d, 2 * f)), cm.empty((d, n)), cm.empty((2 * f, 1)), cm.empty((f, n))
+
+        def step(self):
+            cm.log_probs(self.x, self.labels, *(self.rows + self.lists))
+            cm.layer_norm_grad(self.dy, self.h, self.g, target=self.dh, gain_grad=self.gg, bias_grad=self.gb)
+            cm.dot_gated(self.w.T, self.in_, target=self.y)
+            cm.dot_gated_grad(self.dg, self.w.T, self.in_, self.pre, target=self.t, m1_grad=self.dw, m2_grad=self.dx, bias_grad=self.db)
+
+        def out(self):
+            return self.rows + self.lists + [self.dh, self.gg, self.gb, self.t, self.dw, self.dx, self.db, self.y]
+
+    a, b, c = Set(50001, 3, 300, 200, 5), Set(20000, 17, 130, 40, 3), Set(100000, 2, 64, 700, 14)
+    want = []
+    for s in (a, b, c):
+        s.step()
+        want.append(bits(s.out()))
+    graphs = []
+    for s in (a, b):
+        with cm.Graph() as g:
+            s.step()
+        graphs.append(g)
+    for i in range(4):
+        for s, g, w in zip((a, b), graphs, want):
+            for m in s.out():
+                m.assign(-3.0)
+            c.step()
+            g.launch()
+            c.step()
+            assert all(np.array_equal(p, q) for p, q in zip(bits(s.out()), w)), i
+            assert all(np.array_equal(p, q) for p, q in zip(bits(c.out()), want[2])), i

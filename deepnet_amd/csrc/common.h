@@ -12,7 +12,7 @@ int dn_num_cus();
 // hipMalloc that releases the library's cache of freed matrix blocks and retries when the device is full.
 hipError_t dn_malloc(void** p, size_t bytes);
 
-// Grow-only device workspaces (slot 0: partials and scalar results; slot 1: conv patch matrix).
+// Grow-only device workspaces (slot 0: partials and scalar results; slot 1: conv patch matrix, halves of a gated product).
 void* dn_scratch(size_t bytes, int slot = 0);
 bool dn_scratch_holds(size_t bytes, int slot = 0);   // whether that much is there (launches nothing)
 
@@ -107,6 +107,11 @@ static inline bool dn_launch_fits(dim3 grid, dim3 block) {
 static inline int dn_launch_status() {
   if (g_dn_launch_left_out) { g_dn_launch_left_out = false; return ERROR_UNSUPPORTED; }
   return hipPeekAtLastError() == hipSuccess ? 0 : CUDA_ERROR;
+}
+// The same for the calls that keep a text: null, or what is wrong.
+static inline const char* dn_launch_error() {
+  const int e = dn_launch_status();
+  return e == 0 ? nullptr : e == ERROR_UNSUPPORTED ? "more work items than a launch takes" : hipGetErrorString(hipGetLastError());
 }
 
 static inline bool dn_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -2169,7 +2169,7 @@ static void conv_up_impl(cudamat* images, cudamat* filters, cudamat* targets, in
                              else hipLaunchKernelGGL((k_conv_up_taps<2, CG, KF>), grid64, dim3(256), 0, dn_stream(), a); } while (0)
       if (a.Cg == 3 && k == 5) UP_TAPS(3, 5); else if (a.Cg == 3) UP_TAPS(3, 3); else if (k == 5) UP_TAPS(1, 5); else UP_TAPS(1, 3);
 #undef UP_TAPS
-      if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+      if (const char* what = dn_launch_error()) conv_set_error(where, what);
       return;
     }
     // short reduction, few filters per group: filter bank in registers
@@ -2201,7 +2201,7 @@ static void conv_up_impl(cudamat* images, cudamat* filters, cudamat* targets, in
     if (blocks > dn_num_cus() * 16ll) blocks = dn_num_cus() * 16ll;
     hipLaunchKernelGGL(k_conv_up_direct, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
   }
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 static bool conv_down_args(cudamat* hidActs, cudamat* filters, cudamat* targets, int imgSize, int paddingStart,
@@ -2316,7 +2316,7 @@ static void conv_down_impl(cudamat* hidActs, cudamat* filters, cudamat* targets,
     if (blocks > dn_num_cus() * 16ll) blocks = dn_num_cus() * 16ll;
     hipLaunchKernelGGL(k_conv_down_direct, dim3((unsigned)blocks), dim3(256), 0, dn_stream(), a);
   }
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 // Two chunks in flight per wavefront: with three or four, more of the first requests of the whole
@@ -2467,7 +2467,7 @@ static void conv_outp_impl(cudamat* images, cudamat* hidActs, cudamat* targets, 
       hipLaunchKernelGGL(k_conv_outp_direct, dim3((unsigned)(F * cols)), dim3(256), 0, dn_stream(), a);
     }
   }
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 extern "C" const char* conv_last_error(void) { return g_conv_failed ? g_conv_err : nullptr; }
@@ -2661,7 +2661,7 @@ static ConvRingArgs ring_args(const ConvArgs& a) {
 }
 
 static bool ring_done(const char* where) {
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
   return true;
 }
 

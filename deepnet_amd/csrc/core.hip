@@ -91,7 +91,8 @@ bool dn_capturing() { return g_capturing; }
 // ------------------------------------------------------------------ scratch
 // Grow-only device workspaces.  Slot 0: partials of two-stage reductions and
 // split-K products, scalar results.  Slot 1: the patch matrix of the col2im
-// form of convDown (it is live while a product that may use slot 0 runs).  Slot 2:
+// form of convDown, the halves of a gated product in two launches (live while a product that may
+// use slot 0 runs), the sums of squares of normlimit's rows.  Slot 2:
 // batch-padded copies of conv operands (live across a whole conv call).  Slot 3: the same
 // for operands padded to a multiple of 16 filters.
 static void* g_scratch[4] = {nullptr, nullptr, nullptr, nullptr};

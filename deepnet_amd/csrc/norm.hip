@@ -21,7 +21,7 @@ __device__ __forceinline__ void block_sums(V (&v)[N], V (*red)[4]) {
 
 // ------------------------------------------------------------------ columns that no team holds
 // A workgroup a column, three passes over it (the later ones from the caches): more than 16384 rows, where a lane would have to hold more than
-// 16.  20000 x 1000 106 us (1.5 TB/s), its gradients 257: waits for each pass's loads and its meeting.
+// 16.  20000 x 1000 107 us (1.5 TB/s), its gradients 260: waits for each pass's loads and its meeting.
 // The mean as a pair m + d (m rounded to fp32, d what the deviations from m still sum to) and 1 / sqrt(variance + eps):
 // deviations are taken from m, so that a mean far from zero costs no digits of the variance.  That takes an m that is off by its own rounding only:
 // a lane adds up h / 256 entries, and in 32 bits m was off by so much (1000003 equal entries of 98765.4: by 2.8) that d^2 outweighed

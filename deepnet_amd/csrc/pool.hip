@@ -944,7 +944,7 @@ static void pool_impl(cudamat* images, cudamat* rnd, cudamat* targets, int numFi
     if (v4) hipLaunchKernelGGL((k_pool<4, 1>), dim3(grid), dim3(256), 0, dn_stream(), images->data_device, r, targets->data_device, g);
     else hipLaunchKernelGGL((k_pool<1, 1>), dim3(grid), dim3(256), 0, dn_stream(), images->data_device, r, targets->data_device, g);
   }
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 // ---- MaxPool held back.  deepnet's conv stage calls MaxPool and then ResponseNorm on the pooled map
@@ -1031,7 +1031,7 @@ static void cnorm_impl(cudamat* images, cudamat* meanDiffs, cudamat* denoms, cud
   }
 #undef CNORM_GO
 #undef CNORM_ROWS
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 static void rnorm_undo_impl(cudamat* outGrads, cudamat* denoms, cudamat* inputs, cudamat* acts, cudamat* targets,
@@ -1055,7 +1055,7 @@ static void rnorm_undo_impl(cudamat* outGrads, cudamat* denoms, cudamat* inputs,
     if (qb > 0) {
       norm_lds_launch<true>(qb, false, outGrads->data_device, denoms->data_device, inputs->data_device, acts->data_device,
                             nullptr, targets->data_device, N, S, numFilters, sizeX, -2.f * addScale * powScale, powScale);
-      if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+      if (const char* what = dn_launch_error()) conv_set_error(where, what);
       return;
     }
   }
@@ -1092,7 +1092,7 @@ static void rnorm_undo_impl(cudamat* outGrads, cudamat* denoms, cudamat* inputs,
   }
 #undef RUNDO_GO
 #undef RUNDO_ROWS
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 extern "C" {
@@ -1156,7 +1156,7 @@ void MaxPoolUndo(cudamat* images, cudamat* maxGrads, cudamat* maxActs, cudamat* 
   else
     hipLaunchKernelGGL((k_pool_undo<1>), dim3(grid), dim3(256), 0, dn_stream(), (const float*)images->data_device,
                        (const float*)maxGrads->data_device, (const float*)maxActs->data_device, targets->data_device, g);
-  if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+  if (const char* what = dn_launch_error()) conv_set_error(where, what);
 }
 
 void MaxPoolResponseNorm(cudamat* images, cudamat* pooled, cudamat* denoms, cudamat* targets, int numFilters, int subsX,
@@ -1232,7 +1232,7 @@ void MaxPoolResponseNorm(cudamat* images, cudamat* pooled, cudamat* denoms, cuda
 #undef PN_SU
 #undef PN_SZ
 #undef PN_GO
-    if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+    if (const char* what = dn_launch_error()) conv_set_error(where, what);
     return;
   }
   pool_impl(images, nullptr, pooled, numFilters, subsX, startX, strideX, outputsX, where);
@@ -1290,7 +1290,7 @@ void ResponseNormUndoMaxPoolUndo(cudamat* outGrads, cudamat* denoms, cudamat* in
 #undef NP_SZ
 #undef NP_GO
     if (attr_ok) {
-      if (dn_launch_status()) conv_set_error(where, hipGetErrorString(hipGetLastError()));
+      if (const char* what = dn_launch_error()) conv_set_error(where, what);
       return;
     }
     hipGetLastError();

@@ -1583,8 +1583,8 @@ int normlimit_by_axis(cudamat* mat, cudamat* target, int axis, float norm) {
     if (h <= 0 || w <= 0) return 0;
     // two passes, each at streaming rate: the rows' sums of squares (the axis-1 reduction), then the
     // scaling as a column-vector broadcast (4096 x 4096: 37 us; one workgroup per 64 rows walking
-    // all columns twice took 640 us).  The sums live in scratch slot 1, which nothing else of the
-    // matrix library uses (slot 0 holds the reduction's own partials).
+    // all columns twice took 640 us).  The sums live in scratch slot 1 (slot 0
+    // holds the reduction's own partials).
     float* sq = (float*)dn_scratch((size_t)h * sizeof(float), 1);
     if (!sq) return CUDA_ERROR;
     if (int e = rows_reduce<ROW_SQSUM>(mat->data_device, h, h, w, nullptr, sq, 1.f, 0.f)) return e;

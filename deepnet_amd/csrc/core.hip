@@ -528,12 +528,14 @@ int copy_on_device(cudamat* mat1, cudamat* mat2) {
   if (len <= 0 || mat1->data_device == mat2->data_device) return 0;
   const float* src = mat1->data_device;
   float* dst = mat2->data_device;
-  if (dn_aligned16(src) && dn_aligned16(dst)) {
-    const unsigned blocks = (unsigned)(((len >> 2) + (len & 3) + 255) / 256);
-    if (len >= DN_STREAM_MIN_ELEMS) hipLaunchKernelGGL((k_copy<true, true>), dim3(blocks), dim3(256), 0, dn_stream(), src, dst, len);
-    else hipLaunchKernelGGL((k_copy<true, false>), dim3(blocks), dim3(256), 0, dn_stream(), src, dst, len);
-  } else {
-    hipLaunchKernelGGL((k_copy<false, false>), dim3((unsigned)((len + 255) / 256)), dim3(256), 0, dn_stream(), src, dst, len);
+  const bool vec = dn_aligned16(src) && dn_aligned16(dst);
+  const long long part = (vec ? 1024 : 256) * (DN_MAX_GROUPS - 1);       // (one workgroup more for what is behind the last group of four)
+  for (long long o = 0; o < len; o += part) {
+    const long long n = len - o < part ? len - o : part, lanes = vec ? (n >> 2) + (n & 3) : n;
+    const dim3 grid((unsigned)((lanes + 255) / 256));
+    if (vec && len >= DN_STREAM_MIN_ELEMS) hipLaunchKernelGGL((k_copy<true, true>), grid, dim3(256), 0, dn_stream(), src + o, dst + o, n);
+    else if (vec) hipLaunchKernelGGL((k_copy<true, false>), grid, dim3(256), 0, dn_stream(), src + o, dst + o, n);
+    else hipLaunchKernelGGL((k_copy<false, false>), grid, dim3(256), 0, dn_stream(), src + o, dst + o, n);
   }
   return dn_launch_status() ? CUBLAS_ERROR : 0;
 }

@@ -1,4 +1,6 @@
 """Ends of the ranges of the operators on columns of tokens.  Bounds and helpers of test_gpu_tokens.py."""
+import ctypes as ct
+
 import numpy as np
 import pytest
 
@@ -117,6 +119,24 @@ def test_elementwise_calls_of_more_entries_than_a_launch_takes(cm):
     for c in (0, 1, w // 2, (1 << 17) - 1, 1 << 17, w - 1):
         assert (big.slice(c, c + 1).asarray() == 0.5).all(), c
     release(big)
+
+
+@pytest.mark.parametrize("skip,h,w", [(1, 1 << 16, (1 << 16) + 3), (0, 1 << 17, (1 << 17) + 3)])
+def test_copies_of_more_entries_than_a_launch_takes(cm, skip, h, w):
+    """From an address off 16 bytes an entry a lane, 2^32 of them and some; else four a lane."""
+    whole = cm.empty((h, w + 1))
+    whole.assign(2.5)
+    mat = cm.cudamat()
+    ct.memmove(ct.pointer(mat), whole.p_mat, ct.sizeof(mat))
+    mat.data_device = ct.cast(ct.addressof(mat.data_device.contents) + 4 * skip, type(mat.data_device))
+    mat.owns_data, mat.size[1] = 0, w
+    src = cm.CUDAMatrix(mat)
+    dst = cm.empty((h, w))
+    dst.assign(0.0)
+    dst.assign(src)
+    for c in (0, 1, w // 2, h - 1, h, w - 1):
+        assert (dst.slice(c, c + 1).asarray() == 2.5).all(), c
+    release(dst, whole)
 
 
 def test_a_call_without_a_launch_is_an_error_and_the_next_one_is_none(cm):

@@ -40,9 +40,6 @@ def test_a_grid_that_no_launch_takes_is_refused(lib, new):
     apart = handle(new.cm, 4, w, 1 << 40)
     assert lib.normlimit_by_axis(x, apart, 0, ct.c_float(1.0)) == UNSUPPORTED
     assert lib.max_by_axis(x, row, 0) == UNSUPPORTED
-    # (a copy between places of another alignment takes an entry a lane; its error is the reference's one for copies)
-    a, b = handle(new.cm, 1 << 16, 1 << 16, 1 << 40), handle(new.cm, 1 << 16, 1 << 16, (1 << 41) + 4)
-    assert lib.copy_on_device(a, b) != 0
 
 
 def test_layer_norm_of_columns_that_it_cannot_count_is_refused(lib, new):

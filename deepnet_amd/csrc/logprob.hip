@@ -179,7 +179,8 @@ __device__ __forceinline__ unsigned lp_order(float x) { return (unsigned)(lp_key
 
 // ---- columns (or segments of them) by a workgroup of 256 lanes, eight 16-byte groups a lane on their way
 // Bound by the bytes, 4 an entry: 32768 x 2048 41.8 to 42.2 us, 6.4 TB/s (copy rate: 41.6), 32003 x 2048 43.2; the exponentials take 0.8 of the
-// vector unit's time.  Few columns are split, so that the chip reads them at once: 50000 x 4 in 52 workgroups 4.8 us.  Top lists are found in
+// vector unit's time.  Few columns are split, so that the chip reads them at once: 50000 x 4 in 52 workgroups 4.8 us.
+// Columns of one to three rows come here too, a workgroup each: 3 x 1000000 1177 us.  Top lists are found in
 // the same pass, after it: 32000 x 1024 with 20 best 38.2 us (20.3 by the bytes), 50000 x 4 10.0, a chain of some ten trips to LDS and three to
 // memory, whose steps take 0.4 to 1.4 us each.
 template <bool TOP, bool STREAM>
@@ -574,7 +575,8 @@ __global__ void __launch_bounds__(256) k_log_probs_wave(LogProbArgs a) {
 // target = logp_weight (onehot(label) - p) - entropy_weight p (log p + entropy), log p = mat - log_z, p = e^(log p): one pass.  A unit of 64
 // lanes (columns of up to 1024 rows) or 256 (pieces of 4096) takes up to 16 rows a lane of one column; the rows behind the last group of
 // four go one a lane, so that target may be mat (no row is read by one lane when another may have written it).  8 bytes an entry: 32768 x
-// 1000 45.5 us, 5.8 TB/s (copy rate: 40.6), 32003 x 1000 47.5, 1000 x 20000 31.6.
+// 1000 45.5 us, 5.8 TB/s (copy rate: 40.6), 32003 x 1000 47.5, 1000 x 20000 31.6, 512 x 40000 29.3 (25.4).  A short column leaves lanes without work:
+// 100 x 200000 52.2 (24.8), 64 x 100000 24.9 (7.9), 3 x 1000000 192 (3.7).
 struct LogProbGradArgs {
   const float *mat, *labels, *log_z, *logp_weight, *entropy, *entropy_weight;
   float* target;

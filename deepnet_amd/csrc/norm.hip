@@ -243,8 +243,10 @@ k_layer_norm_cols(const float* mat, const float* gain, const float* bias, float*
 // Backward in one pass over mat and deriv: with m known, sums of the deviations, their squares, g = gain * deriv and g times
 // the deviations come from one round.  The gradients of gain and bias stay in the lanes that have their rows, for all columns of
 // the workgroup; its teams meet in LDS at the end, and a second kernel adds up the workgroups (a single one finishes by itself).  12 bytes an
-// entry: 4096 x 8192 72.8 us, 5.5 TB/s (copy rate: 62.4), of which the second kernel is 4.2; 1024 x 16384 38.9, 4098 x 4099 45.2 (31.2), 1024 x 4
-// 5.1.  A workgroup's teams go in step from barrier to barrier, vector instructions issue in half of the cycles.
+// entry: 4096 x 8192 72.8 us, 5.5 TB/s (copy rate: 62.4), of which the second kernel is 4.2; 1024 x 16384 38.9, 4098 x 4099 45.2 (31.2), 4096 x 4099,
+// whose columns start at a memory line, 42.1, 1026 and 1024 x 8192 26.7 and 23.9 (15.6), 4096 x 1000 19.7 (7.6), 4096 x 300 13.8 (2.3), 16384 x 1024
+// 52.9 (31.2), 1024 x 4 5.1.  What is over the bytes is the partial sums of up to 256 workgroups with their second launch, whatever the columns'
+// number, and the barrier a column, at which a workgroup's teams go in step; vector instructions issue in half of the cycles.
 struct NormGradArgs {
   const float *deriv, *mat, *gain;
   float *target, *partial, *gain_grad, *bias_grad;

@@ -17,7 +17,8 @@
 extern "C" {
 #endif
 
-/* Error codes: cudamat/cudamat.cuh:1-9. */
+/* Error codes: cudamat/cudamat.cuh:1-9.  ERROR_UNSUPPORTED is also the answer of a call that would need a launch of 2^32 work items
+ * or more in one dimension and is not split: nothing is queued (the runtime would run a part of it and report no error). */
 #define ERROR_INCOMPATIBLE_DIMENSIONS -1
 #define CUBLAS_ERROR -2
 #define CUDA_ERROR -3
@@ -333,10 +334,11 @@ int cd_update(cudamat* W, cudamat* bv, cudamat* bh, cudamat* v, cudamat* h, cuda
  * counterpart in the reference.  Nothing is held back, nothing waits.  Matrices that are written may be one that is read where
  * that is said, and share no memory with the others (-9).  layer_norm_grad, log_probs of few columns, dot_gated_grad and dot_gated of
  * products that take more than one launch use the library's workspaces: queued on streams of the caller's (graph_set_stream), such calls may not
- * overlap, and a call records into a graph once the workspaces have their sizes (run it once before). ---- */
+ * overlap, and a call records into a graph once the workspaces have their sizes (run it once before).  Columns and entries that one launch does
+ * not take (2^32 work items) are queued in several. ---- */
 
 /* Layer norm: target = gain * (mat - mean) / sqrt(variance + eps) + bias, mean and (biased) variance of each column.
- * gain, bias: rows x 1 or NULL (ones, zeros); target may be mat; eps >= 0. */
+ * gain, bias: rows x 1 or NULL (ones, zeros); target may be mat; eps >= 0; fewer than 2^30 rows (-9). */
 int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, float eps);
 /* Its gradients from the derivative by its result: target = derivative by mat (may be deriv or mat);
  * gain_grad = beta * gain_grad + mult * (sums over the columns), bias_grad likewise (each may be NULL; beta = 0 reads nothing). */

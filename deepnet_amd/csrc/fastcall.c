@@ -34,6 +34,10 @@ typedef int (*Call)(void* fn, const Arg* a);
   S(, "PPPPPi", (P_, P_, P_, P_, P_, i_), (a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].i))                                         \
   S(, "PPPPPPPPiff", (P_, P_, P_, P_, P_, P_, P_, P_, i_, f_, f_),                                                                  \
     (a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, a[6].p, a[7].p, a[8].i, a[9].f, a[10].f))                                      \
+  S(, "PPPPPPPPi", (P_, P_, P_, P_, P_, P_, P_, P_, i_),                                                                            \
+    (a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, a[6].p, a[7].p, a[8].i))                                                       \
+  S(, "PPPPPPPPffff", (P_, P_, P_, P_, P_, P_, P_, P_, f_, f_, f_, f_),                                                             \
+    (a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, a[6].p, a[7].p, a[8].f, a[9].f, a[10].f, a[11].f))                             \
   S(, "PPPPffiii", (P_, P_, P_, P_, f_, f_, i_, i_, i_),                                                                            \
     (a[0].p, a[1].p, a[2].p, a[3].p, a[4].f, a[5].f, a[6].i, a[7].i, a[8].i))                                                       \
   S(, "PPPPPPP", (P_, P_, P_, P_, P_, P_, P_), (a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, a[6].p))                            \
@@ -59,7 +63,7 @@ static const char* const g_kinds[] = {SIGNATURES(KINDS)};
 #define N_SIGNATURES (sizeof g_kinds / sizeof *g_kinds)
 static const Call g_calls[] = {call_1, call_2, call_3, call_4, call_5, call_6, call_7, call_8, call_9, call_10, call_11, call_12, call_13,
                                call_14, call_15, call_16, call_17, call_18, call_19, call_20, call_21, call_22, call_23,
-                               call_24, call_25, call_26, call_27, call_28, call_29};
+                               call_24, call_25, call_26, call_27, call_28, call_29, call_30, call_31};
 _Static_assert(sizeof g_calls / sizeof *g_calls == sizeof g_kinds / sizeof *g_kinds, "one function per signature");
 
 typedef struct {

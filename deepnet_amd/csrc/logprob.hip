@@ -1,20 +1,9 @@
 // Log probabilities of given tokens, entropies and the best alternatives of columns of logits, and their gradient (no
 // counterpart in cudamat.cu; softmax_ce_grad is the loss of a classifier, which stores its probabilities).
 #include "columns.h"
+#include "tokens.h"
 #include "wide_math.h"
 #include <float.h>
-
-// Orders entries: the greater value first, of equal ones (0 and -0 are) the one further up; NaN ranks with -inf.
-__device__ __forceinline__ unsigned long long lp_key(float x, int i) {
-  x = x != x ? -INFINITY : x + 0.f;
-  const unsigned u = __float_as_uint(x), v = u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-  return ((unsigned long long)v << 32) | (unsigned)~i;
-}
-__device__ __forceinline__ int lp_key_index(unsigned long long k) { return (int)~(unsigned)k; }
-__device__ __forceinline__ float lp_key_value(unsigned long long key) {
-  const unsigned v = (unsigned)(key >> 32);
-  return __uint_as_float(v ^ ((v >> 31) ? 0x80000000u : 0xffffffffu));
-}
 
 // log(1 + r), r >= 0 (NaN stays NaN); 1 + r itself would round a small r away.
 __device__ __forceinline__ double lp_log1p(double u) {

@@ -126,6 +126,9 @@ _SIGNATURES = {
     'dot_gated': (_i, [_M, _M, _M, _M, _M, _i]), 'dot_gated_grad': (_i, [_M, _M, _M, _M, _M, _M, _M, _M, _i, _f, _f]),
     'counter_dropout': (_i, [_M, _M, _M, _M, _f, _f, _u, _u, _u]),
     'log_probs': (_i, [_M, _M, _M, _M, _M, _M, _M]), 'log_probs_grad': (_i, [_M, _M, _M, _M, _M, _M, _M]),
+    'embed': (_i, [_M, _M, _M, _f]), 'embed_grad': (_i, [_M, _M, _M, _f, _f]),
+    'gated_scan': (_i, [_M, _M, _M, _M, _M, _i]), 'gated_scan_grad': (_i, [_M, _M, _M, _M, _M, _M, _M, _M, _i]),
+    'sample_tokens': (_i, [_M, _M, _M, _M, _M, _M, _M, _M, _f, _f, _f, _f]),
     'init_from_sparse_array': (None, [_S, ct.POINTER(ct.c_float), ct.POINTER(ct.c_int), ct.POINTER(ct.c_int),
                                       _i, _i, _i]),
     'allocate_device_memory_sparse': (_i, [_S]), 'copy_sparse_to_device': (_i, [_S]),
@@ -1106,6 +1109,71 @@ def log_probs_grad(mat, labels, log_z, logp_weight=None, entropy=None, entropy_w
     if target is None:
         target = mat
     _check(_cudamat.log_probs_grad(mat.p_mat, _p(labels), log_z.p_mat, _p(logp_weight), _p(entropy), _p(entropy_weight), target.p_mat))
+    return target
+
+
+def embed(mat, labels, target=None, mult=1.0):
+    """Extension of this backend (not in the reference): target (rows of mat x columns) = mult * the column of mat (features x vocabulary) that
+    the labels (1 x columns, as floats) name; 0 where a label is no token (outside [0, vocabulary): padding)."""
+    if target is None:
+        target = empty((mat.shape[0], labels.shape[1]))
+    _check(_cudamat.embed(mat.p_mat, labels.p_mat, target.p_mat, float(mult)))
+    return target
+
+
+def embed_grad(deriv, labels, target, mult=1.0, beta=0.0):
+    """Extension of this backend (not in the reference): the backward pass of embed(mat, labels, mult=mult) from deriv, the derivative by its
+    result: column t of target (the shape of mat) = beta * column t + mult * (sum of the columns of deriv whose label is t, added in an
+    order that depends on the labels alone).  beta = 0 does not read the target and writes all of it; with beta = 1 columns of other tokens are not touched."""
+    _check(_cudamat.embed_grad(deriv.p_mat, labels.p_mat, target.p_mat, float(beta), float(mult)))
+    return target
+
+
+def gated_scan(pre, target=None, offsets=None, sequences=0, state=None, last=None):
+    """Extension of this backend (not in the reference): a gated linear recurrence along the columns of sequences.  With the 2 f rows of
+    pre = [g; u] and a = sigmoid(g),
+        target(:, t) = a_t * target(:, t - 1) + (1 - a_t) * u_t
+    from the sequence's column of state (f x sequences; None: zeros), which stands before its first column.  last (f x sequences, which
+    may be state), where given, receives every sequence's last column, of a sequence without columns its state.
+        offsets     1 x (sequences + 1) whole numbers as floats that do not fall: sequence q has the columns from offsets[q] to before
+                    offsets[q + 1].  Columns that belong to none are left as they are.
+        sequences   without offsets, into how many sequences of equal length the columns are divided (0: as many as the states have, or one).
+                    One column each: a step of decoding."""
+    if target is None:
+        target = empty((pre.shape[0] // 2, pre.shape[1]))
+    _check(_cudamat.gated_scan(pre.p_mat, _p(offsets), _p(state), target.p_mat, _p(last), int(sequences)))
+    return target
+
+
+def gated_scan_grad(deriv, pre, out, target=None, offsets=None, sequences=0, state=None, last_deriv=None, state_grad=None):
+    """Extension of this backend (not in the reference): the backward pass of out = gated_scan(pre, offsets=offsets, sequences=sequences,
+    state=state) from deriv, the derivative by its result, and last_deriv, that by its last columns (f x sequences; None: zeros).
+    target = the derivative by pre (in its place by default); state_grad, where given, that by state (it may be last_deriv)."""
+    if target is None:
+        target = pre
+    _check(_cudamat.gated_scan_grad(deriv.p_mat, pre.p_mat, out.p_mat, _p(offsets), _p(state), _p(last_deriv), target.p_mat, _p(state_grad),
+                                    int(sequences)))
+    return target
+
+
+def sample_tokens(mat, uniform, target=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logp=None):
+    """Extension of this backend (not in the reference): target (1 x columns) = a token of every column of logits (vocabulary x columns),
+    drawn by the column's number in uniform (1 x columns, from [0, 1)).  With weights w_i = exp((x_i - greatest x) / temperature),
+    kept are the entries that come first when they are ordered (the greater first, of equal ones the one further up): at most top_k of them, those
+    whose weight is at least min_p, and of these as few as have top_p of their weight together, one at least.  The token is the first kept
+    one, from the top of the column, up to which the kept weights sum to more than uniform times all of them.  logp (1 x columns), where given,
+    receives the token's log probability among the kept ones.
+        temperature, top_k, top_p, min_p   numbers for all columns, or 1 x columns with each column's own.  temperature 0: the greatest
+                    entry (logp 0); top_k 0, top_p 1, min_p 0: no such limit.
+    Entries of -infinity are never drawn; where there are no others the token is -1 (logp 0), with NaN or +infinity in the column -1 (NaN)."""
+    if target is None:
+        target = empty((1, mat.shape[1]))
+    rows, numbers = [], []
+    for v in (temperature, top_k, top_p, min_p):
+        row = isinstance(v, CUDAMatrix)
+        rows.append(v.p_mat if row else None)
+        numbers.append(0.0 if row else float(v))
+    _check(_cudamat.sample_tokens(mat.p_mat, uniform.p_mat, *rows, target.p_mat, _p(logp), *numbers))
     return target
 
 

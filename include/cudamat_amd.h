@@ -381,6 +381,37 @@ int log_probs(cudamat* mat, cudamat* labels, cudamat* logp, cudamat* entropy, cu
 int log_probs_grad(cudamat* mat, cudamat* labels, cudamat* log_z, cudamat* logp_weight, cudamat* entropy, cudamat* entropy_weight,
                    cudamat* target);
 
+/* Columns of a table by token: target(:, c) = mult * mat(:, labels[c]), 0 where a label is no token (outside [0, columns of mat), NaN).
+ * mat: features x vocabulary (at most 2^24), labels: 1 x columns, tokens as floats. */
+int embed(cudamat* mat, cudamat* labels, cudamat* target, float mult);
+/* Its gradient: target(:, t) = beta * target(:, t) + mult * (sum of the columns of deriv whose label is t).  beta = 0 reads nothing and
+ * writes every column; beta = 1 leaves columns without a label untouched.  The same labels give the same order of addition. */
+int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, float mult);
+
+/* A gated linear recurrence along the columns of sequences: with pre = [g; u] (2 f x columns) and a = sigmoid(g),
+ * target(:, t) = a_t target(:, t - 1) + (1 - a_t) u_t, from the sequence's column of state (f x sequences, or NULL: zeros) before its
+ * first one.  last (f x sequences, may be state, or NULL): the last column of every sequence, of one without columns its state.
+ * offsets: 1 x (sequences + 1) whole numbers as floats, not falling (up to 2^24 columns): sequence q has the columns [offsets[q], offsets[q + 1]);
+ * columns of no sequence are left as they are.  Offsets that fall or leave the matrix give results of no meaning, within the matrices.
+ * NULL: the columns are divided evenly.  sequences: 0 for as many as offsets or states have, or one.
+ * Infinities and NaN make what follows them in their sequence infinite or NaN, and nothing else. */
+int gated_scan(cudamat* pre, cudamat* offsets, cudamat* state, cudamat* target, cudamat* last, int sequences);
+/* Its gradients from deriv, the derivative by out (its target), and last_deriv, that by last (or NULL: zeros): target = derivative by pre (may be
+ * pre), state_grad = derivative by state (or NULL; may be last_deriv). */
+int gated_scan_grad(cudamat* deriv, cudamat* pre, cudamat* out, cudamat* offsets, cudamat* state, cudamat* last_deriv, cudamat* target,
+                    cudamat* state_grad, int sequences);
+
+/* Tokens drawn from columns of logits (vocabulary x columns, at most 2^24 rows) by given uniform numbers (1 x columns).  Weights
+ * w_i = e^((x_i - greatest x) / temperature); in the order of the entries (the greater first, of equal ones the one further up) the first are kept: at most top_k,
+ * those with w_i >= min_p, and of these as few as have top_p of their weight together, one at least.  target (1 x columns): the first kept
+ * entry, from the top of the column, up to which the kept weights sum to more than uniform (taken into [0, 1]) times all of them.  logp (1 x columns, or NULL): its
+ * log probability among the kept ones.  temperature, top_k, top_p, min_p: 1 x columns, or NULL for the numbers all_*.  A temperature that is not
+ * above 0: the greatest entry, logp 0; top_k < 1, top_p >= 1, min_p <= 0 and NaN: no such limit.  Weights are held as whole multiples of 2^-45 (of
+ * more than 2^17 rows less, 2^-38 of 2^24), and entries of less than half of that are never drawn.  A column of nothing but -infinity gives -1 and logp 0,
+ * one with NaN or +infinity -1 and NaN. */
+int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperature, cudamat* top_k, cudamat* top_p, cudamat* min_p, cudamat* target,
+                  cudamat* logp, float all_temperature, float all_top_k, float all_top_p, float all_min_p);
+
 /* ---- HIP graphs: no counterpart in the reference.  graph_capture_begin() makes the library
  * record every following call (with the pointers and scalars it is given) into a HIP graph
  * instead of running it, until graph_capture_end() returns the executable graph;

@@ -19,6 +19,9 @@ bool dn_scratch_holds(size_t bytes, int slot = 0);   // whether that much is the
 // n 32-bit words that are zero between kernels (arrival counters); null when they cannot be had.
 unsigned* dn_zero_words(int n);
 bool dn_zero_words_hold(int n);
+// n 64-bit words that nothing but kernels of one kind writes, all zero at first: what a workgroup hands to another one of its launch
+// stands there with the number of the launch beside it, so nothing has to be cleared in between.  Null when they cannot be had.
+unsigned long long* dn_tagged_words(size_t n);
 // f is called when the last executable graph that this library made has been freed.
 void dn_set_no_graphs_hook(void (*f)());
 

@@ -221,6 +221,32 @@ unsigned* dn_zero_words(int n) {
 }
 bool dn_zero_words_hold(int n) { return n <= g_zero_words_n; }
 
+// Words that name the launch that wrote them (see common.h).
+static unsigned long long* g_tagged_words = nullptr;
+static size_t g_tagged_words_n = 0;
+static bool g_tagged_words_recorded = false;
+
+unsigned long long* dn_tagged_words(size_t n) {
+  dn_flush();
+  if (n > g_tagged_words_n) {
+    if (g_capturing) return nullptr;
+    if (g_tagged_words) {
+      hipDeviceSynchronize();
+      if (g_tagged_words_recorded) g_retired.push_back(g_tagged_words);   // (as for the scratch blocks)
+      else hipFree(g_tagged_words);
+      g_tagged_words_recorded = false;
+      g_tagged_words = nullptr;
+      g_tagged_words_n = 0;
+    }
+    const size_t want = n < (1u << 18) ? (1u << 18) : n;
+    if (dn_malloc((void**)&g_tagged_words, want * sizeof(unsigned long long)) != hipSuccess) { g_tagged_words = nullptr; return nullptr; }
+    if (hipMemset(g_tagged_words, 0, want * sizeof(unsigned long long)) != hipSuccess || hipDeviceSynchronize() != hipSuccess) return nullptr;
+    g_tagged_words_n = want;
+  }
+  if (g_capturing) g_tagged_words_recorded = true;
+  return g_tagged_words;
+}
+
 // ------------------------------------------------------------------ kernels
 
 // Column-major row-band copy: dst(r, c) = src(r + row0, c) for a band of `rows`
@@ -330,6 +356,10 @@ int cuda_set_device(int deviceId) {
     g_zero_words = nullptr;
     g_zero_words_n = 0;
     g_zero_words_recorded = false;
+    if (g_tagged_words) hipFree(g_tagged_words);
+    g_tagged_words = nullptr;
+    g_tagged_words_n = 0;
+    g_tagged_words_recorded = false;
     hipSetDevice(deviceId);
   }
   return 0;
@@ -447,7 +477,7 @@ int graph_free(void* exec) {
     for (void* p : g_retired) hipFree(p);
     g_retired.clear();
     for (bool& r : g_scratch_recorded) r = false;
-    g_zero_words_recorded = false;
+    g_zero_words_recorded = g_tagged_words_recorded = false;
     if (g_no_graphs_hook) g_no_graphs_hook();
   }
   return e == hipSuccess ? 0 : CUDA_ERROR;

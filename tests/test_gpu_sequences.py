@@ -64,7 +64,7 @@ def check_embed_grad(got, dy, labels, n, mult=1.0, old=None, beta=0.0):
     check(got, was + want, U * ((count[None, :] + 2) * size + 3 * (np.abs(was) + np.abs(want))))
 
 
-@pytest.mark.parametrize("h,w,n", EMBED_SHAPES + [(20, 5000, 1), (33, 9000, 7), (130, 3000, 300), (17, 20001, 256), (64, 3000, 40000), (1, 30000, 5), (260, 2049, 2)])
+@pytest.mark.parametrize("h,w,n", EMBED_SHAPES + [(20, 5000, 1), (33, 9000, 7), (130, 3000, 300), (17, 20001, 256), (64, 3000, 40000), (1, 30000, 5), (260, 2049, 2), (1025, 40, 6), (2050, 33, 3), (306177, 3, 2)])
 @pytest.mark.parametrize("skip", [0, 1])
 def test_embed_grad(cm, rng, h, w, n, skip):
     dy, labels = F(rng.standard_normal((h, w))), frequent(rng, n, w)
@@ -96,6 +96,12 @@ def test_embed_grad_of_one_frequent_token(cm, rng, w):
         labels[0, rng.choice(w + 7, 3, replace=False)] = others[1]
         g = cm.embed_grad(cm.CUDAMatrix(dy), cm.CUDAMatrix(labels), cm.CUDAMatrix(F(np.full((h, n), np.nan))))
         check_embed_grad(g.asarray(), dy, labels, n)
+
+
+def test_embed_of_no_vocabulary(cm):
+    y = cm.CUDAMatrix(F(np.full((6, 5), np.nan)))
+    cm.embed(cm.empty((6, 0)), cm.CUDAMatrix(F([[0, 1, -1, 2, 3]])), target=y)
+    assert not y.asarray().any()
 
 
 def test_embed_grad_of_no_columns_and_of_no_tokens(cm, rng):

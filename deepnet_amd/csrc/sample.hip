@@ -74,19 +74,37 @@ __device__ __forceinline__ unsigned long long sample_part_up(double part, unsign
 
 typedef unsigned long long u64;
 
+// Sums of 64-bit numbers over the lanes before and including this one, by the cross-lane paths of the vector unit.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 lane_add_u64(u64 v) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_scan_u64(u64 v) {
+  v = lane_add_u64<0x111, 0xf>(v);           // rows of 16: one, two, four, eight lanes back
+  v = lane_add_u64<0x112, 0xf>(v);
+  v = lane_add_u64<0x114, 0xf>(v);
+  v = lane_add_u64<0x118, 0xf>(v);
+  v = lane_add_u64<0x142, 0xa>(v);           // the row before
+  return lane_add_u64<0x143, 0xc>(v);        // the two rows before
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
+}
+
 #define SAMPLE_LIST 4096           // candidates that are sorted
-#define SAMPLE_SHORT 256           // candidates whose places are counted instead, each by a lane
+#define SAMPLE_SHORT 256           // ... whose places are counted instead
 template <int LANES>
 struct SampleShared {
   static constexpr int WAVES = LANES / 64, BINS = LANES;
   double table[SAMPLE_STEPS];
-  u64 list[SAMPLE_LIST + 2];       // keys of candidates, or the weights of stretches of the column
+  u64 list[SAMPLE_LIST + 2];       // keys of candidates
   u64 masses[BINS];
   u64 sorted[SAMPLE_SHORT];
   int counts[BINS];
   u64 wave_sum[WAVES];
   float wave_max[WAVES], wave_min[WAVES];
-  int wave_bad[WAVES], listed, place, cell;
+  int wave_bad[WAVES], listed, place, owner;
   u64 border, base;
 };
 
@@ -94,8 +112,7 @@ struct SampleShared {
 template <int LANES>
 __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const u64 q = __shfl_up(v, o, WAVE); if (lane >= o) v += q; }
+  v = wave_scan_u64(v);
   __syncthreads();
   if (lane == 63) wave_sum[wv] = v;
   __syncthreads();
@@ -106,7 +123,29 @@ __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
   return v;
 }
 
-// The keys of a list, the greatest first: a bitonic sort of `size` (a power of two, at least the list's length) with zeros behind the list.
+// Bitonic sorts, the greatest first, of `size` keys (a power of two).  One of up to LANES keys, a lane each: lane i gets the i-th; steps within a wavefront
+// are shuffles, the others go through `room`.
+template <int LANES>
+__device__ __forceinline__ u64 sample_sort_lanes(u64 key, u64* room, int size) {
+  const int tid = threadIdx.x;
+  for (int run = 2; run <= size; run *= 2)
+    for (int gap = run / 2; gap > 0; gap /= 2) {
+      u64 other;
+      if (gap < 64) {
+        other = __shfl_xor(key, gap, WAVE);
+      } else {
+        __syncthreads();
+        room[tid] = key;
+        __syncthreads();
+        other = room[tid ^ gap];
+      }
+      const bool greater = ((tid & gap) == 0) == ((tid & run) == 0);
+      key = (other > key) == greater ? other : key;
+    }
+  __syncthreads();
+  return key;
+}
+// One of a list in LDS; zeros are put behind its n keys.
 template <int LANES>
 __device__ __forceinline__ void sample_sort(u64* list, int n, int size) {
   for (int i = n + threadIdx.x; i < size; i += LANES) list[i] = 0;
@@ -122,12 +161,12 @@ __device__ __forceinline__ void sample_sort(u64* list, int n, int size) {
     }
 }
 
-// The entries of a column, four rows a lane and slab: in registers (NV slabs) or, of columns that those do not hold (NV = 0), from memory, where
-// eight slabs are on their way at once.  f(x, row) for a lane's four, rows behind the column being -infinity.
+// The entries of a column: a wavefront has a stretch of it, 256 rows a slab, four of them a lane; in registers (NV slabs) or, of columns that those do not hold
+// (NV = 0), from memory, where eight slabs are on their way at once.  f(x, row, slab) for a lane's four, rows behind the column being -infinity.
 template <int LANES, int NV>
 struct SampleColumn {
   const float* c;
-  int h;
+  int h, from, slabs;              // the stretch's first row of this lane, slabs of a stretch
   float x[NV ? NV : 1][4];
   __device__ __forceinline__ void fetch(float (&v)[4], int row) const {
 #pragma unroll
@@ -139,10 +178,14 @@ struct SampleColumn {
         if (row + e < h) v[e] = c[row + e];
     }
   }
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void init(const float* column, int rows) {
+    c = column; h = rows;
+    slabs = (h + 4 * LANES - 1) / (4 * LANES);
+    from = (int)(threadIdx.x >> 6) * slabs * 256 + 4 * (int)(threadIdx.x & 63);
     if (NV) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) fetch(x[k], 4 * (threadIdx.x + LANES * k));
+      for (int k = 0; k < NV; ++k)
+        if (k < slabs) fetch(x[k], from + 256 * k);
     }
   }
   template <typename F>
@@ -150,49 +193,74 @@ struct SampleColumn {
     if (NV) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (4 * LANES * k < h) {
+        if (k < slabs) {
           float v[4];
+          int row = from + 256 * k;
+          // (what one pass makes of an entry or a row is not kept in registers for the next)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { v[e] = x[k][e]; asm volatile("" : "+v"(v[e])); }      // (what one pass makes of an entry is not kept for the next)
-          int row = 4 * (int)(threadIdx.x + LANES * k);
+          for (int e = 0; e < 4; ++e) { v[e] = x[k][e]; asm volatile("" : "+v"(v[e])); }
           asm volatile("" : "+v"(row));
-          f(v, row);
+          f(v, row, k);
           __builtin_amdgcn_sched_barrier(0);
         }
     } else {
-      for (int k = 0; 4 * LANES * k < h; k += 8) {
+      for (int k = 0; k < slabs; k += 8) {
         float v[8][4];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) fetch(v[q], 4 * (threadIdx.x + LANES * (k + q)));
+        for (int q = 0; q < 8; ++q) fetch(v[q], from + 256 * (k + q));
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          if (4 * LANES * (k + q) < h) f(v[q], 4 * (int)(threadIdx.x + LANES * (k + q)));
+          if (k + q < slabs) { f(v[q], from + 256 * (k + q), k + q); __builtin_amdgcn_sched_barrier(0); }
       }
     }
   }
 };
 
-// Kept entries: those from `border` on in the order of keys whose weight reaches `least`.
+// Kept entries: those from the border on in the order of keys whose weight reaches `least`.
 struct SampleKept {
   float m, far, x;                 // the greatest entry; entries further from it than `far` have no weight; the last kept value,
   int row;                         // and of entries of that value the last kept row
   double c;
   int shift;
+  bool all;                        // no border, no least
   u64 least;
   const double* table;
   __device__ __forceinline__ bool near(float v) const { return v > -INFINITY && m - v <= far; }
   __device__ __forceinline__ bool in(float v, int i) const { return near(v) && (v > x || (v == x && i <= row)); }
   __device__ __forceinline__ u64 weight(float v) const {
     const u64 w = sample_weight(v, m, c, shift, table);
-    __builtin_amdgcn_sched_barrier(0);                     // (one at a time: registers)
     return w >= least ? w : 0;
   }
-  __device__ __forceinline__ void from(u64 border) { x = lp_key_value(border); row = lp_key_index(border); }
+  // of four rows; those of a wavefront without a kept entry are not computed
+  __device__ __forceinline__ void weights(u64 (&w)[4], const float (&v)[4], int i) const {
+    if (all) {
+      const float end = m - far;   // (from there on a weight is nothing)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = sample_weight(fmaxf(v[e], end), m, c, shift, table);
+    } else {
+      bool there[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { there[e] = in(v[e], i + e); w[e] = 0; }
+      if (__any(there[0] || there[1] || there[2] || there[3])) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = there[e] ? weight(v[e]) : 0;
+      }
+    }
+  }
+  __device__ __forceinline__ void from(u64 border) { x = lp_key_value(border); row = lp_key_index(border); all = false; }
 };
-
 __device__ __forceinline__ void sample_out(const SampleArgs& a, int col, const SampleKept& kept, float v, int row, u64 total) {
   a.tokens[col] = (float)row;
   if (a.logp) a.logp[col] = (float)(((double)v - (double)kept.m) * (kept.c * 0.6931471805599453) - dn_log_wide_pos(ldexp((double)total, -a.shift)));
+}
+__device__ __forceinline__ u64 sample_aim(const SampleRule& rule, u64 total) {
+  const u64 at = sample_part((double)rule.u, total);
+  return at < total ? at : total - 1;
+}
+// The weights that top_p asks for.
+__device__ __forceinline__ u64 sample_ask(const SampleRule& rule, u64 total) {
+  const u64 part = rule.top_p < 1.0 ? (rule.top_p > 0.0 ? sample_part_up(rule.top_p, total) : 0) : total;
+  return part > 1 ? part : 1;
 }
 
 // The greatest border that leaves enough: bit by bit, a pass over the column each.  For columns whose border lies among thousands of
@@ -203,7 +271,7 @@ __device__ __forceinline__ u64 sample_bisect(const SampleColumn<LANES, NV>& colu
   for (int bit = 63; bit >= 0; --bit) {
     const u64 trial = border | 1ull << bit;
     u64 sum = 0, all;
-    column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (kept.in(v[e], row + e) && lp_key(v[e], row + e) >= trial) sum += value(v[e]);
@@ -214,50 +282,107 @@ __device__ __forceinline__ u64 sample_bisect(const SampleColumn<LANES, NV>& colu
   return border;
 }
 
-// From n listed candidates: the border, which the list contains, of the first k (by_count: of those the first that have top_p of their weight), or the one where
-// the weights, mass_before ahead of the list, reach `ask`.  Returns 0 where they do not.  A lane has EACH neighbours of the sorted list.
-template <int LANES, int EACH>
-__device__ __forceinline__ u64 sample_cut(const u64* sorted, int n, const SampleRule& rule, const SampleKept& kept, SampleShared<LANES>& sh, bool by_count, u64 mass_before,
-                                          u64 ask) {
+// All that may be kept is listed, n <= LANES entries: draws, unless their weights do not reach `ask` (false; by_count: what top_p asks for of the first k).
+template <int LANES>
+__device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, int n, const SampleRule& rule, const SampleKept& kept, SampleShared<LANES>& sh, bool by_count, u64 ask) {
   const int tid = threadIdx.x;
+  u64 key = 0;
+  int size = 2;
+  while (size < n) size *= 2;
+  if (n <= SAMPLE_SHORT) {                                 // places by counting
+    if (tid < 2) sh.list[n + tid] = 0;
+    __syncthreads();
+    if (tid < n) {
+      const u64 own = sh.list[tid];
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.list + i);
+        rank += (q.x > own ? 1 : 0) + (q.y > own ? 1 : 0);
+      }
+      sh.sorted[rank] = own;
+    }
+    __syncthreads();
+    if (tid < n) key = sh.sorted[tid];
+  } else {
+    key = sample_sort_lanes<LANES>(tid < n ? sh.list[tid] : 0, sh.list, size);
+  }
+  const float v = lp_key_value(key);
+  const int row = lp_key_index(key);
+  u64 w = tid < n && (!by_count || tid < rule.k) ? kept.weight(v) : 0, all;
+  const u64 up_to = sample_scan<LANES>(w, sh.wave_sum, &all) - w;
+  if (by_count) ask = sample_ask(rule, all);
+  if (all < ask) return false;
+  if (up_to >= ask) w = 0;                                 // (not kept)
+  else if (w && up_to + w >= ask) sh.base = up_to + w;     // (one of them)
+  sh.masses[tid] = w;
+  if (n <= SAMPLE_SHORT && tid < n) sh.list[tid] = (u64)(unsigned)row;
+  __syncthreads();
+  const u64 total = sh.base, aim = sample_aim(rule, total);
+  if (n <= SAMPLE_SHORT) {                                 // each adds the weights of those further up in the column
+    if (w) {
+      u64 sum = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) sum += (int)sh.list[i] < row ? sh.masses[i] : 0;
+      if (sum <= aim && sum + w > aim) sample_out(a, col, kept, v, row, total);
+    }
+  } else {
+    const u64 place = sample_sort_lanes<LANES>(w ? (u64)(unsigned)~row << 32 | (unsigned)tid : 0, sh.list, size);
+    const u64 mass = place ? sh.masses[(unsigned)place] : 0, sum = sample_scan<LANES>(mass, sh.wave_sum, &all) - mass;
+    if (mass && sum <= aim && sum + mass > aim) {
+      const int at = (int)~(unsigned)(place >> 32);
+      sample_out(a, col, kept, a.mat[(size_t)col * a.h + at], at, total);
+    }
+  }
+  return true;
+}
+
+// The border, which lies in the list of n: of the first k (by_count), or where the weights, mass_before ahead of the list, reach `ask`.
+template <int LANES>
+__device__ __forceinline__ u64 sample_cut(int n, const SampleRule& rule, const SampleKept& kept, SampleShared<LANES>& sh, bool by_count, u64 mass_before, u64 ask) {
+  constexpr int EACH = SAMPLE_LIST / LANES;
+  const int tid = threadIdx.x;
+  int size = 2;
+  while (size < n) size *= 2;
+  sample_sort<LANES>(sh.list, n, size);
   u64 w[EACH], sum = 0, all;
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
     const int i = EACH * tid + k;
-    w[k] = i < n && (!by_count || i < rule.k) ? kept.weight(lp_key_value(sorted[i])) : 0;
+    w[k] = i < n && (!by_count || i < rule.k) ? kept.weight(lp_key_value(sh.list[i])) : 0;
     sum += w[k];
   }
   u64 up_to = sample_scan<LANES>(sum, sh.wave_sum, &all) - sum + mass_before;
-  if (by_count) ask = rule.top_p < 1.0 ? (rule.top_p > 0.0 ? sample_part_up(rule.top_p, all) : 0) : all;
-  if (ask < 1) ask = 1;
-  if (tid == 0) sh.border = 0;
-  __syncthreads();
+  if (by_count) ask = sample_ask(rule, all);
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
-    if (w[k] && up_to < ask && up_to + w[k] >= ask) { sh.border = sorted[EACH * tid + k]; sh.base = up_to + w[k]; }      // (one of them)
+    if (w[k] && up_to < ask && up_to + w[k] >= ask) sh.border = sh.list[EACH * tid + k];      // (one of them)
     up_to += w[k];
   }
   __syncthreads();
   return sh.border;
 }
 
-// The border that top-k and top-p set, for a pass over the column to draw by (true), or, where all that is kept has been listed and is little, the token
-// itself.  Candidates are chosen by the bin of their distance to the greatest entry.
-// At least k entries lie in the bins up to that of the k-th of the lanes' maxima, and not many more: these are listed.  Without a top-k 128 are, in the hope
-// that they have enough of the weight.  Otherwise all entries are counted (without a top-k: weighed) bin by bin, and those of the bin of the
-// border (with a top-k: of all up to it) are listed.
+// Finds what top-k and top-p keep: the border, for a pass over the column to draw by (true), or, where all that is kept has been listed and is little, draws.
+// Candidates are chosen by the bin of their distance to the greatest entry.  At least k entries lie in the bins up to that of the k-th of 2 LANES maxima of
+// parts of the column, and not many more.  Otherwise, and without a top-k, all entries are counted (weighed) bin by bin, and those of the bins up to
+// the border's are listed, or where they are many those of its own.
 template <int LANES, int NV>
-__device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, const SampleColumn<LANES, NV>& column, const SampleRule& rule, SampleKept& kept, float mine, float least_x,
-                                              SampleShared<LANES>& sh) {
+__device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, const SampleColumn<LANES, NV>& column, const SampleRule& rule, SampleKept& kept, const float (&mine)[2],
+                                              float least_x, SampleShared<LANES>& sh) {
   constexpr int BINS = SampleShared<LANES>::BINS;
   const int tid = threadIdx.x;
   const bool by_count = rule.k < column.h;
   const float scale = fminf((float)BINS / fminf(kept.far, kept.m - least_x), 3e38f);
   auto bin = [&](float v) __attribute__((always_inline)) { return (int)fminf((kept.m - v) * scale, (float)(BINS - 1)); };
-  auto list_bins = [&](int first, int place) __attribute__((always_inline)) {
-    if (tid == 0) sh.listed = 0;
+  auto clear = [&](int place) __attribute__((always_inline)) {
+    sh.counts[tid] = 0;
+    sh.masses[tid] = 0;
+    if (tid == 0) { sh.place = place; sh.listed = 0; }
     __syncthreads();
-    column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
+  };
+  auto list_bins = [&](int first, int place) __attribute__((always_inline)) {
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (kept.near(v[e])) {
@@ -271,112 +396,57 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, cons
     __syncthreads();
     return sh.listed;
   };
-  u64 total = 0, ask = 0;
-  if (!by_count) {
-    u64 sum = 0;
-    column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
-      if (__any(kept.near(v[0]) || kept.near(v[1]) || kept.near(v[2]) || kept.near(v[3]))) {
+  u64 ignored;
+  if (by_count && rule.k <= LANES) {
+    clear(BINS - 1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += kept.near(v[e]) ? kept.weight(v[e]) : 0;
-      }
-    });
-    sample_scan<LANES>(sum, sh.wave_sum, &total);
-    ask = rule.top_p > 0.0 ? sample_part_up(rule.top_p, total) : 1;
-  }
-  const int some = by_count ? rule.k : 128;
-  if (some <= LANES / 2) {
-    sh.counts[tid] = 0;
-    if (tid == 0) sh.place = BINS - 1;
+    for (int k = 0; k < 2; ++k)
+      if (kept.near(mine[k])) atomicAdd(&sh.counts[bin(mine[k])], 1);
     __syncthreads();
-    if (kept.near(mine)) atomicAdd(&sh.counts[bin(mine)], 1);
-    __syncthreads();
-    u64 all;
-    const u64 here = (u64)sh.counts[tid], up = sample_scan<LANES>(here, sh.wave_sum, &all);
-    if (up >= (u64)some && up - here < (u64)some) sh.place = tid;
+    const u64 here = (u64)sh.counts[tid], up = sample_scan<LANES>(here, sh.wave_sum, &ignored);
+    if (up >= (u64)rule.k && up - here < (u64)rule.k) sh.place = tid;
     __syncthreads();
     const int n = list_bins(0, sh.place);
-    if (n <= SAMPLE_SHORT) {
-      // places by counting
-      if (tid < 2) sh.list[n + tid] = 0;
-      __syncthreads();
-      if (tid < n) {
-        const u64 key = sh.list[tid];
-        int rank = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; i += 2) {
-          const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.list + i);
-          rank += (q.x > key ? 1 : 0) + (q.y > key ? 1 : 0);
-        }
-        sh.sorted[rank] = key;
-      }
-      __syncthreads();
-      const u64 border = sample_cut<LANES, 1>(sh.sorted, n, rule, kept, sh, by_count, 0, ask);
-      if (border) {
-        // the kept ones draw: each adds the weights of those further up in the column
-        const u64 key = tid < n ? sh.sorted[tid] : 0, kept_total = sh.base;
-        const float v = lp_key_value(key);
-        const int row = lp_key_index(key);
-        const u64 w = key >= border ? kept.weight(v) : 0;
-        if (tid < SAMPLE_SHORT) { sh.masses[tid] = w; sh.list[tid] = (u64)(unsigned)row; }
-        __syncthreads();
-        const u64 at = sample_part((double)rule.u, kept_total), aim = at < kept_total ? at : kept_total - 1;
-        if (w) {
-          u64 up_to = 0;
-#pragma unroll 4
-          for (int i = 0; i < n; ++i) up_to += (int)sh.list[i] < row ? sh.masses[i] : 0;
-          if (up_to <= aim && up_to + w > aim) sample_out(a, col, kept, v, row, kept_total);
-        }
-        return false;
-      }
-    } else if (n <= SAMPLE_LIST) {
-      int size = 512;
-      while (size < n) size *= 2;
-      sample_sort<LANES>(sh.list, n, size);
-      const u64 border = sample_cut<LANES, SAMPLE_LIST / LANES>(sh.list, n, rule, kept, sh, by_count, 0, ask);
-      if (border) { kept.from(border); return true; }
-    }
+    if (n <= LANES) { sample_from_list<LANES>(a, col, n, rule, kept, sh, true, 0); return false; }
+    if (n <= SAMPLE_LIST) { kept.from(sample_cut<LANES>(n, rule, kept, sh, true, 0, 0)); return true; }
     __syncthreads();
   }
-  sh.counts[tid] = 0;
-  sh.masses[tid] = 0;
-  if (tid == 0) sh.place = BINS;
-  __syncthreads();
-  column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
+  clear(BINS);
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    bool there[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) there[e] = kept.near(v[e]);
+    if (!__any(there[0] || there[1] || there[2] || there[3])) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (kept.near(v[e])) {
+      if (there[e]) {
         const int b = bin(v[e]);
         atomicAdd(&sh.counts[b], 1);
         if (!by_count) atomicAdd(&sh.masses[b], kept.weight(v[e]));
       }
   });
   __syncthreads();
-  u64 ignored;
-  const u64 here = by_count ? (u64)sh.counts[tid] : sh.masses[tid], want = by_count ? (u64)rule.k : ask, up = sample_scan<LANES>(here, sh.wave_sum, &ignored);
-  if (up >= want && up - here < want) { sh.place = tid; sh.base = up - here; }      // (one lane at most)
+  u64 total;
+  const u64 count = (u64)sh.counts[tid], mass = sh.masses[tid], up_count = sample_scan<LANES>(count, sh.wave_sum, &ignored), up_mass = sample_scan<LANES>(mass, sh.wave_sum, &total);
+  const u64 ask = by_count ? 0 : sample_ask(rule, total), want = by_count ? (u64)rule.k : ask, here = by_count ? count : mass, up = by_count ? up_count : up_mass;
+  if (up >= want && up - here < want) { sh.place = tid; sh.base = up_mass - mass; sh.border = up_count; }      // (one lane at most)
   __syncthreads();
   const int place = sh.place;                              // (BINS: fewer candidates than k)
-  const u64 mass_before = by_count ? 0 : sh.base;
-  const int n = list_bins(by_count ? 0 : place, place);
-  if (n <= SAMPLE_LIST) {
-    int size = 2;
-    while (size < n) size *= 2;
-    sample_sort<LANES>(sh.list, n, size);
-    const u64 border = sample_cut<LANES, SAMPLE_LIST / LANES>(sh.list, n, rule, kept, sh, by_count, mass_before, ask);
-    kept.from(border);
-    return true;
-  }
+  const bool all_of_them = by_count || sh.border <= LANES;
+  const u64 mass_before = all_of_them ? 0 : sh.base;
+  const int n = list_bins(all_of_them ? 0 : place, place);
+  if (n <= LANES && all_of_them) { sample_from_list<LANES>(a, col, n, rule, kept, sh, by_count, ask); return false; }
+  if (n <= SAMPLE_LIST) { kept.from(sample_cut<LANES>(n, rule, kept, sh, by_count, mass_before, ask)); return true; }
   if (by_count && place < BINS) kept.from(sample_bisect(column, kept, sh, (u64)rule.k, [](float) { return (u64)1; }));
   if (rule.top_p < 1.0) {
     u64 sum = 0;
-    column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (kept.in(v[e], row + e)) sum += kept.weight(v[e]);
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      u64 w[4];
+      kept.weights(w, v, row);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
     });
     sample_scan<LANES>(sum, sh.wave_sum, &total);
-    const u64 p = rule.top_p > 0.0 ? sample_part_up(rule.top_p, total) : 0;
-    kept.from(sample_bisect(column, kept, sh, p > 1 ? p : 1, [&](float v) __attribute__((always_inline)) { return kept.weight(v); }));
+    kept.from(sample_bisect(column, kept, sh, sample_ask(rule, total), [&](float v) __attribute__((always_inline)) { return kept.weight(v); }));
   }
   return true;
 }
@@ -385,31 +455,28 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, cons
 // Weights are whole numbers (sample_weight), so every sum and with it every border is the same however it is added up.
 template <int LANES, int NV>
 __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
-  constexpr int W = LANES / 64, CELLS = SAMPLE_LIST;
+  constexpr int W = LANES / 64;
   __shared__ SampleShared<LANES> sh;
   const int col = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   SampleColumn<LANES, NV> column;
-  column.c = a.mat + (size_t)col * a.h;
-  column.h = a.h;
-  column.init();
+  column.init(a.mat + (size_t)col * a.h, a.h);
   const SampleRule rule = sample_rule(a, col);
-  float most = -INFINITY, least = INFINITY;
+  float mine[2] = {-INFINITY, -INFINITY}, least = INFINITY;
   bool bad = false;
-  column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
+  if (tid < SAMPLE_STEPS) sh.table[tid] = sample_step(tid);
+  column.each([&](const float (&v)[4], int row, int slab) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       bad |= !(v[e] < INFINITY);
-      most = fmaxf(most, v[e]);
+      mine[e & 1] = fmaxf(mine[e & 1], v[e]);
       least = fminf(least, v[e] > -INFINITY ? v[e] : INFINITY);
     }
   });
-  const float mine = most;
-  most = lanes_sum<64, true>(most);
+  float most = lanes_sum<64, true>(fmaxf(mine[0], mine[1]));
   least = -lanes_sum<64, true>(-least);
   bad = __any(bad);
   if (lane == 0) { sh.wave_max[wv] = most; sh.wave_min[wv] = least; sh.wave_bad[wv] = bad; }
   if (tid == 0) sh.place = a.h;
-  if (tid < SAMPLE_STEPS) sh.table[tid] = sample_step(tid);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < W; ++k) { most = fmaxf(most, sh.wave_max[k]); least = fminf(least, sh.wave_min[k]); bad |= sh.wave_bad[k] != 0; }
@@ -418,7 +485,7 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
     return;
   }
   if (rule.greedy) {
-    column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 3; e >= 0; --e)
         if (v[e] == most) atomicMin(&sh.place, row + e);
@@ -430,70 +497,43 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
   SampleKept kept;
   kept.m = most; kept.x = -INFINITY; kept.row = 0; kept.c = rule.c; kept.shift = a.shift; kept.least = rule.least; kept.table = sh.table;
   kept.far = (float)((a.shift + 1.5) / rule.c);            // (2^-(shift + 1) is nothing; half an octave for the rounding of the distance)
-  if ((rule.k < a.h || rule.top_p < 1.0) && !sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
-  __syncthreads();
-  // the kept weights of every wavefront's part of a slab (256 rows); of more slabs than there is room for, of several slabs
-  const int slabs = (a.h + 4 * LANES - 1) / (4 * LANES), cells = slabs * W, fold = (cells + CELLS - 1) / CELLS;
-  if (fold > 1)
-    for (int k = tid; k < CELLS; k += LANES) sh.list[k] = 0;
-  __syncthreads();
-  column.each([&](const float (&v)[4], int row) __attribute__((always_inline)) {
-    bool in[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) in[e] = kept.in(v[e], row + e);
-    u64 sum = 0;
-    if (__any(in[0] || in[1] || in[2] || in[3])) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += in[e] ? kept.weight(v[e]) : 0;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
-    }
-    if (lane == 0) {
-      const int cell = row / 256;                          // (row: this wavefront's first one)
-      if (fold == 1) sh.list[cell] = sum;
-      else if (sum) atomicAdd(&sh.list[cell / fold], sum);
-    }
+  kept.all = rule.least == 0 && most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
+  if (rule.k < a.h || rule.top_p < 1.0) {
+    __syncthreads();
+    if (!sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
+  }
+  // the weights of every wavefront's stretch, and the stretch that the aim is in
+  u64 sum = 0;
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    u64 w[4];
+    kept.weights(w, v, row);
+    sum += (w[0] + w[1]) + (w[2] + w[3]);
   });
+  sum = lane_u64(wave_scan_u64(sum), 63);
   __syncthreads();
-  constexpr int EACH = CELLS / LANES;
-  u64 w[EACH], sum = 0, total;
-  const int used = (cells + fold - 1) / fold;
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    w[k] = EACH * tid + k < used ? sh.list[EACH * tid + k] : 0;
-    sum += w[k];
-  }
-  u64 up_to = sample_scan<LANES>(sum, sh.wave_sum, &total) - sum;
-  const u64 at = sample_part((double)rule.u, total), aim = at < total ? at : total - 1;
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    if (w[k] && up_to <= aim && up_to + w[k] > aim) { sh.cell = (EACH * tid + k) * fold; sh.base = up_to; }      // (one of them)
-    up_to += w[k];
-  }
+  if (lane == 0) sh.wave_sum[wv] = sum;
   __syncthreads();
-  if (wv > 0) return;
-  // one wavefront: the entry among the 256 (or those of the folded slabs, 256 at a time)
-  u64 base = sh.base;
-  for (int cell = sh.cell; cell < sh.cell + fold; ++cell) {
-    float v[4];
-    const int row = 256 * cell + 4 * lane;
-    column.fetch(v, row);
-    u64 q[4], mine = 0;
+  u64 total = 0, base = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { q[e] = kept.in(v[e], row + e) ? kept.weight(v[e]) : 0; mine += q[e]; }
-    u64 up = mine;
+  for (int k = 0; k < W; ++k) { if (k == wv) base = total; total += sh.wave_sum[k]; }
+  const u64 aim = sample_aim(rule, total);
+  if (aim < base || aim >= base + sum) return;
+  // that wavefront looks for the slab, and the row in it
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    if (base > aim) return;
+    u64 w[4];
+    kept.weights(w, v, row);
+    const u64 own = (w[0] + w[1]) + (w[2] + w[3]), up = wave_scan_u64(own), all = lane_u64(up, 63);
+    if (base + all > aim) {
+      u64 up_to = base + up - own;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const u64 p = __shfl_up(up, o, WAVE); if (lane >= o) up += p; }
-    u64 from = base + up - mine;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (q[e] && from <= aim && from + q[e] > aim) {
-        sample_out(a, col, kept, v[e], row + e, total);
+      for (int e = 0; e < 4; ++e) {
+        if (w[e] && up_to <= aim && up_to + w[e] > aim) sample_out(a, col, kept, v[e], row + e, total);
+        up_to += w[e];
       }
-      from += q[e];
     }
-    base += __shfl(up, 63, WAVE);
-  }
+    base += all;
+  });
 }
 
 extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperature, cudamat* top_k, cudamat* top_p, cudamat* min_p, cudamat* target,

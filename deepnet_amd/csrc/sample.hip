@@ -92,20 +92,20 @@ __device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
   return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
 }
 
-#define SAMPLE_LIST 4096           // candidates that are sorted
-#define SAMPLE_SHORT 256           // ... whose places are counted instead
+#define SAMPLE_SHORT 256           // candidates that are compared with each other
 template <int LANES>
 struct SampleShared {
-  static constexpr int WAVES = LANES / 64, BINS = LANES;
+  static constexpr int WAVES = LANES / 64, BINS = LANES, LIST = 4096;       // LIST: candidates
   double table[SAMPLE_STEPS];
-  u64 list[SAMPLE_LIST + 2];       // keys of candidates
+  u64 few[2 * SAMPLE_SHORT];       // keys with their weights
+  u64 list[LIST];                  // keys of candidates
   u64 masses[BINS];
-  u64 sorted[SAMPLE_SHORT];
   int counts[BINS];
   u64 wave_sum[WAVES];
   float wave_max[WAVES], wave_min[WAVES];
-  int wave_bad[WAVES], listed, place, owner;
-  u64 border, base;
+  int wave_bad[WAVES], listed, place, drawn;
+  unsigned key_max, key_min;
+  u64 border, base, before, total;
 };
 
 // Sums up to a lane (itself included) over a workgroup, and the sum of all.  Every lane calls it; what it uses is free again behind the next barrier.
@@ -121,44 +121,6 @@ __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
   for (int k = 0; k < LANES / 64; ++k) { if (k == wv) v += sum; sum += wave_sum[k]; }
   *all = sum;
   return v;
-}
-
-// Bitonic sorts, the greatest first, of `size` keys (a power of two).  One of up to LANES keys, a lane each: lane i gets the i-th; steps within a wavefront
-// are shuffles, the others go through `room`.
-template <int LANES>
-__device__ __forceinline__ u64 sample_sort_lanes(u64 key, u64* room, int size) {
-  const int tid = threadIdx.x;
-  for (int run = 2; run <= size; run *= 2)
-    for (int gap = run / 2; gap > 0; gap /= 2) {
-      u64 other;
-      if (gap < 64) {
-        other = __shfl_xor(key, gap, WAVE);
-      } else {
-        __syncthreads();
-        room[tid] = key;
-        __syncthreads();
-        other = room[tid ^ gap];
-      }
-      const bool greater = ((tid & gap) == 0) == ((tid & run) == 0);
-      key = (other > key) == greater ? other : key;
-    }
-  __syncthreads();
-  return key;
-}
-// One of a list in LDS; zeros are put behind its n keys.
-template <int LANES>
-__device__ __forceinline__ void sample_sort(u64* list, int n, int size) {
-  for (int i = n + threadIdx.x; i < size; i += LANES) list[i] = 0;
-  __syncthreads();
-  for (int run = 2; run <= size; run *= 2)
-    for (int gap = run / 2; gap > 0; gap /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += LANES) {
-        const int x = 2 * i - (i & (gap - 1)), y = x + gap;
-        const u64 p = list[x], q = list[y];
-        if ((p < q) == ((x & run) == 0)) { list[x] = q; list[y] = p; }
-      }
-      __syncthreads();
-    }
 }
 
 // The entries of a column: a wavefront has a stretch of it, 256 rows a slab, four of them a lane; in registers (NV slabs) or, of columns that those do not hold
@@ -222,7 +184,7 @@ struct SampleKept {
   int row;                         // and of entries of that value the last kept row
   double c;
   int shift;
-  bool all;                        // no border, no least
+  bool plain;                      // m - far is a number far enough from m
   u64 least;
   const double* table;
   __device__ __forceinline__ bool near(float v) const { return v > -INFINITY && m - v <= far; }
@@ -233,21 +195,36 @@ struct SampleKept {
   }
   // of four rows; those of a wavefront without a kept entry are not computed
   __device__ __forceinline__ void weights(u64 (&w)[4], const float (&v)[4], int i) const {
-    if (all) {
-      const float end = m - far;   // (from there on a weight is nothing)
+    const float end = m - far;     // (entries from there on have no weight, nor has this)
+    if (plain && x == -INFINITY && least == 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = sample_weight(fmaxf(v[e], end), m, c, shift, table);
-    } else {
-      bool there[4];
+    } else if (plain) {
+      const float best = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+      const bool borders = __any(v[0] == x || v[1] == x || v[2] == x || v[3] == x);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { there[e] = in(v[e], i + e); w[e] = 0; }
-      if (__any(there[0] || there[1] || there[2] || there[3])) {
+      for (int e = 0; e < 4; ++e) w[e] = 0;
+      if (!__any(best >= x)) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = there[e] ? weight(v[e]) : 0;
+      for (int e = 0; e < 4; ++e) {
+        const u64 q = sample_weight(fmaxf(v[e], end), m, c, shift, table);
+        w[e] = v[e] >= x ? q : 0;
       }
+      if (borders) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v[e] == x && i + e > row) w[e] = 0;
+      }
+      if (least) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = w[e] >= least ? w[e] : 0;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = in(v[e], i + e) ? weight(v[e]) : 0;
     }
   }
-  __device__ __forceinline__ void from(u64 border) { x = lp_key_value(border); row = lp_key_index(border); all = false; }
+  __device__ __forceinline__ void from(u64 border) { x = lp_key_value(border); row = lp_key_index(border); }
 };
 __device__ __forceinline__ void sample_out(const SampleArgs& a, int col, const SampleKept& kept, float v, int row, u64 total) {
   a.tokens[col] = (float)row;
@@ -282,85 +259,169 @@ __device__ __forceinline__ u64 sample_bisect(const SampleColumn<LANES, NV>& colu
   return border;
 }
 
-// All that may be kept is listed, n <= LANES entries: draws, unless their weights do not reach `ask` (false; by_count: what top_p asks for of the first k).
+// Of the few (n2) entries in sh.few: how many are greater than this lane's, and their weights.  (Lanes that have none are here too.)
 template <int LANES>
-__device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, int n, const SampleRule& rule, const SampleKept& kept, SampleShared<LANES>& sh, bool by_count, u64 ask) {
-  const int tid = threadIdx.x;
-  u64 key = 0;
-  int size = 2;
-  while (size < n) size *= 2;
-  if (n <= SAMPLE_SHORT) {                                 // places by counting
-    if (tid < 2) sh.list[n + tid] = 0;
-    __syncthreads();
-    if (tid < n) {
-      const u64 own = sh.list[tid];
-      int rank = 0;
+__device__ __forceinline__ void sample_standing(int n2, SampleShared<LANES>& sh, u64 key, int* rank, u64* mass) {
+  int r = 0;
+  u64 m = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; i += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.list + i);
-        rank += (q.x > own ? 1 : 0) + (q.y > own ? 1 : 0);
-      }
-      sh.sorted[rank] = own;
-    }
-    __syncthreads();
-    if (tid < n) key = sh.sorted[tid];
-  } else {
-    key = sample_sort_lanes<LANES>(tid < n ? sh.list[tid] : 0, sh.list, size);
+  for (int i = 0; i < n2; ++i) {
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
+    r += q.x > key ? 1 : 0;
+    m += q.x > key ? q.y : 0;
   }
-  const float v = lp_key_value(key);
-  const int row = lp_key_index(key);
-  u64 w = tid < n && (!by_count || tid < rule.k) ? kept.weight(v) : 0, all;
-  const u64 up_to = sample_scan<LANES>(w, sh.wave_sum, &all) - w;
-  if (by_count) ask = sample_ask(rule, all);
-  if (all < ask) return false;
-  if (up_to >= ask) w = 0;                                 // (not kept)
-  else if (w && up_to + w >= ask) sh.base = up_to + w;     // (one of them)
-  sh.masses[tid] = w;
-  if (n <= SAMPLE_SHORT && tid < n) sh.list[tid] = (u64)(unsigned)row;
-  __syncthreads();
-  const u64 total = sh.base, aim = sample_aim(rule, total);
-  if (n <= SAMPLE_SHORT) {                                 // each adds the weights of those further up in the column
-    if (w) {
-      u64 sum = 0;
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) sum += (int)sh.list[i] < row ? sh.masses[i] : 0;
-      if (sum <= aim && sum + w > aim) sample_out(a, col, kept, v, row, total);
-    }
-  } else {
-    const u64 place = sample_sort_lanes<LANES>(w ? (u64)(unsigned)~row << 32 | (unsigned)tid : 0, sh.list, size);
-    const u64 mass = place ? sh.masses[(unsigned)place] : 0, sum = sample_scan<LANES>(mass, sh.wave_sum, &all) - mass;
-    if (mass && sum <= aim && sum + mass > aim) {
-      const int at = (int)~(unsigned)(place >> 32);
-      sample_out(a, col, kept, a.mat[(size_t)col * a.h + at], at, total);
-    }
-  }
-  return true;
+  *rank = r;
+  *mass = m;
 }
 
-// The border, which lies in the list of n: of the first k (by_count), or where the weights, mass_before ahead of the list, reach `ask`.
+// From the n listed candidates: the border, of the first k (by_count: of those the first that have top_p of their weight) or where the weights, mass_before
+// ahead of the list, reach `ask`.  `whole`: all that may be kept is in the list, which then draws.  More than a few are divided into bins of even width in the order
+// of the keys, so that only the few of the bin that a border lies in are compared with each other.  Returns false where these are not few (many entries alike).
 template <int LANES>
-__device__ __forceinline__ u64 sample_cut(int n, const SampleRule& rule, const SampleKept& kept, SampleShared<LANES>& sh, bool by_count, u64 mass_before, u64 ask) {
-  constexpr int EACH = SAMPLE_LIST / LANES;
+__device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, int n, const SampleRule& rule, SampleKept& kept, SampleShared<LANES>& sh, bool by_count, bool whole,
+                                                 u64 mass_before, u64 ask) {
+  constexpr int BINS = SampleShared<LANES>::BINS;
   const int tid = threadIdx.x;
-  int size = 2;
-  while (size < n) size *= 2;
-  sample_sort<LANES>(sh.list, n, size);
-  u64 w[EACH], sum = 0, all;
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    const int i = EACH * tid + k;
-    w[k] = i < n && (!by_count || i < rule.k) ? kept.weight(lp_key_value(sh.list[i])) : 0;
-    sum += w[k];
+  if (n <= SAMPLE_SHORT) {
+    u64 key = 0, w = 0, m;
+    int rank;
+    if (tid < n) {
+      key = sh.list[tid];
+      w = kept.weight(lp_key_value(key));
+      sh.few[2 * tid] = key;
+      sh.few[2 * tid + 1] = w;
+    }
+    __syncthreads();
+    if (tid < n) {
+      sample_standing<LANES>(n, sh, key, &rank, &m);
+      if (by_count && rank == (rule.k < n ? rule.k : n) - 1) { sh.border = key; sh.total = m + w; }
+    }
+    __syncthreads();
+    if (by_count) ask = sample_ask(rule, sh.total);
+    if (!by_count || rule.top_p < 1.0) {
+      __syncthreads();
+      if (tid < n && w && mass_before + m < ask && mass_before + m + w >= ask) { sh.border = key; sh.total = mass_before + m + w; }
+      __syncthreads();
+    }
+    const u64 border = sh.border, total = sh.total;
+    if (!whole) { kept.from(border); return true; }
+    if (key >= border && w) {
+      const u64 aim = sample_aim(rule, total);
+      const int row = lp_key_index(key);
+      u64 sum = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
+        sum += lp_key_index(q.x) < row && q.x >= border ? q.y : 0;
+      }
+      if (sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
+    }
+    sh.drawn = 1;
+    return true;
   }
-  u64 up_to = sample_scan<LANES>(sum, sh.wave_sum, &all) - sum + mass_before;
-  if (by_count) ask = sample_ask(rule, all);
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    if (w[k] && up_to < ask && up_to + w[k] >= ask) sh.border = sh.list[EACH * tid + k];      // (one of them)
-    up_to += w[k];
+  if (tid == 0) { sh.key_max = 0; sh.key_min = ~0u; }
+  sh.counts[tid] = 0;
+  sh.masses[tid] = 0;
+  __syncthreads();
+  unsigned high = 0, low = ~0u;
+  for (int i = tid; i < n; i += LANES) {
+    const unsigned o = (unsigned)(sh.list[i] >> 32);
+    high = o > high ? o : high;
+    low = o < low ? o : low;
+  }
+  atomicMax(&sh.key_max, high);
+  atomicMin(&sh.key_min, low);
+  __syncthreads();
+  const float most = lp_key_value((u64)sh.key_max << 32), scale = fminf((float)BINS / (most - lp_key_value((u64)sh.key_min << 32)), 3e38f);
+  auto bin = [&](u64 key) __attribute__((always_inline)) { return (int)fminf((most - lp_key_value(key)) * scale, (float)(BINS - 1)); };
+  u64 all_count, all_mass;
+  for (int i = tid; i < n; i += LANES) {
+    const u64 key = sh.list[i];
+    const int b = bin(key);
+    atomicAdd(&sh.counts[b], 1);
+    const u64 w = kept.weight(lp_key_value(key));
+    if (w) atomicAdd(&sh.masses[b], w);
   }
   __syncthreads();
-  return sh.border;
+  const u64 count = (u64)sh.counts[tid], mass = sh.masses[tid], up_count = sample_scan<LANES>(count, sh.wave_sum, &all_count), up_mass = sample_scan<LANES>(mass, sh.wave_sum, &all_mass);
+  u64 border = 0, total = 0;
+  // first the k-th, then the share of the weight
+  for (int step = by_count ? 0 : 1; step < 2; ++step) {
+    if (step == 1 && by_count) {
+      if (rule.top_p >= 1.0) break;
+      ask = sample_ask(rule, total);
+    }
+    const u64 want = step ? ask - mass_before : (u64)(rule.k < n ? rule.k : n);
+    if (tid == 0) { sh.place = 0; sh.base = 0; sh.before = 0; sh.listed = 0; }
+    __syncthreads();
+    const u64 here = step ? mass : count, up = step ? up_mass : up_count;
+    if (up >= want && up - here < want) { sh.place = tid; sh.base = up_mass - mass; sh.before = up_count - count; }      // (one lane)
+    __syncthreads();
+    const int place = sh.place;
+    const u64 base = sh.base, before = sh.before;
+    for (int i = tid; i < n; i += LANES) {
+      const u64 key = sh.list[i];
+      if (bin(key) == place) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < SAMPLE_SHORT) { sh.few[2 * at] = key; sh.few[2 * at + 1] = kept.weight(lp_key_value(key)); }
+      }
+    }
+    __syncthreads();
+    const int n2 = sh.listed;
+    if (n2 > SAMPLE_SHORT) return false;
+    if (tid < n2) {
+      const u64 key = sh.few[2 * tid], w = sh.few[2 * tid + 1];
+      int rank;
+      u64 m;
+      sample_standing<LANES>(n2, sh, key, &rank, &m);
+      const bool it = step ? w && base + m < want && base + m + w >= want : before + (u64)rank == want - 1;
+      if (it) { sh.border = key; sh.total = base + m + w + mass_before; }
+    }
+    __syncthreads();
+    border = sh.border;
+    total = sh.total;
+  }
+  if (!whole) { kept.from(border); return true; }
+  // The row: the stretch of the column (one for every lane) in which the kept weights reach the aim, then those of its entries further up.
+  const u64 aim = sample_aim(rule, total);
+  const int stretch = (a.h + LANES - 1) / LANES;
+  __syncthreads();
+  if (tid == 0) sh.listed = 0;
+  sh.masses[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += LANES) {
+    const u64 key = sh.list[i], w = key >= border ? kept.weight(lp_key_value(key)) : 0;
+    if (w) atomicAdd(&sh.masses[lp_key_index(key) / stretch], w);
+  }
+  __syncthreads();
+  const u64 part = sh.masses[tid], up_part = sample_scan<LANES>(part, sh.wave_sum, &all_mass);
+  if (part && up_part - part <= aim && up_part > aim) { sh.place = tid; sh.base = up_part - part; }      // (one lane)
+  __syncthreads();
+  const int place = sh.place;
+  const u64 base = sh.base;
+  for (int i = tid; i < n; i += LANES) {
+    const u64 key = sh.list[i], w = key >= border && lp_key_index(key) / stretch == place ? kept.weight(lp_key_value(key)) : 0;
+    if (w) {
+      const int to = atomicAdd(&sh.listed, 1);
+      if (to < SAMPLE_SHORT) { sh.few[2 * to] = key; sh.few[2 * to + 1] = w; }
+    }
+  }
+  __syncthreads();
+  const int n2 = sh.listed;
+  if (n2 > SAMPLE_SHORT) { kept.from(border); sh.drawn = 0; return true; }      // (of tall columns: by a pass over the column)
+  if (tid < n2) {
+    const u64 key = sh.few[2 * tid], w = sh.few[2 * tid + 1];
+    const int row = lp_key_index(key);
+    u64 sum = base;
+#pragma unroll 4
+    for (int i = 0; i < n2; ++i) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
+      sum += lp_key_index(q.x) < row ? q.y : 0;
+    }
+    if (sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
+  }
+  sh.drawn = 1;
+  return true;
 }
 
 // Finds what top-k and top-p keep: the border, for a pass over the column to draw by (true), or, where all that is kept has been listed and is little, draws.
@@ -368,9 +429,9 @@ __device__ __forceinline__ u64 sample_cut(int n, const SampleRule& rule, const S
 // parts of the column, and not many more.  Otherwise, and without a top-k, all entries are counted (weighed) bin by bin, and those of the bins up to
 // the border's are listed, or where they are many those of its own.
 template <int LANES, int NV>
-__device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, const SampleColumn<LANES, NV>& column, const SampleRule& rule, SampleKept& kept, const float (&mine)[2],
+__device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, SampleColumn<LANES, NV>& column, const SampleRule& rule, SampleKept& kept, const float (&mine)[2],
                                               float least_x, SampleShared<LANES>& sh) {
-  constexpr int BINS = SampleShared<LANES>::BINS;
+  constexpr int BINS = SampleShared<LANES>::BINS, LIST = SampleShared<LANES>::LIST;
   const int tid = threadIdx.x;
   const bool by_count = rule.k < column.h;
   const float scale = fminf((float)BINS / fminf(kept.far, kept.m - least_x), 3e38f);
@@ -382,21 +443,26 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, cons
     __syncthreads();
   };
   auto list_bins = [&](int first, int place) __attribute__((always_inline)) {
+    // (bins up to `place` lie within this of the greatest entry, with room for the roundings; one comparison rules most entries out)
+    const float reach = (float)(place + 1) / scale * 1.0001f, end = place >= BINS - 1 ? -INFINITY : kept.m - reach - 1e-6f * fabsf(kept.m);
     column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= end)) return;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (kept.near(v[e])) {
+        if (v[e] >= end && kept.near(v[e])) {
           const int b = bin(v[e]);
           if (b >= first && b <= place) {
             const int at = atomicAdd(&sh.listed, 1);
-            if (at < SAMPLE_LIST) sh.list[at] = lp_key(v[e], row + e);
+            if (at < LIST) sh.list[at] = lp_key(v[e], row + e);
           }
         }
     });
     __syncthreads();
     return sh.listed;
   };
-  u64 ignored;
+  u64 ignored, mass_before = 0, ask = 0;
+  int n = LIST + 1, place = BINS;
+  bool whole = true;
   if (by_count && rule.k <= LANES) {
     clear(BINS - 1);
 #pragma unroll
@@ -406,40 +472,44 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, cons
     const u64 here = (u64)sh.counts[tid], up = sample_scan<LANES>(here, sh.wave_sum, &ignored);
     if (up >= (u64)rule.k && up - here < (u64)rule.k) sh.place = tid;
     __syncthreads();
-    const int n = list_bins(0, sh.place);
-    if (n <= LANES) { sample_from_list<LANES>(a, col, n, rule, kept, sh, true, 0); return false; }
-    if (n <= SAMPLE_LIST) { kept.from(sample_cut<LANES>(n, rule, kept, sh, true, 0, 0)); return true; }
+    n = list_bins(0, sh.place);
     __syncthreads();
   }
-  clear(BINS);
-  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-    bool there[4];
+  if (n > LIST) {
+    clear(BINS);
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      bool there[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) there[e] = kept.near(v[e]);
-    if (!__any(there[0] || there[1] || there[2] || there[3])) return;
+      for (int e = 0; e < 4; ++e) there[e] = kept.near(v[e]);
+      if (!__any(there[0] || there[1] || there[2] || there[3])) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (there[e]) {
-        const int b = bin(v[e]);
-        atomicAdd(&sh.counts[b], 1);
-        if (!by_count) atomicAdd(&sh.masses[b], kept.weight(v[e]));
-      }
-  });
-  __syncthreads();
-  u64 total;
-  const u64 count = (u64)sh.counts[tid], mass = sh.masses[tid], up_count = sample_scan<LANES>(count, sh.wave_sum, &ignored), up_mass = sample_scan<LANES>(mass, sh.wave_sum, &total);
-  const u64 ask = by_count ? 0 : sample_ask(rule, total), want = by_count ? (u64)rule.k : ask, here = by_count ? count : mass, up = by_count ? up_count : up_mass;
-  if (up >= want && up - here < want) { sh.place = tid; sh.base = up_mass - mass; sh.border = up_count; }      // (one lane at most)
-  __syncthreads();
-  const int place = sh.place;                              // (BINS: fewer candidates than k)
-  const bool all_of_them = by_count || sh.border <= LANES;
-  const u64 mass_before = all_of_them ? 0 : sh.base;
-  const int n = list_bins(all_of_them ? 0 : place, place);
-  if (n <= LANES && all_of_them) { sample_from_list<LANES>(a, col, n, rule, kept, sh, by_count, ask); return false; }
-  if (n <= SAMPLE_LIST) { kept.from(sample_cut<LANES>(n, rule, kept, sh, by_count, mass_before, ask)); return true; }
-  if (by_count && place < BINS) kept.from(sample_bisect(column, kept, sh, (u64)rule.k, [](float) { return (u64)1; }));
+      for (int e = 0; e < 4; ++e)
+        if (there[e]) {
+          const int b = bin(v[e]);
+          atomicAdd(&sh.counts[b], 1);
+          if (!by_count) atomicAdd(&sh.masses[b], kept.weight(v[e]));
+        }
+    });
+    __syncthreads();
+    u64 total;
+    const u64 count = (u64)sh.counts[tid], mass = sh.masses[tid], up_count = sample_scan<LANES>(count, sh.wave_sum, &ignored), up_mass = sample_scan<LANES>(mass, sh.wave_sum, &total);
+    ask = by_count ? 0 : sample_ask(rule, total);
+    const u64 want = by_count ? (u64)rule.k : ask, here = by_count ? count : mass, up = by_count ? up_count : up_mass;
+    if (up >= want && up - here < want) { sh.place = tid; sh.base = up_mass - mass; sh.border = up_count; }      // (one lane at most)
+    __syncthreads();
+    place = sh.place;                                      // (BINS: fewer candidates than k)
+    whole = by_count || sh.border <= LIST;
+    if (!whole) mass_before = sh.base;
+    n = list_bins(whole ? 0 : place, place);
+  }
+  if (n <= LIST && sample_from_list<LANES>(a, col, n, rule, kept, sh, by_count, whole, mass_before, ask)) return !whole || !sh.drawn;
+  column.init(column.c, column.h);
+  if (by_count) {
+    const u64 border = sample_bisect(column, kept, sh, (u64)rule.k, [](float) { return (u64)1; });
+    if (border) kept.from(border);                         // (none: fewer candidates than k)
+  }
   if (rule.top_p < 1.0) {
-    u64 sum = 0;
+    u64 sum = 0, total;
     column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
       u64 w[4];
       kept.weights(w, v, row);
@@ -497,10 +567,11 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
   SampleKept kept;
   kept.m = most; kept.x = -INFINITY; kept.row = 0; kept.c = rule.c; kept.shift = a.shift; kept.least = rule.least; kept.table = sh.table;
   kept.far = (float)((a.shift + 1.5) / rule.c);            // (2^-(shift + 1) is nothing; half an octave for the rounding of the distance)
-  kept.all = rule.least == 0 && most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
+  kept.plain = most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
   if (rule.k < a.h || rule.top_p < 1.0) {
     __syncthreads();
     if (!sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
+    column.init(column.c, a.h);                            // (the registers are the lists' meanwhile)
   }
   // the weights of every wavefront's stretch, and the stretch that the aim is in
   u64 sum = 0;
@@ -557,7 +628,6 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   else if (h <= 4096) SAMPLE_GO(256, 4);
   else if (h <= 16384) SAMPLE_GO(1024, 4);
   else if (h <= 32768) SAMPLE_GO(1024, 8);
-  else if (h <= 65536) SAMPLE_GO(1024, 16);
   else SAMPLE_GO(1024, 0);
 #undef SAMPLE_GO
   return dn_launch_status();

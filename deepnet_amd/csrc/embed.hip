@@ -172,6 +172,7 @@ struct EmbedSums {
   const int *starts, *sorted;
   const EmbedSlot* slots;
   int h, n, slot_count, tiles, rows;      // rows of a tile
+  unsigned first;                  // item of a launch
   float beta, mult;
 };
 // A team (T lanes, NV groups of W rows each) and its rows of a column.
@@ -222,7 +223,7 @@ __device__ __forceinline__ void embed_out(const EmbedRows<T, NV, W, TAIL>& rows,
 // as does what a token without columns gets.  Four columns are on their way at once.  Bytes: the columns and, with beta = 0, the table.
 template <int T, int NV, int W, bool TAIL, bool STREAM>
 __global__ void __launch_bounds__(256) k_embed_sums(EmbedSums a) {
-  unsigned item = blockIdx.x * (256 / T) + (T == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : threadIdx.x / T);
+  const unsigned item = a.first + blockIdx.x * (256 / T) + (T == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : threadIdx.x / T);
   const unsigned which = item / a.tiles, tile = item - which * a.tiles;
   if (which >= (unsigned)a.slot_count + a.n) return;
   const int row0 = tile * a.rows;
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(EmbedSums a) {
 // The sums of the pieces of every long run, in their order, sixteen on their way at once.
 template <int T, int W, bool TAIL>
 __global__ void __launch_bounds__(256) k_embed_join(EmbedSums a) {
-  unsigned item = blockIdx.x * (256 / T) + (T == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : threadIdx.x / T);
+  const unsigned item = a.first + blockIdx.x * (256 / T) + (T == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : threadIdx.x / T);
   const unsigned which = item / a.tiles, tile = item - which * a.tiles;
   if (which >= (unsigned)a.slot_count || (int)which >= embed_slot(a.starts[a.n])) return;
   const EmbedSlot s = a.slots[which];
@@ -359,7 +360,15 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
   o.range = (int)((n + sorters - 1) / sorters);
   hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)((n + o.range - 1) / o.range)), dim3(1024), 0, dn_stream(), o);
   const bool stream = (long long)h * (w > n ? w : n) >= DN_STREAM_MIN_ELEMS;
-#define SUMS3(T, NV, W, TAIL, S) hipLaunchKernelGGL((k_embed_sums<T, NV, W, TAIL, S>), dim3((unsigned)((sums + 256 / T - 1) / (256 / T))), dim3(256), 0, dn_stream(), s)
+  // (items of one launch: teams of 16 or 64 lanes)
+  auto launches = [&](long long items, int team, auto go) {
+    const long long most = DN_MAX_GROUPS * (256 / team);
+    for (long long i = 0; i < items; i += most) {
+      s.first = (unsigned)i;
+      go(dim3((unsigned)(((items - i < most ? items - i : most) + 256 / team - 1) / (256 / team))));
+    }
+  };
+#define SUMS3(T, NV, W, TAIL, S) launches(sums, T, [&](dim3 grid) { hipLaunchKernelGGL((k_embed_sums<T, NV, W, TAIL, S>), grid, dim3(256), 0, dn_stream(), s); })
 #define SUMS2(T, NV, W, TAIL) do { if (stream) SUMS3(T, NV, W, TAIL, true); else SUMS3(T, NV, W, TAIL, false); } while (0)
 #define SUMS(T, NV, W) do { if (h % 4 && W == 4) SUMS2(T, NV, W, true); else SUMS2(T, NV, W, false); } while (0)
   if (h < 4) SUMS(16, 1, 1);
@@ -374,7 +383,7 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
   if (s.slot_count) {
     embed_tiles(s, 256);
     const long long joins = (long long)s.slot_count * s.tiles;
-#define JOIN(T, W, TAIL) hipLaunchKernelGGL((k_embed_join<T, W, TAIL>), dim3((unsigned)((joins + 256 / T - 1) / (256 / T))), dim3(256), 0, dn_stream(), s)
+#define JOIN(T, W, TAIL) launches(joins, T, [&](dim3 grid) { hipLaunchKernelGGL((k_embed_join<T, W, TAIL>), grid, dim3(256), 0, dn_stream(), s); })
     if (h < 4) JOIN(16, 1, false);
     else if (h <= 64) { if (h % 4) JOIN(16, 4, true); else JOIN(16, 4, false); }
     else if (h % 4) JOIN(64, 4, true);

@@ -13,19 +13,20 @@ struct SampleArgs {
 };
 
 // The weight e^((x - m) / T) of an entry, x <= m, as a whole multiple of 2^-shift: the same one wherever it is computed, and sums of
-// them do not depend on their order, so a border between two sums is one border.  c = log2(e) / T.  2^t with t = (n + f) / 256, n whole and |f| <= 1/2: 2^(n / 256) from
-// a table of 256 steps and the whole part, 2^(f / 256) by its Taylor sum (remainder (ln 2 / 512)^5 / 5! < 4e-17).  Adding 2^52 leaves the rounded whole number in the low bits.
-// Entries that have none (too far from m) are not asked for.
+// them do not depend on their order, so a border between two sums is one border.  c = 256 log2(e) / T.  (x - m) c = n + f, n whole and |f| <= 1/2: 2^(n / 256) from
+// a table of 256 steps (times 2^shift) and the whole part, 2^(f / 256) by its Taylor sum (remainder (ln 2 / 512)^5 / 5! < 4e-17).  Adding 2^52 leaves the rounded
+// whole number in the low bits.  Entries that have none (too far from m) are not asked for.
+// 2048 steps and one term less take as long, and 1.2 us more to fill the table.
 #define SAMPLE_STEPS 256
-__device__ __forceinline__ unsigned long long sample_weight(float x, float m, double c, int shift, const double* table) {
-  const double t = ((double)x - (double)m) * (c * 256.0), b = t + 6755399441055744.0, f = t - (b - 6755399441055744.0);      // (3 * 2^51: the low bits are n)
+__device__ __forceinline__ unsigned long long sample_weight(float x, float m, double c, const double* table) {
+  const double d = (double)x - (double)m, b = fma(d, c, 6755399441055744.0), f = fma(d, c, 6755399441055744.0 - b);      // (3 * 2^51: the low bits are n)
   const int n = (int)__double_as_longlong(b);
-  double p = 2.239395190875157e-12;           // (ln2 / 256)^4 / 4!
+  double p = 2.239395190875157e-12;            // (ln2 / 256)^4 / 4!
   p = fma(p, f, 3.308302680541371e-09);
   p = fma(p, f, 3.665565596910106e-06);
-  p = fma(p, f, 2.7076061740622863e-03);
-  p = fma(p, f, 1.0) * table[n & 255];
-  const double w = __hiloint2double(__double2hiint(p) + (((n >> 8) + shift) << 20), __double2loint(p)) + 4503599627370496.0;
+  p = fma(p, f, 0.0027076061740622863);
+  const double step = table[n & (SAMPLE_STEPS - 1)], s = __hiloint2double(__double2hiint(step) + ((n >> 8) << 20), __double2loint(step));
+  const double w = fma(s * f, p, s) + 4503599627370496.0;
   return (unsigned long long)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 // 2^(n / 256), by its Taylor sum from the nearer end (remainder (ln 2 / 2)^13 / 13! < 2e-16)
@@ -180,41 +181,33 @@ struct SampleColumn {
 
 // Kept entries: those from the border on in the order of keys whose weight reaches `least`.
 struct SampleKept {
-  float m, far, x;                 // the greatest entry; entries further from it than `far` have no weight; the last kept value,
+  float m, far, x, above;          // the greatest entry; entries further from it than `far` have no weight; the last kept value (and the next greater),
   int row;                         // and of entries of that value the last kept row
-  double c;
-  int shift;
-  bool plain;                      // m - far is a number far enough from m
+  double c;                        // 256 log2(e) / temperature
+  bool plain, bordered;            // plain: m - far is a number far enough from m
   u64 least;
   const double* table;
   __device__ __forceinline__ bool near(float v) const { return v > -INFINITY && m - v <= far; }
   __device__ __forceinline__ bool in(float v, int i) const { return near(v) && (v > x || (v == x && i <= row)); }
   __device__ __forceinline__ u64 weight(float v) const {
-    const u64 w = sample_weight(v, m, c, shift, table);
+    const u64 w = sample_weight(v, m, c, table);
     return w >= least ? w : 0;
   }
   // of four rows; those of a wavefront without a kept entry are not computed
   __device__ __forceinline__ void weights(u64 (&w)[4], const float (&v)[4], int i) const {
     const float end = m - far;     // (entries from there on have no weight, nor has this)
-    if (plain && x == -INFINITY && least == 0) {
+    if (plain && !bordered && least == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = sample_weight(fmaxf(v[e], end), m, c, shift, table);
+      for (int e = 0; e < 4; ++e) w[e] = sample_weight(fmaxf(v[e], end), m, c, table);
     } else if (plain) {
-      const float best = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-      const bool borders = __any(v[0] == x || v[1] == x || v[2] == x || v[3] == x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = 0;
-      if (!__any(best >= x)) return;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const u64 q = sample_weight(fmaxf(v[e], end), m, c, shift, table);
-        w[e] = v[e] >= x ? q : 0;
+      // (rows up to the last kept one keep its value, those behind it the next greater)
+      const float here = i <= row ? x : above;
+      if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= here || (i <= row && row < i + 3))) {
+        w[0] = w[1] = w[2] = w[3] = 0;
+        return;
       }
-      if (borders) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v[e] == x && i + e > row) w[e] = 0;
-      }
+      for (int e = 0; e < 4; ++e) w[e] = sample_weight(v[e] >= (e && i + e > row ? above : here) ? v[e] : end, m, c, table);
       if (least) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = w[e] >= least ? w[e] : 0;
@@ -224,11 +217,16 @@ struct SampleKept {
       for (int e = 0; e < 4; ++e) w[e] = in(v[e], i + e) ? weight(v[e]) : 0;
     }
   }
-  __device__ __forceinline__ void from(u64 border) { x = lp_key_value(border); row = lp_key_index(border); }
+  __device__ __forceinline__ void from(u64 border) {
+    x = lp_key_value(border);
+    row = lp_key_index(border);
+    above = lp_key_value(((border >> 32) + 1) << 32);
+    bordered = true;
+  }
 };
 __device__ __forceinline__ void sample_out(const SampleArgs& a, int col, const SampleKept& kept, float v, int row, u64 total) {
   a.tokens[col] = (float)row;
-  if (a.logp) a.logp[col] = (float)(((double)v - (double)kept.m) * (kept.c * 0.6931471805599453) - dn_log_wide_pos(ldexp((double)total, -a.shift)));
+  if (a.logp) a.logp[col] = (float)(((double)v - (double)kept.m) * (kept.c * (0.6931471805599453 / 256.0)) - dn_log_wide_pos(ldexp((double)total, -a.shift)));
 }
 __device__ __forceinline__ u64 sample_aim(const SampleRule& rule, u64 total) {
   const u64 at = sample_part((double)rule.u, total);
@@ -443,13 +441,17 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
     __syncthreads();
   };
   auto list_bins = [&](int first, int place) __attribute__((always_inline)) {
-    // (bins up to `place` lie within this of the greatest entry, with room for the roundings; one comparison rules most entries out)
-    const float reach = (float)(place + 1) / scale * 1.0001f, end = place >= BINS - 1 ? -INFINITY : kept.m - reach - 1e-6f * fabsf(kept.m);
+    // (the values of these bins, with room for the roundings: two comparisons rule most entries out)
+    const float slack = 1e-6f * fabsf(kept.m), end = place >= BINS - 1 ? -INFINITY : kept.m - (float)(place + 1) / scale * 1.0001f - slack;
+    const float start = first > 0 ? kept.m - (float)first / scale * 0.9999f + slack : INFINITY;
     column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-      if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= end)) return;
+      bool there[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) there[e] = v[e] >= end && v[e] <= start;
+      if (!__any(there[0] || there[1] || there[2] || there[3]) || *(volatile int*)&sh.listed > LIST) return;      // (too many already)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (v[e] >= end && kept.near(v[e])) {
+        if (there[e] && kept.near(v[e])) {
           const int b = bin(v[e]);
           if (b >= first && b <= place) {
             const int at = atomicAdd(&sh.listed, 1);
@@ -478,29 +480,45 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
   if (n > LIST) {
     clear(BINS);
     column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-      bool there[4];
+      if (by_count) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) there[e] = kept.near(v[e]);
-      if (!__any(there[0] || there[1] || there[2] || there[3])) return;
+        for (int e = 0; e < 4; ++e)
+          if (kept.near(v[e])) atomicAdd(&sh.counts[bin(v[e])], 1);
+      } else {
+        u64 w[4];
+        kept.weights(w, v, row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (there[e]) {
-          const int b = bin(v[e]);
-          atomicAdd(&sh.counts[b], 1);
-          if (!by_count) atomicAdd(&sh.masses[b], kept.weight(v[e]));
-        }
+        for (int e = 0; e < 4; ++e)
+          if (w[e]) atomicAdd(&sh.masses[bin(v[e])], w[e]);
+      }
     });
     __syncthreads();
+    const u64 here = by_count ? (u64)sh.counts[tid] : sh.masses[tid];
     u64 total;
-    const u64 count = (u64)sh.counts[tid], mass = sh.masses[tid], up_count = sample_scan<LANES>(count, sh.wave_sum, &ignored), up_mass = sample_scan<LANES>(mass, sh.wave_sum, &total);
+    const u64 up = sample_scan<LANES>(here, sh.wave_sum, &total);
     ask = by_count ? 0 : sample_ask(rule, total);
-    const u64 want = by_count ? (u64)rule.k : ask, here = by_count ? count : mass, up = by_count ? up_count : up_mass;
-    if (up >= want && up - here < want) { sh.place = tid; sh.base = up_mass - mass; sh.border = up_count; }      // (one lane at most)
+    const u64 want = by_count ? (u64)rule.k : ask;
+    if (up >= want && up - here < want) { sh.place = tid; sh.base = up - here; }      // (one lane at most)
     __syncthreads();
     place = sh.place;                                      // (BINS: fewer candidates than k)
-    whole = by_count || sh.border <= LIST;
-    if (!whole) mass_before = sh.base;
-    n = list_bins(whole ? 0 : place, place);
+    if (!by_count && column.slabs > 1) {                   // many, going by the first slab of every stretch: those of the border's bin alone
+      float v[4];
+      u64 some = 0;
+      column.fetch(v, column.from);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) some += kept.near(v[e]) && bin(v[e]) <= place ? 1 : 0;
+      sample_scan<LANES>(some, sh.wave_sum, &some);
+      whole = some * column.slabs <= LIST;
+    }
+    if (whole) n = list_bins(0, place);
+    if (!by_count && (!whole || n > LIST)) {
+      whole = false;
+      mass_before = sh.base;
+      __syncthreads();
+      if (tid == 0) sh.listed = 0;
+      __syncthreads();
+      n = list_bins(place, place);
+    }
   }
   if (n <= LIST && sample_from_list<LANES>(a, col, n, rule, kept, sh, by_count, whole, mass_before, ask)) return !whole || !sh.drawn;
   column.init(column.c, column.h);
@@ -521,7 +539,23 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
   return true;
 }
 
-// A workgroup a column, which it holds in registers (of more than 65536 rows: reads again, from the caches).
+// The weights of a slab, `base` being those before it; draws if the aim is among them.
+__device__ __forceinline__ u64 sample_slab(const SampleArgs& a, int col, const SampleKept& kept, const float (&v)[4], int row, u64 base, u64 aim, u64 total) {
+  u64 w[4];
+  kept.weights(w, v, row);
+  const u64 own = (w[0] + w[1]) + (w[2] + w[3]), up = wave_scan_u64(own), all = lane_u64(up, 63);
+  if (base + all > aim) {
+    u64 up_to = base + up - own;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (w[e] && up_to <= aim && up_to + w[e] > aim) sample_out(a, col, kept, v[e], row + e, total);
+      up_to += w[e];
+    }
+  }
+  return all;
+}
+
+// A workgroup a column, which it holds in registers, of up to 16384 rows, or reads again, from the caches (32768 x 512 takes as long either way).
 // Weights are whole numbers (sample_weight), so every sum and with it every border is the same however it is added up.
 template <int LANES, int NV>
 __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
@@ -533,7 +567,7 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
   const SampleRule rule = sample_rule(a, col);
   float mine[2] = {-INFINITY, -INFINITY}, least = INFINITY;
   bool bad = false;
-  if (tid < SAMPLE_STEPS) sh.table[tid] = sample_step(tid);
+  if (tid < SAMPLE_STEPS) sh.table[tid] = ldexp(sample_step(tid), a.shift);
   column.each([&](const float (&v)[4], int row, int slab) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -565,9 +599,11 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
     return;
   }
   SampleKept kept;
-  kept.m = most; kept.x = -INFINITY; kept.row = 0; kept.c = rule.c; kept.shift = a.shift; kept.least = rule.least; kept.table = sh.table;
+  kept.m = most; kept.row = 0; kept.c = rule.c * 256.0; kept.least = rule.least; kept.table = sh.table;
   kept.far = (float)((a.shift + 1.5) / rule.c);            // (2^-(shift + 1) is nothing; half an octave for the rounding of the distance)
   kept.plain = most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
+  kept.bordered = false;
+  kept.x = kept.above = kept.plain ? most - kept.far : -INFINITY;
   if (rule.k < a.h || rule.top_p < 1.0) {
     __syncthreads();
     if (!sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
@@ -585,26 +621,56 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
   if (lane == 0) sh.wave_sum[wv] = sum;
   __syncthreads();
   u64 total = 0, base = 0;
+  if (NV) {
 #pragma unroll
-  for (int k = 0; k < W; ++k) { if (k == wv) base = total; total += sh.wave_sum[k]; }
+    for (int k = 0; k < W; ++k) { if (k == wv) base = total; total += sh.wave_sum[k]; }
+    const u64 aim = sample_aim(rule, total);
+    if (aim < base || aim >= base + sum) return;
+    // that wavefront looks for the slab, and the row in it
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      if (base > aim) return;
+      base += sample_slab(a, col, kept, v, row, base, aim, total);
+    });
+    return;
+  }
+  // all wavefronts look for the part of that stretch (of one slab, or so many that there are at most as many parts as lanes), and one for the row in it
+  int owner = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) total += sh.wave_sum[k];
   const u64 aim = sample_aim(rule, total);
-  if (aim < base || aim >= base + sum) return;
-  // that wavefront looks for the slab, and the row in it
-  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-    if (base > aim) return;
-    u64 w[4];
-    kept.weights(w, v, row);
-    const u64 own = (w[0] + w[1]) + (w[2] + w[3]), up = wave_scan_u64(own), all = lane_u64(up, 63);
-    if (base + all > aim) {
-      u64 up_to = base + up - own;
+  u64 up_to = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (w[e] && up_to <= aim && up_to + w[e] > aim) sample_out(a, col, kept, v[e], row + e, total);
-        up_to += w[e];
-      }
+  for (int k = 0; k < W; ++k) {
+    if (up_to <= aim) { owner = k; base = up_to; }
+    up_to += sh.wave_sum[k];
+  }
+  const int first = owner * column.slabs * 256 + 4 * lane, fold = (column.slabs + LANES - 1) / LANES;
+  sh.masses[tid] = 0;
+  __syncthreads();
+  for (int part = wv; part * fold < column.slabs; part += W) {
+    sum = 0;
+    for (int k = part * fold; k < (part + 1) * fold && k < column.slabs; ++k) {
+      float v[4];
+      u64 w[4];
+      column.fetch(v, first + 256 * k);
+      kept.weights(w, v, first + 256 * k);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
     }
-    base += all;
-  });
+    sum = lane_u64(wave_scan_u64(sum), 63);
+    if (lane == 0) sh.masses[part] = sum;
+  }
+  __syncthreads();
+  u64 all;
+  const u64 here = sh.masses[tid], up = base + sample_scan<LANES>(here, sh.wave_sum, &all);
+  if (here && up - here <= aim && up > aim) { sh.place = tid; sh.base = up - here; }      // (one lane)
+  __syncthreads();
+  if (wv) return;
+  base = sh.base;
+  for (int k = sh.place * fold; k < (sh.place + 1) * fold && k < column.slabs && base <= aim; ++k) {
+    float v[4];
+    column.fetch(v, first + 256 * k);
+    base += sample_slab(a, col, kept, v, first + 256 * k, base, aim, total);
+  }
 }
 
 extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperature, cudamat* top_k, cudamat* top_p, cudamat* min_p, cudamat* target,
@@ -621,14 +687,18 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   if (w <= 0) return 0;
   int bits = 0;
   while ((1 << bits) < h) ++bits;
-  const SampleArgs a = {mat->data_device, uniform->data_device, tok_data(temperature), tok_data(top_k), tok_data(top_p), tok_data(min_p), target->data_device,
-                        tok_data(logp), all_temperature, all_top_k, all_top_p, all_min_p, h, w, 62 - bits < 45 ? 62 - bits : 45};
-#define SAMPLE_GO(LANES, NV) hipLaunchKernelGGL((k_sample_tokens<LANES, NV>), dim3(w), dim3(LANES), 0, dn_stream(), a)
-  if (h <= 1024) SAMPLE_GO(256, 1);
-  else if (h <= 4096) SAMPLE_GO(256, 4);
-  else if (h <= 16384) SAMPLE_GO(1024, 4);
-  else if (h <= 32768) SAMPLE_GO(1024, 8);
-  else SAMPLE_GO(1024, 0);
+  const long long most = h <= 4096 ? DN_MAX_GROUPS : DN_MAX_GROUPS / 4;            // columns of a launch
+  for (long long c0 = 0; c0 < w; c0 += most) {
+    const int n = (int)(w - c0 < most ? w - c0 : most);
+    auto from = [c0](const cudamat* m) { return m ? m->data_device + c0 : nullptr; };
+    const SampleArgs a = {mat->data_device + c0 * h, from(uniform), from(temperature), from(top_k), from(top_p), from(min_p), from(target), from(logp),
+                          all_temperature, all_top_k, all_top_p, all_min_p, h, n, 62 - bits < 45 ? 62 - bits : 45};
+#define SAMPLE_GO(LANES, NV) hipLaunchKernelGGL((k_sample_tokens<LANES, NV>), dim3(n), dim3(LANES), 0, dn_stream(), a)
+    if (h <= 1024) SAMPLE_GO(256, 1);
+    else if (h <= 4096) SAMPLE_GO(256, 4);
+    else if (h <= 16384) SAMPLE_GO(1024, 4);
+    else SAMPLE_GO(1024, 0);
 #undef SAMPLE_GO
+  }
   return dn_launch_status();
 }

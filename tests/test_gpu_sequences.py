@@ -405,6 +405,30 @@ def test_columns_beyond_two_to_the_31_entries(cm, rng):
     assert [int(v) for v in t] == [seq.sample_token(top[:, i], u[0, w - n + i], top_k=20)[0] for i in range(n)]
 
 
+def test_more_columns_than_a_launch_takes(cm, rng):
+    """Calls of several launches: the columns around their borders."""
+    w = (1 << 24) + 1000
+    x, u = cm.empty((2, w)), cm.empty((1, w))
+    x.assign(0.0)
+    u.assign(0.25)
+    u.slice(w - 1001, w - 999).assign(0.75)
+    u.slice(w - 3, w).assign(0.75)
+    t = cm.sample_tokens(x, u).asarray()[0]
+    assert t.sum() == 5 and (t[-3:] == 1).all() and (t[w - 1001:w - 999] == 1).all()
+    w = (1 << 30) + 5                                                       # three rows: columns beyond 2^31 rows go into another launch
+    e, labels, y = cm.CUDAMatrix(F(rng.standard_normal((3, 4)))), cm.empty((1, w)), cm.empty((3, w))
+    labels.assign(2.0)
+    tail = F([[0, 1, -1, 3] * 5])
+    at = (1 << 31) // 3 - 10
+    labels.slice(at, at + 20).assign(cm.CUDAMatrix(tail))
+    labels.slice(w - 20, w).assign(cm.CUDAMatrix(tail))
+    cm.embed(e, labels, target=y)
+    for a in (at, w - 20):
+        assert np.array_equal(y.slice(a, a + 20).asarray(), F(seq.embed(e.asarray(), tail)))
+    for a in (0, at - 20, at + 20, w - 40):
+        assert np.array_equal(y.slice(a, a + 20).asarray(), np.tile(e.asarray()[:, 2:3], (1, 20)))
+
+
 def test_scans_beyond_two_to_the_31_entries(cm, rng):
     f, w = 4096, (1 << 18) + 300                                           # pre has 2^31 entries and more
     pre, y, o = cm.empty((2 * f, w)), cm.empty((f, w)), [0, 100, w - 200, w]

@@ -52,6 +52,19 @@ __device__ __forceinline__ int embed_piece(int count) {
 }
 __device__ __forceinline__ int embed_slot(int sorted) { return (int)(((unsigned)sorted + EMBED_SLOT - 1) / EMBED_SLOT); }
 
+// Of the lanes in `all`, those with the same x (of `bits` bits): how many are before this one, and how many there are.  (The whole wavefront is here.)
+__device__ __forceinline__ void embed_same(unsigned long long all, int x, int bits, int* rank, int* count) {
+  unsigned lo = (unsigned)all, hi = (unsigned)(all >> 32);
+  for (int b = 0; b < bits; ++b) {
+    const int bit = (int)((unsigned)x << (31 - b)) >> 31;  // 0 or -1
+    const unsigned long long set = __ballot(bit);
+    lo &= ~((unsigned)set ^ bit);
+    hi &= ~((unsigned)(set >> 32) ^ bit);
+  }
+  *rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+  *count = __popc(lo) + __popc(hi);
+}
+
 struct EmbedSlot { int from, count, token, pieces; };      // a piece of a long run; pieces: of its first one, how many there are (0 in the others)
 struct EmbedSort {
   const float* labels;
@@ -149,17 +162,12 @@ __global__ void __launch_bounds__(1024) k_embed_sort(EmbedSort a) {
         const unsigned long long all = __ballot(in);
         if (all == 0) continue;
         const int x = (int)l[k][e] - lo;
-        unsigned same_lo = (unsigned)all, same_hi = (unsigned)(all >> 32);
-        for (int b = 0; b < bits; ++b) {
-          const int bit = (int)((unsigned)x << (31 - b)) >> 31;          // 0 or -1
-          const unsigned long long set = __ballot(bit);
-          same_lo &= ~((unsigned)set ^ bit);
-          same_hi &= ~((unsigned)(set >> 32) ^ bit);
-        }
+        int rank, count;
+        embed_same(all, x, bits, &rank, &count);
         if (in) {
-          const int at = next[x], rank = __builtin_amdgcn_mbcnt_hi(same_hi, __builtin_amdgcn_mbcnt_lo(same_lo, 0));
+          const int at = next[x];
           a.sorted[at + rank] = (int)(c0 + 256 * k + 4 * lane + e);
-          if (rank == 0) next[x] = at + __popc(same_lo) + __popc(same_hi);
+          if (rank == 0) next[x] = at + count;
         }
       }
     }
@@ -295,6 +303,119 @@ __global__ void __launch_bounds__(256) k_embed_join(EmbedSums a) {
   embed_out<T, 1, W, TAIL, false>(rows, a.target + (size_t)s.token * a.h + row0, sum, a.beta, a.mult);
 }
 
+// Few columns (at most EMBED_FEW): one launch.  A workgroup has a range of tokens and, of the table, 256 rows (T = 16: 64): it sorts its columns in LDS, its teams
+// take the tokens of up to EMBED_RUN columns in turn, and all of them share those of more, whose parts meet in LDS in their order.
+// 1001 x 4099 of 256 tokens 13 us (as three launches 18).
+#define EMBED_FEW 8192
+#define EMBED_FEW_RANGE 8
+template <int T, int W, bool TAIL, bool STREAM>
+__global__ void __launch_bounds__(1024) k_embed_few(EmbedSort a, EmbedSums b) {
+  constexpr int WAVES = 16, TEAMS = 1024 / T, PER = EMBED_FEW / WAVES / 256;
+  __shared__ int counts[WAVES][EMBED_FEW_RANGE], starts[EMBED_FEW_RANGE + 1], waves[WAVES], longs[EMBED_FEW_RANGE], long_count;
+  __shared__ unsigned short list[EMBED_FEW];
+  __shared__ float parts[TEAMS][T * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int range = blockIdx.x / b.tiles, tile = blockIdx.x - range * b.tiles, lo = range * a.range, size = a.n - lo < a.range ? a.n - lo : a.range;
+  const int per = (a.w + WAVES * 256 - 1) / (WAVES * 256) * 256, from = wv * per, to = from + per < a.w ? from + per : a.w;
+  float l[PER][4];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = from + 256 * k + 4 * lane;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l[k][e] = -1.f;
+    if (256 * k >= per) continue;
+    if (c + 4 <= to) col_load<false>(l[k], a.labels + c);
+    else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (c + e < to) l[k][e] = a.labels[c + e];
+    }
+  }
+  for (int k = tid; k < WAVES * EMBED_FEW_RANGE; k += 1024) (&counts[0][0])[k] = 0;
+  if (tid == 0) long_count = 0;
+  __syncthreads();
+  const float first = (float)lo, behind = (float)(lo + size);
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (l[k][e] >= first && l[k][e] < behind) atomicAdd(&counts[wv][(int)l[k][e] - lo], 1);
+  __syncthreads();
+  int mine = 0;
+  if (tid < size)
+    for (int k = 0; k < WAVES; ++k) mine += counts[k][tid];
+  int up = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { const int q = __shfl_up(up, o, WAVE); if (lane >= o) up += q; }
+  if (lane == 63) waves[wv] = up;
+  __syncthreads();
+  int start = up - mine;
+  for (int k = 0; k < wv; ++k) start += waves[k];
+  if (tid < size) {
+    starts[tid] = start;
+    if (tid == size - 1) starts[size] = start + mine;
+    if (mine > EMBED_RUN) longs[atomicAdd(&long_count, 1)] = tid;
+    for (int k = 0, at = start; k < WAVES; ++k) { const int q = counts[k][tid]; counts[k][tid] = at; at += q; }
+  }
+  __syncthreads();
+  volatile int* const next = counts[wv];
+  const int bits = 32 - __builtin_clz(a.range);
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = l[k][e] >= first && l[k][e] < behind;
+      const unsigned long long all = __ballot(in);
+      if (all == 0) continue;
+      const int x = (int)l[k][e] - lo;
+      int rank, count;
+      embed_same(all, x, bits, &rank, &count);
+      if (in) {
+        const int at = next[x];
+        list[at + rank] = (unsigned short)(from + 256 * k + 4 * lane + e);
+        if (rank == 0) next[x] = at + count;
+      }
+    }
+  __syncthreads();
+  const int row0 = tile * b.rows, team = T == 64 ? wv : tid / T;
+  EmbedRows<T, 1, W, TAIL> rows;
+  rows.init(tid % T, b.h - row0 < b.rows ? b.h - row0 : b.rows);
+  const float* const deriv = b.deriv + row0;
+  auto add = [&](float (&sum)[1][4], int at, int count) __attribute__((always_inline)) {
+    for (int k = 0; k < count; k += 8) {                  // (the last one again in the place of those that are not there)
+      float v[8][1][4];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rows.template load<STREAM>(v[q], deriv + (size_t)list[at + (k + q < count ? k + q : count - 1)] * b.h);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (k + q < count) embed_add<1, W>(sum, v[q]);
+    }
+  };
+  for (int t = team; t < size; t += TEAMS) {
+    const int at = starts[t], count = starts[t + 1] - at;
+    if (count > EMBED_RUN || (count == 0 && b.beta == 1.f)) continue;
+    float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+    add(sum, at, count);
+    embed_out<T, 1, W, TAIL, STREAM>(rows, b.target + (size_t)(lo + t) * b.h + row0, sum, b.beta, b.mult);
+  }
+  const int many = long_count;
+  for (int i = 0; i < many; ++i) {
+    const int t = longs[i], at = starts[t], count = starts[t + 1] - at, each = (count + TEAMS - 1) / TEAMS, used = (count + each - 1) / each;
+    float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+    if (team < used) add(sum, at + team * each, count - team * each < each ? count - team * each : each);
+#pragma unroll
+    for (int e = 0; e < W; ++e) parts[team][tid % T * W + e] = sum[0][e];
+    __syncthreads();
+    if (team == i % TEAMS) {
+      for (int k = 0; k < used; ++k)
+#pragma unroll
+        for (int e = 0; e < W; ++e) sum[0][e] = k ? sum[0][e] + parts[k][tid % T * W + e] : parts[0][tid % T * W + e];
+      embed_out<T, 1, W, TAIL, false>(rows, b.target + (size_t)(lo + t) * b.h + row0, sum, b.beta, b.mult);
+    }
+    __syncthreads();
+  }
+}
+
 // Tiles of at most `most` rows, a multiple of four; the last one has a group of four rows too.
 static void embed_tiles(EmbedSums& s, int most) {
   s.tiles = (s.h + most - 1) / most;
@@ -339,7 +460,28 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
   if (h <= 0 || n <= 0) return 0;
   EmbedSums s;
   s.deriv = deriv->data_device; s.target = target->data_device; s.h = h; s.n = n; s.beta = beta; s.mult = mult;
-  s.slot_count = w > EMBED_RUN ? (w + EMBED_SLOT - 1) / EMBED_SLOT : 0;
+  const bool stream = (long long)h * (w > n ? w : n) >= DN_STREAM_MIN_ELEMS;
+  EmbedSort o;
+  o.labels = labels->data_device; o.w = w; o.n = n;
+  embed_tiles(s, h <= 64 ? 64 : 256);
+  // One launch while the frequent tokens, which a workgroup has by itself, are not many columns (us, three launches / one: 1024 x 64 of 256 tokens 10.4 / 5.8, x 4000
+  // 16.6 / 12.7, x 6000 21.6 / 21.5, x 8000 24.5 / 27.4; 64 x 8000 of 1000 18.4 / 11.2; 4096 x 1000 of 200 16.0 / 14.1, x 4000 30.3 / 38.7).  Fewer workgroups for few
+  // columns (1024 x 64 in 1024 8.6, x 4000 in 512 15.4).
+  if (w <= EMBED_FEW && (long long)h * w <= 1 << 22 && (long long)n * s.tiles <= 4096) {
+    const int want = w <= 512 ? 512 : 1024;
+    o.range = (int)(((long long)n * s.tiles + want - 1) / want);
+    const long long groups = (long long)((n + o.range - 1) / o.range) * s.tiles;
+#define FEW2(T, W, TAIL) do { if (stream) hipLaunchKernelGGL((k_embed_few<T, W, TAIL, true>), dim3((unsigned)groups), dim3(1024), 0, dn_stream(), o, s); \
+                              else hipLaunchKernelGGL((k_embed_few<T, W, TAIL, false>), dim3((unsigned)groups), dim3(1024), 0, dn_stream(), o, s); } while (0)
+#define FEW(T, W) do { if (h % 4 && W == 4) FEW2(T, W, true); else FEW2(T, W, false); } while (0)
+    if (h < 4) FEW(16, 1);
+    else if (h <= 64) FEW(16, 4);
+    else FEW(64, 4);
+#undef FEW
+#undef FEW2
+    return dn_launch_status();
+  }
+  s.slot_count = (w + EMBED_SLOT - 1) / EMBED_SLOT;
   embed_tiles(s, 1024);
   const long long sums = ((long long)s.slot_count + n) * s.tiles;
   if (sums >= 1ll << 31) return ERROR_UNSUPPORTED;
@@ -347,19 +489,16 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
   const size_t ints = ((size_t)n + 1 + w + 3) / 4 * 4, slots = (size_t)(w + EMBED_SLOT - 1) / EMBED_SLOT;
   char* scratch = (char*)dn_scratch(4 * ints + sizeof(EmbedSlot) * slots + 4 * (size_t)s.slot_count * h);
   if (!scratch) return CUDA_ERROR;
-  EmbedSort o;
-  o.labels = labels->data_device; o.w = w; o.n = n;
   o.starts = (int*)scratch; o.sorted = o.starts + n + 1; o.slots = (EmbedSlot*)(scratch + 4 * ints);
   s.starts = o.starts; s.sorted = o.sorted; s.slots = o.slots; s.partials = (float*)(o.slots + slots);
   // Few tokens a workgroup that sorts (its turns are as many as it has different tokens among 64 columns), unless the labels are so many that
   // reading them that often would take long.
-  long long sorters = (1ll << 25) / (w > 0 ? w : 1);
+  long long sorters = (1ll << 25) / w;
   sorters = sorters < 512 ? sorters : 512;
   const long long least = ((long long)n + EMBED_RANGE - 1) / EMBED_RANGE;
   sorters = sorters > least ? sorters : least;
   o.range = (int)((n + sorters - 1) / sorters);
   hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)((n + o.range - 1) / o.range)), dim3(1024), 0, dn_stream(), o);
-  const bool stream = (long long)h * (w > n ? w : n) >= DN_STREAM_MIN_ELEMS;
   // (items of one launch: teams of 16 or 64 lanes)
   auto launches = [&](long long items, int team, auto go) {
     const long long most = DN_MAX_GROUPS * (256 / team);
@@ -380,7 +519,7 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
 #undef SUMS
 #undef SUMS2
 #undef SUMS3
-  if (s.slot_count) {
+  {
     embed_tiles(s, 256);
     const long long joins = (long long)s.slot_count * s.tiles;
 #define JOIN(T, W, TAIL) launches(joins, T, [&](dim3 grid) { hipLaunchKernelGGL((k_embed_join<T, W, TAIL>), grid, dim3(256), 0, dn_stream(), s); })

@@ -64,7 +64,7 @@ def check_embed_grad(got, dy, labels, n, mult=1.0, old=None, beta=0.0):
     check(got, was + want, U * ((count[None, :] + 2) * size + 3 * (np.abs(was) + np.abs(want))))
 
 
-@pytest.mark.parametrize("h,w,n", EMBED_SHAPES + [(20, 5000, 1), (33, 9000, 7), (130, 3000, 300), (17, 20001, 256), (64, 3000, 40000), (1, 30000, 5), (260, 2049, 2), (1025, 40, 6), (2050, 33, 3), (306177, 3, 2)])
+@pytest.mark.parametrize("h,w,n", EMBED_SHAPES + [(20, 5000, 1), (33, 9000, 7), (130, 3000, 300), (17, 20001, 256), (64, 3000, 40000), (1, 30000, 5), (260, 2049, 2), (1025, 40, 6), (2050, 33, 3), (306177, 3, 2), (512, 8192, 9), (512, 8193, 9), (3, 8000, 2000), (64, 600, 4096), (65, 513, 4090), (300, 512, 2048), (300, 513, 2049), (68, 4000, 1)])
 @pytest.mark.parametrize("skip", [0, 1])
 def test_embed_grad(cm, rng, h, w, n, skip):
     dy, labels = F(rng.standard_normal((h, w))), frequent(rng, n, w)

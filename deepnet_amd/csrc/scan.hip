@@ -51,7 +51,7 @@ struct ScanCut {
 #define SCAN_GROUP 16
 #define SCAN_TILES 1024            // of one launch
 #define SCAN_WORDS (16 * SCAN_TILES)   // a counter a tile, each in a memory line of its own
-#define SCAN_POLLS (1 << 18)       // (a wait lasts some microseconds; one that lasts this long gives NaN)
+#define SCAN_POLLS (1 << 20)       // (a wait lasts some microseconds; one that lasts this long, about a second, gives NaN)
 
 // Which launch this is, and which of a tile's workgroups.  A tile's counter has the launches in its upper 36 bits; the last place taken moves it on,
 // and those of tiles that this launch does not have, so that all of them always agree on the launch.

@@ -274,6 +274,35 @@ def test_gated_scan_gives_the_same_bits_every_time(cm, rng):
         assert all(np.array_equal(p, q) for p, q in zip(r, runs[0]))
 
 
+def test_gated_scan_of_many_sizes_in_turn(cm):
+    """What workgroups hand to each other stands where other sizes, and other launches of the same size, have left theirs: every call has the bits of
+    its first one, in whatever order the sizes come, eagerly and replayed."""
+    rng = np.random.default_rng(12)
+    sets = []
+    for f, w in ((64, 3000), (65, 2500), (300, 700), (1, 9000), (30, 40000), (200, 5000), (700, 1300), (64, 60000), (1100, 400)):
+        pre, state, dy, _ = scan_inputs(rng, f, w, 1)
+        s = dict(P=cm.CUDAMatrix(pre), S=cm.CUDAMatrix(state), D=cm.CUDAMatrix(dy), y=cm.empty((f, w)), dp=cm.empty((2 * f, w)), ds=cm.empty((f, 1)))
+        def step(s=s):
+            cm.gated_scan(s['P'], target=s['y'], state=s['S'])
+            cm.gated_scan_grad(s['D'], s['P'], s['y'], target=s['dp'], state=s['S'], state_grad=s['ds'])
+        step()
+        s['want'] = bits([s['y'], s['dp'], s['ds']])
+        want, _, off, _ = seq.gated_scan(pre[:, :300], [0, 300], state)
+        check(s['y'].asarray()[:, :300], want, STEP * U * off)
+        s['step'] = step
+        sets.append(s)
+    for s in sets:
+        with cm.Graph() as g:
+            s['step']()
+        s['graph'] = g
+    for turn in range(150):
+        s = sets[int(rng.integers(len(sets)))]
+        for name in ('y', 'dp', 'ds'):
+            s[name].assign(7.0)
+        s['graph'].launch() if turn % 3 == 0 else s['step']()
+        assert all(np.array_equal(p, q) for p, q in zip(bits([s['y'], s['dp'], s['ds']]), s['want'])), turn
+
+
 def test_gated_scan_gradients_against_differences(cm):
     """The device's gradients along random directions against differences of the oracle's recurrence."""
     rng = np.random.default_rng(6)
@@ -362,6 +391,12 @@ def test_sample_tokens_of_ties_masks_and_special_columns(cm, rng, h):
             check_sample(cm, x[:, few], u[few], **rule)
     u = F(np.array([np.nan, -1.0, 1.0, 7.0] * 4))
     check_sample(cm, F(np.tile(np.log([[3.0], [1.0], [2.0]]), (1, 16))), u)
+
+
+def test_sample_tokens_of_no_rows(cm):
+    logp = cm.CUDAMatrix(F([[5.0, 5.0]]))
+    t = cm.sample_tokens(cm.empty((0, 2)), cm.CUDAMatrix(F([[0.5, 0.5]])), logp=logp)
+    assert (t.asarray() == -1).all() and not logp.asarray().any()
 
 
 def test_sample_tokens_draws_by_the_shares(cm):

@@ -125,8 +125,8 @@ __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
 }
 
 // The entries of a column: a wavefront has a stretch of it, 256 rows a slab, four of them a lane; in registers (NV slabs) or, of columns that those do not hold
-// (NV = 0), from memory, where eight slabs are on their way at once.  f(x, row, slab) for a lane's four, rows behind the column being -infinity.
-template <int LANES, int NV>
+// (NV = 0), from memory, where AHEAD slabs are on their way at once.  f(x, row, slab) for a lane's four, rows behind the column being -infinity.
+template <int LANES, int NV, int AHEAD = 8>
 struct SampleColumn {
   const float* c;
   int h, from, slabs;              // the stretch's first row of this lane, slabs of a stretch
@@ -167,12 +167,12 @@ struct SampleColumn {
           __builtin_amdgcn_sched_barrier(0);
         }
     } else {
-      for (int k = 0; k < slabs; k += 8) {
-        float v[8][4];
+      for (int k = 0; k < slabs; k += AHEAD) {
+        float v[AHEAD][4];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) fetch(v[q], from + 256 * (k + q));
+        for (int q = 0; q < AHEAD; ++q) fetch(v[q], from + 256 * (k + q));
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < AHEAD; ++q)
           if (k + q < slabs) { f(v[q], from + 256 * (k + q), k + q); __builtin_amdgcn_sched_barrier(0); }
       }
     }
@@ -557,8 +557,8 @@ __device__ __forceinline__ u64 sample_slab(const SampleArgs& a, int col, const S
 
 // A workgroup a column, which it holds in registers, of up to 16384 rows, or reads again, from the caches (32768 x 512 takes as long either way).
 // Weights are whole numbers (sample_weight), so every sum and with it every border is the same however it is added up.
-template <int LANES, int NV>
-__global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
+template <int LANES, int NV, bool LIMITS>
+__global__ void __launch_bounds__(LANES, LIMITS || LANES < 1024 || NV == 0 ? 1 : 8) k_sample_tokens(SampleArgs a) {
   constexpr int W = LANES / 64;
   __shared__ SampleShared<LANES> sh;
   const int col = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -604,10 +604,12 @@ __global__ void __launch_bounds__(LANES) k_sample_tokens(SampleArgs a) {
   kept.plain = most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
   kept.bordered = false;
   kept.x = kept.above = kept.plain ? most - kept.far : -INFINITY;
-  if (rule.k < a.h || rule.top_p < 1.0) {
-    __syncthreads();
-    if (!sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
-    column.init(column.c, a.h);                            // (the registers are the lists' meanwhile)
+  if constexpr (LIMITS) {
+    if (rule.k < a.h || rule.top_p < 1.0) {
+      __syncthreads();
+      if (!sample_border<LANES, NV>(a, col, column, rule, kept, mine, least, sh)) return;
+      column.init(column.c, a.h);                          // (the registers are the lists' meanwhile)
+    }
   }
   // the weights of every wavefront's stretch, and the stretch that the aim is in
   u64 sum = 0;
@@ -687,13 +689,16 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   if (w <= 0) return 0;
   int bits = 0;
   while ((1 << bits) < h) ++bits;
+  // From the whole distribution, as the numbers say: without the lists two workgroups fit a CU.
+  const bool limits = top_k || top_p || min_p || (all_top_k >= 1.f && all_top_k < (float)h) || all_top_p < 1.f || all_min_p > 0.f;
   const long long most = h <= 4096 ? DN_MAX_GROUPS : DN_MAX_GROUPS / 4;            // columns of a launch
   for (long long c0 = 0; c0 < w; c0 += most) {
     const int n = (int)(w - c0 < most ? w - c0 : most);
     auto from = [c0](const cudamat* m) { return m ? m->data_device + c0 : nullptr; };
     const SampleArgs a = {mat->data_device + c0 * h, from(uniform), from(temperature), from(top_k), from(top_p), from(min_p), from(target), from(logp),
                           all_temperature, all_top_k, all_top_p, all_min_p, h, n, 62 - bits < 45 ? 62 - bits : 45};
-#define SAMPLE_GO(LANES, NV) hipLaunchKernelGGL((k_sample_tokens<LANES, NV>), dim3(n), dim3(LANES), 0, dn_stream(), a)
+#define SAMPLE_GO(LANES, NV) do { if (limits) hipLaunchKernelGGL((k_sample_tokens<LANES, NV, true>), dim3(n), dim3(LANES), 0, dn_stream(), a); \
+                                  else hipLaunchKernelGGL((k_sample_tokens<LANES, NV, false>), dim3(n), dim3(LANES), 0, dn_stream(), a); } while (0)
     if (h <= 1024) SAMPLE_GO(256, 1);
     else if (h <= 4096) SAMPLE_GO(256, 4);
     else if (h <= 16384) SAMPLE_GO(1024, 4);

@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(1024) k_embed_sort(EmbedSort a) {
         const bool in = l[k][e] >= first && l[k][e] < behind;
         const unsigned long long all = __ballot(in);
         if (all == 0) continue;
-        const int x = (int)l[k][e] - lo;
+        const int x = in ? (int)l[k][e] - lo : 0;
         int rank, count;
         embed_same(all, x, bits, &rank, &count);
         if (in) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(1024) k_embed_few(EmbedSort a, EmbedSums b) {
       const bool in = l[k][e] >= first && l[k][e] < behind;
       const unsigned long long all = __ballot(in);
       if (all == 0) continue;
-      const int x = (int)l[k][e] - lo;
+      const int x = in ? (int)l[k][e] - lo : 0;
       int rank, count;
       embed_same(all, x, bits, &rank, &count);
       if (in) {
@@ -493,7 +493,7 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
   s.starts = o.starts; s.sorted = o.sorted; s.slots = o.slots; s.partials = (float*)(o.slots + slots);
   // Few tokens a workgroup that sorts (its turns are as many as it has different tokens among 64 columns), unless the labels are so many that
   // reading them that often would take long.
-  long long sorters = (1ll << 25) / w;
+  long long sorters = w > 0 ? (1ll << 25) / w : 512;
   sorters = sorters < 512 ? sorters : 512;
   const long long least = ((long long)n + EMBED_RANGE - 1) / EMBED_RANGE;
   sorters = sorters > least ? sorters : least;

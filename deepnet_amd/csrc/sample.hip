@@ -432,7 +432,7 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
   constexpr int BINS = SampleShared<LANES>::BINS, LIST = SampleShared<LANES>::LIST;
   const int tid = threadIdx.x;
   const bool by_count = rule.k < column.h;
-  const float scale = fminf((float)BINS / fminf(kept.far, kept.m - least_x), 3e38f);
+  const float scale = fminf((float)BINS / fminf(fminf(kept.far, kept.m - least_x), 3.402823466e38f), 3e38f);      // (a distance may overflow: the last bin)
   auto bin = [&](float v) __attribute__((always_inline)) { return (int)fminf((kept.m - v) * scale, (float)(BINS - 1)); };
   auto clear = [&](int place) __attribute__((always_inline)) {
     sh.counts[tid] = 0;
@@ -680,6 +680,7 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   cudamat* const all[8] = {mat, uniform, temperature, top_k, top_p, min_p, target, logp};
   if (int e = tok_check_device(all)) return e;
   const int h = mat->size[0], w = mat->size[1];
+  if (!uniform || !target) return ERROR_INCOMPATIBLE_DIMENSIONS;
   for (int i = 1; i < 8; ++i)
     if (!tok_shape(all[i], 1, w)) return ERROR_INCOMPATIBLE_DIMENSIONS;
   if (h > (1 << 24)) return ERROR_UNSUPPORTED;

@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(1024) k_gated_scan(ScanArgs a, ScanCut cut) {
   unsigned tag = 0;
   if (cut.chunks > 1) {
     const ScanPlace o = scan_take_place(cut.words, tile, cut.tiles, cut.chunks, &place);
+    if (o.chunk >= cut.chunks) return;                     // (only where calls overlap, which they may not)
     chunk = __builtin_amdgcn_readfirstlane(o.chunk);
     tag = __builtin_amdgcn_readfirstlane((unsigned)o.launch + 1u);
   }

@@ -89,8 +89,8 @@ def gated_scan_grad(dy, pre, out, at, state=None, last_deriv=None):
 
 # ---- sampling
 
-def sample_token(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """(token, log probability, the kept entries) of one column."""
+def sample_token(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, part=1.0):
+    """(token, log probability, the kept entries) of one column.  part: a factor of what top_p asks for."""
     x = np.asarray(x, dtype=np.float32).astype(np.float64)
     temperature, top_k, top_p, min_p, u = (float(np.float32(v)) for v in (temperature, top_k, top_p, min_p, uniform))
     h = x.size
@@ -110,7 +110,7 @@ def sample_token(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         kept = [i for i in kept if w[i] >= min(min_p, 1.0)]
     if top_p < 1:
         total, up_to, n = math.fsum(w[i] for i in kept), 0.0, 0
-        while n == 0 or up_to < top_p * total:
+        while n == 0 or (n < len(kept) and up_to < part * top_p * total):
             up_to += w[kept[n]]
             n += 1
         kept = kept[:n]

@@ -114,6 +114,15 @@ def test_embed_grad_of_no_columns_and_of_no_tokens(cm, rng):
             assert np.array_equal(g.asarray(), want)
 
 
+@pytest.mark.parametrize("h,n", [(6, 5000), (1030, 5000), (3, 1 << 20)])
+def test_embed_grad_of_no_columns_and_many_tokens(cm, rng, h, n):
+    old = F(rng.standard_normal((h, n)))
+    for beta, want in ((0.0, np.zeros((h, n))), (1.0, old), (0.5, F(0.5) * old)):
+        g = cm.CUDAMatrix(old)
+        cm.embed_grad(cm.empty((h, 0)), cm.empty((1, 0)), g, beta=beta)
+        assert np.array_equal(g.asarray(), want)
+
+
 def test_embed_grad_gives_the_same_bits_every_time(cm, rng):
     h, w, n = 200, 30000, 5000
     d, l = cm.CUDAMatrix(F(rng.standard_normal((h, w)))), cm.CUDAMatrix(frequent(rng, n, w))
@@ -336,7 +345,17 @@ def check_sample(cm, x, u, skip=0, **rule):
     got, got_logp = tokens.asarray()[0], logp.asarray()[0]
     assert np.array_equal(again.asarray()[0], got), 'without logp'
     for c in range(w):
-        token, lp, kept = seq.sample_token(x[:, c], u[c], **{k: v[c] if np.ndim(v) else v for k, v in rule.items()})
+        own = {k: v[c] if np.ndim(v) else v for k, v in rule.items()}
+        token, lp, kept = seq.sample_token(x[:, c], u[c], **own)
+        if got[c] != token and own.get('top_p', 1.0) < 1:
+            # Every weight is rounded by at most half of 2^-45 (h of up to 2^17), so their sum, which is 1 or more, by at most h 2^-46 of itself, and so is a
+            # border in it: where top_p of the sum is the weight of some first entries to within that (75 of 100 equal ones and 600 of
+            # 4e-15 each, which are 0 as multiples, with top_p = 0.75), one entry more or less is kept.
+            assert h <= 1 << 17
+            for p in (1 - h * 2.0 ** -46, 1 + h * 2.0 ** -46):
+                near = seq.sample_token(x[:, c], u[c], part=p, **own)
+                if near[0] == got[c]:
+                    token, lp, kept = near
         assert got[c] == token, (c, got[c], token, lp, len(kept), u[c], {k: v[c] if np.ndim(v) else v for k, v in rule.items()})
         assert got_logp[c] == lp or (np.isnan(lp) and np.isnan(got_logp[c])) or abs(got_logp[c] - lp) <= 2 * U * abs(lp) + 1e-10, (c, got_logp[c], lp)
 
@@ -391,6 +410,17 @@ def test_sample_tokens_of_ties_masks_and_special_columns(cm, rng, h):
             check_sample(cm, x[:, few], u[few], **rule)
     u = F(np.array([np.nan, -1.0, 1.0, 7.0] * 4))
     check_sample(cm, F(np.tile(np.log([[3.0], [1.0], [2.0]]), (1, 16))), u)
+
+
+@pytest.mark.parametrize("h", [700, 3000, 20000])
+def test_sample_tokens_of_distances_that_overflow(cm, rng, h):
+    far, rows = 3e38, np.arange(h)
+    x = np.stack([np.where(rows % 2, -far, far), np.where(rows % 5, far, -far + rows / h * 1e38), np.where(rows % 7, -far * (0.1 + 0.8 * rows / h), far), np.where(rows == 3, far, -far),
+                  rng.uniform(-far, far, h)], axis=1)
+    w = x.shape[1]
+    for temperature in (float('inf'), 3e38, 1e38, 1e37):
+        for rule in (dict(top_p=0.45), dict(top_p=0.75), dict(top_p=0.98), dict(top_k=h - 5), dict(top_k=100, top_p=0.9), dict(min_p=0.3), dict()):
+            check_sample(cm, F(x), F(rng.random(w)), temperature=temperature, **rule)
 
 
 def test_sample_tokens_of_no_rows(cm):

@@ -160,6 +160,9 @@ def test_sample_tokens_refusals(cm):
     assert call(a) == UNSUPPORTED
     a = list(good); a[0] = handle(cm, (1 << 24) + 1, 3, 1 << 42)
     assert call(a) == UNSUPPORTED
+    for i in (1, 6):
+        a = list(good); a[i] = None
+        assert call(a) == INCOMPATIBLE
 
 
 def test_calls_without_columns_queue_nothing(cm):

@@ -3,6 +3,7 @@
 #include "columns.h"
 #include "tokens.h"
 #include "wide_math.h"
+#include <type_traits>
 
 struct SampleArgs {
   const float *mat, *uniform, *temperature, *top_k, *top_p, *min_p;
@@ -129,7 +130,7 @@ __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
 template <int LANES, int NV, int AHEAD = 8>
 struct SampleColumn {
   const float* c;
-  int h, from, slabs;              // the stretch's first row of this lane, slabs of a stretch
+  int h, from, slabs;              // behind the last row; the stretch's first row of this lane, slabs of a stretch
   float x[NV ? NV : 1][4];
   __device__ __forceinline__ void fetch(float (&v)[4], int row) const {
 #pragma unroll
@@ -141,10 +142,10 @@ struct SampleColumn {
         if (row + e < h) v[e] = c[row + e];
     }
   }
-  __device__ __forceinline__ void init(const float* column, int rows) {
-    c = column; h = rows;
-    slabs = (h + 4 * LANES - 1) / (4 * LANES);
-    from = (int)(threadIdx.x >> 6) * slabs * 256 + 4 * (int)(threadIdx.x & 63);
+  __device__ __forceinline__ void init(const float* column, int end, int first = 0) {
+    c = column; h = end;
+    slabs = (h - first + 4 * LANES - 1) / (4 * LANES);
+    from = first + (int)(threadIdx.x >> 6) * slabs * 256 + 4 * (int)(threadIdx.x & 63);
     if (NV) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -224,6 +225,16 @@ struct SampleKept {
     bordered = true;
   }
 };
+// What may be kept before any border is known.
+__device__ __forceinline__ SampleKept sample_kept(const SampleArgs& a, const SampleRule& rule, float most, const double* table) {
+  SampleKept kept;
+  kept.m = most; kept.row = 0; kept.c = rule.c * 256.0; kept.least = rule.least; kept.table = table;
+  kept.far = (float)((a.shift + 1.5) / rule.c);            // (2^-(shift + 1) is nothing; half an octave for the rounding of the distance)
+  kept.plain = most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
+  kept.bordered = false;
+  kept.x = kept.above = kept.plain ? most - kept.far : -INFINITY;
+  return kept;
+}
 __device__ __forceinline__ void sample_out(const SampleArgs& a, int col, const SampleKept& kept, float v, int row, u64 total) {
   a.tokens[col] = (float)row;
   if (a.logp) a.logp[col] = (float)(((double)v - (double)kept.m) * (kept.c * (0.6931471805599453 / 256.0)) - dn_log_wide_pos(ldexp((double)total, -a.shift)));
@@ -257,19 +268,46 @@ __device__ __forceinline__ u64 sample_bisect(const SampleColumn<LANES, NV>& colu
   return border;
 }
 
-// Of the few (n2) entries in sh.few: how many are greater than this lane's, and their weights.  (Lanes that have none are here too.)
+// Sums over the LANES / SAMPLE_SHORT lanes that have one of few entries together; every one of them gets it.
+template <int TEAM>
+__device__ __forceinline__ u64 team_sum_u64(u64 v) {
+  static_assert(TEAM == 1 || TEAM == 4, "a lane or a quad");
+  if (TEAM == 4) {
+    auto move = [&](u64 x, auto step) __attribute__((always_inline)) {
+      constexpr int CTRL = decltype(step)::value;
+      const unsigned lo = __builtin_amdgcn_mov_dpp((int)(unsigned)x, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp((int)(unsigned)(x >> 32), CTRL, 0xf, 0xf, true);
+      return (u64)hi << 32 | lo;
+    };
+    v += move(v, std::integral_constant<int, 0xB1>());
+    v += move(v, std::integral_constant<int, 0x4E>());
+  }
+  return v;
+}
+// Of the few (n2) entries in sh.few: how many are greater than that of this lane's team, and their weights.  (Lanes that have none are here too.)
 template <int LANES>
 __device__ __forceinline__ void sample_standing(int n2, SampleShared<LANES>& sh, u64 key, int* rank, u64* mass) {
-  int r = 0;
-  u64 m = 0;
+  constexpr int TEAM = LANES / SAMPLE_SHORT;
+  u64 r = 0, m = 0;
 #pragma unroll 4
-  for (int i = 0; i < n2; ++i) {
+  for (int i = threadIdx.x % TEAM; i < n2; i += TEAM) {
     const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
     r += q.x > key ? 1 : 0;
     m += q.x > key ? q.y : 0;
   }
-  *rank = r;
-  *mass = m;
+  *rank = (int)team_sum_u64<TEAM>(r);
+  *mass = team_sum_u64<TEAM>(m);
+}
+// The weights of those of them that are kept and further up than a row.
+template <int LANES>
+__device__ __forceinline__ u64 sample_further_up(int n2, SampleShared<LANES>& sh, u64 border, int row) {
+  constexpr int TEAM = LANES / SAMPLE_SHORT;
+  u64 m = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x % TEAM; i < n2; i += TEAM) {
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
+    m += lp_key_index(q.x) < row && q.x >= border ? q.y : 0;
+  }
+  return team_sum_u64<TEAM>(m);
 }
 
 // From the n listed candidates: the border, of the first k (by_count: of those the first that have top_p of their weight) or where the weights, mass_before
@@ -280,40 +318,35 @@ __device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, i
                                                  u64 mass_before, u64 ask) {
   constexpr int BINS = SampleShared<LANES>::BINS;
   const int tid = threadIdx.x;
+  constexpr int TEAM = LANES / SAMPLE_SHORT;
+  const int who = tid / TEAM;      // (the entry that this lane has with its team)
+  const bool leads = tid % TEAM == 0;
   if (n <= SAMPLE_SHORT) {
     u64 key = 0, w = 0, m;
     int rank;
-    if (tid < n) {
-      key = sh.list[tid];
+    if (who < n) {
+      key = sh.list[who];
       w = kept.weight(lp_key_value(key));
-      sh.few[2 * tid] = key;
-      sh.few[2 * tid + 1] = w;
+      if (leads) { sh.few[2 * who] = key; sh.few[2 * who + 1] = w; }
     }
     __syncthreads();
-    if (tid < n) {
-      sample_standing<LANES>(n, sh, key, &rank, &m);
-      if (by_count && rank == (rule.k < n ? rule.k : n) - 1) { sh.border = key; sh.total = m + w; }
+    sample_standing<LANES>(n, sh, key, &rank, &m);
+    if (by_count) {
+      if (leads && who < n && rank == (rule.k < n ? rule.k : n) - 1) { sh.border = key; sh.total = m + w; }
+      __syncthreads();
+      ask = sample_ask(rule, sh.total);
     }
-    __syncthreads();
-    if (by_count) ask = sample_ask(rule, sh.total);
     if (!by_count || rule.top_p < 1.0) {
       __syncthreads();
-      if (tid < n && w && mass_before + m < ask && mass_before + m + w >= ask) { sh.border = key; sh.total = mass_before + m + w; }
-      __syncthreads();
+      if (leads && who < n && w && mass_before + m < ask && mass_before + m + w >= ask) { sh.border = key; sh.total = mass_before + m + w; }
     }
+    __syncthreads();
     const u64 border = sh.border, total = sh.total;
     if (!whole) { kept.from(border); return true; }
-    if (key >= border && w) {
-      const u64 aim = sample_aim(rule, total);
-      const int row = lp_key_index(key);
-      u64 sum = 0;
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
-        sum += lp_key_index(q.x) < row && q.x >= border ? q.y : 0;
-      }
-      if (sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
-    }
+    const u64 aim = sample_aim(rule, total);
+    const int row = lp_key_index(key);
+    const u64 sum = sample_further_up<LANES>(n, sh, border, row);
+    if (leads && who < n && key >= border && w && sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
     sh.drawn = 1;
     return true;
   }
@@ -367,13 +400,13 @@ __device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, i
     __syncthreads();
     const int n2 = sh.listed;
     if (n2 > SAMPLE_SHORT) return false;
-    if (tid < n2) {
-      const u64 key = sh.few[2 * tid], w = sh.few[2 * tid + 1];
+    {
+      const u64 key = who < n2 ? sh.few[2 * who] : 0, w = who < n2 ? sh.few[2 * who + 1] : 0;
       int rank;
       u64 m;
       sample_standing<LANES>(n2, sh, key, &rank, &m);
       const bool it = step ? w && base + m < want && base + m + w >= want : before + (u64)rank == want - 1;
-      if (it) { sh.border = key; sh.total = base + m + w + mass_before; }
+      if (it && leads && who < n2) { sh.border = key; sh.total = base + m + w + mass_before; }
     }
     __syncthreads();
     border = sh.border;
@@ -407,19 +440,48 @@ __device__ __forceinline__ bool sample_from_list(const SampleArgs& a, int col, i
   __syncthreads();
   const int n2 = sh.listed;
   if (n2 > SAMPLE_SHORT) { kept.from(border); sh.drawn = 0; return true; }      // (of tall columns: by a pass over the column)
-  if (tid < n2) {
-    const u64 key = sh.few[2 * tid], w = sh.few[2 * tid + 1];
-    const int row = lp_key_index(key);
-    u64 sum = base;
-#pragma unroll 4
-    for (int i = 0; i < n2; ++i) {
-      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sh.few + 2 * i);
-      sum += lp_key_index(q.x) < row ? q.y : 0;
-    }
-    if (sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
-  }
+  const u64 key = who < n2 ? sh.few[2 * who] : 0, w = who < n2 ? sh.few[2 * who + 1] : 0;
+  const int row = lp_key_index(key);
+  const u64 sum = base + sample_further_up<LANES>(n2, sh, border, row);
+  if (leads && w && sum <= aim && sum + w > aim) sample_out(a, col, kept, lp_key_value(key), row, total);
   sh.drawn = 1;
   return true;
+}
+
+// Bins of even width by the distance to the greatest entry (one that overflows is in the last bin).
+__device__ __forceinline__ float sample_scale(const SampleKept& kept, float least, int bins) {
+  return fminf((float)bins / fminf(fminf(kept.far, kept.m - least), 3.402823466e38f), 3e38f);
+}
+__device__ __forceinline__ int sample_bin(const SampleKept& kept, float v, float scale, int bins) { return (int)fminf((kept.m - v) * scale, (float)(bins - 1)); }
+
+// Lists the entries of the bins first to place, as long as there is room.  AHEAD: returns the weights of this lane's entries in the bins before them.
+template <bool AHEAD, int LANES, int NV>
+__device__ __forceinline__ u64 sample_list(const SampleColumn<LANES, NV>& column, const SampleKept& kept, float scale, int bins, int first, int place, int* listed, u64* list) {
+  constexpr int LIST = SampleShared<LANES>::LIST;
+  // (the values of these bins, with room for the roundings: two comparisons rule most entries out)
+  const float slack = 1e-6f * fabsf(kept.m), end = place >= bins - 1 ? -INFINITY : kept.m - (float)(place + 1) / scale * 1.0001f - slack;
+  const float start = !AHEAD && first > 0 ? kept.m - (float)first / scale * 0.9999f + slack : INFINITY;
+  u64 sum = 0;
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    bool there[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) there[e] = v[e] >= end && v[e] <= start;
+    if (!__any(there[0] || there[1] || there[2] || there[3]) || (!AHEAD && *(volatile int*)listed > LIST)) return;      // (too many already)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (AHEAD) there[e] = there[e] && kept.near(v[e]);
+      int b = AHEAD ? sample_bin(kept, v[e], scale, bins) : 0;
+      if (AHEAD) { const u64 w = kept.weight(there[e] ? v[e] : kept.m); sum += there[e] && b < first ? w : 0; }
+      if (there[e] && (AHEAD || kept.near(v[e]))) {
+        if (!AHEAD) b = sample_bin(kept, v[e], scale, bins);
+        if (b >= first && b <= place) {
+          const int at = atomicAdd(listed, 1);
+          if (at < LIST) list[at] = lp_key(v[e], row + e);
+        }
+      }
+    }
+  });
+  return sum;
 }
 
 // Finds what top-k and top-p keep: the border, for a pass over the column to draw by (true), or, where all that is kept has been listed and is little, draws.
@@ -432,8 +494,8 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
   constexpr int BINS = SampleShared<LANES>::BINS, LIST = SampleShared<LANES>::LIST;
   const int tid = threadIdx.x;
   const bool by_count = rule.k < column.h;
-  const float scale = fminf((float)BINS / fminf(fminf(kept.far, kept.m - least_x), 3.402823466e38f), 3e38f);      // (a distance may overflow: the last bin)
-  auto bin = [&](float v) __attribute__((always_inline)) { return (int)fminf((kept.m - v) * scale, (float)(BINS - 1)); };
+  const float scale = sample_scale(kept, least_x, BINS);
+  auto bin = [&](float v) __attribute__((always_inline)) { return sample_bin(kept, v, scale, BINS); };
   auto clear = [&](int place) __attribute__((always_inline)) {
     sh.counts[tid] = 0;
     sh.masses[tid] = 0;
@@ -441,24 +503,7 @@ __device__ __forceinline__ bool sample_border(const SampleArgs& a, int col, Samp
     __syncthreads();
   };
   auto list_bins = [&](int first, int place) __attribute__((always_inline)) {
-    // (the values of these bins, with room for the roundings: two comparisons rule most entries out)
-    const float slack = 1e-6f * fabsf(kept.m), end = place >= BINS - 1 ? -INFINITY : kept.m - (float)(place + 1) / scale * 1.0001f - slack;
-    const float start = first > 0 ? kept.m - (float)first / scale * 0.9999f + slack : INFINITY;
-    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-      bool there[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) there[e] = v[e] >= end && v[e] <= start;
-      if (!__any(there[0] || there[1] || there[2] || there[3]) || *(volatile int*)&sh.listed > LIST) return;      // (too many already)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (there[e] && kept.near(v[e])) {
-          const int b = bin(v[e]);
-          if (b >= first && b <= place) {
-            const int at = atomicAdd(&sh.listed, 1);
-            if (at < LIST) sh.list[at] = lp_key(v[e], row + e);
-          }
-        }
-    });
+    sample_list<false>(column, kept, scale, BINS, first, place, &sh.listed, sh.list);
     __syncthreads();
     return sh.listed;
   };
@@ -555,6 +600,82 @@ __device__ __forceinline__ u64 sample_slab(const SampleArgs& a, int col, const S
   return all;
 }
 
+// Draws from one stretch of a column, whose first slab begins at `first` (of this lane) and which the aim is in; `base`: the weights before it.
+// All wavefronts look for the part of the stretch (of one slab, or so many that there are at most as many parts as lanes), and one for the row in it.
+template <int LANES, int NV>
+__device__ __forceinline__ void sample_draw_stretch(const SampleArgs& a, int col, const SampleColumn<LANES, NV>& column, const SampleKept& kept, SampleShared<LANES>& sh, int first, u64 base,
+                                                    u64 aim, u64 total) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, fold = (column.slabs + LANES - 1) / LANES;
+  sh.masses[tid] = 0;
+  __syncthreads();
+  for (int part = wv; part * fold < column.slabs; part += LANES / 64) {
+    u64 sum = 0;
+    for (int k = part * fold; k < (part + 1) * fold && k < column.slabs; ++k) {
+      float v[4];
+      u64 w[4];
+      column.fetch(v, first + 256 * k);
+      kept.weights(w, v, first + 256 * k);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    sum = lane_u64(wave_scan_u64(sum), 63);
+    if (lane == 0) sh.masses[part] = sum;
+  }
+  __syncthreads();
+  u64 all;
+  const u64 here = sh.masses[tid], up = base + sample_scan<LANES>(here, sh.wave_sum, &all);
+  if (here && up - here <= aim && up > aim) { sh.place = tid; sh.base = up - here; }      // (one lane)
+  __syncthreads();
+  if (wv) return;
+  base = sh.base;
+  for (int k = sh.place * fold; k < (sh.place + 1) * fold && k < column.slabs && base <= aim; ++k) {
+    float v[4];
+    column.fetch(v, first + 256 * k);
+    base += sample_slab(a, col, kept, v, first + 256 * k, base, aim, total);
+  }
+}
+
+// Draws from what is kept of a column.
+template <int LANES, int NV>
+__device__ __forceinline__ void sample_draw(const SampleArgs& a, int col, const SampleColumn<LANES, NV>& column, const SampleKept& kept, const SampleRule& rule, SampleShared<LANES>& sh) {
+  constexpr int W = LANES / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  // the weights of every wavefront's stretch, and the stretch that the aim is in
+  u64 sum = 0;
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    u64 w[4];
+    kept.weights(w, v, row);
+    sum += (w[0] + w[1]) + (w[2] + w[3]);
+  });
+  sum = lane_u64(wave_scan_u64(sum), 63);
+  __syncthreads();
+  if (lane == 0) sh.wave_sum[wv] = sum;
+  __syncthreads();
+  u64 total = 0, base = 0;
+  if (NV) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) { if (k == wv) base = total; total += sh.wave_sum[k]; }
+    const u64 aim = sample_aim(rule, total);
+    if (aim < base || aim >= base + sum) return;
+    // that wavefront looks for the slab, and the row in it
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      if (base > aim) return;
+      base += sample_slab(a, col, kept, v, row, base, aim, total);
+    });
+    return;
+  }
+  int owner = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) total += sh.wave_sum[k];
+  const u64 aim = sample_aim(rule, total);
+  u64 up_to = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if (up_to <= aim) { owner = k; base = up_to; }
+    up_to += sh.wave_sum[k];
+  }
+  sample_draw_stretch(a, col, column, kept, sh, owner * column.slabs * 256 + 4 * lane, base, aim, total);
+}
+
 // A workgroup a column, which it holds in registers, of up to 16384 rows, or reads again, from the caches (32768 x 512 takes as long either way).
 // Weights are whole numbers (sample_weight), so every sum and with it every border is the same however it is added up.
 template <int LANES, int NV, bool LIMITS>
@@ -598,12 +719,7 @@ __global__ void __launch_bounds__(LANES, LIMITS || LANES < 1024 || NV == 0 ? 1 :
     if (tid == 0) { a.tokens[col] = (float)sh.place; if (a.logp) a.logp[col] = 0.f; }
     return;
   }
-  SampleKept kept;
-  kept.m = most; kept.row = 0; kept.c = rule.c * 256.0; kept.least = rule.least; kept.table = sh.table;
-  kept.far = (float)((a.shift + 1.5) / rule.c);            // (2^-(shift + 1) is nothing; half an octave for the rounding of the distance)
-  kept.plain = most - kept.far > -INFINITY && ((double)most - (double)(most - kept.far)) * rule.c >= a.shift + 1.0;
-  kept.bordered = false;
-  kept.x = kept.above = kept.plain ? most - kept.far : -INFINITY;
+  SampleKept kept = sample_kept(a, rule, most, sh.table);
   if constexpr (LIMITS) {
     if (rule.k < a.h || rule.top_p < 1.0) {
       __syncthreads();
@@ -611,68 +727,261 @@ __global__ void __launch_bounds__(LANES, LIMITS || LANES < 1024 || NV == 0 ? 1 :
       column.init(column.c, a.h);                          // (the registers are the lists' meanwhile)
     }
   }
-  // the weights of every wavefront's stretch, and the stretch that the aim is in
-  u64 sum = 0;
-  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-    u64 w[4];
-    kept.weights(w, v, row);
-    sum += (w[0] + w[1]) + (w[2] + w[3]);
-  });
-  sum = lane_u64(wave_scan_u64(sum), 63);
-  __syncthreads();
-  if (lane == 0) sh.wave_sum[wv] = sum;
-  __syncthreads();
-  u64 total = 0, base = 0;
-  if (NV) {
+  sample_draw(a, col, column, kept, rule, sh);
+}
+
+// ------------------------------------------------------------------ few tall columns
+// A column is divided into parts, a workgroup each, in four launches: the parts' greatest entries; their weights, bin by bin where top-p (or a large top-k)
+// asks for a border; the candidates of the border's bins; and a workgroup a column that finds the border among those and draws, from the rows of
+// one part.  The same sums of whole numbers, so the same tokens and bits as a workgroup a column gives.  What the lists do not hold
+// (thousands of entries that are alike) that one does by itself.
+struct SamplePart { float most, least; int bad, first, listed; };      // first: row of the greatest entry (temperature 0)
+struct SampleParts {
+  int parts, rows;                 // of a column; of a part
+  SamplePart* part;
+  float* maxima;                   // one a lane, of every part
+  u64 *bins, *lists, *sums;        // sums: of kept weights ahead of the list, 16 stretches a part
+};
+#define SAMPLE_PARTS 64            // of a column at most: a lane each where they meet
+#define SAMPLE_BINS 2048           // two a lane: of 128003 logits a border's bin then has so few that they are compared with each other
+typedef SampleShared<1024> SampleHere;
+__device__ __forceinline__ SamplePart sample_meet(const SampleParts& s, int col) {
+  const int lane = threadIdx.x & 63;
+  const SamplePart* p = s.part + (size_t)col * s.parts + (lane < s.parts ? lane : 0);
+  SamplePart o = {};
+  const float most = p->most;
+  o.most = lanes_sum<64, true>(most);
+  o.least = -lanes_sum<64, true>(-p->least);
+  o.bad = __any(p->bad);
+  const unsigned long long who = __ballot(most == o.most);
+  o.first = who ? __builtin_amdgcn_readlane(p->first, (int)__builtin_ctzll(who)) : 0;
+  return o;
+}
+// Which of the ways a column goes: by a list of the first k, by bins of counts or weights, or only its weights' sum.
+__device__ __forceinline__ bool sample_short(const SampleArgs& a, const SampleRule& rule) { return rule.k < a.h && rule.k <= 1024; }
+__device__ __forceinline__ bool sample_whole(const SampleArgs& a, const SampleRule& rule) { return rule.k >= a.h && rule.top_p >= 1.0; }
+
+// This lane's two bins of all parts.
+__device__ __forceinline__ ulonglong2 sample_bins(const SampleParts& s, int col) {
+  const ulonglong2* const bins = (const ulonglong2*)s.bins + (size_t)col * s.parts * (SAMPLE_BINS / 2) + threadIdx.x;
+  ulonglong2 sum = {0, 0};
+  for (int k = 0; k < s.parts; k += 4) {
+    ulonglong2 x[4];
 #pragma unroll
-    for (int k = 0; k < W; ++k) { if (k == wv) base = total; total += sh.wave_sum[k]; }
-    const u64 aim = sample_aim(rule, total);
-    if (aim < base || aim >= base + sum) return;
-    // that wavefront looks for the slab, and the row in it
+    for (int q = 0; q < 4; ++q) x[q] = bins[SAMPLE_BINS / 2 * (k + q < s.parts ? k + q : k)];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (k + q < s.parts) { sum.x += x[q].x; sum.y += x[q].y; }
+  }
+  return sum;
+}
+
+template <bool LIMITS>
+__global__ void __launch_bounds__(1024) k_sample_parts_most(SampleArgs a, SampleParts s) {
+  __shared__ float wave_max[16], wave_min[16];
+  __shared__ int wave_bad[16], place;
+  const int col = blockIdx.x / s.parts, part = blockIdx.x - col * s.parts, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, first = part * s.rows;
+  SampleColumn<1024, 0> column;
+  column.init(a.mat + (size_t)col * a.h, first + s.rows < a.h ? first + s.rows : a.h, first);
+  const SampleRule rule = sample_rule(a, col);
+  float mine[2] = {-INFINITY, -INFINITY}, least = INFINITY;
+  bool bad = false;
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bad |= !(v[e] < INFINITY);
+      mine[e & 1] = fmaxf(mine[e & 1], v[e]);
+      least = fminf(least, v[e] > -INFINITY ? v[e] : INFINITY);
+    }
+  });
+  float most = fmaxf(mine[0], mine[1]);
+  if (LIMITS && sample_short(a, rule)) s.maxima[(size_t)blockIdx.x * 1024 + tid] = most;
+  most = lanes_sum<64, true>(most);
+  least = -lanes_sum<64, true>(-least);
+  bad = __any(bad);
+  if (lane == 0) { wave_max[wv] = most; wave_min[wv] = least; wave_bad[wv] = bad; }
+  if (tid == 0) place = a.h;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 16; ++k) { most = fmaxf(most, wave_max[k]); least = fminf(least, wave_min[k]); bad |= wave_bad[k] != 0; }
+  if (rule.greedy) {
     column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
-      if (base > aim) return;
-      base += sample_slab(a, col, kept, v, row, base, aim, total);
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (v[e] == most) atomicMin(&place, row + e);
     });
+    __syncthreads();
+  }
+  if (tid == 0) s.part[blockIdx.x] = SamplePart{most, least, bad ? 1 : 0, place, 0};
+}
+
+template <bool LIMITS>
+__global__ void __launch_bounds__(1024) k_sample_parts_weigh(SampleArgs a, SampleParts s) {
+  __shared__ __align__(16) u64 bins[LIMITS ? SAMPLE_BINS : 2];
+  __shared__ double table[SAMPLE_STEPS];
+  const int col = blockIdx.x / s.parts, part = blockIdx.x - col * s.parts, tid = threadIdx.x, first = part * s.rows;
+  const SampleRule rule = sample_rule(a, col);
+  const SamplePart met = sample_meet(s, col);
+  if (met.bad || !(met.most > -INFINITY) || rule.greedy || (LIMITS && sample_short(a, rule))) return;
+  SampleColumn<1024, 0> column;
+  column.init(a.mat + (size_t)col * a.h, first + s.rows < a.h ? first + s.rows : a.h, first);
+  const SampleKept kept = sample_kept(a, rule, met.most, table);
+  if (tid < SAMPLE_STEPS) table[tid] = ldexp(sample_step(tid), a.shift);
+  if (LIMITS) reinterpret_cast<ulonglong2*>(bins)[tid] = ulonglong2{0, 0};
+  __syncthreads();
+  if (!LIMITS || sample_whole(a, rule)) {
+    u64 sum = 0;
+    column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+      u64 w[4];
+      kept.weights(w, v, row);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    });
+    sum = lane_u64(wave_scan_u64(sum), 63);
+    if ((tid & 63) == 0) s.sums[blockIdx.x * 16 + (tid >> 6)] = sum;
     return;
   }
-  // all wavefronts look for the part of that stretch (of one slab, or so many that there are at most as many parts as lanes), and one for the row in it
-  int owner = 0;
+  const bool by_count = rule.k < a.h;
+  const float scale = sample_scale(kept, met.least, SAMPLE_BINS);
+  column.each([&](const float (&v)[4], int row, int) __attribute__((always_inline)) {
+    if (by_count) {
 #pragma unroll
-  for (int k = 0; k < W; ++k) total += sh.wave_sum[k];
-  const u64 aim = sample_aim(rule, total);
-  u64 up_to = 0;
-#pragma unroll
-  for (int k = 0; k < W; ++k) {
-    if (up_to <= aim) { owner = k; base = up_to; }
-    up_to += sh.wave_sum[k];
-  }
-  const int first = owner * column.slabs * 256 + 4 * lane, fold = (column.slabs + LANES - 1) / LANES;
-  sh.masses[tid] = 0;
-  __syncthreads();
-  for (int part = wv; part * fold < column.slabs; part += W) {
-    sum = 0;
-    for (int k = part * fold; k < (part + 1) * fold && k < column.slabs; ++k) {
-      float v[4];
+      for (int e = 0; e < 4; ++e)
+        if (kept.near(v[e])) atomicAdd(&bins[sample_bin(kept, v[e], scale, SAMPLE_BINS)], 1ull);
+    } else {
       u64 w[4];
-      column.fetch(v, first + 256 * k);
-      kept.weights(w, v, first + 256 * k);
-      sum += (w[0] + w[1]) + (w[2] + w[3]);
+      kept.weights(w, v, row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (w[e]) atomicAdd(&bins[sample_bin(kept, v[e], scale, SAMPLE_BINS)], w[e]);
     }
-    sum = lane_u64(wave_scan_u64(sum), 63);
-    if (lane == 0) sh.masses[part] = sum;
+  });
+  __syncthreads();
+  ((ulonglong2*)s.bins)[(size_t)blockIdx.x * 1024 + tid] = reinterpret_cast<ulonglong2*>(bins)[tid];
+}
+
+__global__ void __launch_bounds__(1024) k_sample_parts_list(SampleArgs a, SampleParts s) {
+  __shared__ double table[SAMPLE_STEPS];
+  __shared__ __align__(8) int counts[SAMPLE_BINS];
+  __shared__ u64 wave_sum[16];
+  __shared__ int found, listed;
+  const int col = blockIdx.x / s.parts, part = blockIdx.x - col * s.parts, tid = threadIdx.x, first = part * s.rows;
+  const SampleRule rule = sample_rule(a, col);
+  const SamplePart met = sample_meet(s, col);
+  if (met.bad || !(met.most > -INFINITY) || rule.greedy || sample_whole(a, rule)) return;
+  SampleColumn<1024, 0> column;
+  column.init(a.mat + (size_t)col * a.h, first + s.rows < a.h ? first + s.rows : a.h, first);
+  const SampleKept kept = sample_kept(a, rule, met.most, table);
+  const float scale = sample_scale(kept, met.least, SAMPLE_BINS);
+  const bool by_count = rule.k < a.h, brief = sample_short(a, rule);
+  if (!by_count && tid < SAMPLE_STEPS) table[tid] = ldexp(sample_step(tid), a.shift);
+  reinterpret_cast<int2*>(counts)[tid] = int2{0, 0};
+  if (tid == 0) { found = brief ? SAMPLE_BINS - 1 : SAMPLE_BINS; listed = 0; }
+  __syncthreads();
+  ulonglong2 here;
+  if (brief) {
+    const float* const maxima = s.maxima + (size_t)col * s.parts * 1024 + tid;
+    for (int k = 0; k < s.parts; k += 8) {
+      float x[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = maxima[1024 * (k + q < s.parts ? k + q : k)];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (k + q < s.parts && kept.near(x[q])) atomicAdd(&counts[sample_bin(kept, x[q], scale, SAMPLE_BINS)], 1);
+    }
+    __syncthreads();
+    const int2 two = reinterpret_cast<const int2*>(counts)[tid];
+    here = ulonglong2{(u64)two.x, (u64)two.y};
+  } else here = sample_bins(s, col);
+  u64 total;
+  const u64 up = sample_scan<1024>(here.x + here.y, wave_sum, &total), want = by_count ? (u64)rule.k : sample_ask(rule, total), base = up - here.x - here.y;
+  if (up >= want && base < want) found = 2 * tid + (base + here.x < want ? 1 : 0);      // (one lane at most)
+  __syncthreads();
+  const int place = found;
+  u64* const list = s.lists + (size_t)blockIdx.x * SampleHere::LIST;
+  if (by_count) sample_list<false>(column, kept, scale, SAMPLE_BINS, 0, place, &listed, list);
+  else {
+    const u64 sum = lane_u64(wave_scan_u64(sample_list<true>(column, kept, scale, SAMPLE_BINS, place, place, &listed, list)), 63);
+    if ((tid & 63) == 0) s.sums[blockIdx.x * 16 + (tid >> 6)] = sum;
   }
   __syncthreads();
-  u64 all;
-  const u64 here = sh.masses[tid], up = base + sample_scan<LANES>(here, sh.wave_sum, &all);
-  if (here && up - here <= aim && up > aim) { sh.place = tid; sh.base = up - here; }      // (one lane)
-  __syncthreads();
-  if (wv) return;
-  base = sh.base;
-  for (int k = sh.place * fold; k < (sh.place + 1) * fold && k < column.slabs && base <= aim; ++k) {
-    float v[4];
-    column.fetch(v, first + 256 * k);
-    base += sample_slab(a, col, kept, v, first + 256 * k, base, aim, total);
+  if (tid == 0) s.part[blockIdx.x].listed = listed;
+}
+
+template <bool LIMITS>
+__global__ void __launch_bounds__(1024) k_sample_parts_draw(SampleArgs a, SampleParts s) {
+  __shared__ SampleHere sh;
+  const int col = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), stretches = 16 * s.parts;
+  const SampleRule rule = sample_rule(a, col);
+  const SamplePart met = sample_meet(s, col);
+  if (met.bad || !(met.most > -INFINITY)) {                // (nothing to draw)
+    if (tid == 0) { a.tokens[col] = -1.f; if (a.logp) a.logp[col] = met.bad ? NAN : 0.f; }
+    return;
   }
+  if (rule.greedy) {
+    if (tid == 0) { a.tokens[col] = (float)met.first; if (a.logp) a.logp[col] = 0.f; }
+    return;
+  }
+  SampleKept kept = sample_kept(a, rule, met.most, sh.table);
+  const bool by_count = rule.k < a.h, whole = !LIMITS || sample_whole(a, rule);
+  u64 sum = !by_count && tid < stretches ? s.sums[(size_t)col * stretches + tid] : 0, before, total;
+  if (tid < SAMPLE_STEPS) sh.table[tid] = ldexp(sample_step(tid), a.shift);
+  SampleColumn<1024, 0> column;
+  if constexpr (LIMITS) {
+    if (!whole) {
+      int up = lane < s.parts ? s.part[(size_t)col * s.parts + lane].listed : 0;      // (where a part's list ends)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const int q = __shfl_up(up, o, WAVE); if (lane >= o) up += q; }
+      const int n = __builtin_amdgcn_readlane(up, 63);
+      bool found = false;
+      if (n <= SampleHere::LIST) {
+        for (int k = wv; k < s.parts; k += 16) {
+          const int to = __builtin_amdgcn_readlane(up, k), from = k ? __builtin_amdgcn_readlane(up, k - 1) : 0;
+          const u64* const list = s.lists + ((size_t)col * s.parts + k) * SampleHere::LIST;
+          for (int i = from + lane; i < to; i += 64) sh.list[i] = list[i - from];
+        }
+        u64 ask = 0;
+        before = 0;
+        if (!by_count) {
+          const ulonglong2 two = sample_bins(s, col);
+          sample_scan<1024>(two.x + two.y, sh.wave_sum, &total);
+          ask = sample_ask(rule, total);
+          sample_scan<1024>(sum, sh.wave_sum, &before);
+        }
+        __syncthreads();
+        found = sample_from_list<1024>(a, col, n, rule, kept, sh, by_count, by_count, before, ask);
+        if (found && by_count && sh.drawn) return;
+      }
+      if (!found || by_count) {                            // by the whole column
+        const float none[2] = {-INFINITY, -INFINITY};
+        column.init(a.mat + (size_t)col * a.h, a.h);
+        __syncthreads();
+        if (found || sample_border<1024, 0>(a, col, column, rule, kept, none, met.least, sh)) sample_draw(a, col, column, kept, rule, sh);
+        return;
+      }
+      // the listed ones that are kept, stretch by stretch
+      const u64 border = sh.border;
+      const int full = s.rows / 16, last = (a.h - (s.parts - 1) * s.rows + 4095) / 4096 * 256;
+      __syncthreads();
+      sh.masses[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += 1024) {
+        const u64 key = sh.list[i], w = key >= border ? kept.weight(lp_key_value(key)) : 0;
+        const int row = lp_key_index(key), part = row / s.rows;
+        if (w) atomicAdd(&sh.masses[16 * part + (row - part * s.rows) / (part == s.parts - 1 ? last : full)], w);
+      }
+      __syncthreads();
+      sum += sh.masses[tid];
+    }
+  }
+  // the stretch that the aim is in
+  const u64 up = sample_scan<1024>(sum, sh.wave_sum, &total), aim = sample_aim(rule, total);
+  if (sum && up - sum <= aim && up > aim) { sh.place = tid; sh.base = up - sum; }      // (one lane)
+  __syncthreads();
+  const int place = sh.place, first = (place >> 4) * s.rows;
+  before = sh.base;
+  column.init(a.mat + (size_t)col * a.h, first + s.rows < a.h ? first + s.rows : a.h, first);
+  __syncthreads();
+  sample_draw_stretch(a, col, column, kept, sh, first + (place & 15) * column.slabs * 256 + 4 * lane, before, aim, total);
 }
 
 extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperature, cudamat* top_k, cudamat* top_p, cudamat* min_p, cudamat* target,
@@ -692,6 +1001,42 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   while ((1 << bits) < h) ++bits;
   // From the whole distribution, as the numbers say: without the lists two workgroups fit a CU.
   const bool limits = top_k || top_p || min_p || (all_top_k >= 1.f && all_top_k < (float)h) || all_top_p < 1.f || all_min_p > 0.f;
+  const int slabs = (int)(((long long)h + 4095) / 4096);
+  // Divided where that pays (us, a workgroup a column / divided: 65536 x 8 from the whole distribution 19.9 / 14.3, 32000 x 8 12.8 / 14.1; greatest entries 9.1 / 7.6,
+  // 6.4 / 7.5; top-p 49.6 / 34.2, 30.7 / 29.9; in two parts, 65536 x 128, 20.8 / 19.5, 9.5 / 8.9, 51.5 / 50.9; up to 1024 best, which take only one pass more,
+  // 98304 x 8 17.3 / 20.7, 200000 x 8 27.3 / 21.3, x 64 30.8 / 29.5, x 128 39.0 / 45.6).
+  const bool brief = !top_k && all_top_k >= 1.f && all_top_k < (float)h && all_top_k < 1025.f, greedy = !temperature && !(all_temperature > 0.f);
+  int parts = dn_num_cus() / w;
+  if (brief && !greedy ? slabs < 40 || parts < 4 : slabs <= 8) parts = 1;
+  parts = parts < slabs ? parts : slabs;
+  parts = parts < SAMPLE_PARTS ? parts : SAMPLE_PARTS;
+  if (parts > 1) {
+    SampleParts s;
+    const int per = (slabs + parts - 1) / parts;
+    s.rows = 4096 * per;
+    s.parts = parts = (slabs + per - 1) / per;
+    const size_t all_parts = (size_t)parts * w, each = sizeof(SamplePart) + 16 * sizeof(u64) + (limits ? 1024 * sizeof(float) + (SAMPLE_BINS + SampleHere::LIST) * sizeof(u64) : 0);
+    if (char* scratch = (char*)dn_scratch(all_parts * each)) {
+      s.sums = (u64*)scratch;
+      s.lists = s.sums + 16 * all_parts;
+      s.bins = s.lists + (limits ? all_parts * SampleHere::LIST : 0);
+      s.maxima = (float*)(s.bins + (limits ? all_parts * SAMPLE_BINS : 0));
+      s.part = (SamplePart*)(s.maxima + (limits ? all_parts * 1024 : 0));
+      const SampleArgs a = {mat->data_device, tok_data(uniform), tok_data(temperature), tok_data(top_k), tok_data(top_p), tok_data(min_p), target->data_device, tok_data(logp),
+                            all_temperature, all_top_k, all_top_p, all_min_p, h, w, 62 - bits < 45 ? 62 - bits : 45};
+      const dim3 grid((unsigned)all_parts), block(1024);
+      if (limits) hipLaunchKernelGGL(k_sample_parts_most<true>, grid, block, 0, dn_stream(), a, s);
+      else hipLaunchKernelGGL(k_sample_parts_most<false>, grid, block, 0, dn_stream(), a, s);
+      if (!greedy && !brief) {
+        if (limits) hipLaunchKernelGGL(k_sample_parts_weigh<true>, grid, block, 0, dn_stream(), a, s);
+        else hipLaunchKernelGGL(k_sample_parts_weigh<false>, grid, block, 0, dn_stream(), a, s);
+      }
+      if (!greedy && limits) hipLaunchKernelGGL(k_sample_parts_list, grid, block, 0, dn_stream(), a, s);
+      if (limits) hipLaunchKernelGGL(k_sample_parts_draw<true>, dim3(w), block, 0, dn_stream(), a, s);
+      else hipLaunchKernelGGL(k_sample_parts_draw<false>, dim3(w), block, 0, dn_stream(), a, s);
+      return dn_launch_status();
+    }
+  }
   const long long most = h <= 4096 ? DN_MAX_GROUPS : DN_MAX_GROUPS / 4;            // columns of a launch
   for (long long c0 = 0; c0 < w; c0 += most) {
     const int n = (int)(w - c0 < most ? w - c0 : most);

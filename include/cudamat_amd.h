@@ -333,9 +333,9 @@ int cd_update(cudamat* W, cudamat* bv, cudamat* bh, cudamat* v, cudamat* h, cuda
 /* ---- Extension: the parts of a net over tokens that work on one column (a token's features or logits) at a time, and on the columns
  * of a sequence; no counterpart in the reference.  Nothing is held back, nothing waits.  Matrices that are written may be one that is read where
  * that is said, and share no memory with the others (-9).  layer_norm_grad, log_probs of few columns, dot_gated_grad and dot_gated of
- * products that take more than one launch, embed_grad and the gated scans use the library's workspaces: queued on streams of the caller's
- * (graph_set_stream), such calls may not overlap, and a call records into a graph once the workspaces have their sizes (run it once before).
- * Columns and entries that one launch does not take (2^32 work items) are queued in several. ---- */
+ * products that take more than one launch, embed_grad, the gated scans and sample_tokens of few tall columns use the library's workspaces: queued
+ * on streams of the caller's (graph_set_stream), such calls may not overlap, and a call records into a graph once the workspaces have their sizes (run
+ * it once before).  Columns and entries that one launch does not take (2^32 work items) are queued in several. ---- */
 
 /* Layer norm: target = gain * (mat - mean) / sqrt(variance + eps) + bias, mean and (biased) variance of each column.
  * gain, bias: rows x 1 or NULL (ones, zeros); target may be mat; eps >= 0; fewer than 2^30 rows (-9). */

@@ -448,6 +448,70 @@ def test_sample_tokens_from_logits_in_a_narrow_band(cm, rng):
             check_sample(cm, x, F(rng.random(8)), **rule)
 
 
+@pytest.mark.parametrize("h,w", [(36865, 1), (45057, 3), (65537, 128), (163841, 5), (266240, 2), (262145, 1), (1050000, 1), (33000, 129), (200000, 65)])
+def test_sample_tokens_of_divided_columns(cm, rng, h, w):
+    """Few tall columns are divided among workgroups: parts of one row, parts that end with the column, rules of every kind in one call."""
+    x = F(rng.standard_normal((h, w)) * rng.uniform(0.5, 4.0, (1, w)))
+    x[:, 0] = F(np.where(rng.random(h) < 0.4, -np.inf, x[:, 0]))
+    x[h - 1, w - 1] = 40.0                                               # (nearly all of it, in the last row)
+    few = np.unique(np.concatenate([np.arange(min(w, 3)), [w - 1]]))
+    u = F(rng.random(w))
+    def call(cols=None, **rule):
+        given = {k: cm.CUDAMatrix(F(np.reshape(v, (1, w)))) if np.ndim(v) else v for k, v in rule.items()}
+        tokens, logp = cm.empty((1, w)), cm.empty((1, w))
+        cm.sample_tokens(cm.CUDAMatrix(x), cm.CUDAMatrix(F(u.reshape(1, w))), target=tokens, logp=logp, **given)
+        for c in few:
+            token, lp, _ = seq.sample_token(x[:, c], u[c], **{k: v[c] if np.ndim(v) else v for k, v in rule.items()})
+            assert tokens.asarray()[0, c] == token and abs(logp.asarray()[0, c] - lp) <= 2 * U * abs(lp) + 1e-9, (c, rule)
+    call()
+    call(temperature=0.0)
+    call(top_k=30)
+    call(top_k=900, top_p=0.9)
+    call(top_k=3000)
+    call(top_p=0.8, min_p=1e-4)
+    kinds = rng.permutation(np.resize(np.arange(6), w))
+    call(temperature=F(np.where(kinds == 0, 0.0, 0.9)), top_k=F(np.where(kinds == 1, 20, np.where(kinds == 2, 2000, 0))), top_p=F(np.where(kinds == 3, 0.7, 1.0)),
+         min_p=F(np.where(kinds == 4, 0.01, 0.0)))
+
+
+def test_sample_tokens_divided_and_special_columns(cm, rng):
+    h = 140000
+    x = F(rng.standard_normal((h, 6)))
+    x[h // 2, 0], x[h - 1, 1], x[:, 2] = np.nan, np.inf, -np.inf
+    x[:, 3] = -np.inf
+    x[70000, 3] = -5.0
+    for rule in (dict(), dict(temperature=0.0), dict(top_p=0.5), dict(top_k=3), dict(top_k=5000)):
+        check_sample(cm, x, F(rng.random(6)), **rule)
+
+
+def test_recorded_sampling_of_divided_columns(cm, rng):
+    """Two recordings and eager calls share the workspace, which grows in between."""
+    sizes = [(140000, 3, dict(top_p=0.9)), (60000, 20, dict(top_k=2000, temperature=0.8))]
+    mats, nums, outs, want, graphs = [], [], [], [], []
+    for h, w, rule in sizes:
+        mats.append(cm.CUDAMatrix(F(rng.standard_normal((h, w)))))
+        nums.append(cm.CUDAMatrix(F(rng.random((1, w)))))
+        outs.append((cm.empty((1, w)), cm.empty((1, w))))
+    def call(i):
+        cm.sample_tokens(mats[i], nums[i], target=outs[i][0], logp=outs[i][1], **sizes[i][2])
+    for i in (0, 1):
+        call(i)
+        want.append(bits(outs[i]))
+        with cm.Graph() as g:
+            call(i)
+        graphs.append(g)
+    big = cm.CUDAMatrix(F(rng.standard_normal((40000, 120))))
+    for turn in range(4):
+        for i in (0, 1, 0):
+            for o in outs[i]:
+                o.assign(-7)
+            graphs[i].launch()
+            assert all(np.array_equal(p, q) for p, q in zip(bits(outs[i]), want[i]))
+        cm.sample_tokens(big, cm.CUDAMatrix(F(rng.random((1, 120)))), target=cm.empty((1, 120)), top_p=0.5)
+        call(turn % 2)
+        assert all(np.array_equal(p, q) for p, q in zip(bits(outs[turn % 2]), want[turn % 2]))
+
+
 # ------------------------------------------------------------------ large
 
 def test_columns_beyond_two_to_the_31_entries(cm, rng):

@@ -678,6 +678,9 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, int col, const 
 
 // A workgroup a column, which it holds in registers, of up to 16384 rows, or reads again, from the caches (32768 x 512 takes as long either way).
 // Weights are whole numbers (sample_weight), so every sum and with it every border is the same however it is added up.
+// Bytes: 4 an entry.  32768 x 512 from the whole distribution 32 us (10 by the bytes): the first pass with the greatest entry takes as long as the greatest entries
+// alone (19 with the search for them), the rest is the weights' arithmetic in 64 bits.  One column, 50000 x 1 with limits 15: its read by one CU and some
+// twenty meetings of the workgroup.
 template <int LANES, int NV, bool LIMITS>
 __global__ void __launch_bounds__(LANES, LIMITS || LANES < 1024 || NV == 0 ? 1 : 8) k_sample_tokens(SampleArgs a) {
   constexpr int W = LANES / 64;
@@ -735,6 +738,8 @@ __global__ void __launch_bounds__(LANES, LIMITS || LANES < 1024 || NV == 0 ? 1 :
 // asks for a border; the candidates of the border's bins; and a workgroup a column that finds the border among those and draws, from the rows of
 // one part.  The same sums of whole numbers, so the same tokens and bits as a workgroup a column gives.  What the lists do not hold
 // (thousands of entries that are alike) that one does by itself.
+// 128003 x 64, a rule of its own a column, 56 us (a workgroup a column 100): 6 to 10 for the greatest entries, 12 for the weights, 16 for the candidates, 19 for
+// the borders; from the whole distribution 21 (37).
 struct SamplePart { float most, least; int bad, first, listed; };      // first: row of the greatest entry (temperature 0)
 struct SampleParts {
   int parts, rows;                 // of a column; of a part
@@ -1003,11 +1008,11 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
   const bool limits = top_k || top_p || min_p || (all_top_k >= 1.f && all_top_k < (float)h) || all_top_p < 1.f || all_min_p > 0.f;
   const int slabs = (int)(((long long)h + 4095) / 4096);
   // Divided where that pays (us, a workgroup a column / divided: 65536 x 8 from the whole distribution 19.9 / 14.3, 32000 x 8 12.8 / 14.1; greatest entries 9.1 / 7.6,
-  // 6.4 / 7.5; top-p 49.6 / 34.2, 30.7 / 29.9; in two parts, 65536 x 128, 20.8 / 19.5, 9.5 / 8.9, 51.5 / 50.9; up to 1024 best, which take only one pass more,
-  // 98304 x 8 17.3 / 20.7, 200000 x 8 27.3 / 21.3, x 64 30.8 / 29.5, x 128 39.0 / 45.6).
+  // 6.4 / 7.5; top-p 49.6 / 34.2, 30.7 / 29.9; in two parts, 65536 x 128, 20.8 / 19.5, 9.5 / 8.9, 51.5 / 50.9; 50 best, which take only one pass more,
+  // 98304 x 8 17.3 / 20.7, 128003 x 64 22.2 / 21.4, 200000 x 8 27.3 / 21.3, x 128 39.0 / 45.6; 400 best 31.7 / 30.2, 37.6 / 33.0, 43.0 / 31.2, 50.1 / 56.7).
   const bool brief = !top_k && all_top_k >= 1.f && all_top_k < (float)h && all_top_k < 1025.f, greedy = !temperature && !(all_temperature > 0.f);
   int parts = dn_num_cus() / w;
-  if (brief && !greedy ? slabs < 40 || parts < 4 : slabs <= 8) parts = 1;
+  if (brief && !greedy ? slabs < 32 || parts < 4 : slabs <= 8) parts = 1;
   parts = parts < slabs ? parts : slabs;
   parts = parts < SAMPLE_PARTS ? parts : SAMPLE_PARTS;
   if (parts > 1) {
@@ -1045,8 +1050,11 @@ extern "C" int sample_tokens(cudamat* mat, cudamat* uniform, cudamat* temperatur
                           all_temperature, all_top_k, all_top_p, all_min_p, h, n, 62 - bits < 45 ? 62 - bits : 45};
 #define SAMPLE_GO(LANES, NV) do { if (limits) hipLaunchKernelGGL((k_sample_tokens<LANES, NV, true>), dim3(n), dim3(LANES), 0, dn_stream(), a); \
                                   else hipLaunchKernelGGL((k_sample_tokens<LANES, NV, false>), dim3(n), dim3(LANES), 0, dn_stream(), a); } while (0)
-    if (h <= 1024) SAMPLE_GO(256, 1);
-    else if (h <= 4096) SAMPLE_GO(256, 4);
+    // (us, 256 / 1024 lanes: 2900 x 256 from the whole distribution 5.1 / 5.4, of 50 best 10.0 / 9.0, of 400 15.7 / 18.7; 4096 x 512 6.8 / 8.2, 11.1 / 16.6, 17.3 / 35.6.
+    // Above 4096 rows, registers of 1024 lanes against memory and 256: 8192 x 128 6.5 / 7.8, 9.4 / 11.8, 19.5 / 21.3, but with limits in more columns than CUs
+    // x 1000 34 / 24, 74 / 40, top-p 0.9 92 / 58; 16384 x 512 19.8 / 16.3, 42 / 31, 60 / 55; 32768 x 1000 54 / 52, 104 / 99, 135 / 147.)
+    if (h <= 4096) SAMPLE_GO(256, 4);
+    else if (h <= 16384 && limits && w > dn_num_cus()) hipLaunchKernelGGL((k_sample_tokens<256, 0, true>), dim3(n), dim3(256), 0, dn_stream(), a);
     else if (h <= 16384) SAMPLE_GO(1024, 4);
     else SAMPLE_GO(1024, 0);
 #undef SAMPLE_GO

@@ -412,6 +412,20 @@ def test_sample_tokens_of_ties_masks_and_special_columns(cm, rng, h):
     check_sample(cm, F(np.tile(np.log([[3.0], [1.0], [2.0]]), (1, 16))), u)
 
 
+@pytest.mark.parametrize("h,w", [(4097, 300), (9001, 257), (16384, 260)])
+def test_limits_in_more_columns_than_compute_units(cm, rng, h, w):
+    x = F(rng.standard_normal((h, w)) * rng.uniform(0.3, 4.0, (1, w)))
+    x[:, 5], x[: h // 2, 7] = F(np.arange(h) % 3), -np.inf
+    few = np.r_[0:9, w - 1]
+    for rule in (dict(top_k=40), dict(top_k=300, top_p=0.9), dict(top_k=h // 2), dict(top_p=0.9), dict(min_p=0.05)):
+        u = F(rng.random(w))
+        tokens, logp = cm.empty((1, w)), cm.empty((1, w))
+        cm.sample_tokens(cm.CUDAMatrix(x), cm.CUDAMatrix(F(u.reshape(1, w))), target=tokens, logp=logp, **rule)
+        for c in few:
+            token, lp, _ = seq.sample_token(x[:, c], u[c], **rule)
+            assert tokens.asarray()[0, c] == token and abs(logp.asarray()[0, c] - lp) <= 2 * U * abs(lp) + 1e-10, (c, rule)
+
+
 @pytest.mark.parametrize("h", [700, 3000, 20000])
 def test_sample_tokens_of_distances_that_overflow(cm, rng, h):
     far, rows = 3e38, np.arange(h)

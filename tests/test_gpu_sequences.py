@@ -201,6 +201,16 @@ def test_gated_scan_of_sequences_of_any_lengths(cm, rng, f, w, skip):
     check_scan(cm, rng, f, w, 2, [0, w // 2, w], skip, states=False)
 
 
+@pytest.mark.parametrize("f,w,n", [(65606, 150, 2), (131072, 130, 1)])
+def test_gated_scan_of_more_units_than_a_launch_takes(cm, rng, f, w, n):
+    check_scan(cm, rng, f, w, n)
+
+
+@pytest.mark.parametrize("f", [449, 512, 963, 1024, 2001])
+def test_gated_scan_of_tiles_that_xcds_share(cm, rng, f):
+    check_scan(cm, rng, f, 700, 3, [0, 5, 400, 699], skip=1)
+
+
 def test_gated_scan_of_no_columns(cm, rng):
     state = F(rng.standard_normal((5, 3)))
     last = cm.empty((5, 3))

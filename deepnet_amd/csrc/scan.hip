@@ -298,9 +298,23 @@ __global__ void __launch_bounds__(1024) k_gated_scan(ScanArgs a, ScanCut cut) {
       for (int j = 0; j < S; ++j)
         if (done >> j & 1) states[((GRAD ? firsts : ends)[own + j] - 1) * f + i] = GRAD ? x[j] : u[j];
     }
-    if (a.offsets && chunk == 0)
-      for (int q = strand; q < a.n; q += strands)
-        if (scan_border(a, q) >= scan_border(a, q + 1)) states[q * f + i] = handed ? handed[q * f + i] : 0.f;
+  }
+  if (states && a.offsets) {         // every wavefront of a tile looks through some of the sequences
+    const int each = WIDE ? strands : strands << cut.shift >> 6, waves = cut.chunks * each;
+    const int wave = chunk * each + (WIDE ? strand : __builtin_amdgcn_readfirstlane(strand << cut.shift >> 6));
+    const int batch = (a.n + waves - 1) / waves < 64 ? (a.n + waves - 1) / waves : 64;
+    for (long long q0 = (long long)batch * wave; q0 < a.n; q0 += (long long)batch * waves) {
+      const int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), q = (int)q0 + l;
+      unsigned long long none = __ballot(l < batch && q < a.n && scan_border(a, q < a.n ? q : a.n) >= scan_border(a, q < a.n ? q + 1 : a.n));
+      while (none) {                 // two on their way at once (the first one again in the place of one that is not there)
+        const size_t x = (size_t)(q0 + __builtin_ctzll(none)) * f + i;
+        none &= none - 1;
+        const size_t y = none ? (size_t)(q0 + __builtin_ctzll(none)) * f + i : x;
+        none &= none - 1;            // (0 & -1: stays 0)
+        const float v = handed ? handed[x] : 0.f, w = handed ? handed[y] : 0.f;
+        if (live) { states[x] = v; states[y] = w; }
+      }
+    }
   }
 }
 

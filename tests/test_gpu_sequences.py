@@ -211,6 +211,12 @@ def test_gated_scan_of_tiles_that_xcds_share(cm, rng, f):
     check_scan(cm, rng, f, 700, 3, [0, 5, 400, 699], skip=1)
 
 
+@pytest.mark.parametrize("f,w,n", [(376, 814, 450), (65, 3, 1000), (20, 40, 700), (64, 700, 65), (130, 1, 64), (7, 900, 3000)])
+def test_gated_scan_of_many_sequences_most_of_them_empty(cm, rng, f, w, n):
+    check_scan(cm, rng, f, w, n, np.sort(rng.integers(0, w + 1, n + 1)), skip=1)
+    check_scan(cm, rng, f, w, n, np.r_[[0] * (n // 2), [w] * (n + 1 - n // 2)])
+
+
 def test_gated_scan_of_no_columns(cm, rng):
     state = F(rng.standard_normal((5, 3)))
     last = cm.empty((5, 3))

@@ -126,9 +126,10 @@ __device__ __forceinline__ u64 sample_scan(u64 v, u64* wave_sum, u64* all) {
 }
 
 // The entries of a column: a wavefront has a stretch of it, 256 rows a slab, four of them a lane; in registers (NV slabs) or, of columns that those do not hold
-// (NV = 0), from memory, where AHEAD slabs are on their way at once.  f(x, row, slab) for a lane's four, rows behind the column being -infinity.
-template <int LANES, int NV, int AHEAD = 8>
+// (NV = 0), from memory, where eight slabs are on their way at once.  f(x, row, slab) for a lane's four, rows behind the column being -infinity.
+template <int LANES, int NV>
 struct SampleColumn {
+  static constexpr int AHEAD = 8;
   const float* c;
   int h, from, slabs;              // behind the last row; the stretch's first row of this lane, slabs of a stretch
   float x[NV ? NV : 1][4];

@@ -434,7 +434,7 @@ int embed(cudamat* mat, cudamat* labels, cudamat* target, float mult) {
   if (n > (1 << 24) || !tok_apart(mat, target) || !tok_apart(labels, target)) return ERROR_UNSUPPORTED;
   if (h <= 0 || w <= 0) return 0;
   const bool by4 = h >= 4, stream = (long long)h * w >= DN_STREAM_MIN_ELEMS;
-  const uint32_t groups = by4 ? (h + 3) / 4 : h;
+  const uint32_t groups = by4 ? ((uint32_t)h + 3) / 4 : h;                              // (h + 3 may pass 31 bits)
   const FastDiv div = make_fastdiv(groups);
   const float* const from = n > 0 ? mat->data_device : target->data_device;            // (lanes without a token read its first entries)
   const long long most = (1ll << 31) / groups > 0 ? (1ll << 31) / groups : 1;           // columns of a launch

@@ -588,6 +588,56 @@ def test_more_columns_than_a_launch_takes(cm, rng):
         assert np.array_equal(y.slice(a, a + 20).asarray(), np.tile(e.asarray()[:, 2:3], (1, 20)))
 
 
+MANY_ROWS = (1 << 31) - 2                                                   # (a multiple of 6; no multiple of 4)
+
+
+def tall(cm, rng, w):
+    """MANY_ROWS x w, column c holding (c + 1) / 8 and random numbers at its first, some middle and its last six rows: the matrix, and those (18 x w)."""
+    big, part = cm.empty((MANY_ROWS, w)), F(rng.standard_normal((18, w)))
+    for c in range(w):
+        big.slice(c, c + 1).assign((c + 1) / 8)
+        for at, rows in zip(tall_places(), np.split(part[:, c:c + 1], 3)):
+            src = cm.CUDAMatrix(F(rows.T))
+            tall_rows(big, c, at).assign(src)
+            src.free_device_memory()
+    return big, part
+
+
+def tall_places():
+    return 0, 1 << 30, MANY_ROWS - 6
+
+
+def tall_rows(big, c, at, n=6):
+    """Rows [at, at + n) of a column of a tall matrix, on the device."""
+    rows = big.slice(c, c + 1)
+    rows.reshape((1, MANY_ROWS))
+    return rows.slice(at, at + n)
+
+
+def tall_read(big, c):
+    """What `tall` returns of a column, and whether those between are all alike (their value)."""
+    part = np.concatenate([tall_rows(big, c, at).asarray().ravel() for at in tall_places()])
+    rest = [tall_rows(big, c, at, 1000).asarray() for at in (6, (1 << 30) - 1000, (1 << 30) + 6, MANY_ROWS - 1006)]
+    assert all((r == rest[0][0, 0]).all() for r in rest)
+    return part, rest[0][0, 0]
+
+
+def release(*mats):
+    for m in mats:
+        m.free_device_memory()
+
+
+def test_embed_of_nearly_two_to_the_31_rows(cm, rng):
+    e, part = tall(cm, rng, 2)
+    y = cm.empty((MANY_ROWS, 5))
+    y.assign(-7.0)
+    cm.embed(e, cm.CUDAMatrix(F([[1, -1, 0, 1, 1]])), target=y, mult=2.0)
+    for c, t in enumerate((1, -1, 0, 1, 1)):
+        got, rest = tall_read(y, c)
+        assert np.array_equal(got, 2 * part[:, t] if t >= 0 else np.zeros(18)) and rest == (t + 1) / 4, c
+    release(e, y)
+
+
 def test_scans_beyond_two_to_the_31_entries(cm, rng):
     f, w = 4096, (1 << 18) + 300                                           # pre has 2^31 entries and more
     pre, y, o = cm.empty((2 * f, w)), cm.empty((f, w)), [0, 100, w - 200, w]

@@ -418,10 +418,11 @@ __global__ void __launch_bounds__(1024) k_embed_few(EmbedSort a, EmbedSums b) {
 
 // Tiles of at most `most` rows, a multiple of four; the last one has a group of four rows too.
 static void embed_tiles(EmbedSums& s, int most) {
-  s.tiles = (s.h + most - 1) / most;
-  s.rows = s.tiles > 1 ? ((s.h + s.tiles - 1) / s.tiles + 3) / 4 * 4 : s.h;
-  while (s.tiles > 1 && s.h % s.rows && s.h % s.rows < 4) s.rows -= 4;
-  s.tiles = (s.h + s.rows - 1) / s.rows;
+  const long long h = s.h;         // (h + most may pass 31 bits)
+  long long tiles = (h + most - 1) / most, rows = tiles > 1 ? ((h + tiles - 1) / tiles + 3) / 4 * 4 : h;
+  while (tiles > 1 && h % rows && h % rows < 4) rows -= 4;
+  s.tiles = (int)((h + rows - 1) / rows);
+  s.rows = (int)rows;
 }
 
 extern "C" {

@@ -638,6 +638,20 @@ def test_embed_of_nearly_two_to_the_31_rows(cm, rng):
     release(e, y)
 
 
+def test_embed_grad_of_nearly_two_to_the_31_rows(cm, rng):
+    """Bound: three roundings of sums below 20."""
+    dy, part = tall(cm, rng, 3)
+    for labels, beta in (([1, 1, 0], 0.0), ([1, -1, 1], 1.0)):
+        g, old = tall(cm, rng, 2)
+        cm.embed_grad(dy, cm.CUDAMatrix(F([labels])), g, mult=2.0, beta=beta)
+        for t in (0, 1):
+            of = [c for c in range(3) if labels[c] == t]
+            got, rest = tall_read(g, t)
+            assert np.max(np.abs(got - (beta * old[:, t] + 2 * part[:, of].sum(axis=1)))) < 3 * U * 20 and rest == beta * (t + 1) / 8 + sum((c + 1) / 4 for c in of), (labels, t)
+        release(g)
+    release(dy)
+
+
 def test_scans_beyond_two_to_the_31_entries(cm, rng):
     f, w = 4096, (1 << 18) + 300                                           # pre has 2^31 entries and more
     pre, y, o = cm.empty((2 * f, w)), cm.empty((f, w)), [0, 100, w - 200, w]

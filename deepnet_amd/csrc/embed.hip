@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(1024) k_embed_sort(EmbedSort a) {
     int x = 0;
     for (int step = EMBED_RANGE / 2; step > 0; step /= 2)
       if (embed_slot(starts[x + step]) <= q) x += step;
-    const int s = starts[x], count = starts[x + 1] - s, piece = embed_piece(count), k = q - embed_slot(s), pieces = (count + piece - 1) / piece;
+    const int s = starts[x], count = starts[x + 1] - s, piece = embed_piece(count), k = q - embed_slot(s), pieces = (int)(((unsigned)count + piece - 1) / piece);
     EmbedSlot o = {0, 0, 0, 0};
     if (count > EMBED_RUN && k < pieces) o = EmbedSlot{s + k * piece, count - k * piece < piece ? count - k * piece : piece, lo + x, k ? 0 : pieces};
     a.slots[q] = o;
@@ -482,12 +482,12 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
 #undef FEW2
     return dn_launch_status();
   }
-  s.slot_count = (w + EMBED_SLOT - 1) / EMBED_SLOT;
+  s.slot_count = (int)(((long long)w + EMBED_SLOT - 1) / EMBED_SLOT);
   embed_tiles(s, 1024);
   const long long sums = ((long long)s.slot_count + n) * s.tiles;
   if (sums >= 1ll << 31) return ERROR_UNSUPPORTED;
   // starts, sorted columns, slots (16-byte ones), partial sums
-  const size_t ints = ((size_t)n + 1 + w + 3) / 4 * 4, slots = (size_t)(w + EMBED_SLOT - 1) / EMBED_SLOT;
+  const size_t ints = ((size_t)n + 1 + w + 3) / 4 * 4, slots = (size_t)s.slot_count;
   char* scratch = (char*)dn_scratch(4 * ints + sizeof(EmbedSlot) * slots + 4 * (size_t)s.slot_count * h);
   if (!scratch) return CUDA_ERROR;
   o.starts = (int*)scratch; o.sorted = o.starts + n + 1; o.slots = (EmbedSlot*)(scratch + 4 * ints);

@@ -652,6 +652,29 @@ def test_embed_grad_of_nearly_two_to_the_31_rows(cm, rng):
     release(dy)
 
 
+def test_embed_grad_of_nearly_two_to_the_31_columns(cm, rng):
+    """Whole numbers: exact.  Nearly all columns have one token, or none."""
+    w = (1 << 31) - 1
+    dy, labels = cm.empty((1, w)), cm.empty((1, w))
+    dy.assign(0.0)
+    tail = F([np.arange(1, 9)])
+    for at in (0, 1 << 30, w - 8):
+        dy.slice(at, at + 8).assign(cm.CUDAMatrix(tail))
+    for rest in (1.0, -1.0):
+        labels.assign(rest)
+        for at in (0, 1 << 30, w - 8):
+            labels.slice(at, at + 8).assign(cm.CUDAMatrix(F([[0, 1, 1, 0, rest, 0, 0, rest]])))
+        g = cm.CUDAMatrix(F([[-1, -1, -1]]))
+        cm.embed_grad(dy, labels, g, beta=1.0)
+        want = np.zeros(3)
+        for at in (0, 1, 2):
+            for c, t in enumerate([0, 1, 1, 0, rest, 0, 0, rest]):
+                if t >= 0:
+                    want[int(t)] += c + 1
+        assert np.array_equal(g.asarray()[0], want - 1), rest
+    release(dy, labels)
+
+
 def test_scans_beyond_two_to_the_31_entries(cm, rng):
     f, w = 4096, (1 << 18) + 300                                           # pre has 2^31 entries and more
     pre, y, o = cm.empty((2 * f, w)), cm.empty((f, w)), [0, 100, w - 200, w]

@@ -366,15 +366,20 @@ static int scan_launch(const ScanArgs& a) {
   const bool stream = (long long)a.f * a.w >= DN_STREAM_MIN_ELEMS;
   for (cut.first_tile = 0; cut.first_tile < tiles; cut.first_tile += most_tiles) {
     cut.tiles = tiles - cut.first_tile < most_tiles ? tiles - cut.first_tile : most_tiles;
-    const dim3 grid((unsigned)((long long)cut.chunks * cut.tiles)), block((unsigned)(cut.strands << cut.shift));
+    const dim3 block((unsigned)(cut.strands << cut.shift));
+    // (what one launch does not take goes on in the next: workgroups have the chunks in the order in which they start)
+    const long long most = ((1ll << 32) - 1) / block.x / cut.tiles;
+    for (long long c0 = 0; c0 < cut.chunks; c0 += most) {
+      const dim3 grid((unsigned)((cut.chunks - c0 < most ? cut.chunks - c0 : most) * cut.tiles));
 #define SCAN_GO(S, WIDE) do { if (stream) hipLaunchKernelGGL((k_gated_scan<S, WIDE, GRAD, true>), grid, block, 0, dn_stream(), a, cut); \
                               else hipLaunchKernelGGL((k_gated_scan<S, WIDE, GRAD, false>), grid, block, 0, dn_stream(), a, cut); } while (0)
-    if (!wide) SCAN_GO(4, false);
-    else if (s == 1) SCAN_GO(1, true);
-    else if (s == 4) SCAN_GO(4, true);
-    else if (s == 8) SCAN_GO(8, true);
-    else if constexpr (!GRAD) SCAN_GO(16, true);
+      if (!wide) SCAN_GO(4, false);
+      else if (s == 1) SCAN_GO(1, true);
+      else if (s == 4) SCAN_GO(4, true);
+      else if (s == 8) SCAN_GO(8, true);
+      else if constexpr (!GRAD) SCAN_GO(16, true);
 #undef SCAN_GO
+    }
   }
   return dn_launch_status();
 }

@@ -696,6 +696,39 @@ def test_scans_beyond_two_to_the_31_entries(cm, rng):
     assert not pre.slice(w - 300, w - 200).asarray().any()
 
 
+def test_scans_of_more_columns_than_a_launch_takes(cm, rng):
+    """Four lanes a column: 2^32 of them go into two launches, the second one from column 2^30 - 256 on.  Gates of 1 hand on what comes, and inputs and derivatives
+    of 0 add nothing, so the oracle sees the other columns alone."""
+    w, n = (1 << 30) + 1000, 40
+    places = (0, (1 << 30) - 256 - n // 2, w - n)
+    pre, y, dy = cm.empty((2, w)), cm.empty((1, w)), cm.empty((1, w))
+    pre.assign(1000.0)
+    dy.assign(0.0)
+    p, state, d, dlast = scan_inputs(rng, 1, 3 * n, 1)
+    for i, at in enumerate(places):
+        pre.slice(at, at + n).assign(cm.CUDAMatrix(F(p[:, n * i:n * i + n])))
+        dy.slice(at, at + n).assign(cm.CUDAMatrix(F(d[:, n * i:n * i + n])))
+    last = cm.empty((1, 1))
+    cm.gated_scan(pre, target=y, state=cm.CUDAMatrix(state), last=last)
+    got = np.concatenate([y.slice(at, at + n).asarray() for at in places], axis=1)
+    want, want_last, off, last_off = seq.gated_scan(p, [0, 3 * n], state)
+    check(got, want, STEP * U * off)
+    assert last.asarray()[0, 0] == got[0, -1]
+    # What is handed on was joined from the links of one or two chunks and of what came before them, not added up column by column: at most 4 joins, each a
+    # rounding of what `off` has counted once at that column.  Links of gates of 1 and sums of 0 are joined exactly.
+    for i, (a, b) in enumerate(zip(places, places[1:])):
+        at = n * i + n - 1
+        for c in [c for c in (a + n, (a + b) // 2, b - 1000) if c + 1000 <= b]:
+            assert (np.abs(y.slice(c, c + 1000).asarray() - want[0, at]) <= (STEP + 4) * U * off[0, at]).all(), (i, c)
+    ds = cm.empty((1, 1))
+    cm.gated_scan_grad(dy, pre, y, state=cm.CUDAMatrix(state), last_deriv=cm.CUDAMatrix(dlast), state_grad=ds)
+    want, want_state, off, state_off = seq.gated_scan_grad(d, p, got, [0, 3 * n], state, dlast)
+    check(np.concatenate([pre.slice(at, at + n).asarray() for at in places], axis=1), want, STEP * U * (off + np.abs(want)))
+    check(ds.asarray(), want_state, STEP * U * state_off + U * np.abs(want_state))
+    assert not pre.slice(n, n + 1000).asarray().any() and not pre.slice(places[1] - 1000, places[1]).asarray().any()
+    release(pre, y, dy)
+
+
 # ------------------------------------------------------------------ together
 
 class Net(object):

@@ -329,7 +329,10 @@ static int scan_launch(const ScanArgs& a) {
   if (a.w <= 0) {
     float* to = GRAD ? a.state_grad : a.last;
     const long long n = (long long)a.f * a.n;
-    if (to) hipLaunchKernelGGL(k_scan_states, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dn_stream(), GRAD ? a.last_deriv : a.state, to, n);
+    const float* from = GRAD ? a.last_deriv : a.state;
+    const long long most = 256 * DN_MAX_GROUPS;
+    for (long long i = 0; to && i < n; i += most)
+      hipLaunchKernelGGL(k_scan_states, dim3((unsigned)(((n - i < most ? n - i : most) + 255) / 256)), dim3(256), 0, dn_stream(), from ? from + i : from, to + i, n - i);
     return dn_launch_status();
   }
   ScanCut cut;

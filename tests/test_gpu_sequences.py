@@ -729,6 +729,20 @@ def test_scans_of_more_columns_than_a_launch_takes(cm, rng):
     release(pre, y, dy)
 
 
+def test_scans_without_columns_and_states_of_more_entries_than_a_launch_takes(cm, rng):
+    f, n = 1 << 21, (1 << 11) + 1
+    state, last, tail = cm.empty((f, n)), cm.empty((f, n)), F(rng.standard_normal((f, 2)))
+    state.assign(0.5)
+    last.assign(-1.0)
+    state.slice(n - 2, n).assign(cm.CUDAMatrix(tail))
+    cm.gated_scan(cm.empty((2 * f, 0)), target=cm.empty((f, 0)), state=state, last=last)
+    assert np.array_equal(last.slice(n - 2, n).asarray(), tail)
+    assert all((last.slice(c, c + 1).asarray() == 0.5).all() for c in (0, n // 2, n - 3))
+    cm.gated_scan_grad(cm.empty((f, 0)), cm.empty((2 * f, 0)), cm.empty((f, 0)), state_grad=last, sequences=n)
+    assert not any(last.slice(c, c + 1).asarray().any() for c in (0, n // 2, n - 3, n - 2, n - 1))
+    release(state, last)
+
+
 # ------------------------------------------------------------------ together
 
 class Net(object):

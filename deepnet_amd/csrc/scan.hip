@@ -396,6 +396,9 @@ static int scan_sequences(int asked, const cudamat* offsets, const cudamat* s0, 
   return 1;
 }
 
+// Offsets are floats, and the kernel steps through the sequences by up to 2^22.
+static bool scan_beyond(const cudamat* offsets, int w, int n) { return offsets && (w > (1 << 24) || (w > 0 && n > (1 << 30))); }
+
 extern "C" {
 
 int gated_scan(cudamat* pre, cudamat* offsets, cudamat* state, cudamat* target, cudamat* last, int sequences) {
@@ -406,7 +409,7 @@ int gated_scan(cudamat* pre, cudamat* offsets, cudamat* state, cudamat* target, 
       !tok_shape(state, f, n) || !tok_shape(last, f, n))
     return ERROR_INCOMPATIBLE_DIMENSIONS;
   if (!tok_apart(pre, target) || !tok_apart(offsets, target) || !tok_apart(state, target) || !tok_apart(pre, last) || !tok_apart(offsets, last) ||
-      !tok_apart(target, last) || (state && last && !tok_same_or_apart(state, last)) || (offsets && w > (1 << 24)))
+      !tok_apart(target, last) || (state && last && !tok_same_or_apart(state, last)) || scan_beyond(offsets, w, n))
     return ERROR_UNSUPPORTED;
   if (f <= 0 || (w <= 0 && !last)) return 0;
   const ScanArgs a = {pre->data_device, tok_data(offsets), tok_data(state), nullptr, nullptr, nullptr, target->data_device, tok_data(last), nullptr, f, w, n, w / n};
@@ -422,7 +425,7 @@ int gated_scan_grad(cudamat* deriv, cudamat* pre, cudamat* out, cudamat* offsets
       !tok_shape(offsets, 1, n + 1) || (!offsets && w % n) || !tok_shape(state, f, n) || !tok_shape(last_deriv, f, n) || !tok_shape(state_grad, f, n))
     return ERROR_INCOMPATIBLE_DIMENSIONS;
   if (!tok_same_or_apart(pre, target) || (last_deriv && state_grad && !tok_same_or_apart(last_deriv, state_grad)) || !tok_apart(pre, state_grad) ||
-      !tok_apart(target, state_grad) || !tok_apart(last_deriv, target) || (offsets && w > (1 << 24)))
+      !tok_apart(target, state_grad) || !tok_apart(last_deriv, target) || scan_beyond(offsets, w, n))
     return ERROR_UNSUPPORTED;
   for (const cudamat* m : {deriv, out, offsets, state})
     if (!tok_apart(m, target) || !tok_apart(m, state_grad)) return ERROR_UNSUPPORTED;

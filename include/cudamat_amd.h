@@ -391,7 +391,7 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
 /* A gated linear recurrence along the columns of sequences: with pre = [g; u] (2 f x columns) and a = sigmoid(g),
  * target(:, t) = a_t target(:, t - 1) + (1 - a_t) u_t, from the sequence's column of state (f x sequences, or NULL: zeros) before its
  * first one.  last (f x sequences, may be state, or NULL): the last column of every sequence, of one without columns its state.
- * offsets: 1 x (sequences + 1) whole numbers as floats, not falling (up to 2^24 columns): sequence q has the columns [offsets[q], offsets[q + 1]);
+ * offsets: 1 x (sequences + 1) whole numbers as floats, not falling (up to 2^24 columns and 2^30 sequences): sequence q has the columns [offsets[q], offsets[q + 1]);
  * columns of no sequence are left as they are.  Offsets that fall or leave the matrix give results of no meaning, within the matrices.
  * NULL: the columns are divided evenly.  sequences: 0 for as many as offsets or states have, or one.
  * Infinities and NaN make what follows them in their sequence infinite or NaN, and nothing else. */

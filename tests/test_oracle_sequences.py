@@ -135,6 +135,14 @@ def test_gated_scan_refusals(cm):
     assert grad(*a) == UNSUPPORTED
 
 
+def test_gated_scan_refuses_more_sequences_than_it_counts(cm):
+    """Of 2^30 sequences every number that the kernels step through them by stays below 2^31."""
+    lib, new, n = cm._cudamat, Space(cm), (1 << 30) + 1
+    pre, y, o = new(2, 12), new(1, 12), handle(cm, 1, n + 1, 1 << 42)
+    assert lib.gated_scan(pre, o, None, y, None, 0) == UNSUPPORTED and lib.gated_scan(pre, o, None, y, handle(cm, 1, n, 1 << 43), n) == UNSUPPORTED
+    assert lib.gated_scan_grad(new(1, 12), pre, y, o, None, None, new(2, 12), None, 0) == UNSUPPORTED
+
+
 def test_sample_tokens_refusals(cm):
     lib, new = cm._cudamat, Space(cm)
     shapes = [(9, 3)] + [(1, 3)] * 7

@@ -2,6 +2,7 @@
 // pre and a = sigmoid(g):  h_t = a_t h_{t-1} + (1 - a_t) u_t.
 #include "columns.h"
 #include "gated_act.h"
+#include "scan_launch.h"
 #include "tokens.h"
 
 struct ScanArgs {
@@ -65,11 +66,11 @@ __device__ __forceinline__ ScanPlace scan_take_place(unsigned long long* counter
   const ScanPlace o = *shared;
   if (o.chunk == chunks - 1)
     for (int k = tile + threadIdx.x * tiles; k < SCAN_TILES; k += blockDim.x * tiles)
-      __hip_atomic_store(counters + 16 * k, (o.launch + 1) << 28, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(counters + 16 * k, scan_next(o.launch) << 28, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return o;
 }
 // A link as two words that each have the launch's number in their upper half: the words need no order between them, and nothing is cleared (what is
-// there from before has another number, until one stays unwritten for 2^32 launches).
+// there from before has another number, but where it has stayed unwritten for exactly as many launches as there are numbers, 2^32 - 1).
 __device__ __forceinline__ void scan_put(unsigned long long* at, ScanLink l, unsigned tag) {
   __hip_atomic_store(at, (unsigned long long)tag << 32 | __float_as_uint(l.p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __hip_atomic_store(at + 64, (unsigned long long)tag << 32 | __float_as_uint(l.b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(1024) k_gated_scan(ScanArgs a, ScanCut cut) {
     const ScanPlace o = scan_take_place(cut.words, tile, cut.tiles, cut.chunks, &place);
     if (o.chunk >= cut.chunks) return;                     // (only where calls overlap, which they may not)
     chunk = __builtin_amdgcn_readfirstlane(o.chunk);
-    tag = __builtin_amdgcn_readfirstlane((unsigned)o.launch + 1u);
+    tag = __builtin_amdgcn_readfirstlane(scan_tag(o.launch));
   }
   const bool live = unit < a.f;
   const size_t f = a.f, i = live ? unit : a.f - 1;

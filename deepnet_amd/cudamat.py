@@ -1136,11 +1136,13 @@ def gated_scan(pre, target=None, offsets=None, sequences=0, state=None, last=Non
     from the sequence's column of state (f x sequences; None: zeros), which stands before its first column.  last (f x sequences, which
     may be state), where given, receives every sequence's last column, of a sequence without columns its state.
         offsets     1 x (sequences + 1) whole numbers as floats that do not fall: sequence q has the columns from offsets[q] to before
-                    offsets[q + 1].  Columns that belong to none are left as they are.
+                    offsets[q + 1].  Columns that belong to none are left as they are (of a target that is made here, 0).
         sequences   without offsets, into how many sequences of equal length the columns are divided (0: as many as the states have, or one).
                     One column each: a step of decoding."""
     if target is None:
         target = empty((pre.shape[0] // 2, pre.shape[1]))
+        if offsets is not None:
+            target.assign(0.0)
     _check(_cudamat.gated_scan(pre.p_mat, _p(offsets), _p(state), target.p_mat, _p(last), int(sequences)))
     return target
 

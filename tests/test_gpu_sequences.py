@@ -286,6 +286,23 @@ def test_offsets_out_of_place_stay_within_the_matrix(cm, rng):
             neighbours_untouched(m, 4)
 
 
+@pytest.mark.parametrize("f,w,at", [(5, 40, [3, 20, 33]), (70, 900, [0, 0, 500, 899]), (64, 10, [4, 4])])
+def test_a_scan_into_a_matrix_of_its_own_has_zeros_in_columns_of_no_sequence(cm, rng, f, w, at):
+    """Whatever its memory held."""
+    pre, state = scan_inputs(rng, f, w, len(at) - 1)[:2]
+    want, _, off, _ = seq.gated_scan(pre, at, state)
+    outside = np.ones(w, dtype=bool)
+    outside[at[0]:at[-1]] = False
+    for _ in range(3):
+        was = cm.CUDAMatrix(F(np.full((f, w), np.nan)))
+        was.free_device_memory()                                         # (its block is the next one of this size)
+        y = cm.gated_scan(cm.CUDAMatrix(pre), offsets=cm.CUDAMatrix(F([at])), state=cm.CUDAMatrix(state))
+        got = y.asarray()
+        assert outside.any() and not got[:, outside].any()
+        check(got[:, ~outside], want[:, ~outside], STEP * U * off[:, ~outside])
+    assert cm.gated_scan(cm.empty((2 * f, 0)), offsets=cm.CUDAMatrix(F([[0, 0]]))).shape == (f, 0)
+
+
 def test_gated_scan_gives_the_same_bits_every_time(cm, rng):
     f, w = 300, 9000
     pre, state, dy, _ = scan_inputs(rng, f, w, 1)

@@ -1150,8 +1150,9 @@ def gated_scan(pre, target=None, offsets=None, sequences=0, state=None, last=Non
 def gated_scan_grad(deriv, pre, out, target=None, offsets=None, sequences=0, state=None, last_deriv=None, state_grad=None):
     """Extension of this backend (not in the reference): the backward pass of out = gated_scan(pre, offsets=offsets, sequences=sequences,
     state=state) from deriv, the derivative by its result, and last_deriv, that by its last columns (f x sequences; None: zeros).
-    target = the derivative by pre (in its place by default; columns of no sequence are left as they are); state_grad, where given, that by
-    state (it may be last_deriv)."""
+    target = the derivative by pre (in its place by default); state_grad, where given, that by state (it may be last_deriv).  Columns of no
+    sequence are left as they are: in place they still hold pre there, which is no derivative.  A program whose next products take these
+    columns too gives a target that holds zeros there, or clears them."""
     if target is None:
         target = pre
     _check(_cudamat.gated_scan_grad(deriv.p_mat, pre.p_mat, out.p_mat, _p(offsets), _p(state), _p(last_deriv), target.p_mat, _p(state_grad),

@@ -397,7 +397,7 @@ int embed_grad(cudamat* deriv, cudamat* labels, cudamat* target, float beta, flo
  * Infinities and NaN make what follows them in their sequence infinite or NaN, and nothing else. */
 int gated_scan(cudamat* pre, cudamat* offsets, cudamat* state, cudamat* target, cudamat* last, int sequences);
 /* Its gradients from deriv, the derivative by out (its target), and last_deriv, that by last (or NULL: zeros): target = derivative by pre (may be
- * pre; columns of no sequence are left as they are), state_grad = derivative by state (or NULL; may be last_deriv). */
+ * pre; columns of no sequence are left as they are, over pre therefore no derivatives), state_grad = derivative by state (or NULL; may be last_deriv). */
 int gated_scan_grad(cudamat* deriv, cudamat* pre, cudamat* out, cudamat* offsets, cudamat* state, cudamat* last_deriv, cudamat* target,
                     cudamat* state_grad, int sequences);
 

@@ -864,6 +864,31 @@ def test_a_net_over_packed_texts_forward_and_backward(cm, rng):
         assert abs(np.sum(got * way) - slope) < 1e-4 * np.max(np.abs(want)) * np.sqrt(want.size) + 1e-6 * (1 + abs(value)), name
 
 
+class ZerosBehind(object):
+    """The library, but that the derivative by the gates and inputs goes into a matrix of zeros first, for products that take the padding too."""
+
+    def __init__(self, cm, shape):
+        self.cm, self.zeros = cm, cm.CUDAMatrix(F(np.zeros(shape)))
+
+    def __getattr__(self, name):
+        return getattr(self.cm, name)
+
+    def gated_scan_grad(self, deriv, pre, out, **args):
+        pre.assign(self.cm.gated_scan_grad(deriv, pre, out, target=self.zeros, **args))
+
+
+def test_a_net_over_packed_and_padded_texts(cm, rng):
+    """Every gradient, with padding behind the last text; bounds as above."""
+    b = Net(cm, rng)
+    b.cm = ZerosBehind(cm, b.m['pre'].shape)
+    for _ in range(2):
+        b.step()
+        value, grads, o = b.oracle(b.host)
+        for name in b.GRADS:
+            got, want = b.m[name].asarray(), grads[name]
+            assert np.max(np.abs(got - want)) < 2e-5 * np.max(np.abs(want)), name
+
+
 def test_recorded_nets_and_eager_calls_between_them(cm):
     """Two recordings of different sizes that share the library's workspaces, replayed in turn with eager calls of a third size between them."""
     sizes = (dict(), dict(d=200, f=130, v=3000, at=(0, 700, 1500), pad=0), dict(d=33, f=20, v=100, at=(0, 5, 3000), pad=3))

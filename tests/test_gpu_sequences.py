@@ -345,6 +345,56 @@ def test_gated_scan_of_many_sizes_in_turn(cm):
         assert all(np.array_equal(p, q) for p, q in zip(bits([s['y'], s['dp'], s['ds']]), s['want'])), turn
 
 
+def rare(rng, f, w, at):
+    """Inputs of a scan over very many columns in which something happens only every 400 columns or so, in one unit each: a gate of 1/2 there, of 1 elsewhere
+    (sigmoid(1000), whose other side is 0), where inputs and derivatives are 0 as well.  What a stretch of columns hands on thus stays to be seen until the unit's next
+    one.  Returns the inputs and the columns that the oracle has to look at: those, the ones before them and the ends of sequences."""
+    n, each = len(at) - 1, 400
+    pre, dy = np.zeros((2 * f, w), dtype=np.float32), np.zeros((f, w), dtype=np.float32)
+    pre[:f] = 1000.0
+    events = np.minimum(np.arange(0, w, each) + rng.integers(0, each, -(-w // each)), w - 1)
+    units = rng.integers(0, f, events.size)
+    pre[units, events], pre[f + units, events] = 0.0, rng.standard_normal(events.size)
+    dy[units, events] = rng.standard_normal(events.size)
+    at = np.asarray(at)
+    cols = np.unique(np.concatenate([events, events - 1, at[:-1], at[1:] - 1]))
+    return F(pre), F(rng.standard_normal((f, n))), F(dy), F(rng.standard_normal((f, n))), cols[(cols >= at[0]) & (cols < at[-1])]
+
+
+@pytest.mark.parametrize("f,w,at", [(64, 20011, None), (130, 40000, None), (30, 40000, None), (1, 80000, None), (64, 530000, None), (20, 530000, None), (64, 20011, [5, 700, 700, 9000, 19711]),
+                                    (130, 40000, [0, 3, 12345, 39990, 40000]), (30, 40000, [0, 17000, 40000]), (1, 80000, [100, 101, 9000, 79990]), (64, 530000, [9, 300000, 529000]),
+                                    (7, 1060000, [0, 12345, 1060000])])
+def test_gated_scan_hands_on_through_many_chunks(cm, rng, f, w, at):
+    """More than 256 chunks, and more than 4096, so that links of 16 chunks, of 256 and of 4096 are joined: every column, the states and all derivatives.  Of gates of 1 and
+    inputs of 0 the links are joined exactly; other joins round what `off` counts for the columns that the links are of, damped by the gates behind them, but for those
+    that come last: at most three of each of four levels and two of the workgroup's own, less than 16 of the magnitudes at the last column where anything happened."""
+    at = at or [0, w]
+    pre, state, dy, dlast, cols = rare(rng, f, w, at)
+    few = np.searchsorted(cols, at)
+    o, S = cm.CUDAMatrix(F([at])), cm.CUDAMatrix(state)
+    P, y, last = cm.CUDAMatrix(pre), cm.CUDAMatrix(F(np.zeros((f, w)))), cm.CUDAMatrix(F(np.zeros(state.shape)))
+    cm.gated_scan(P, target=y, offsets=o, state=S, last=last)
+    got = y.asarray().copy()
+    want, want_last, off, last_off = seq.gated_scan(pre[:, cols], few, state)
+    inside = np.arange(at[0], at[-1])
+    seen = np.searchsorted(cols, inside, side='right') - 1                # (the first column of a sequence is one of them)
+    check(got[:, inside], want[:, seen], (STEP + 16) * U * off[:, seen], 'y')
+    assert not got[:, :at[0]].any() and not got[:, at[-1]:].any()
+    check(last.asarray(), want_last, (STEP + 16) * U * last_off + U * np.abs(want_last), 'last')
+    D, ds = cm.CUDAMatrix(dy), cm.CUDAMatrix(F(np.zeros(state.shape)))
+    dp = cm.CUDAMatrix(F(np.zeros((2 * f, w))))
+    cm.gated_scan_grad(D, P, y, target=dp, offsets=o, state=S, last_deriv=cm.CUDAMatrix(dlast), state_grad=ds)
+    want, want_state, off, state_off = seq.gated_scan_grad(dy[:, cols], pre[:, cols], got[:, cols], few, state, dlast)
+    g = dp.asarray()
+    check(g[:, cols], want, (STEP + 16) * U * (off + np.abs(want)), 'dpre')
+    rest = np.ones(w, dtype=bool)
+    rest[cols] = False
+    assert not g[:, rest].any()                                            # (1 - gate is 0)
+    check(ds.asarray(), want_state, (STEP + 16) * U * state_off + U * np.abs(want_state), 'dstate')
+    assert np.abs(want_state).max() > 0.1 and np.abs(want_last).max() > 0.1
+    release(P, y, D, dp)
+
+
 def test_gated_scan_gradients_against_differences(cm):
     """The device's gradients along random directions against differences of the oracle's recurrence."""
     rng = np.random.default_rng(6)

@@ -39,8 +39,9 @@ __global__ void __launch_bounds__(256) k_embed(const float* mat, const float* la
 
 // ------------------------------------------------------------------ gradient of the table
 // Columns are first sorted by token (k_embed_sort), then every token's run of columns is added up (k_embed_sums), long runs in pieces whose
-// sums k_embed_join adds: every order of addition follows from the labels alone, and nobody adds more than a few dozen columns by itself
-// where a token is frequent.
+// sums k_embed_join adds: every order of addition follows from the labels alone.  Of a token with n > 16 columns a piece is up to sqrt(n / 2) of them, one
+// after the other (n <= 2048: 16), and then up to sqrt(8 n) sums of pieces are added likewise, in 32 bits: at most 4608 roundings in a row for 2^21 columns.  In one launch
+// (k_embed_few) these are n / 16 and 16, of up to 64 rows n / 64 and 64.
 #define EMBED_RUN 16               // columns that one team adds for a token
 #define EMBED_SLOT 8               // one slot for as many sorted columns: a run of more than EMBED_RUN has at least as many slots as pieces
 #define EMBED_RANGE 512            // tokens of a workgroup that sorts

@@ -98,6 +98,30 @@ def test_embed_grad_of_one_frequent_token(cm, rng, w):
         check_embed_grad(g.asarray(), dy, labels, n)
 
 
+@pytest.mark.parametrize("h,w", [(12, 2000), (12, 8192), (100, 8192), (3, 8192), (12, 8193), (12, 70000), (300, 70000), (1, 1 << 21)])
+def test_embed_grad_of_a_frequent_token_adds_in_short_chains(cm, h, w):
+    """2^25, where a step of fp32 is 4, and ones: added one after the other these would all be lost.  Bound: as many roundings as follow each other in the longest
+    chain, and the scaling's."""
+    if w <= 8192:
+        teams = 16 if h > 64 else 64
+        chain = -(-w // teams) + teams
+    else:
+        piece = 16
+        while 8 * piece * piece < w:
+            piece *= 2
+        chain = piece + -(-w // piece)
+    dy, labels = cm.empty((h, w)), cm.empty((1, w))
+    dy.assign(1.0)
+    labels.assign(3.0)
+    for at in (0, w // 2, w - 1):
+        dy.slice(at, at + 1).assign(float(1 << 25))
+        g = cm.embed_grad(dy, labels, cm.CUDAMatrix(F(np.full((h, 5), np.nan)))).asarray()
+        dy.slice(at, at + 1).assign(1.0)
+        total = (1 << 25) + w - 1
+        assert np.abs(g[:, 3] - float(total)).max() <= U * (chain + 1) * total < w / 2, (at, g[0, 3] - total)
+        assert not g[:, [0, 1, 2, 4]].any()
+
+
 def test_embed_of_no_vocabulary(cm):
     y = cm.CUDAMatrix(F(np.full((6, 5), np.nan)))
     cm.embed(cm.empty((6, 0)), cm.CUDAMatrix(F([[0, 1, -1, 2, 3]])), target=y)

@@ -250,8 +250,9 @@ __device__ __forceinline__ u64 sample_ask(const SampleRule& rule, u64 total) {
   return part > 1 ? part : 1;
 }
 
-// The greatest border that leaves enough: bit by bit, a pass over the column each.  For columns whose border lies among thousands of
-// entries that are alike or nearly so.
+// The greatest border that leaves enough: bit by bit, a pass over the column each.  For more than LIST best ones, and for columns whose border lies among more than
+// SAMPLE_SHORT entries that are alike or nearly so.  128003 x 64 by 6000 best 1390 us (by 4000 57), by top-p 0.9 of logits in steps of 1/64 2720 (54 of others): slower than
+// elementary operations, and right.
 template <int LANES, int NV, typename F>
 __device__ __forceinline__ u64 sample_bisect(const SampleColumn<LANES, NV>& column, const SampleKept& kept, SampleShared<LANES>& sh, u64 enough, F value) {
   u64 border = 0;
